@@ -114,6 +114,25 @@ int kr_softmax_cdf(const uint16_t* logits, int N, int V, long long ld, int32_t* 
 int kr_softmax_probs(const uint16_t* logits, int N, int V, long long ld, float* probs,
                      void* stream);
 
+/* Scores of tokens, for callers that want a text's cost or a model's next
+ * tokens without a coder (no reference counterpart): per row of logits (fp16,
+ * or fp32 with logits_f32; any row stride ld >= V, any V), in nats,
+ *   logprob[row]  = ln softmax(row)[tokens[row]]; 0 where tokens[row] = -1 (a
+ *                   row without a token), NaN for any other id outside 0..V-1;
+ *   entropy[row]  = -sum p ln p;
+ *   top_logprob, top_token [N, n_top]: the n_top most likely tokens, largest
+ *                   first, equal ones by lower id (n_top <= 64 and <= V; 0:
+ *                   none, both pointers may be NULL).
+ * A logit of -inf is a masked token: probability 0, never among the top ones
+ * (missing ones are -1 with -inf). A row of only masked tokens has logprob
+ * -inf and entropy 0; a row with a NaN or +inf has NaN everywhere and top
+ * tokens -1. Sums are fp32 in an order that does not depend on N. These are
+ * the softmax's own probabilities: the coder's integer CDF adds a floor of one
+ * count per token and rounds to 2^-cdf_precision. */
+int kr_token_scores(const void* logits, int logits_f32, int N, int V, long long ld,
+                    const int32_t* tokens, float* logprob, float* entropy, int n_top,
+                    float* top_logprob, int32_t* top_token, void* stream);
+
 /* Fused compress stage: per row only the interval of symbols[row],
  * pairs[row] = (cdf[sym], cdf[sym+1]) — replaces det_softmax_cdf + cumsum +
  * the coder's two reads (cpp_path.py:499-500, encode_kernel.cu:110-111). */

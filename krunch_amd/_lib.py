@@ -60,6 +60,7 @@ _SIGS = {
     "kr_probs_to_cdf": ([P, I, I, LL, P, I, P], I),
     "kr_softmax_cdf": ([P, I, I, LL, P, I, I, P], I),
     "kr_softmax_probs": ([P, I, I, LL, P, P], I),
+    "kr_token_scores": ([P, I, I, I, LL, P, P, P, I, P, P, P], I),
     "kr_softmax_cdf_pairs": ([P, I, I, LL, P, P, I, P], I),
     "kr_softmax_cdf_decode": ([P, I, I, LL, P, U32, P, P, P, P, P, LL, P, P, I, P], I),
     # GEMM / layers / model

@@ -169,6 +169,48 @@ def softmax_probs(logits):
     return out
 
 
+def _on(t):
+    """The stream to launch on for tensors of t's device: that device's current
+    stream, with the device made current where it is not."""
+    return torch.cuda.device(t.device)
+
+
+TOP_TOKENS_MAX = 64
+
+
+def token_scores(logits, tokens, n_top: int = 0):
+    """Log probabilities of given tokens, entropies and the most likely tokens
+    of rows of logits, in nats: logits [N, V] fp16 or fp32 (rows may be strided),
+    tokens int32 [N] -> (logprob [N], entropy [N], top_logprob [N, n_top],
+    top_token int32 [N, n_top]). A token of -1 is none (logprob 0); other ids
+    outside 0..V-1 give NaN. Logits of -inf are masked tokens: never among the
+    top ones, whose missing places hold -1 and -inf. A row of only masked tokens
+    has logprob -inf and entropy 0, one with a NaN or +inf is NaN. Equal logits
+    are ranked by lower id. n_top <= 64."""
+    _check(logits.is_cuda, "logits must be a device tensor")
+    _check(logits.dtype in (torch.float16, torch.float32),
+           f"logits must be float16 or float32, got {logits.dtype}")
+    _check(logits.dim() == 2, "logits must be [N, V]")
+    N, V = logits.shape
+    ld = logits.stride(0) if N > 1 else V
+    _check(V >= 1 and (V == 1 or logits.stride(1) == 1) and ld >= V,
+           "logits rows must be contiguous and not overlap")
+    _cuda(tokens, torch.int32, "tokens")
+    _check(tokens.device == logits.device, "tokens and logits must be on one device")
+    _check(tokens.dim() == 1 and tokens.numel() == N, f"tokens must be [N] = [{N}]")
+    _check(0 <= n_top <= min(TOP_TOKENS_MAX, V),
+           f"n_top must be in 0..{min(TOP_TOKENS_MAX, V)}, got {n_top}")
+    dev = logits.device
+    with _on(logits):
+        logprob, entropy = torch.empty((2, N), dtype=torch.float32, device=dev)
+        top_logprob = torch.empty((N, n_top), dtype=torch.float32, device=dev)
+        top_token = torch.empty((N, n_top), dtype=torch.int32, device=dev)
+        _lib.call("kr_token_scores", logits.data_ptr(), logits.dtype == torch.float32, N, V, ld,
+                  tokens.data_ptr(), logprob.data_ptr(), entropy.data_ptr(), n_top,
+                  top_logprob.data_ptr(), top_token.data_ptr(), _lib.stream_ptr())
+    return logprob, entropy, top_logprob, top_token
+
+
 # ---------------------------------------------------------------------------
 # matmul / layer ops (layer_cpp.cpp)
 # ---------------------------------------------------------------------------
