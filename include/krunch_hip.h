@@ -250,6 +250,33 @@ typedef struct kr_layer_q8 {
     kr_matrix_q8 K, V, R, O, fK, fV, fR;
 } kr_layer_q8;
 
+/* 4-bit weights with group scales (no reference counterpart; beside w8a8, for
+ * products over few rows, where the weights are most of what is read): integers
+ * q in -8..7 and one fp16 scale per output and group of 32, 64 or 128 inputs,
+ * weight = q * s. kr_quantize_w4 makes them from W [K, N] fp16 (element (k, n)
+ * at W[k * ldk + n * ldn], so either orientation): s = fp16(max |w| / 7), q =
+ * w / s to the nearest integer, ties to even, at most 7 in size, 0 where s is
+ * 0; a group with an infinity or NaN gets a NaN scale. K % 32 == 0, any N.
+ * q holds kr_w4_bytes(N, K) bytes, 16-byte aligned: blocks of 16 outputs x 128
+ * inputs, 1 KB, outputs major; lane l of a block holds four 32-bit words, word
+ * c the inputs 32 c + 8 (l / 16) + e of output l % 16 as nibbles q + 8, e = 0,
+ * 2, 4, 6, 1, 3, 5, 7 from the low nibble up; outputs and inputs past N and K
+ * are q = 0. scales is fp16 [ceil(K / group), N rounded up to 16], 8-byte
+ * aligned, 0 past N. */
+size_t kr_w4_bytes(int N, int K);
+int kr_quantize_w4(const uint16_t* W, long long ldk, long long ldn, int N, int K, int group, void* q,
+                   uint16_t* scales, void* stream);
+
+/* out = epilogue(x [M, K] @ W) with W in 4 bits; epilogues, res and gate as
+ * kr_det_matmul. x rows have stride ldx (a multiple of 8, x 16-byte aligned),
+ * out rows any stride ldo >= N. Products q x are exact, their sums and the
+ * scaling fp32: c_g = chain of v_mfma_f32_16x16x32_f16 over group g, P =
+ * fma(s_g, c_g, P) over the groups of a 512-wide slice of K from zero, acc = P_0
+ * + P_1 + ... left to right; so a row has the same bits for any M. */
+int kr_det_matmul_w4(const uint16_t* x, long long ldx, int M, int K, const void* q,
+                     const uint16_t* scales, int group, int N, void* out, long long ldo, int epilogue,
+                     const uint16_t* res, const uint16_t* gate, void* stream);
+
 typedef struct kr_layer_weights {
     const void *ln1_w, *ln1_b;            /* fp16 [C] */
     const void *tm_k, *tm_v, *tm_r;       /* fp16 [C] */

@@ -17,6 +17,7 @@ kernel phases rather than the reference's eleven.
 from __future__ import annotations
 
 import weakref
+from dataclasses import dataclass
 
 import torch
 
@@ -261,6 +262,81 @@ def det_matmul(x, W, out_dtype=None):
     wt, _, _keep = _copies(W, False)
     _lib.call("kr_det_matmul", x.data_ptr(), M, K, wt, K, N, out.data_ptr(), N,
               ep, None, None, _lib.stream_ptr())
+    return out
+
+
+@dataclass
+class W4:
+    """A [K, N] weight in 4 bits (kr_quantize_w4): q int32 [kr_w4_bytes / 4] in
+    blocks of 16 outputs x 128 inputs, scales fp16 [ceil(K / group), N rounded up
+    to 16], one per output and group of 32, 64 or 128 inputs."""
+    q: torch.Tensor
+    scales: torch.Tensor
+    K: int
+    N: int
+    group: int = 64
+
+
+def quantize_w4(W, group: int = 64) -> W4:
+    """W fp16 [K, N] (y = x @ W; a transposed view will do) -> W4: weight q * s
+    with s = fp16(max |w| / 7) over a group, q = w / s to the nearest integer in
+    -7..7. K must be a multiple of 32. 4 bits a weight and 16 / group for its scale."""
+    _check(W.is_cuda and W.dtype == torch.float16, "W must be a float16 device tensor")
+    _check(W.dim() == 2, "W must be [K, N]")
+    K, N = W.shape
+    ldk, ldn = W.stride()
+    _check(K >= 32 and K % 32 == 0, f"K = {K} must be a multiple of 32")
+    _check(N >= 1 and ldk >= 1 and ldn >= 1, "W must not be empty or broadcast")
+    _check(group in (32, 64, 128), f"group must be 32, 64 or 128, got {group}")
+    with _on(W):
+        q = torch.empty(_lib.lib().kr_w4_bytes(N, K) // 4, dtype=torch.int32, device=W.device)
+        scales = torch.empty(((K + group - 1) // group, (N + 15) // 16 * 16), dtype=torch.float16,
+                             device=W.device)
+        _lib.call("kr_quantize_w4", W.data_ptr(), ldk, ldn, N, K, group, q.data_ptr(),
+                  scales.data_ptr(), _lib.stream_ptr())
+    return W4(q, scales, K, N, group)
+
+
+EPILOGUES_W4 = {"none": 1, "sigmoid": 2, "relu2": 3, "residual": 4, "gated": 5}
+
+
+def det_matmul_w4(x, W: W4, out_dtype=None, epilogue: str = "none", res=None, gate=None):
+    """y = x @ W, x fp16 [M, K] (rows may be strided), W in 4 bits; exact products,
+    fp32 sums and scales in a fixed order, so each row's result does not depend on
+    M. fp16 out, or fp32 with epilogue "none". Epilogues on h = fp16(acc): "sigmoid"
+    (h), "relu2" max(h, 0)^2, "residual" res + h, "gated" res + fp16(gate * h), with
+    res and gate fp16 [M, N]."""
+    _check(x.is_cuda and x.dtype == torch.float16, "x must be a float16 device tensor")
+    _check(x.dim() == 2, "x must be [M, K]")
+    M, K = x.shape
+    N, group = W.N, W.group
+    _check(K == W.K, f"inner dimensions differ: x has {K}, W {W.K}")
+    ldx = x.stride(0) if M > 1 else K
+    _check(x.stride(1) == 1 and ldx >= K and ldx % 8 == 0 and x.data_ptr() % 16 == 0,
+           "x rows must be contiguous, 16-byte aligned and not overlap")
+    _check(group in (32, 64, 128), f"group must be 32, 64 or 128, got {group}")
+    _check(K >= 32 and K % 32 == 0 and N >= 1, f"bad W4 shape [{K}, {N}]")
+    N16 = (N + 15) // 16 * 16
+    _check(W.q.dtype == torch.int32 and W.q.is_contiguous()
+           and W.q.numel() == N16 * ((K + 127) // 128) * 16, "W.q does not hold a [K, N] weight")
+    _check(W.scales.dtype == torch.float16 and W.scales.is_contiguous()
+           and W.scales.shape == ((K + group - 1) // group, N16), "W.scales must be [groups, N16]")
+    _check(W.q.device == x.device and W.scales.device == x.device, "x and W must be on one device")
+    dtype = out_dtype or torch.float16
+    _check(dtype in (torch.float16, torch.float32), f"out_dtype must be float16 or float32, got {dtype}")
+    _check(epilogue in EPILOGUES_W4, f"epilogue must be one of {sorted(EPILOGUES_W4)}")
+    _check(dtype == torch.float16 or epilogue == "none", "an epilogue's output is float16")
+    for t, name, need in ((res, "res", epilogue in ("residual", "gated")),
+                          (gate, "gate", epilogue == "gated")):
+        _check((t is not None) == need, f"epilogue {epilogue} takes {'a' if need else 'no'} {name}")
+        if need:
+            _cuda(t, torch.float16, name)
+            _check(t.shape == (M, N) and t.device == x.device, f"{name} must be [{M}, {N}]")
+    with _on(x):
+        out = torch.empty((M, N), dtype=dtype, device=x.device)
+        _lib.call("kr_det_matmul_w4", x.data_ptr(), ldx, M, K, W.q.data_ptr(), W.scales.data_ptr(),
+                  group, N, out.data_ptr(), N, 0 if dtype == torch.float32 else EPILOGUES_W4[epilogue],
+                  _lib.ptr(res), _lib.ptr(gate), _lib.stream_ptr())
     return out
 
 
