@@ -385,6 +385,28 @@ int kr_wkv(int B, int T, int C, const float* decay, const float* first, const fl
            const float* v, const uint16_t* r, float* aa, float* bb, float* pp, uint16_t* ry,
            void* stream);
 
+/* WKV with heads (no reference counterpart; beside kr_wkv, for models whose
+ * recurrence keeps a D x D matrix per head): r, k, v fp16 [B, T, H, D] by token
+ * strides ldr, ldk, ldv (elements, multiples of 8; streams follow at T tokens),
+ * state fp32 [B, H, D, D] (key channel major) updated in place, decay (w) and
+ * first (u) fp32 [H], y fp16 by ldy:
+ *   y_t = r_t (S + u k_t' v_t);  S <- e^w S + k_t' v_t
+ * w above 0 counts as 0, -inf is no memory. D is 64 or 128. lens (nullable = T)
+ * gives each stream's tokens, clamped to 0..T: its state stops there and its
+ * later rows of y are zeros, whatever r, k, v hold there. chunked = 0: token by
+ * token in fp32; T tokens in one call have the bits of T calls of one. chunked =
+ * 1: 64 tokens at a time on the matrix units, for prompts: equal to that up to
+ * rounding, and in an order that depends on B * H and T (the time axis is split
+ * over workgroups where heads are few). A NaN or infinity of a token then also
+ * reaches y of up to 63 tokens before it. Calls of at most 16 tokens
+ * are the same in both. ws: kr_wkv_heads_workspace_bytes (chunked only, may be
+ * 0), 16-byte aligned, as r, k, v, state and y. */
+size_t kr_wkv_heads_workspace_bytes(int B, int T, int H, int D);
+int kr_wkv_heads(int B, int T, int H, int D, const uint16_t* r, long long ldr, const uint16_t* k,
+                 long long ldk, const uint16_t* v, long long ldv, const float* decay,
+                 const float* first, const int32_t* lens, float* state, uint16_t* y, long long ldy,
+                 int chunked, void* ws, size_t ws_bytes, void* stream);
+
 /* All layers over x [B*T, C] (cpp_path.forward_packed_window's layer loop,
  * :155-160; forward_stepped_batched's with T = 1, :451-456). */
 int kr_forward_layers(const kr_model_weights* m, void* x, int B, int T, void* state, void* ws,

@@ -85,6 +85,8 @@ _SIGS = {
     "kr_layer_step_noalloc": ([ctypes.POINTER(KrLayerWeights), I, I, P, I, I, P, P, P, P, P, P],
                               I),
     "kr_wkv": ([I, I, I, P, P, P, P, P, P, P, P, P, P], I),
+    "kr_wkv_heads_workspace_bytes": ([I, I, I, I], SZ),
+    "kr_wkv_heads": ([I, I, I, I, P, LL, P, LL, P, LL, P, P, P, P, P, LL, I, P, SZ, P], I),
     "kr_phase_profile": ([I], I),
     "kr_phase_count": ([], I),
     "kr_phase_name": ([I], ctypes.c_char_p),

@@ -340,6 +340,51 @@ def det_matmul_w4(x, W: W4, out_dtype=None, epilogue: str = "none", res=None, ga
     return out
 
 
+def wkv_heads(r, k, v, decay, first, state, lens=None, chunked: bool = True):
+    """WKV with a matrix state per head: y_t = r_t (S + u k_t' v_t), then S <- e^w S
+    + k_t' v_t. r, k, v fp16 [B, T, H, D], D 64 or 128 (heads contiguous; token
+    strides free, so slices of one projection will do), decay (w <= 0) and first
+    (u) fp32 [H], state fp32 [B, H, D, D] updated in place; returns y fp16
+    [B, T, H, D]. lens int32 [B]: each stream's tokens (its state stops there, later
+    rows of y are 0). chunked=True (prompts, scoring) takes 64 tokens at a time on
+    the matrix units; chunked=False, and calls of at most 16 tokens, go token by
+    token, and T tokens then have the bits of T calls, as a codec's two directions need."""
+    _check(r.dim() == 4, "r must be [B, T, H, D]")
+    B, T, H, D = r.shape
+    _check(D in (64, 128), f"D must be 64 or 128, got {D}")
+    _check(H >= 1, "r must have a head")
+    dev = r.device
+    ld = []
+    for t, name in ((r, "r"), (k, "k"), (v, "v")):
+        _check(t.is_cuda and t.dtype == torch.float16, f"{name} must be a float16 device tensor")
+        _check(t.shape == r.shape and t.device == dev, f"{name} must be [B, T, H, D] on r's device")
+        sb, st, sh, sd = t.stride()
+        if t.numel():
+            if T == 1:
+                st = sb if B > 1 else H * D
+            _check(sd == 1 and (H == 1 or sh == D) and st >= H * D and (B == 1 or sb == T * st)
+                   and st % 8 == 0 and t.data_ptr() % 16 == 0,
+                   f"{name}: heads must be contiguous, tokens evenly spaced and 16-byte aligned")
+        ld.append(st if t.numel() else H * D)
+    for t, name in ((decay, "decay"), (first, "first")):
+        _cuda(t, torch.float32, name)
+        _check(t.numel() == H and t.device == dev, f"{name} must be [H] = [{H}]")
+    _cuda(state, torch.float32, "state")
+    _check(state.shape == (B, H, D, D) and state.device == dev and state.data_ptr() % 16 == 0,
+           f"state must be [B, H, D, D] = [{B}, {H}, {D}, {D}], 16-byte aligned")
+    if lens is not None:
+        _cuda(lens, torch.int32, "lens")
+        _check(lens.numel() == B and lens.device == dev, f"lens must be [B] = [{B}]")
+    with _on(r):
+        y = torch.empty((B, T, H, D), dtype=torch.float16, device=dev)
+        nbytes = _lib.lib().kr_wkv_heads_workspace_bytes(B, T, H, D) if chunked else 0
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        _lib.call("kr_wkv_heads", B, T, H, D, r.data_ptr(), ld[0], k.data_ptr(), ld[1], v.data_ptr(),
+                  ld[2], decay.data_ptr(), first.data_ptr(), _lib.ptr(lens), state.data_ptr(),
+                  y.data_ptr(), H * D, 1 if chunked else 0, _lib.ptr(ws), nbytes, _lib.stream_ptr())
+    return y
+
+
 def _layer_struct(x, att_xx, aa, bb, pp, ffn_xx, ln1_w, ln1_b, tm_k, tm_v, tm_r, time_decay,
                   time_first, Kw, Vw, Rw, Ow, ln2_w, ln2_b, ffn_tm_k, ffn_tm_r, ffn_Kw, ffn_Vw,
                   ffn_Rw):
