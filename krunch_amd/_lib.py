@@ -136,7 +136,7 @@ def exported_symbols():
 
 def call(name: str, *args):
     """Call an int-returning entry point and raise KrunchError on failure."""
-    rc = getattr(lib(), name)(*args)
+    rc = getattr(_lib or lib(), name)(*args)
     if rc != 0:
         msg = lib().kr_last_error().decode(errors="replace")
         raise KrunchError(f"{name} failed ({rc}): {msg}")
@@ -165,7 +165,20 @@ def ptr(t) -> int | None:
     return t.data_ptr()
 
 
+_raw_stream = None
+
+
 def stream_ptr(stream=None) -> int | None:
-    import torch
-    s = stream if stream is not None else torch.cuda.current_stream()
-    return s.cuda_stream
+    """hipStream_t of a torch stream, or of the current device's current one (by
+    torch's raw-stream query where it has one: 0.3 us a call, 2.5 through a
+    Stream object)."""
+    global _raw_stream
+    if stream is not None:
+        return stream.cuda_stream
+    if _raw_stream is None:
+        import torch
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        device = torch.cuda.current_device
+        _raw_stream = ((lambda: raw(device())) if raw is not None
+                       else (lambda: torch.cuda.current_stream().cuda_stream))
+    return _raw_stream()

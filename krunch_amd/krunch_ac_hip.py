@@ -170,10 +170,22 @@ def softmax_probs(logits):
     return out
 
 
-def _on(t):
-    """The stream to launch on for tensors of t's device: that device's current
-    stream, with the device made current where it is not."""
-    return torch.cuda.device(t.device)
+# The operators below launch on the current stream of their tensors' device, and
+# check with "condition or _refuse(message)": a message is only made for a call
+# that is refused (a small call's time is the host's).
+
+def _refuse(msg):
+    raise RuntimeError(msg)
+
+
+def _on_device_of(t, op, *args):
+    """op(*args) with t's device current."""
+    with torch.cuda.device(t.device):
+        return op(*args)
+
+
+def _elsewhere(t):
+    return t.get_device() != torch.cuda.current_device()
 
 
 TOP_TOKENS_MAX = 64
@@ -188,27 +200,32 @@ def token_scores(logits, tokens, n_top: int = 0):
     top ones, whose missing places hold -1 and -inf. A row of only masked tokens
     has logprob -inf and entropy 0, one with a NaN or +inf is NaN. Equal logits
     are ranked by lower id. n_top <= 64."""
-    _check(logits.is_cuda, "logits must be a device tensor")
-    _check(logits.dtype in (torch.float16, torch.float32),
-           f"logits must be float16 or float32, got {logits.dtype}")
-    _check(logits.dim() == 2, "logits must be [N, V]")
+    logits.is_cuda or _refuse("logits must be a device tensor")
+    f32 = logits.dtype is torch.float32
+    f32 or logits.dtype is torch.float16 or _refuse(
+        f"logits must be float16 or float32, got {logits.dtype}")
+    logits.dim() == 2 or _refuse("logits must be [N, V]")
     N, V = logits.shape
-    ld = logits.stride(0) if N > 1 else V
-    _check(V >= 1 and (V == 1 or logits.stride(1) == 1) and ld >= V,
-           "logits rows must be contiguous and not overlap")
-    _cuda(tokens, torch.int32, "tokens")
-    _check(tokens.device == logits.device, "tokens and logits must be on one device")
-    _check(tokens.dim() == 1 and tokens.numel() == N, f"tokens must be [N] = [{N}]")
-    _check(0 <= n_top <= min(TOP_TOKENS_MAX, V),
-           f"n_top must be in 0..{min(TOP_TOKENS_MAX, V)}, got {n_top}")
-    dev = logits.device
-    with _on(logits):
-        logprob, entropy = torch.empty((2, N), dtype=torch.float32, device=dev)
-        top_logprob = torch.empty((N, n_top), dtype=torch.float32, device=dev)
-        top_token = torch.empty((N, n_top), dtype=torch.int32, device=dev)
-        _lib.call("kr_token_scores", logits.data_ptr(), logits.dtype == torch.float32, N, V, ld,
-                  tokens.data_ptr(), logprob.data_ptr(), entropy.data_ptr(), n_top,
-                  top_logprob.data_ptr(), top_token.data_ptr(), _lib.stream_ptr())
+    ld, step = logits.stride()
+    if N <= 1:
+        ld = V
+    (V >= 1 and (step == 1 or V == 1) and ld >= V) or _refuse(
+        "logits rows must be contiguous and not overlap")
+    (tokens.is_cuda and tokens.dtype is torch.int32 and tokens.is_contiguous()) or _refuse(
+        "tokens must be a contiguous int32 device tensor")
+    tokens.get_device() == logits.get_device() or _refuse("tokens and logits must be on one device")
+    tokens.shape == (N,) or _refuse(f"tokens must be [N] = [{N}]")
+    0 <= n_top <= min(TOP_TOKENS_MAX, V) or _refuse(
+        f"n_top must be in 0..{min(TOP_TOKENS_MAX, V)}, got {n_top}")
+    if _elsewhere(logits):
+        return _on_device_of(logits, token_scores, logits, tokens, n_top)
+    logprob = torch.empty_like(tokens, dtype=torch.float32)
+    entropy = torch.empty_like(logprob)
+    top_logprob = logprob.new_empty((N, n_top))
+    top_token = tokens.new_empty((N, n_top))
+    _lib.call("kr_token_scores", logits.data_ptr(), f32, N, V, ld, tokens.data_ptr(),
+              logprob.data_ptr(), entropy.data_ptr(), n_top, top_logprob.data_ptr(),
+              top_token.data_ptr(), _lib.stream_ptr())
     return logprob, entropy, top_logprob, top_token
 
 
@@ -281,19 +298,19 @@ def quantize_w4(W, group: int = 64) -> W4:
     """W fp16 [K, N] (y = x @ W; a transposed view will do) -> W4: weight q * s
     with s = fp16(max |w| / 7) over a group, q = w / s to the nearest integer in
     -7..7. K must be a multiple of 32. 4 bits a weight and 16 / group for its scale."""
-    _check(W.is_cuda and W.dtype == torch.float16, "W must be a float16 device tensor")
-    _check(W.dim() == 2, "W must be [K, N]")
+    (W.is_cuda and W.dtype is torch.float16) or _refuse("W must be a float16 device tensor")
+    W.dim() == 2 or _refuse("W must be [K, N]")
     K, N = W.shape
     ldk, ldn = W.stride()
-    _check(K >= 32 and K % 32 == 0, f"K = {K} must be a multiple of 32")
-    _check(N >= 1 and ldk >= 1 and ldn >= 1, "W must not be empty or broadcast")
-    _check(group in (32, 64, 128), f"group must be 32, 64 or 128, got {group}")
-    with _on(W):
-        q = torch.empty(_lib.lib().kr_w4_bytes(N, K) // 4, dtype=torch.int32, device=W.device)
-        scales = torch.empty(((K + group - 1) // group, (N + 15) // 16 * 16), dtype=torch.float16,
-                             device=W.device)
-        _lib.call("kr_quantize_w4", W.data_ptr(), ldk, ldn, N, K, group, q.data_ptr(),
-                  scales.data_ptr(), _lib.stream_ptr())
+    (K >= 32 and K % 32 == 0) or _refuse(f"K = {K} must be a multiple of 32")
+    (N >= 1 and ldk >= 1 and ldn >= 1) or _refuse("W must not be empty or broadcast")
+    group in (32, 64, 128) or _refuse(f"group must be 32, 64 or 128, got {group}")
+    if _elsewhere(W):
+        return _on_device_of(W, quantize_w4, W, group)
+    q = torch.empty(_lib.lib().kr_w4_bytes(N, K) // 4, dtype=torch.int32, device=W.device)
+    scales = W.new_empty(((K + group - 1) // group, (N + 15) // 16 * 16))
+    _lib.call("kr_quantize_w4", W.data_ptr(), ldk, ldn, N, K, group, q.data_ptr(),
+              scales.data_ptr(), _lib.stream_ptr())
     return W4(q, scales, K, N, group)
 
 
@@ -306,37 +323,42 @@ def det_matmul_w4(x, W: W4, out_dtype=None, epilogue: str = "none", res=None, ga
     M. fp16 out, or fp32 with epilogue "none". Epilogues on h = fp16(acc): "sigmoid"
     (h), "relu2" max(h, 0)^2, "residual" res + h, "gated" res + fp16(gate * h), with
     res and gate fp16 [M, N]."""
-    _check(x.is_cuda and x.dtype == torch.float16, "x must be a float16 device tensor")
-    _check(x.dim() == 2, "x must be [M, K]")
+    (x.is_cuda and x.dtype is torch.float16) or _refuse("x must be a float16 device tensor")
+    x.dim() == 2 or _refuse("x must be [M, K]")
     M, K = x.shape
-    N, group = W.N, W.group
-    _check(K == W.K, f"inner dimensions differ: x has {K}, W {W.K}")
-    ldx = x.stride(0) if M > 1 else K
-    _check(x.stride(1) == 1 and ldx >= K and ldx % 8 == 0 and x.data_ptr() % 16 == 0,
-           "x rows must be contiguous, 16-byte aligned and not overlap")
-    _check(group in (32, 64, 128), f"group must be 32, 64 or 128, got {group}")
-    _check(K >= 32 and K % 32 == 0 and N >= 1, f"bad W4 shape [{K}, {N}]")
+    q, scales, N, group = W.q, W.scales, W.N, W.group
+    K == W.K or _refuse(f"inner dimensions differ: x has {K}, W {W.K}")
+    ldx, step = x.stride()
+    if M <= 1:
+        ldx = K
+    xp = x.data_ptr()
+    (step == 1 and ldx >= K and ldx % 8 == 0 and xp % 16 == 0) or _refuse(
+        "x rows must be contiguous, 16-byte aligned and not overlap")
+    group in (32, 64, 128) or _refuse(f"group must be 32, 64 or 128, got {group}")
+    (K >= 32 and K % 32 == 0 and N >= 1) or _refuse(f"bad W4 shape [{K}, {N}]")
     N16 = (N + 15) // 16 * 16
-    _check(W.q.dtype == torch.int32 and W.q.is_contiguous()
-           and W.q.numel() == N16 * ((K + 127) // 128) * 16, "W.q does not hold a [K, N] weight")
-    _check(W.scales.dtype == torch.float16 and W.scales.is_contiguous()
-           and W.scales.shape == ((K + group - 1) // group, N16), "W.scales must be [groups, N16]")
-    _check(W.q.device == x.device and W.scales.device == x.device, "x and W must be on one device")
-    dtype = out_dtype or torch.float16
-    _check(dtype in (torch.float16, torch.float32), f"out_dtype must be float16 or float32, got {dtype}")
-    _check(epilogue in EPILOGUES_W4, f"epilogue must be one of {sorted(EPILOGUES_W4)}")
-    _check(dtype == torch.float16 or epilogue == "none", "an epilogue's output is float16")
-    for t, name, need in ((res, "res", epilogue in ("residual", "gated")),
-                          (gate, "gate", epilogue == "gated")):
-        _check((t is not None) == need, f"epilogue {epilogue} takes {'a' if need else 'no'} {name}")
+    (q.dtype is torch.int32 and q.is_contiguous() and q.numel() == N16 * ((K + 127) // 128) * 16
+     and q.data_ptr() % 16 == 0) or _refuse("W.q does not hold a [K, N] weight")
+    (scales.dtype is torch.float16 and scales.is_contiguous() and scales.data_ptr() % 8 == 0
+     and scales.shape == ((K + group - 1) // group, N16)) or _refuse("W.scales must be [groups, N16]")
+    dev = x.get_device()
+    q.get_device() == scales.get_device() == dev or _refuse("x and W must be on one device")
+    f32 = out_dtype is torch.float32
+    f32 or out_dtype in (None, torch.float16) or _refuse(
+        f"out_dtype must be float16 or float32, got {out_dtype}")
+    epilogue in EPILOGUES_W4 or _refuse(f"epilogue must be one of {sorted(EPILOGUES_W4)}")
+    f32 and epilogue != "none" and _refuse("an epilogue's output is float16")
+    code = 0 if f32 else EPILOGUES_W4[epilogue]
+    for t, name, need in ((res, "res", code >= 4), (gate, "gate", code == 5)):
+        (t is not None) == need or _refuse(f"epilogue {epilogue} takes {'a' if need else 'no'} {name}")
         if need:
             _cuda(t, torch.float16, name)
-            _check(t.shape == (M, N) and t.device == x.device, f"{name} must be [{M}, {N}]")
-    with _on(x):
-        out = torch.empty((M, N), dtype=dtype, device=x.device)
-        _lib.call("kr_det_matmul_w4", x.data_ptr(), ldx, M, K, W.q.data_ptr(), W.scales.data_ptr(),
-                  group, N, out.data_ptr(), N, 0 if dtype == torch.float32 else EPILOGUES_W4[epilogue],
-                  _lib.ptr(res), _lib.ptr(gate), _lib.stream_ptr())
+            (t.shape == (M, N) and t.get_device() == dev) or _refuse(f"{name} must be [{M}, {N}]")
+    if _elsewhere(x):
+        return _on_device_of(x, det_matmul_w4, x, W, out_dtype, epilogue, res, gate)
+    out = x.new_empty((M, N), dtype=torch.float32) if f32 else x.new_empty((M, N))
+    _lib.call("kr_det_matmul_w4", xp, ldx, M, K, q.data_ptr(), scales.data_ptr(), group, N,
+              out.data_ptr(), N, code, _lib.ptr(res), _lib.ptr(gate), _lib.stream_ptr())
     return out
 
 
@@ -349,39 +371,49 @@ def wkv_heads(r, k, v, decay, first, state, lens=None, chunked: bool = True):
     rows of y are 0). chunked=True (prompts, scoring) takes 64 tokens at a time on
     the matrix units; chunked=False, and calls of at most 16 tokens, go token by
     token, and T tokens then have the bits of T calls, as a codec's two directions need."""
-    _check(r.dim() == 4, "r must be [B, T, H, D]")
-    B, T, H, D = r.shape
-    _check(D in (64, 128), f"D must be 64 or 128, got {D}")
-    _check(H >= 1, "r must have a head")
-    dev = r.device
+    r.dim() == 4 or _refuse("r must be [B, T, H, D]")
+    shape = r.shape
+    B, T, H, D = shape
+    (D in (64, 128) and H >= 1) or _refuse(f"r must have heads of 64 or 128 channels, got {tuple(shape)}")
+    dev = r.get_device()
+    C = H * D
     ld = []
     for t, name in ((r, "r"), (k, "k"), (v, "v")):
-        _check(t.is_cuda and t.dtype == torch.float16, f"{name} must be a float16 device tensor")
-        _check(t.shape == r.shape and t.device == dev, f"{name} must be [B, T, H, D] on r's device")
+        (t.is_cuda and t.dtype is torch.float16) or _refuse(f"{name} must be a float16 device tensor")
+        (t.shape == shape and t.get_device() == dev) or _refuse(
+            f"{name} must be {tuple(shape)} on r's device")
+        if B * T == 0:
+            ld.append(C)
+            continue
         sb, st, sh, sd = t.stride()
-        if t.numel():
-            if T == 1:
-                st = sb if B > 1 else H * D
-            _check(sd == 1 and (H == 1 or sh == D) and st >= H * D and (B == 1 or sb == T * st)
-                   and st % 8 == 0 and t.data_ptr() % 16 == 0,
-                   f"{name}: heads must be contiguous, tokens evenly spaced and 16-byte aligned")
-        ld.append(st if t.numel() else H * D)
+        if T == 1:
+            st = sb if B > 1 else C
+        (sd == 1 and (sh == D or H == 1) and st >= C and (sb == T * st or B == 1) and st % 8 == 0
+         and t.data_ptr() % 16 == 0) or _refuse(
+            f"{name}: heads must be contiguous, tokens evenly spaced and 16-byte aligned")
+        ld.append(st)
     for t, name in ((decay, "decay"), (first, "first")):
-        _cuda(t, torch.float32, name)
-        _check(t.numel() == H and t.device == dev, f"{name} must be [H] = [{H}]")
-    _cuda(state, torch.float32, "state")
-    _check(state.shape == (B, H, D, D) and state.device == dev and state.data_ptr() % 16 == 0,
-           f"state must be [B, H, D, D] = [{B}, {H}, {D}, {D}], 16-byte aligned")
-    if lens is not None:
-        _cuda(lens, torch.int32, "lens")
-        _check(lens.numel() == B and lens.device == dev, f"lens must be [B] = [{B}]")
-    with _on(r):
-        y = torch.empty((B, T, H, D), dtype=torch.float16, device=dev)
-        nbytes = _lib.lib().kr_wkv_heads_workspace_bytes(B, T, H, D) if chunked else 0
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        _lib.call("kr_wkv_heads", B, T, H, D, r.data_ptr(), ld[0], k.data_ptr(), ld[1], v.data_ptr(),
-                  ld[2], decay.data_ptr(), first.data_ptr(), _lib.ptr(lens), state.data_ptr(),
-                  y.data_ptr(), H * D, 1 if chunked else 0, _lib.ptr(ws), nbytes, _lib.stream_ptr())
+        (t.is_cuda and t.dtype is torch.float32 and t.is_contiguous() and t.numel() == H
+         and t.get_device() == dev) or _refuse(
+            f"{name} must be a contiguous float32 device tensor [H] = [{H}] on r's device")
+    (state.is_cuda and state.dtype is torch.float32 and state.is_contiguous()
+     and state.shape == (B, H, D, D) and state.get_device() == dev
+     and state.data_ptr() % 16 == 0) or _refuse(
+        f"state must be a contiguous float32 device tensor {(B, H, D, D)} on r's device, 16-byte aligned")
+    lens is None or (lens.is_cuda and lens.dtype is torch.int32 and lens.is_contiguous()
+                     and lens.numel() == B and lens.get_device() == dev) or _refuse(
+        f"lens must be a contiguous int32 device tensor [B] = [{B}] on r's device")
+    if _elsewhere(r):
+        return _on_device_of(r, wkv_heads, r, k, v, decay, first, state, lens, chunked)
+    y = r.new_empty(shape)
+    ws, nbytes = None, 0
+    if chunked and T > 1:
+        nbytes = _lib.lib().kr_wkv_heads_workspace_bytes(B, T, H, D)
+        if nbytes:
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=r.device)
+    _lib.call("kr_wkv_heads", B, T, H, D, r.data_ptr(), ld[0], k.data_ptr(), ld[1], v.data_ptr(),
+              ld[2], decay.data_ptr(), first.data_ptr(), _lib.ptr(lens), state.data_ptr(),
+              y.data_ptr(), C, 1 if chunked else 0, _lib.ptr(ws), nbytes, _lib.stream_ptr())
     return y
 
 
