@@ -6,9 +6,8 @@
 //
 // q x has at most 15 significant bits, so c_g is a chain of exact products on
 // v_mfma_f32_16x16x32_f16 (k ascending, from zero), and the scale is applied in
-// fp32. Reduction contract, whatever the kernel: slices of 512 inputs, in a
-// slice P = fma(s_g, c_g, P) over its groups in order from zero, then y = P_0
-// + P_1 + ... left to right; so a row has the same bits for any M.
+// fp32. Reduction contract, whatever the kernel: y = fma(s_g, c_g, y) over the
+// groups in order, from zero; so a row has the same bits for any M.
 //
 // Layout (kr_w4_bytes): blocks of 16 outputs x 128 inputs, 1 KB, (N / 16) major
 // and K / 128 minor. Lane l holds 4 words, word c the inputs 32 c + 8 (l / 16)
@@ -23,8 +22,8 @@
 
 namespace {
 
-constexpr int kBlockK = 128, kSliceK = 512;
-constexpr int kMaxSplit = 8;                 // waves that share a tile's slices
+constexpr int kBlockK = 128;
+constexpr int kMaxSplit = 8;                 // waves that share a tile
 
 typedef kr_half kr_half2 __attribute__((ext_vector_type(2)));
 typedef kr_half4 kr_half4_any __attribute__((aligned(2)));
@@ -39,17 +38,28 @@ struct W4Args {
     kr_gemm_args o;           // out, ldo, res, gate, M, N, K
 };
 
-// The 8 weights of a word as an MFMA operand.
-__device__ __forceinline__ kr_half8 unpack(uint32_t w) {
-    const kr_half2 k1024 = {(kr_half)-1032.0f, (kr_half)-1032.0f};
-    const kr_half2 k64 = {(kr_half)-72.0f, (kr_half)-72.0f};
-    const uint32_t v = w >> 8;
-    const kr_half2 a = __builtin_bit_cast(kr_half2, (w & 0x000F000Fu) | 0x64006400u) + k1024;
-    const kr_half2 b = __builtin_bit_cast(kr_half2, (w & 0x00F000F0u) | 0x54005400u) + k64;
-    const kr_half2 c = __builtin_bit_cast(kr_half2, (v & 0x000F000Fu) | 0x64006400u) + k1024;
-    const kr_half2 d = __builtin_bit_cast(kr_half2, (v & 0x00F000F0u) | 0x54005400u) + k64;
-    return kr_half8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-}
+// The 8 weights of a word as an MFMA operand. The masks and magic numbers are
+// held in registers the compiler does not see into: as literals (one per
+// instruction) they make AND and OR two operations instead of v_and_or_b32.
+struct Unpacker {
+    uint32_t low, high, magic_low, magic_high;
+    __device__ __forceinline__ Unpacker() {
+        __asm__("s_mov_b32 %0, 0x000f000f" : "=s"(low));
+        __asm__("s_mov_b32 %0, 0x00f000f0" : "=s"(high));
+        __asm__("v_mov_b32 %0, 0x64006400" : "=v"(magic_low));
+        __asm__("v_mov_b32 %0, 0x54005400" : "=v"(magic_high));
+    }
+    __device__ __forceinline__ kr_half8 operator()(uint32_t w) const {
+        const kr_half2 k1024 = {(kr_half)-1032.0f, (kr_half)-1032.0f};
+        const kr_half2 k64 = {(kr_half)-72.0f, (kr_half)-72.0f};
+        const uint32_t v = w >> 8;
+        const kr_half2 a = __builtin_bit_cast(kr_half2, (w & low) | magic_low) + k1024;
+        const kr_half2 b = __builtin_bit_cast(kr_half2, (w & high) | magic_high) + k64;
+        const kr_half2 c = __builtin_bit_cast(kr_half2, (v & low) | magic_low) + k1024;
+        const kr_half2 d = __builtin_bit_cast(kr_half2, (v & high) | magic_high) + k64;
+        return kr_half8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+    }
+};
 
 // Columns n..n+3 of row m; rows of out start at any element.
 template <int EP>
@@ -68,115 +78,380 @@ __device__ __forceinline__ void store4(const kr_gemm_args& g, int m, int n, kr_f
     }
 }
 
-__device__ __forceinline__ kr_float4 scale4(const kr_half* s) {
-    const kr_half4 h = *reinterpret_cast<const kr_half4*>(s);
-    return kr_float4{(float)h[0], (float)h[1], (float)h[2], (float)h[3]};
-}
-
-// One slice of one 16-output tile against MT x 16 rows, x read from memory.
-// GS = k-steps per group.
-template <int MT, int GS>
-__device__ __forceinline__ void slice_rows(const W4Args& g, int tile, int k_begin, int k_end,
-                                           const kr_half* const (&xr)[MT], kr_float4 (&P)[MT]) {
+// Groups [g_begin, g_end) of one 16-output tile against 16 rows, x read from
+// memory: each group's chain to take(group, chain). GS = k-steps per group.
+template <int GS, typename Take>
+__device__ __forceinline__ void tile_groups(const W4Args& g, const Unpacker& unpack, int tile, int g_begin,
+                                            int g_end, const kr_half* xr, Take take) {
+    constexpr int GPB = 4 / GS;
     const int lane = threadIdx.x & 63;
     const int kb_all = (g.o.K + kBlockK - 1) / kBlockK;
-    const kr_int4* q = g.q + ((size_t)tile * kb_all + k_begin / kBlockK) * 64 + lane;
-    const kr_half* sc = g.scales + (size_t)(k_begin / (32 * GS)) * g.n16 + 16 * tile + 4 * (lane >> 4);
-    #pragma unroll
-    for (int t = 0; t < MT; t++) P[t] = kr_float4{0, 0, 0, 0};
-    for (int k0 = k_begin; k0 < k_end; k0 += kBlockK, q += 64) {
+    const kr_int4* q = g.q + ((size_t)tile * kb_all + g_begin / GPB) * 64 + lane;
+    for (int g0 = g_begin; g0 < g_end; g0 += GPB, q += 64) {
         const kr_int4 w = *q;
-        kr_float4 c[MT];
         #pragma unroll
-        for (int t = 0; t < MT; t++) c[t] = kr_float4{0, 0, 0, 0};
-        #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int k = k0 + 32 * i;
-            if (k >= k_end) break;
-            const kr_half8 a = unpack((uint32_t)w[i]);
+        for (int j = 0; j < GPB; j++) {
+            if (g0 + j >= g_end) break;
+            kr_float4 c = {0, 0, 0, 0};
             #pragma unroll
-            for (int t = 0; t < MT; t++)
-                c[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                    a, *reinterpret_cast<const kr_half8*>(xr[t] + k), c[t], 0, 0, 0);
-            if ((i + 1) % GS == 0 || k + 32 >= k_end) {
-                const kr_float4 s = scale4(sc);
-                sc += g.n16;
-                #pragma unroll
-                for (int t = 0; t < MT; t++) {
-                    #pragma unroll
-                    for (int r = 0; r < 4; r++) P[t][r] = __builtin_fmaf(s[r], c[t][r], P[t][r]);
-                    c[t] = kr_float4{0, 0, 0, 0};
-                }
+            for (int i = 0; i < GS; i++) {
+                const int k = (g0 + j) * 32 * GS + 32 * i;
+                if (i > 0 && k >= g.o.K) break;
+                c = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                    unpack((uint32_t)w[j * GS + i]), *reinterpret_cast<const kr_half8*>(xr + k), c, 0, 0, 0);
             }
+            take(g0 + j, c);
         }
     }
 }
 
-// Few rows: a wave has a 16-output tile against up to 16 MT rows. With SPLIT,
-// the workgroup's waves share one tile, wave w its slices w, w + waves, ...,
-// joined in LDS in slice order; else each wave has a tile of its own.
-template <int MT, int GS, int EP, bool SPLIT>
-__global__ void __launch_bounds__(SPLIT ? 64 * kMaxSplit : 256) w4_rows_kernel(W4Args g) {
+__device__ __forceinline__ void add_group(kr_half4 s, kr_float4 c, kr_float4& y) {
+    #pragma unroll
+    for (int r = 0; r < 4; r++) y[r] = __builtin_fmaf((float)s[r], c[r], y[r]);
+}
+
+// Up to 16 rows: 16 outputs for a wave, its weights read once, x from the L1.
+// With SPLIT, the workgroup's waves share one tile, each a run of its blocks, and
+// leave every group's chains (of the rows there are) and scales in LDS, from where
+// wave 0 adds them in order, `room` groups at a time; else each wave has a tile of
+// its own.
+// Bound: latency (a launch, a read of memory, the chains of a wave's blocks).
+template <int GS, int EP, bool SPLIT>
+__global__ void __launch_bounds__(SPLIT ? 64 * kMaxSplit : 256) w4_rows_kernel(W4Args g, int room) {
+    constexpr int GPB = 4 / GS;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const int tile = SPLIT ? blockIdx.x : blockIdx.x * waves + wave;
-    const int m0 = blockIdx.y * 16 * MT;
     if (!SPLIT && 16 * tile >= g.n16) return;
-    const kr_half* xr[MT];
-    #pragma unroll
-    for (int t = 0; t < MT; t++) {
-        const int m = m0 + 16 * t + (lane & 15);       // rows past M read the last one
-        xr[t] = g.x + (size_t)(m < g.o.M ? m : g.o.M - 1) * g.ldx + 8 * (lane >> 4);
-    }
-    const int slices = (g.o.K + kSliceK - 1) / kSliceK;
-    kr_float4 total[MT], P[MT];
+    const Unpacker unpack;
+    const int m = lane & 15, q4 = lane >> 4, n = 16 * tile + 4 * q4;     // rows past M read the last one
+    const kr_half* xr = g.x + (size_t)(m < g.o.M ? m : g.o.M - 1) * g.ldx + 8 * q4;
+    const kr_half* sc = g.scales + n;
+    auto scales = [&](int i) { return *reinterpret_cast<const kr_half4*>(sc + (size_t)i * g.n16); };
+    const int groups = (g.o.K + 32 * GS - 1) / (32 * GS);
+    kr_float4 y = {0, 0, 0, 0};
     if constexpr (SPLIT) {
-        extern __shared__ kr_float4 part[];           // [slices][MT][64]
-        for (int z = wave; z < slices; z += waves) {
-            const int k1 = (z + 1) * kSliceK < g.o.K ? (z + 1) * kSliceK : g.o.K;
-            slice_rows<MT, GS>(g, tile, z * kSliceK, k1, xr, P);
-            #pragma unroll
-            for (int t = 0; t < MT; t++) part[(z * MT + t) * 64 + lane] = P[t];
+        extern __shared__ kr_float4 chains[];           // [room][4][M], then the scales [room][4]
+        const int M = g.o.M;
+        kr_half4* held = reinterpret_cast<kr_half4*>(chains + room * 4 * M);
+        for (int at = 0; at < groups; at += room) {
+            const int end = groups - at < room ? groups : at + room;
+            const int run = ((end - at + GPB - 1) / GPB + waves - 1) / waves * GPB;
+            const int g0 = at + wave * run, g1 = g0 + run < end ? g0 + run : end;
+            tile_groups<GS>(g, unpack, tile, g0, g1, xr, [&](int i, kr_float4 c) {
+                const int k = (i - at) * 4 + q4;
+                if (m == 0) held[k] = scales(i);
+                if (m < M) chains[k * M + m] = c;
+            });
+            __syncthreads();
+            if (wave == 0 && m < M) {
+                #pragma unroll 8
+                for (int i = 0; i < end - at; i++) add_group(held[i * 4 + q4], chains[(i * 4 + q4) * M + m], y);
+            }
+            if (end < groups) __syncthreads();
         }
-        __syncthreads();
-        for (int t = wave; t < MT; t += waves) {
-            kr_float4 y = part[t * 64 + lane];
-            for (int z = 1; z < slices; z++) y += part[(z * MT + t) * 64 + lane];
-            store4<EP>(g.o, m0 + 16 * t + (lane & 15), 16 * tile + 4 * (lane >> 4), y);
-        }
+        if (wave == 0) store4<EP>(g.o, m, n, y);
     } else {
-        for (int z = 0; z < slices; z++) {
-            const int k1 = (z + 1) * kSliceK < g.o.K ? (z + 1) * kSliceK : g.o.K;
-            slice_rows<MT, GS>(g, tile, z * kSliceK, k1, xr, P);
-            #pragma unroll
-            for (int t = 0; t < MT; t++) total[t] = z == 0 ? P[t] : total[t] + P[t];
-        }
-        #pragma unroll
-        for (int t = 0; t < MT; t++)
-            store4<EP>(g.o, m0 + 16 * t + (lane & 15), 16 * tile + 4 * (lane >> 4), total[t]);
+        tile_groups<GS>(g, unpack, tile, 0, groups, xr, [&](int i, kr_float4 c) { add_group(scales(i), c, y); });
+        store4<EP>(g.o, m, n, y);
     }
 }
 
-template <int MT, int GS, int EP>
+template <int GS, int EP>
 int launch_rows(const W4Args& g, hipStream_t s) {
-    const int tiles = g.n16 / 16, slices = (g.o.K + kSliceK - 1) / kSliceK;
-    const int mt = (g.o.M + 16 * MT - 1) / (16 * MT);
-    const size_t lds = (size_t)slices * MT * 64 * sizeof(kr_float4);
-    if (slices > 1 && (long long)tiles * mt < 1024 && lds <= 65536) {
-        const int waves = slices < kMaxSplit ? slices : kMaxSplit;
-        w4_rows_kernel<MT, GS, EP, true><<<dim3(tiles, mt), 64 * waves, lds, s>>>(g);
+    const int tiles = g.n16 / 16, blocks = (g.o.K + kBlockK - 1) / kBlockK;
+    // 1024 tiles are a wave for each SIMD without a split
+    if (blocks > 1 && tiles < 1024) {
+        const int waves = blocks < kMaxSplit ? blocks : kMaxSplit;
+        const int groups = (g.o.K + 32 * GS - 1) / (32 * GS);
+        const int a_group = 64 * g.o.M + 32;                       // bytes of LDS
+        const int turns = (groups * a_group + 65535) / 65536;
+        const int room = (blocks + turns - 1) / turns * (4 / GS);
+        w4_rows_kernel<GS, EP, true><<<tiles, 64 * waves, (size_t)room * a_group, s>>>(g, room);
     } else {
-        w4_rows_kernel<MT, GS, EP, false><<<dim3((tiles + 3) / 4, mt), 256, 0, s>>>(g);
+        w4_rows_kernel<GS, EP, false><<<(tiles + 3) / 4, 256, 0, s>>>(g, 0);
     }
     KR_LAUNCHED();
     return KR_OK;
 }
 
+// More rows, any K: a workgroup has 64 outputs, 16 for each of its 4 waves, against
+// 32 rows. x goes through LDS in blocks of 128 inputs (two buffers, one barrier a
+// block); the weights go straight to their wave's registers, and are unpacked
+// once for the 32 rows. Both are asked for kTileAhead blocks ahead.
+// Bound: latency, where the kernels below have too few units of work.
+// us by blocks ahead, 1 / 3: 64 x 768 x 768, groups of 32 6.2 / 5.5, 64 5.4 / 4.8,
+// 128 5.8 / 5.7; 64 x 2048 x 8192 14.0 / 11.6, 11.9 / 10.0, 13.1 / 14.8. Tiles of
+// 64 x 64 and 128 x 64 are slower on both (8.0 / 7.5 and 11.1 at groups of 32).
+template <int GS, int EP>
+__global__ void __launch_bounds__(256, 2) w4_tile_kernel(W4Args g) {
+    constexpr int MT = 2, ROWS = 16 * MT;
+    constexpr int kTileAhead = GS == 4 ? 1 : 3;
+    constexpr int GPB = 4 / GS;                             // groups per block
+    __shared__ kr_half8 xs[2][ROWS * 16];                   // unit c of row m at 16 m + (c ^ m % 16)
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l16 = lane & 15, q4 = lane >> 4;
+    const int tiles = g.n16 / 16, tile = blockIdx.x * 4 + wave;
+    const int t_read = tile < tiles ? tile : tiles - 1;               // past N: the last tile, not stored
+    const int m0 = blockIdx.y * ROWS;
+    const int kb_all = (g.o.K + kBlockK - 1) / kBlockK, groups = (g.o.K + 32 * GS - 1) / (32 * GS);
+    const Unpacker unpack;
+    const kr_int4* qp = g.q + (size_t)t_read * kb_all * 64 + lane;
+    const kr_half* sp = g.scales + 16 * t_read + 4 * q4;
+    const kr_half* xp[MT];
+    #pragma unroll
+    for (int i = 0; i < MT; i++) {
+        const int m = m0 + 16 * i + tid / 16;                         // past M: the last row, not stored
+        xp[i] = g.x + (size_t)(m < g.o.M ? m : g.o.M - 1) * g.ldx;
+    }
+    kr_half8 xv[kTileAhead][MT];
+    kr_int4 w[kTileAhead];
+    kr_half4 sc[kTileAhead][GPB];
+    auto fetch = [&](int kb, kr_half8 (&xn)[MT], kr_int4& wn, kr_half4 (&sn)[GPB]) {
+        if (kb >= kb_all) return;
+        // inputs past K are zeros, and so the products with them, whatever scale is read
+        const int k = kb * kBlockK + 8 * (tid & 15);
+        #pragma unroll
+        for (int i = 0; i < MT; i++) {
+            xn[i] = kr_half8{0, 0, 0, 0, 0, 0, 0, 0};
+            if (k < g.o.K) xn[i] = *reinterpret_cast<const kr_half8*>(xp[i] + k);
+        }
+        wn = qp[(size_t)kb * 64];
+        #pragma unroll
+        for (int j = 0; j < GPB; j++) {
+            const int gi = kb * GPB + j < groups ? kb * GPB + j : groups - 1;
+            sn[j] = *reinterpret_cast<const kr_half4*>(sp + (size_t)gi * g.n16);
+        }
+    };
+    kr_float4 y[MT];
+    #pragma unroll
+    for (int t = 0; t < MT; t++) y[t] = kr_float4{0, 0, 0, 0};
+    #pragma unroll
+    for (int a = 0; a < kTileAhead; a++) fetch(a, xv[a], w[a], sc[a]);
+    for (int kb = 0; kb < kb_all; kb++) {
+        kr_half8* xb = xs[kb & 1];
+        #pragma unroll
+        for (int i = 0; i < MT; i++) xb[(16 * i + tid / 16) * 16 + ((tid & 15) ^ (tid / 16))] = xv[0][i];
+        const kr_int4 wc = w[0];
+        kr_half4 sg[GPB];
+        #pragma unroll
+        for (int j = 0; j < GPB; j++) sg[j] = sc[0][j];
+        #pragma unroll
+        for (int a = 1; a < kTileAhead; a++) {
+            #pragma unroll
+            for (int i = 0; i < MT; i++) xv[a - 1][i] = xv[a][i];
+            w[a - 1] = w[a];
+            #pragma unroll
+            for (int j = 0; j < GPB; j++) sc[a - 1][j] = sc[a][j];
+        }
+        fetch(kb + kTileAhead, xv[kTileAhead - 1], w[kTileAhead - 1], sc[kTileAhead - 1]);
+        __syncthreads();      // and with it, every wave is done with the buffer of kb - 1
+        kr_float4 c[MT];
+        #pragma unroll
+        for (int s = 0; s < 4; s++) {
+            const kr_half8 a = unpack((uint32_t)wc[s]);
+            #pragma unroll
+            for (int t = 0; t < MT; t++) {
+                if (s % GS == 0) c[t] = kr_float4{0, 0, 0, 0};
+                c[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                    a, xb[(16 * t + l16) * 16 + ((4 * s + q4) ^ l16)], c[t], 0, 0, 0);
+            }
+            if ((s + 1) % GS == 0) {
+                #pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const float f = (float)sg[s / GS][r];
+                    #pragma unroll
+                    for (int t = 0; t < MT; t++) y[t][r] = __builtin_fmaf(f, c[t][r], y[t][r]);
+                }
+            }
+        }
+    }
+    if (tile < tiles) {
+        #pragma unroll
+        for (int t = 0; t < MT; t++) store4<EP>(g.o, m0 + 16 * t + l16, 16 * tile + 4 * q4, y[t]);
+    }
+}
+
+template <int GS, int EP>
+int launch_tile(const W4Args& g, hipStream_t s) {
+    // outputs in steps of 8 workgroups: those of an XCD (every eighth) keep
+    // their weights in its L2 from one row tile to the next
+    const int groups = (g.n16 / 16 + 3) / 4;
+    const int gx = groups >= 8 ? (groups + 7) / 8 * 8 : groups;
+    w4_tile_kernel<GS, EP><<<dim3(gx, (g.o.M + 31) / 32), 256, 0, s>>>(g);
+    KR_LAUNCHED();
+    return KR_OK;
+}
+
+// Rows held: a workgroup has all of K of 16 MT rows in LDS, zeros past K, and its
+// waves take units of 16 NT outputs one after another, each on its own: no barrier
+// after the rows are in. Weights come kAhead blocks ahead into registers.
+constexpr int kHeldUnits = 163840 / 16;      // all of a CU's LDS: one workgroup each
+
+template <int NT, int MT, int GS, int EP, int kAhead, int kHeldWaves>
+__global__ void __launch_bounds__(64 * kHeldWaves, kHeldWaves / 4) w4_held_kernel(W4Args g, int ranges) {
+    constexpr int GPB = 4 / GS;
+    __shared__ kr_half8 xs[kHeldUnits];      // unit c of row m of block b at 16 (16 MT b + m) + (c ^ m % 16)
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l16 = lane & 15, q4 = lane >> 4;
+    // workgroups of one range of outputs are 8 apart: on one XCD, whose L2 then
+    // has the weights for all of them
+    const int row_tiles = (g.o.M + 16 * MT - 1) / (16 * MT);
+    const int range = blockIdx.x % 8 + blockIdx.x / 8 / row_tiles * 8, m0 = blockIdx.x / 8 % row_tiles * 16 * MT;
+    const int kb_all = (g.o.K + kBlockK - 1) / kBlockK, groups = (g.o.K + 32 * GS - 1) / (32 * GS);
+    const int tiles = g.n16 / 16, units = (tiles + NT - 1) / NT;
+    for (int i = tid; i < 16 * MT * kb_all * 16; i += 64 * kHeldWaves) {
+        const int m = i / (kb_all * 16), c = i - m * (kb_all * 16);   // neighbours along a row
+        kr_half8 v = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (m0 + m < g.o.M && 8 * c < g.o.K)
+            v = *reinterpret_cast<const kr_half8*>(g.x + (size_t)(m0 + m) * g.ldx + 8 * c);
+        xs[16 * (c / 16 * 16 * MT + m) + ((c ^ m) & 15)] = v;
+    }
+    __syncthreads();
+    const Unpacker unpack;
+    const kr_half8* xl[4];
+    #pragma unroll
+    for (int s = 0; s < 4; s++) xl[s] = xs + l16 * 16 + ((4 * s + q4) ^ l16);
+    const int step = ranges * kHeldWaves;
+    int unit = range + ranges * wave;
+    if (range >= ranges || unit >= units) return;
+
+    // blocks in flight: next_unit, next_kb is the first not yet asked for
+    kr_int4 w[kAhead][NT];
+    kr_half4 sc[kAhead][NT][GPB];
+    int next_unit = unit, next_kb = 0;
+    const kr_int4* qp[NT];
+    const kr_half* sp[NT];
+    auto point = [&]() {
+        #pragma unroll
+        for (int i = 0; i < NT; i++) {
+            const int tile = next_unit * NT + i < tiles ? next_unit * NT + i : tiles - 1;
+            qp[i] = g.q + (size_t)tile * kb_all * 64 + lane;
+            sp[i] = g.scales + 16 * tile + 4 * q4;
+        }
+    };
+    auto fetch = [&](kr_int4 (&wn)[NT], kr_half4 (&sn)[NT][GPB]) {
+        if (next_unit >= units) return;
+        #pragma unroll
+        for (int i = 0; i < NT; i++) {
+            wn[i] = qp[i][next_kb * 64];
+            #pragma unroll
+            for (int j = 0; j < GPB; j++) {
+                const int gi = next_kb * GPB + j < groups ? next_kb * GPB + j : groups - 1;   // the products are 0
+                sn[i][j] = *reinterpret_cast<const kr_half4*>(sp[i] + (size_t)gi * g.n16);
+            }
+        }
+        if (++next_kb == kb_all) {
+            next_kb = 0;
+            next_unit += step;
+            point();
+        }
+    };
+    point();
+    #pragma unroll
+    for (int a = 0; a < kAhead; a++) fetch(w[a], sc[a]);
+    for (; unit < units; unit += step) {
+        kr_float4 y[NT][MT];
+        #pragma unroll
+        for (int i = 0; i < NT; i++)
+            #pragma unroll
+            for (int t = 0; t < MT; t++) y[i][t] = kr_float4{0, 0, 0, 0};
+        for (int kb = 0; kb < kb_all; kb++) {
+            kr_int4 wc[NT];
+            kr_half4 sg[NT][GPB];
+            #pragma unroll
+            for (int i = 0; i < NT; i++) {
+                wc[i] = w[0][i];
+                #pragma unroll
+                for (int j = 0; j < GPB; j++) sg[i][j] = sc[0][i][j];
+                #pragma unroll
+                for (int a = 1; a < kAhead; a++) {
+                    w[a - 1][i] = w[a][i];
+                    #pragma unroll
+                    for (int j = 0; j < GPB; j++) sc[a - 1][i][j] = sc[a][i][j];
+                }
+            }
+            fetch(w[kAhead - 1], sc[kAhead - 1]);
+            kr_float4 c[NT][MT];
+            #pragma unroll
+            for (int s = 0; s < 4; s++) {
+                kr_half8 x[MT];
+                #pragma unroll
+                for (int t = 0; t < MT; t++) x[t] = xl[s][256 * (MT * kb + t)];
+                #pragma unroll
+                for (int i = 0; i < NT; i++) {
+                    const kr_half8 a = unpack((uint32_t)wc[i][s]);
+                    #pragma unroll
+                    for (int t = 0; t < MT; t++) {
+                        if (s % GS == 0) c[i][t] = kr_float4{0, 0, 0, 0};
+                        c[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, x[t], c[i][t], 0, 0, 0);
+                    }
+                }
+                if ((s + 1) % GS == 0) {
+                    #pragma unroll
+                    for (int i = 0; i < NT; i++)
+                        #pragma unroll
+                        for (int r = 0; r < 4; r++) {
+                            const float f = (float)sg[i][s / GS][r];
+                            #pragma unroll
+                            for (int t = 0; t < MT; t++) y[i][t][r] = __builtin_fmaf(f, c[i][t][r], y[i][t][r]);
+                        }
+                }
+            }
+        }
+        #pragma unroll
+        for (int t = 0; t < MT; t++)
+            #pragma unroll
+            for (int i = 0; i < NT; i++)
+                if (unit * NT + i < tiles)
+                    store4<EP>(g.o, m0 + 16 * t + l16, 16 * (unit * NT + i) + 4 * q4, y[i][t]);
+    }
+}
+
+// Whether 16 MT rows of this K fit, and give every wave of 256 workgroups a unit.
+bool held_fits(const W4Args& g, int MT) {
+    return (long long)(g.o.K + kBlockK - 1) / kBlockK * 16 * 16 * MT <= kHeldUnits;
+}
+bool held_fills(const W4Args& g, int NT, int MT, int waves) {
+    return held_fits(g, MT) && (long long)((g.n16 / 16 + NT - 1) / NT) * ((g.o.M + 16 * MT - 1) / (16 * MT)) >=
+                                   256 * waves;
+}
+
+template <int NT, int MT, int GS, int EP, int kAhead, int kHeldWaves>
+int launch_held(const W4Args& g, hipStream_t s) {
+    const int row_tiles = (g.o.M + 16 * MT - 1) / (16 * MT);
+    const int units = (g.n16 / 16 + NT - 1) / NT;
+    const int most = (units + kHeldWaves - 1) / kHeldWaves;
+    int ranges = (256 + row_tiles - 1) / row_tiles;
+    if (ranges > most) ranges = most;
+    w4_held_kernel<NT, MT, GS, EP, kAhead, kHeldWaves>
+        <<<(ranges + 7) / 8 * 8 * row_tiles, 64 * kHeldWaves, 0, s>>>(g, ranges);
+    KR_LAUNCHED();
+    return KR_OK;
+}
+
+// Kernel by the work there is, us on MI355X at groups of 32 / 64 / 128:
+//   up to 16 rows, fewer than 1536 tiles of 16 outputs: rows, else held (16 x 16).
+//     1 x 768 x 16384 rows 4.9 / 5.1 / 4.5, held 8.0 / 6.5 / 5.9; 1 x 768 x 32768
+//     9.5 / 10.2 / 8.8 and 8.2 / 6.9 / 6.3; 16 x 768 x 50277 16.5 / 16.7 / 15.6 and
+//     10.0 / 8.8 / 8.4.
+//   more rows: held with 64 rows, else with 32, where that gives each of the 12
+//     waves of 256 workgroups a unit of 32 outputs; else tiles. 512 x 768 x 16384
+//     (4096 units) 24.3 / 20.0 / 17.5, tiles 36 / 30 / 28; 512 x 768 x 8192 (2048
+//     units of 64 rows, 4096 of 32) held 64 18.7 / 16.2 / 14.4, held 32 15.3 / 12.5
+//     / 11.3, tiles 20 / 17 / 16; 128 x 768 x 16384 (2048 of 32) held 32 12.3 / 10.2
+//     / 9.3, tiles 11.1 / 9.3 / 9.2.
 template <int GS, int EP>
 int launch_by_rows(const W4Args& g, hipStream_t s) {
-    if (g.o.M <= 16) return launch_rows<1, GS, EP>(g, s);
-    if (g.o.M <= 32) return launch_rows<2, GS, EP>(g, s);
-    return launch_rows<4, GS, EP>(g, s);
+    if (g.o.M <= 16) {
+        if (g.n16 / 16 >= 1536 && held_fits(g, 1)) return launch_held<1, 1, GS, EP, 3, 16>(g, s);
+        return launch_rows<GS, EP>(g, s);
+    }
+    if (held_fills(g, 2, 4, 12)) return launch_held<2, 4, GS, EP, 1, 12>(g, s);
+    if (held_fills(g, 2, 2, 12)) return launch_held<2, 2, GS, EP, 1, 12>(g, s);
+    return launch_tile<GS, EP>(g, s);
 }
 
 template <int EP>
