@@ -121,7 +121,7 @@ int kr_softmax_probs(const uint16_t* logits, int N, int V, long long ld, float* 
  *                   row without a token), NaN for any other id outside 0..V-1;
  *   entropy[row]  = -sum p ln p;
  *   top_logprob, top_token [N, n_top]: the n_top most likely tokens, largest
- *                   first, equal ones by lower id (n_top <= 64 and <= V; 0:
+ *                   first, equal ones by lower id (n_top <= 32 and <= V; 0:
  *                   none, both pointers may be NULL).
  * A logit of -inf is a masked token: probability 0, never among the top ones
  * (missing ones are -1 with -inf). A row of only masked tokens has logprob

@@ -4,45 +4,43 @@
 //   m = max x;  s = sum e^(x - m);  t = sum e^(x - m) (x - m)
 //   ln p(i) = (x_i - m) - ln s;     H = ln s - t / s
 //
-// A row is held in registers (fp16 as it comes, two to a register), so the
-// maximum is known before the sums start and memory is read once; rows longer
-// than 64 elements a thread of 1024 (32 in fp32) are taken in segments, whose
-// (m, s, t) are joined. Sums are fp32, in an order given by the element's index
+// One pass over memory: a thread keeps a running maximum and the two sums relative
+// to it, rescaled where a block of its chunks has a larger one; the threads' are
+// joined at the row's end. Sums are fp32, in an order given by the element's index
 // alone, so a row's results do not depend on N or on where the row lies.
-// Exponentials are 2^(x log2 e - m log2 e): one fused multiply-add and the
-// hardware's exp2, the rounding of m log2 e taken back in the sums.
+// Exponentials are 2^(x log2 e - m log2 e): for fp16 one fused multiply-add and the
+// hardware's exp2, sums being relative to the rounded m log2 e.
 //
-// Top tokens: T, the n_top-th largest of 64 disjoint groups' maxima, has at
-// least n_top elements >= T and few more where the logits are spread over the
-// groups (group = lane: 8 neighbouring tokens, then every 512th). Those go
-// to a list in LDS, and each of them counts how many are before it (larger, or
-// equal with a lower index): that is its rank. A row with more candidates than
-// the list holds (long ties) takes its n_top largest one by one instead.
+// Top tokens: T, the n_top-th largest of 16 (n_top <= 8) or 64 disjoint groups'
+// maxima, has at least n_top elements >= T and few more where the logits are
+// spread over the groups (64: lanes, so 8 neighbouring tokens, then every 512th).
+// Threads with a maximum >= T, few, are listed and their chunks read again (from
+// the L2; a row of one wave has them in registers), and each element >= T counts how many are before it (larger, or
+// equal with a lower index): that is its rank. A row with more of them than there
+// is room for (long ties) takes its n_top largest one by one instead.
 #include "kr_common.h"
 #include "kr_wave.h"
 #include "krunch_hip.h"
+
+#include <type_traits>
 
 namespace {
 
 constexpr float kLog2e = 0x1.715476p+0f;
 constexpr float kLn2 = 0x1.62e43p-1f;
-constexpr int kMaxTop = 64;
-constexpr int kListRoom = 512;      // candidates held beside the running top tokens
-
-typedef kr_half8 kr_half8_any __attribute__((aligned(2)));     // rows start at any element
-typedef kr_float4 kr_float4_any __attribute__((aligned(4)));
+constexpr int kMaxTop = 32;
 
 template <typename T> struct Chunk;
 template <> struct Chunk<kr_half> {
     static constexpr int n = 8;
     typedef kr_half8 vec;
-    typedef kr_half8_any any;
 };
 template <> struct Chunk<float> {
     static constexpr int n = 4;
     typedef kr_float4 vec;
-    typedef kr_float4_any any;
 };
+
+typedef kr_int4 int4_any __attribute__((aligned(4)));
 
 struct ScoreArgs {
     const void* logits;
@@ -83,31 +81,88 @@ __device__ __forceinline__ float sort_step(float v, int lane) {
     const bool larger = ((lane & O) == 0) == (SIZE == 64 || (lane & SIZE) == 0);
     return larger ? fmaxf(v, w) : fminf(v, w);
 }
-// The 64 lanes' values in descending order.
-__device__ __forceinline__ float wave_sort_down(float v, int lane) {
+// The k-th largest of the 64 lanes' values, or with k <= 8 of the maxima of the 16
+// groups of lanes l, l + 16, l + 32, l + 48: less spread over the row, but half
+// the steps, and without exchanges between the wave's quarters.
+__device__ __forceinline__ float kth_largest(float v, int lane, int k) {
+    if (k <= 8) {
+        v = fmaxf(v, kr_xor<16>(v));
+        v = fmaxf(v, kr_xor<32>(v));
+    }
     v = sort_step<2, 1>(v, lane);
     v = sort_step<4, 2>(v, lane); v = sort_step<4, 1>(v, lane);
     v = sort_step<8, 4>(v, lane); v = sort_step<8, 2>(v, lane); v = sort_step<8, 1>(v, lane);
     v = sort_step<16, 8>(v, lane); v = sort_step<16, 4>(v, lane); v = sort_step<16, 2>(v, lane);
     v = sort_step<16, 1>(v, lane);
-    v = sort_step<32, 16>(v, lane); v = sort_step<32, 8>(v, lane); v = sort_step<32, 4>(v, lane);
-    v = sort_step<32, 2>(v, lane); v = sort_step<32, 1>(v, lane);
-    v = sort_step<64, 32>(v, lane); v = sort_step<64, 16>(v, lane); v = sort_step<64, 8>(v, lane);
-    v = sort_step<64, 4>(v, lane); v = sort_step<64, 2>(v, lane); v = sort_step<64, 1>(v, lane);
-    return v;
+    if (k > 8) {
+        v = sort_step<32, 16>(v, lane); v = sort_step<32, 8>(v, lane); v = sort_step<32, 4>(v, lane);
+        v = sort_step<32, 2>(v, lane); v = sort_step<32, 1>(v, lane);
+        v = sort_step<64, 32>(v, lane); v = sort_step<64, 16>(v, lane); v = sort_step<64, 8>(v, lane);
+        v = sort_step<64, 4>(v, lane); v = sort_step<64, 2>(v, lane); v = sort_step<64, 1>(v, lane);
+    }
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), k - 1));
 }
 
 // What the threads of one row share. W waves work on a row.
 template <int W, bool TOP>
 struct RowShared {
+    static constexpr int kThreads = TOP ? 96 : 1;        // with candidates
+    static constexpr int kList = TOP ? 384 : 1;          // candidates
     float lane_max[W > 1 ? W : 1][64];
     float sum[W], tsum[W];
     float threshold;
-    int count;
-    uint64_t list[TOP ? kListRoom + kMaxTop : 1];
+    int threads, count;
+    int thread[kThreads];
+    uint64_t list[kList];
     uint64_t top[TOP ? kMaxTop : 1];
     uint64_t best[W];
 };
+
+// Element words of a row shorter than a chunk, and -inf past it.
+template <typename T>
+__device__ __forceinline__ kr_int4 read_short(const T* x, int i, int n) {
+    kr_int4 v;
+    #pragma unroll
+    for (int j = 0; j < 4; j++) {
+        if constexpr (sizeof(T) == 4) {
+            v[j] = i + j < n ? __float_as_int((float)x[i + j]) : (int)0xFF800000;
+        } else {
+            const uint16_t* h = reinterpret_cast<const uint16_t*>(x);
+            const uint32_t lo = i + 2 * j < n ? h[i + 2 * j] : 0xFC00u;
+            const uint32_t hi = i + 2 * j + 1 < n ? h[i + 2 * j + 1] : 0xFC00u;
+            v[j] = (int)(lo | hi << 16);
+        }
+    }
+    return v;
+}
+template <typename T>
+__device__ __forceinline__ float chunk_max(kr_int4 raw) {
+    const typename Chunk<T>::vec v = __builtin_bit_cast(typename Chunk<T>::vec, raw);
+    if constexpr (sizeof(T) == 2) {
+        typedef kr_half half2v __attribute__((ext_vector_type(2)));
+        const kr_half4 h = __builtin_elementwise_max(__builtin_shufflevector(v, v, 0, 1, 2, 3),
+                                                     __builtin_shufflevector(v, v, 4, 5, 6, 7));
+        const half2v p = __builtin_elementwise_max(__builtin_shufflevector(h, h, 0, 1),
+                                                   __builtin_shufflevector(h, h, 2, 3));
+        return (float)__builtin_elementwise_max(p[0], p[1]);
+    } else {
+        return fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
+    }
+}
+// The first d elements of a chunk become -inf.
+template <typename T>
+__device__ __forceinline__ kr_int4 without_first(kr_int4 v, int d) {
+    #pragma unroll
+    for (int j = 0; j < 4; j++) {
+        if constexpr (sizeof(T) == 4) {
+            if (j < d) v[j] = (int)0xFF800000;
+        } else {
+            const uint32_t w = (uint32_t)v[j];
+            v[j] = (int)(2 * j + 1 < d ? 0xFC00FC00u : 2 * j < d ? (w & 0xFFFF0000u) | 0xFC00u : w);
+        }
+    }
+    return v;
+}
 
 // A barrier of the row's threads: the workgroup's, or the wave's own order.
 template <int W>
@@ -119,212 +174,267 @@ __device__ __forceinline__ void row_sync() {
     }
 }
 
-// W waves per row, U chunks of 16 bytes per thread, 4 / W rows (at least one)
-// per workgroup.
+// W waves per row, U chunks of 16 bytes per thread at a time; four rows a workgroup
+// with W = 1, else one.
 template <typename T, int W, int U, bool TOP>
-__global__ void __launch_bounds__(W >= 4 ? 64 * W : 256, W == 16 ? (sizeof(T) == 2 ? 8 : 4) : 6)
+__global__ void __launch_bounds__(W > 1 ? 64 * W : 256, 8)
 scores_kernel(ScoreArgs g) {
-    constexpr int kRows = W >= 4 ? 1 : 4 / W;
-    constexpr int CH = Chunk<T>::n, TH = 64 * W, kSegment = TH * CH * U;
+    constexpr int kRows = W > 1 ? 1 : 4;
+    constexpr int CH = Chunk<T>::n, TH = 64 * W;
     typedef typename Chunk<T>::vec vec;
     __shared__ RowShared<W, TOP> shared_rows[kRows];
     const int lane = threadIdx.x & 63;
-    const int wave = W > 1 ? threadIdx.x / 64 % W : 0;
+    const int wave = W > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / 64 % W) : 0;
     const int tid = 64 * wave + lane;
     const int slot = kRows > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / TH) : 0;
     RowShared<W, TOP>& sh = shared_rows[slot];
     const long long row = (long long)blockIdx.x * kRows + slot;
     if (kRows > 1 && row >= g.N) return;    // a whole wave: rows of W = 1 share nothing
-    const T* x0 = reinterpret_cast<const T*>(g.logits) + row * g.ld;
+    const int V = g.V;
+    const T* x = reinterpret_cast<const T*>(g.logits) + row * g.ld;
     const int token = g.tokens[row];
-    const bool named = token >= 0 && token < g.V;
-    const float x_token = named ? (float)x0[token] : 0.0f;
+    const bool named = token >= 0 && token < V;
+    const float x_token = named ? (float)x[token] : 0.0f;
 
-    float M = -INFINITY, S = 0.0f, Q = 0.0f;   // running maximum, sums of e and e * (x - M) log2 e
-    int kept = 0;                               // entries of sh.top
-    for (int base = 0; base < g.V; base += kSegment) {
-        const T* xs = x0 + base;
-        const int n = g.V - base < kSegment ? g.V - base : kSegment;
-        vec x[U];
+    // Chunk c of the row starts at element c * CH; one that ends past the row is
+    // read from the row's last 16 bytes, without what belongs to the one before.
+    auto chunk_start = [&](int c) { return min(c * CH, V - CH); };
+    const int chunks = (V + CH - 1) / CH;
+    // U chunks of the thread from chunk c0 + lane on, TH apart. fp16 rows that start
+    // in the middle of a 4-byte word are read by the words around: reads of 16 bytes
+    // run at full speed from any 4-byte boundary, and 26% slower over rows of which
+    // half have none (8192 x 50277 held in registers: 165 us, 209).
+    auto read_block = [&](int c0, kr_int4 (&raw)[U], auto odd_row) {
+        constexpr bool ODD = decltype(odd_row)::value;
+        int next[U];
         #pragma unroll
         for (int u = 0; u < U; u++) {
-            const int i = (u * TH + tid) * CH;
+            const int* words =
+                reinterpret_cast<const int*>(x + chunk_start(c0 + u * TH + lane) - (ODD ? 1 : 0));
+            raw[u] = *reinterpret_cast<const int4_any*>(words);
+            if (ODD) next[u] = words[4];
+        }
+        if (ODD) {
             #pragma unroll
-            for (int e = 0; e < CH; e++) x[u][e] = (T)-INFINITY;
-            if (i + CH <= n) {
-                x[u] = *reinterpret_cast<const typename Chunk<T>::any*>(xs + i);
-            } else if (i < n) {
+            for (int u = 0; u < U; u++)
                 #pragma unroll
-                for (int e = 0; e < CH; e++)
-                    if (i + e < n) x[u][e] = xs[i + e];
-            }
+                for (int j = 0; j < 4; j++)
+                    raw[u][j] = (int)__builtin_amdgcn_alignbit(
+                        (uint32_t)(j < 3 ? raw[u][j + 1] : next[u]), (uint32_t)raw[u][j], 16);
         }
-        T chunk_max[U];
-        float mine = -INFINITY;
-        #pragma unroll
-        for (int u = 0; u < U; u++) {
-            vec v = x[u];
-            if constexpr (CH == 8) {
-                kr_half4 h = __builtin_elementwise_max(
-                    __builtin_shufflevector(v, v, 0, 1, 2, 3), __builtin_shufflevector(v, v, 4, 5, 6, 7));
-                typedef kr_half half2v __attribute__((ext_vector_type(2)));
-                half2v p = __builtin_elementwise_max(__builtin_shufflevector(h, h, 0, 1),
-                                                     __builtin_shufflevector(h, h, 2, 3));
-                chunk_max[u] = __builtin_elementwise_max(p[0], p[1]);
-            } else {
-                chunk_max[u] = (T)fmaxf(fmaxf((float)v[0], (float)v[1]), fmaxf((float)v[2], (float)v[3]));
-            }
-            mine = fmaxf(mine, (float)chunk_max[u]);
-        }
-        // maximum per lane over the row's waves (the groups of T), then of all
-        float group = mine;
-        if constexpr (W > 1) {
-            sh.lane_max[wave][lane] = mine;
-            row_sync<W>();
+        if ((c0 + (U - 1) * TH + 64) * CH > V) {
             #pragma unroll
-            for (int w = 0; w < W; w++) group = fmaxf(group, sh.lane_max[w][lane]);
-        }
-        float m = kr_wave_reduce(group, [](float a, float b) { return fmaxf(a, b); });
-        if (TOP && wave == 0) {
-            const float sorted = wave_sort_down(group, lane);
-            const float th = __int_as_float(
-                __builtin_amdgcn_readlane(__float_as_int(sorted), g.n_top - 1));
-            if (lane == 0) {
-                sh.threshold = th;
-                sh.count = 0;
+            for (int u = 0; u < U; u++) {
+                const int c = c0 + u * TH + lane;
+                raw[u] = without_first<T>(raw[u], c * CH - chunk_start(c));
             }
         }
-        if (m == -INFINITY) m = 0.0f;           // nothing above -inf: every e is 0 (or NaN)
-        float s = 0.0f, q = 0.0f;
-        const float ml = m * kLog2e;
+    };
+    const std::integral_constant<bool, true> odd;
+    const std::integral_constant<bool, false> even;
+    const bool is_odd = sizeof(T) == 2 && ((uintptr_t)x & 2);
+    // m: maximum; ref: what the sums s of e and q of e a are relative to, in log2
+    // (fp32: the maximum itself, whose log2 e multiple may overflow)
+    float m = -INFINITY, ref = 0.0f, s = 0.0f, q = 0.0f;
+    auto reference = [](float top) { return top == -INFINITY ? 0.0f : CH == 8 ? top * kLog2e : top; };
+    auto add = [&](const kr_int4 (&raw)[U]) {
         #pragma unroll
         for (int u = 0; u < U; u++) {
-            if ((u * TH + 64 * wave) * CH >= n) break;     // wave-uniform: nothing of the row here
+            const vec v = __builtin_bit_cast(vec, raw[u]);
             #pragma unroll
             for (int e = 0; e < CH; e++) {
                 float a;
-                if constexpr (CH == 8) a = __builtin_fmaf((float)x[u][e], kLog2e, -ml);
-                else a = ((float)x[u][e] - m) * kLog2e;
+                if constexpr (CH == 8) a = __builtin_fmaf((float)v[e], kLog2e, -ref);
+                else a = ((float)v[e] - ref) * kLog2e;
                 const float ex = __builtin_amdgcn_exp2f(a);
                 s += ex;
                 q = __builtin_fmaf(ex, fmaxf(a, -1000.0f), q);   // e^-inf * -inf = 0
             }
         }
-        s = kr_wave_reduce(s, [](float a, float b) { return a + b; });
-        q = kr_wave_reduce(q, [](float a, float b) { return a + b; });
-        if constexpr (W > 1) {
-            if (lane == 0) {
-                sh.sum[wave] = s;
-                sh.tsum[wave] = q;
-            }
-            row_sync<W>();
-            s = 0.0f;
-            q = 0.0f;
-            #pragma unroll
-            for (int w = 0; w < W; w++) {
-                s += sh.sum[w];
-                q += sh.tsum[w];
-            }
-        } else {
-            row_sync<W>();
-        }
-        if constexpr (CH == 8) {
-            // every e is 2^b too large, b the rounding of ml
-            const float b = __builtin_fmaf(m, kLog2e, -ml), f = __builtin_amdgcn_exp2f(-b);
-            q = f * __builtin_fmaf(-b, s, q);
+    };
+    // s and q relative to `to`, which is not below ref; with m = -inf, nothing is
+    // in them but, perhaps, NaN
+    auto rescale = [&](float to) {
+        if (m != -INFINITY) {
+            const float d = fmaxf(CH == 8 ? ref - to : (ref - to) * kLog2e, -1000.0f);
+            const float f = __builtin_amdgcn_exp2f(d);
+            q = f * __builtin_fmaf(d, s, q);
             s = f * s;
         }
-        if (base == 0) {
-            M = m;
-            S = s;
-            Q = q;
-        } else if (s != 0.0f) {                 // (NaN too)
-            // join: both sides relative to the larger maximum; an empty side adds nothing
-            if (S == 0.0f) {
-                M = m;
-                S = s;
-                Q = q;
-            } else {
-                const float top = fmaxf(M, m);
-                const float d0 = fmaxf((M - top) * kLog2e, -1000.0f);
-                const float d1 = fmaxf((m - top) * kLog2e, -1000.0f);
-                const float f0 = __builtin_amdgcn_exp2f(d0), f1 = __builtin_amdgcn_exp2f(d1);
-                Q = f0 * __builtin_fmaf(d0, S, Q) + f1 * __builtin_fmaf(d1, s, q);
-                S = f0 * S + f1 * s;
-                M = top;
-            }
-        }
-        if constexpr (TOP) {
-            // chunks with a candidate, few: read again, so that no element stays
-            // converted, with its key, from the sums on (146 spilled registers)
-            const float th = sh.threshold;
-            uint32_t hit = 0;
+        ref = to;
+    };
+    kr_int4 raw[U];
+    if constexpr (W == 1) {
+        // the whole row is one block of its wave
+        if (V < CH) {
             #pragma unroll
-            for (int u = 0; u < U; u++)
-                hit |= ((float)chunk_max[u] >= th && (float)chunk_max[u] > -INFINITY) ? 1u << u : 0u;
-            while (hit) {
-                const int i = ((__ffs(hit) - 1) * TH + tid) * CH;
-                hit &= hit - 1;
-                #pragma unroll 1
-                for (int e = 0; e < CH && i + e < n; e++) {
-                    const float xe = (float)xs[i + e];
-                    if (xe >= th && xe > -INFINITY) {
-                        const int at = atomicAdd(&sh.count, 1);
-                        if (at < kListRoom) sh.list[at] = order_key(xe, (uint32_t)(base + i + e));
+            for (int u = 0; u < U; u++) raw[u] = read_short(x, (u * TH + lane) * CH, V);
+        } else if (is_odd) {
+            read_block(0, raw, odd);
+        } else {
+            read_block(0, raw, even);
+        }
+        #pragma unroll
+        for (int u = 0; u < U; u++) m = fmaxf(m, chunk_max<T>(raw[u]));
+    } else {
+        auto walk = [&](auto odd_row) {
+            for (int c0 = 64 * wave; c0 < chunks; c0 += U * TH) {
+                read_block(c0, raw, odd_row);
+                float top = -INFINITY;
+                #pragma unroll
+                for (int u = 0; u < U; u++) top = fmaxf(top, chunk_max<T>(raw[u]));
+                if (__any(top > m)) {
+                    top = fmaxf(top, m);
+                    rescale(reference(top));
+                    m = top;
+                }
+                add(raw);
+            }
+        };
+        if (is_odd) walk(odd);
+        else walk(even);
+    }
+
+    // maximum per lane over the row's waves (the groups of T), then of all
+    float group = m;
+    if constexpr (W > 1) {
+        sh.lane_max[wave][lane] = m;
+        row_sync<W>();
+        #pragma unroll
+        for (int w = 0; w < W; w++) group = fmaxf(group, sh.lane_max[w][lane]);
+    }
+    const float M = kr_wave_reduce(group, [](float a, float b) { return fmaxf(a, b); });
+    if constexpr (W == 1) {
+        ref = reference(M);
+        add(raw);
+    } else {
+        rescale(reference(M));
+    }
+    s = kr_wave_reduce(s, [](float a, float b) { return a + b; });
+    q = kr_wave_reduce(q, [](float a, float b) { return a + b; });
+    if (TOP && wave == W - 1) {
+        const float th = kth_largest(group, lane, g.n_top);
+        if (lane == 0) {
+            sh.threshold = th;
+            sh.threads = 0;
+            sh.count = 0;
+        }
+    }
+    if constexpr (W > 1) {
+        if (lane == 0) {
+            sh.sum[wave] = s;
+            sh.tsum[wave] = q;
+        }
+    }
+    row_sync<W>();
+    int kept = 0;
+    if constexpr (TOP) {
+        const float th = sh.threshold;
+        int all = 0;
+        bool room = true;
+        if constexpr (W == 1) {
+            #pragma unroll
+            for (int u = 0; u < U; u++) {
+                if (!__any(chunk_max<T>(raw[u]) >= th)) continue;
+                const vec v = __builtin_bit_cast(vec, raw[u]);
+                const int start = V < CH ? lane * CH : chunk_start(u * TH + lane);
+                #pragma unroll
+                for (int e = 0; e < CH; e++) {
+                    const float xe = (float)v[e];
+                    const bool in = xe >= th && xe > -INFINITY;
+                    const uint64_t mask = __ballot(in);
+                    const int at = all + __popcll(mask & ((1ull << lane) - 1));
+                    if (in && at < sh.kList) sh.list[at] = order_key(xe, (uint32_t)(start + e));
+                    all += __popcll(mask);
+                }
+            }
+            row_sync<W>();
+            room = all <= sh.kList;
+        } else {
+            if (m >= th && m > -INFINITY) {
+                const int at = atomicAdd(&sh.threads, 1);
+                if (at < sh.kThreads) sh.thread[at] = tid;
+            }
+            row_sync<W>();
+            const int threads = sh.threads;
+            if (threads <= sh.kThreads) {
+                const int per = (chunks + TH - 1) / TH;       // chunks of a thread
+                for (int i = tid; i < threads * per; i += TH) {
+                    const int c = sh.thread[i / per] + i % per * TH;
+                    if (c >= chunks) continue;
+                    const int start = chunk_start(c);
+                    vec v;
+                    __builtin_memcpy(&v, x + start, 16);
+                    #pragma unroll
+                    for (int e = 0; e < CH; e++) {
+                        const float xe = (float)v[e];
+                        if (xe >= th && xe > -INFINITY && start + e >= c * CH) {
+                            const int at = atomicAdd(&sh.count, 1);
+                            if (at < sh.kList) sh.list[at] = order_key(xe, (uint32_t)(start + e));
+                        }
                     }
                 }
             }
             row_sync<W>();
-            const int found = sh.count;
-            if (found <= kListRoom) {
-                // rank among the candidates and the earlier segments' top tokens
-                if (tid < kept) sh.list[found + tid] = sh.top[tid];
-                row_sync<W>();
-                const int all = found + kept;
-                for (int c = tid; c < all; c += TH) {
-                    const uint64_t k = sh.list[c];
-                    int rank = 0;
-                    for (int j = 0; j < all; j++) rank += sh.list[j] > k;
-                    if (rank < g.n_top) sh.top[rank] = k;
+            all = sh.count;
+            room = threads <= sh.kThreads && all <= sh.kList;
+        }
+        if (room) {
+            if (wave > 0) return;
+            for (int c = lane; c < all; c += 64) {
+                const uint64_t k = sh.list[c];
+                int rank = 0;
+                #pragma unroll 4
+                for (int j = 0; j < all; j++) rank += sh.list[j] > k;
+                if (rank < g.n_top) sh.top[rank] = k;
+            }
+            kept = all < g.n_top ? all : g.n_top;
+            row_sync<1>();
+        } else {
+            // one after the other, each the largest below the one before
+            uint64_t last = ~0ull;
+            for (; kept < g.n_top; kept++) {
+                uint64_t k = 0;
+                #pragma unroll 1
+                for (int i = tid; i < V; i += TH) {
+                    const float v = (float)x[i];
+                    const uint64_t c = order_key(v, (uint32_t)i);
+                    if (v > -INFINITY && c < last && c > k) k = c;
                 }
-                kept = all < g.n_top ? all : g.n_top;
-            } else {
-                // one after the other, each the largest below the one before
-                if (tid < kept) sh.list[tid] = sh.top[tid];
-                row_sync<W>();
-                const int had = kept;
-                uint64_t last = ~0ull;
-                for (kept = 0; kept < g.n_top; kept++) {
-                    uint64_t k = 0;
-                    #pragma unroll 1
-                    for (int i = tid; i < n; i += TH) {
-                        const float xe = (float)xs[i];
-                        const uint64_t c = order_key(xe, (uint32_t)(base + i));
-                        if (xe > -INFINITY && c < last && c > k) k = c;
-                    }
-                    if (tid < had && sh.list[tid] < last && sh.list[tid] > k) k = sh.list[tid];
-                    k = wave_max_key(k);
-                    if constexpr (W > 1) {
-                        if (lane == 0) sh.best[wave] = k;
-                        row_sync<W>();
-                        for (int w = 0; w < W; w++) k = sh.best[w] > k ? sh.best[w] : k;
-                        row_sync<W>();
-                    }
-                    if (k == 0) break;          // the row has no more
-                    if (tid == 0) sh.top[kept] = k;
-                    last = k;
+                k = wave_max_key(k);
+                if constexpr (W > 1) {
+                    if (lane == 0) sh.best[wave] = k;
+                    row_sync<W>();
+                    for (int w = 0; w < W; w++) k = sh.best[w] > k ? sh.best[w] : k;
+                    row_sync<W>();
                 }
+                if (k == 0) break;          // the row has no more
+                if (tid == 0) sh.top[kept] = k;
+                last = k;
             }
             row_sync<W>();
         }
     }
+    if (wave > 0) return;
 
-    // S: 0 = nothing above -inf, NaN = a NaN or +inf in the row
-    const float ln_s = __logf(S);
-    if (tid == 0) {
-        float lp = (x_token - M) - ln_s;
-        float h = ln_s - kLn2 * (Q / S);
-        if (S == 0.0f) {
+    if constexpr (W > 1) {
+        s = 0.0f;
+        q = 0.0f;
+        #pragma unroll
+        for (int w = 0; w < W; w++) {
+            s += sh.sum[w];
+            q += sh.tsum[w];
+        }
+    }
+    // s: 0 = nothing above -inf, NaN = a NaN or +inf in the row. With M log2 e
+    // rounded by b, every e is 2^b too large
+    const float base = M == -INFINITY ? 0.0f : M;
+    const float b = CH == 8 ? __builtin_fmaf(base, kLog2e, -ref) : 0.0f;
+    const float ln_s = __logf(s) - b * kLn2;
+    if (lane == 0) {
+        float lp = (x_token - base) - ln_s;
+        float h = __logf(s) - kLn2 * (q / s);
+        if (s == 0.0f) {
             lp = -INFINITY;
             h = 0.0f;
         }
@@ -333,19 +443,18 @@ scores_kernel(ScoreArgs g) {
         g.logprob[row] = lp;
         g.entropy[row] = h;
     }
-    if (TOP && tid < g.n_top) {
-        const bool good = S == S, there = good && tid < kept;
-        const uint64_t k = there ? sh.top[tid] : 0;
-        const size_t o = (size_t)row * g.n_top + tid;
-        g.top_logprob[o] = there ? (key_value(k) - M) - ln_s : good ? -INFINITY : NAN;
+    if (TOP && lane < g.n_top) {
+        const bool good = s == s, there = good && lane < kept;
+        const uint64_t k = there ? sh.top[lane] : 0;
+        const size_t o = (size_t)row * g.n_top + lane;
+        g.top_logprob[o] = there ? (key_value(k) - base) - ln_s : good ? -INFINITY : NAN;
         g.top_token[o] = there ? (int32_t)key_index(k) : -1;
     }
 }
 
 template <typename T, int W, int U>
 void launch(const ScoreArgs& g, hipStream_t s) {
-    constexpr int rows = W >= 4 ? 1 : 4 / W;
-    const int threads = W >= 4 ? 64 * W : 256;
+    constexpr int rows = W > 1 ? 1 : 4, threads = W > 1 ? 64 * W : 256;
     const int grid = (g.N - 1) / rows + 1;
     if (g.n_top) scores_kernel<T, W, U, true><<<grid, threads, 0, s>>>(g);
     else scores_kernel<T, W, U, false><<<grid, threads, 0, s>>>(g);
@@ -356,8 +465,9 @@ void launch_by_width(const ScoreArgs& g, hipStream_t s) {
     constexpr int CH = Chunk<T>::n;
     if (g.V <= 64 * CH) launch<T, 1, 1>(g, s);
     else if (g.V <= 256 * CH) launch<T, 1, 4>(g, s);
-    else if (g.V <= 4 * 256 * CH) launch<T, 4, 4>(g, s);
-    else launch<T, 16, 8>(g, s);
+    else if (g.V <= 1024 * CH) launch<T, 2, 4>(g, s);
+    else if (g.V <= 4096 * CH) launch<T, 4, 4>(g, s);
+    else launch<T, 8, 4>(g, s);
 }
 
 }  // namespace

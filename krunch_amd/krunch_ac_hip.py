@@ -188,7 +188,7 @@ def _elsewhere(t):
     return t.get_device() != torch.cuda.current_device()
 
 
-TOP_TOKENS_MAX = 64
+TOP_TOKENS_MAX = 32
 
 
 def token_scores(logits, tokens, n_top: int = 0):
@@ -199,7 +199,7 @@ def token_scores(logits, tokens, n_top: int = 0):
     outside 0..V-1 give NaN. Logits of -inf are masked tokens: never among the
     top ones, whose missing places hold -1 and -inf. A row of only masked tokens
     has logprob -inf and entropy 0, one with a NaN or +inf is NaN. Equal logits
-    are ranked by lower id. n_top <= 64."""
+    are ranked by lower id. n_top <= 32."""
     logits.is_cuda or _refuse("logits must be a device tensor")
     f32 = logits.dtype is torch.float32
     f32 or logits.dtype is torch.float16 or _refuse(

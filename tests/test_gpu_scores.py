@@ -81,7 +81,7 @@ def test_widths(dtype, V):
     check(x, tok, min(V, 9))
 
 
-@pytest.mark.parametrize("k", [0, 1, 2, 20, 63, 64])
+@pytest.mark.parametrize("k", [0, 1, 2, 8, 9, 20, 31, 32])
 @pytest.mark.parametrize("V", [256, 1500, 5000, 50277, 70001])
 def test_top_counts(V, k):
     x, tok = rand(3, V, torch.float16, V + k)
@@ -104,7 +104,7 @@ def test_ties_clusters_and_long_candidate_lists(dtype, V):
     x[6, ::2] = -0.0
     x[7] = torch.clamp(x[7], max=1.0)
     check(x, tok, 17)
-    check(x, tok, 64)
+    check(x, tok, 32)
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
