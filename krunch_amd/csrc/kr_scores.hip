@@ -75,11 +75,21 @@ __device__ __forceinline__ uint64_t wave_max_key(uint64_t k) {
     return k;
 }
 
-template <int SIZE, int O>
+// One step of a bitonic sort. LAST: of the last merge, all descending.
+template <int SIZE, int O, bool LAST = SIZE == 64>
 __device__ __forceinline__ float sort_step(float v, int lane) {
     const float w = kr_xor<O>(v);
-    const bool larger = ((lane & O) == 0) == (SIZE == 64 || (lane & SIZE) == 0);
+    const bool larger = ((lane & O) == 0) == (LAST || (lane & SIZE) == 0);
     return larger ? fmaxf(v, w) : fminf(v, w);
+}
+template <bool LAST>
+__device__ __forceinline__ float sort_16(float v, int lane) {
+    v = sort_step<2, 1>(v, lane);
+    v = sort_step<4, 2>(v, lane); v = sort_step<4, 1>(v, lane);
+    v = sort_step<8, 4>(v, lane); v = sort_step<8, 2>(v, lane); v = sort_step<8, 1>(v, lane);
+    v = sort_step<16, 8, LAST>(v, lane); v = sort_step<16, 4, LAST>(v, lane);
+    v = sort_step<16, 2, LAST>(v, lane);
+    return sort_step<16, 1, LAST>(v, lane);
 }
 // The k-th largest of the 64 lanes' values, or with k <= 8 of the maxima of the 16
 // groups of lanes l, l + 16, l + 32, l + 48: less spread over the row, but half
@@ -89,11 +99,7 @@ __device__ __forceinline__ float kth_largest(float v, int lane, int k) {
         v = fmaxf(v, kr_xor<16>(v));
         v = fmaxf(v, kr_xor<32>(v));
     }
-    v = sort_step<2, 1>(v, lane);
-    v = sort_step<4, 2>(v, lane); v = sort_step<4, 1>(v, lane);
-    v = sort_step<8, 4>(v, lane); v = sort_step<8, 2>(v, lane); v = sort_step<8, 1>(v, lane);
-    v = sort_step<16, 8>(v, lane); v = sort_step<16, 4>(v, lane); v = sort_step<16, 2>(v, lane);
-    v = sort_step<16, 1>(v, lane);
+    v = sort_16<false>(v, lane);
     if (k > 8) {
         v = sort_step<32, 16>(v, lane); v = sort_step<32, 8>(v, lane); v = sort_step<32, 4>(v, lane);
         v = sort_step<32, 2>(v, lane); v = sort_step<32, 1>(v, lane);
@@ -452,6 +458,179 @@ scores_kernel(ScoreArgs g) {
     }
 }
 
+// Short rows: 16 lanes have a row, so a wave's reductions and sort serve four. U
+// chunks of 16 bytes per lane, in registers; n_top <= 8, T the n_top-th largest of
+// the 16 lanes' maxima. Rows of one wave may start at different halves of a word, so
+// fp16 is always read as five words and shifted by 0 or 16 bits.
+// Bound: issue (the wave's reductions, sort and lists); 16 rows a workgroup.
+constexpr int kShortChunks = 24, kShortList = 64;      // with candidates, and candidates, of a row
+
+template <typename T, int U, bool TOP>
+__global__ void __launch_bounds__(256, 8) scores_short_kernel(ScoreArgs g) {
+    constexpr int CH = Chunk<T>::n;
+    typedef typename Chunk<T>::vec vec;
+    __shared__ kr_int4 hit_chunk[TOP ? 16 : 1][kShortChunks];
+    __shared__ int hit_at[TOP ? 16 : 1][kShortChunks];
+    __shared__ int hits[16], found[16];
+    __shared__ uint64_t list[TOP ? 16 : 1][kShortList];
+    __shared__ uint64_t best[TOP ? 16 : 1][8];
+    const int lane = threadIdx.x & 63, l = lane & 15, slot = threadIdx.x >> 4;
+    const long long row = (long long)blockIdx.x * 16 + slot;
+    const bool there = row < g.N;
+    const long long r = there ? row : g.N - 1;      // past N: the last row, not written
+    const int V = g.V;
+    const T* x = reinterpret_cast<const T*>(g.logits) + r * g.ld;
+    const int token = g.tokens[r];
+    const bool named = token >= 0 && token < V;
+    const float x_token = named ? (float)x[token] : 0.0f;
+    if (TOP && l == 0) hits[slot] = found[slot] = 0;
+    auto chunk_start = [&](int u) { return V < CH ? l * CH : min((u * 16 + l) * CH, V - CH); };
+    kr_int4 raw[U];
+    float m = -INFINITY;
+    if (V < CH) {
+        #pragma unroll
+        for (int u = 0; u < U; u++) raw[u] = read_short(x, (u * 16 + l) * CH, V);
+    } else {
+        const int odd = sizeof(T) == 2 ? (int)((uintptr_t)x >> 1 & 1) : 0;
+        int next[U];
+        #pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int* words = reinterpret_cast<const int*>(x + chunk_start(u) - odd);
+            raw[u] = *reinterpret_cast<const int4_any*>(words);
+            if (sizeof(T) == 2) next[u] = words[3 + odd];
+        }
+        #pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (sizeof(T) == 2) {
+                #pragma unroll
+                for (int j = 0; j < 4; j++)
+                    raw[u][j] = (int)__builtin_amdgcn_alignbit(
+                        (uint32_t)(j < 3 ? raw[u][j + 1] : next[u]), (uint32_t)raw[u][j], 16 * odd);
+            }
+            if ((u + 1) * 16 * CH > V) raw[u] = without_first<T>(raw[u], (u * 16 + l) * CH - chunk_start(u));
+        }
+    }
+    #pragma unroll
+    for (int u = 0; u < U; u++) m = fmaxf(m, chunk_max<T>(raw[u]));
+    float M = m;
+    M = fmaxf(M, kr_xor<8>(M));
+    M = fmaxf(M, kr_xor<4>(M));
+    M = fmaxf(M, kr_xor<2>(M));
+    M = fmaxf(M, kr_xor<1>(M));
+    const float base = M == -INFINITY ? 0.0f : M;
+    const float ref = CH == 8 ? base * kLog2e : base;
+    float s = 0.0f, q = 0.0f;
+    #pragma unroll
+    for (int u = 0; u < U; u++) {
+        const vec v = __builtin_bit_cast(vec, raw[u]);
+        #pragma unroll
+        for (int e = 0; e < CH; e++) {
+            const float a = CH == 8 ? __builtin_fmaf((float)v[e], kLog2e, -ref) : ((float)v[e] - ref) * kLog2e;
+            const float ex = __builtin_amdgcn_exp2f(a);
+            s += ex;
+            q = __builtin_fmaf(ex, fmaxf(a, -1000.0f), q);
+        }
+    }
+    s += kr_xor<8>(s);
+    s += kr_xor<4>(s);
+    s += kr_xor<2>(s);
+    s += kr_xor<1>(s);
+    q += kr_xor<8>(q);
+    q += kr_xor<4>(q);
+    q += kr_xor<2>(q);
+    q += kr_xor<1>(q);
+    const float b = CH == 8 ? __builtin_fmaf(base, kLog2e, -ref) : 0.0f;
+    const float log_s = __logf(s), ln_s = log_s - b * kLn2;
+    if (there && l == 0) {
+        float lp = (x_token - base) - ln_s;
+        float h = log_s - kLn2 * (q / s);
+        if (s == 0.0f) {
+            lp = -INFINITY;
+            h = 0.0f;
+        }
+        if (token == -1) lp = 0.0f;
+        else if (!named) lp = NAN;
+        g.logprob[row] = lp;
+        g.entropy[row] = h;
+    }
+    if constexpr (TOP) {
+        const float th = __shfl(sort_16<true>(m, lane), (lane & 48) + g.n_top - 1);
+        row_sync<1>();
+        #pragma unroll
+        for (int u = 0; u < U; u++) {
+            const float c = chunk_max<T>(raw[u]);
+            if (c >= th && c > -INFINITY) {
+                const int at = atomicAdd(&hits[slot], 1);
+                if (at < kShortChunks) {
+                    hit_chunk[slot][at] = raw[u];
+                    hit_at[slot][at] = chunk_start(u);
+                }
+            }
+        }
+        row_sync<1>();
+        const int chunks = hits[slot];
+        int kept = 0;
+        if (chunks <= kShortChunks) {
+            for (int i = l; i < chunks * CH; i += 16) {
+                const float v = (float)reinterpret_cast<const T*>(hit_chunk[slot])[i];
+                if (v >= th && v > -INFINITY) {
+                    const int at = atomicAdd(&found[slot], 1);
+                    if (at < kShortList)
+                        list[slot][at] = order_key(v, (uint32_t)(hit_at[slot][i / CH] + i % CH));
+                }
+            }
+            if (l < 8) best[slot][l] = 0;
+        }
+        row_sync<1>();
+        const int all = found[slot];
+        if (chunks <= kShortChunks && all <= kShortList) {
+            for (int i = l; i < all; i += 16) {
+                const uint64_t k = list[slot][i];
+                int rank = 0;
+                #pragma unroll 4
+                for (int j = 0; j < all; j++) rank += list[slot][j] > k;
+                if (rank < g.n_top) best[slot][rank] = k;
+            }
+            row_sync<1>();
+            kept = g.n_top;
+        } else {
+            // one after the other, each the largest below the one before
+            uint64_t last = ~0ull;
+            for (; kept < g.n_top; kept++) {
+                uint64_t k = 0;
+                #pragma unroll 1
+                for (int i = l; i < V; i += 16) {
+                    const float v = (float)x[i];
+                    const uint64_t c = order_key(v, (uint32_t)i);
+                    if (v > -INFINITY && c < last && c > k) k = c;
+                }
+                #pragma unroll
+                for (int o = 8; o >= 1; o >>= 1) {
+                    const uint64_t other = __shfl_xor(k, o);
+                    k = other > k ? other : k;
+                }
+                if (l == 0) best[slot][kept] = k;     // 0: the row has no more
+                last = k;
+            }
+            row_sync<1>();
+        }
+        if (there && l < g.n_top) {
+            const bool good = s == s;
+            const uint64_t k = good ? best[slot][l] : 0;
+            const size_t o = (size_t)row * g.n_top + l;
+            g.top_logprob[o] = k ? (key_value(k) - base) - ln_s : good ? -INFINITY : NAN;
+            g.top_token[o] = k ? (int32_t)key_index(k) : -1;
+        }
+    }
+}
+
+template <typename T, int U>
+void launch_short(const ScoreArgs& g, hipStream_t s) {
+    const int grid = (g.N - 1) / 16 + 1;
+    if (g.n_top) scores_short_kernel<T, U, true><<<grid, 256, 0, s>>>(g);
+    else scores_short_kernel<T, U, false><<<grid, 256, 0, s>>>(g);
+}
+
 template <typename T, int W, int U>
 void launch(const ScoreArgs& g, hipStream_t s) {
     constexpr int rows = W > 1 ? 1 : 4, threads = W > 1 ? 64 * W : 256;
@@ -463,7 +642,9 @@ void launch(const ScoreArgs& g, hipStream_t s) {
 template <typename T>
 void launch_by_width(const ScoreArgs& g, hipStream_t s) {
     constexpr int CH = Chunk<T>::n;
-    if (g.V <= 64 * CH) launch<T, 1, 1>(g, s);
+    if (g.V <= 256 && g.n_top <= 8) launch_short<T, 16 / CH>(g, s);
+    else if (g.V <= 512 && g.n_top <= 8) launch_short<T, 32 / CH>(g, s);
+    else if (g.V <= 64 * CH) launch<T, 1, 1>(g, s);
     else if (g.V <= 256 * CH) launch<T, 1, 4>(g, s);
     else if (g.V <= 1024 * CH) launch<T, 2, 4>(g, s);
     else if (g.V <= 4096 * CH) launch<T, 4, 4>(g, s);

@@ -73,12 +73,14 @@ def rand(N, V, dtype, seed, scale=3.0):
 # one element; around a chunk, a wave's row, four waves' row, sixteen waves' row
 # and one segment of it, by type; the codec's vocabulary; several segments
 @pytest.mark.parametrize("dtype,V", [(torch.float16, v) for v in (
-    1, 2, 7, 8, 9, 256, 257, 511, 512, 513, 2047, 2048, 2049, 8191, 8192, 8193, 50277, 65535, 65536,
+    1, 2, 7, 8, 9, 127, 255, 256, 257, 511, 512, 513, 2047, 2048, 2049, 8191, 8192, 8193, 50277, 65535, 65536,
     65537, 131080, 151937)] + [(torch.float32, v) for v in (
-    1, 3, 4, 5, 255, 256, 257, 1023, 1024, 1025, 4096, 4097, 32768, 32769, 50277, 65543)])
+    1, 3, 4, 5, 63, 255, 256, 257, 511, 512, 513, 1023, 1024, 1025, 4096, 4097, 32768, 32769, 50277, 65543)])
 def test_widths(dtype, V):
     x, tok = rand(5, V, dtype, V)
     check(x, tok, min(V, 9))
+    check(x, tok, min(V, 8))      # (short rows have a kernel up to 8)
+    check(x, tok, 0)
 
 
 @pytest.mark.parametrize("k", [0, 1, 2, 8, 9, 20, 31, 32])
@@ -89,7 +91,7 @@ def test_top_counts(V, k):
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
-@pytest.mark.parametrize("V", [300, 3000, 9000, 66000])
+@pytest.mark.parametrize("V", [200, 300, 600, 3000, 9000, 66000])
 def test_ties_clusters_and_long_candidate_lists(dtype, V):
     """All equal, many equal maxima, sorted up and down, all mass in one chunk,
     zeros of both signs: lists that overflow and ranks by id."""
@@ -103,6 +105,7 @@ def test_ties_clusters_and_long_candidate_lists(dtype, V):
     x[6] = 0.0
     x[6, ::2] = -0.0
     x[7] = torch.clamp(x[7], max=1.0)
+    check(x, tok, 5)
     check(x, tok, 17)
     check(x, tok, 32)
 
@@ -126,6 +129,7 @@ def test_masks_nan_and_infinities(dtype, V):
     x[11, :] = -inf; x[11, 3] = float("nan")      # NaN among masked ones
     tok[6] = -1
     check(x, tok, 10)
+    check(x, tok, 6)
     check(x, tok, 0)
 
 
