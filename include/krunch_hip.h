@@ -398,7 +398,7 @@ int kr_wkv(int B, int T, int C, const float* decay, const float* first, const fl
  * 1: 64 tokens at a time on the matrix units, for prompts: equal to that up to
  * rounding, and in an order that depends on B * H and T (the time axis is split
  * over workgroups where heads are few). A NaN or infinity of a token then also
- * reaches y of up to 63 tokens before it. Calls of at most 16 tokens
+ * reaches y of up to 63 tokens before it. Calls of at most 8 tokens
  * are the same in both. ws: kr_wkv_heads_workspace_bytes (chunked only, may be
  * 0), 16-byte aligned, as r, k, v, state and y. */
 size_t kr_wkv_heads_workspace_bytes(int B, int T, int H, int D);

@@ -16,6 +16,8 @@
 #include "kr_wave.h"
 #include "krunch_hip.h"
 
+#include <type_traits>
+
 namespace {
 
 constexpr float kLog2e = 0x1.715476p+0f;
@@ -53,6 +55,9 @@ __device__ __forceinline__ int stream_tokens(const HeadArgs& g, int b) {
 // Recurrent form. A wave has 16 columns of a head's state in registers: lane
 // l the columns 4 (l % 4) .. + 3 of rows D/16 (l / 4) .. + D/16 - 1, so y is
 // summed over a lane's rows and then over 16 lanes, with no LDS.
+// Bound, for one token: the state, read and written once. Measured on MI355X, heads
+// of 64: 512 streams x 12 heads 37 us (203 MB, 5.4 TB/s; a copy runs at 5.1), one
+// stream 3.0; a further token about 0.4 us at one stream, 0.9 at 64.
 // ---------------------------------------------------------------------------
 template <int D>
 __global__ void __launch_bounds__(4 * D) heads_step_kernel(HeadArgs g) {
@@ -118,8 +123,20 @@ __global__ void __launch_bounds__(4 * D) heads_step_kernel(HeadArgs g) {
 }
 
 // ---------------------------------------------------------------------------
-// Chunked form: a workgroup of 4 waves has one head of one stream (or one
-// segment of its time axis) and walks its chunks.
+// Chunked form: a workgroup has one head of one stream (or one segment of its time
+// axis) and walks its chunks, a wave for each 16 columns of the state, which stays
+// in the wave's registers as the matrix unit leaves it: as such it is the operand
+// of r S, too. r, k and v of a chunk are read ahead into registers, then go to
+// LDS by token (r, k) and transposed by channel (k, v). The first four waves make
+// (r k') e^.. for 16 tokens each, halves of it above the diagonal left out.
+// Bound: with many heads, the VALU work of taking values apart (about 500
+// instructions a chunk and wave beside 50 products) and the three barriers, with 3
+// workgroups a CU for D = 64 and one for 128; with few heads, latency. Measured on
+// MI355X, heads of 64: 256 x 1024 tokens x 12 heads 400 us (1.71 GB, 4.3 TB/s), 128
+// streams of 256..1024 161 us (619 MB, 3.8 TB/s; 172 in the order they come), 1 x 4096
+// 25.5; heads of 128: 128 x 1024 x 6 272 us (3.3 TB/s), 1 x 1777 x 8 27. With the
+// scaling always done, without the registers' limit (2 workgroups a CU): 256 x 1024
+// 412 and 430.
 // ---------------------------------------------------------------------------
 
 // Powers of two that bring a largest value x to 2^13..2^14, and back. Zero and
@@ -129,6 +146,18 @@ __device__ __forceinline__ void power_scale(float x, float& up, float& down) {
     e = e < 14 ? 14 : e;
     up = __uint_as_float((uint32_t)(267 - e) << 23);
     down = __uint_as_float((uint32_t)(e - 13) << 23);
+}
+
+// Whether values up to `big` can be taken apart as they are: in fp16's range, and
+// their low parts' spacing (2^-24) at most 2^-21 of it. Zeros can, too.
+__device__ __forceinline__ bool plain_parts(float big) {
+    return big == 0.0f || (big >= 0.125f && big <= 32768.0f);
+}
+// x as a high and a low fp16 part. (Without kr_f16's barrier: hi is the rounding of
+// x whichever way it is made, x being exact or already fp32.)
+__device__ __forceinline__ void two_parts(float x, kr_half& hi, kr_half& lo) {
+    hi = (kr_half)x;
+    lo = (kr_half)(x - (float)hi);
 }
 
 // LDS tiles in 16-byte units. Token-major [64][D]: unit c of token t. Channel-
@@ -148,16 +177,32 @@ struct ChunkShared {
 
 // SUM: only the state that a segment's tokens add to zero.
 template <int D, bool SUM>
-__global__ void __launch_bounds__(256) heads_chunk_kernel(HeadArgs g) {
+__global__ void __launch_bounds__(4 * D, D == 64 ? 3 : 2) heads_chunk_kernel(HeadArgs g) {
     constexpr int KS = D / 32;            // k-steps over the channels
-    constexpr int MC = D / 64;            // 16-column tiles of a wave
-    constexpr int NP = D / 64;            // token pairs a thread stages
     __shared__ ChunkShared<D> sh;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l16 = lane & 15, q4 = lane >> 4;
-    const int head = blockIdx.x, h = head % g.H, b = head / g.H, seg = blockIdx.y;
-    const int heads = gridDim.x;
+    const int heads = gridDim.x, seg = blockIdx.y, h = blockIdx.x % g.H;
+    int b = blockIdx.x / g.H;
+    if (!SUM && g.lens && g.segments == 1 && g.B <= 4 * D) {
+        // longest streams first, so that no long one is left for the end: thread i
+        // ranks stream i (the sh.ph are written after the next barrier only)
+        int* lens = reinterpret_cast<int*>(sh.ph);
+        if (tid < g.B) lens[tid] = stream_tokens(g, tid);
+        __syncthreads();
+        int rank = 0;
+        if (tid < g.B) {
+            const int mine = lens[tid];
+            #pragma unroll 8
+            for (int j = 0; j < g.B; j++) rank += lens[j] > mine || (lens[j] == mine && j < tid);
+            if (rank == b) reinterpret_cast<int*>(sh.pl)[0] = tid;
+        }
+        __syncthreads();
+        b = __builtin_amdgcn_readfirstlane(reinterpret_cast<int*>(sh.pl)[0]);
+        __syncthreads();
+    }
+    const int head = b * g.H + h;
     const int t_begin = seg * g.seg_tokens;
     const int t_end = g.T - t_begin < g.seg_tokens ? g.T : t_begin + g.seg_tokens;
     const int live = stream_tokens(g, b);
@@ -165,44 +210,45 @@ __global__ void __launch_bounds__(256) heads_chunk_kernel(HeadArgs g) {
     const float w2 = decay_log2(g.decay[h]);
     const size_t row0 = (size_t)b * g.T + t_begin;
 
-    // state: column m = D/4 wave + 16 c + l16; S[c][2s], S[c][2s + 1] hold rows
-    // 32 s + 8 q4 + r and + 4, so that the pair is the operand of k-step s
-    kr_float4 S[MC][2 * KS];
-    const size_t state_at = (size_t)(8 * q4) * D + (D / 4) * wave + l16;
+    // state: column m = 16 wave + l16; S[2s], S[2s + 1] hold rows 32 s + 8 q4 + r and
+    // + 4, so that the pair is the operand of k-step s
+    kr_float4 S[2 * KS];
+    const int m = 16 * wave + l16;
+    const size_t state_at = (size_t)(8 * q4) * D + m;
     const float* s_in = nullptr;
     if (!SUM)
         s_in = (g.segments > 1 ? g.seg_state + ((size_t)seg * heads + head) * D * D
                                : g.state + (size_t)head * D * D) + state_at;
     #pragma unroll
-    for (int c = 0; c < MC; c++)
+    for (int s = 0; s < KS; s++)
         #pragma unroll
-        for (int s = 0; s < KS; s++)
-            #pragma unroll
-            for (int e = 0; e < 8; e++)
-                S[c][2 * s + e / 4][e % 4] = SUM ? 0.0f : s_in[(size_t)(32 * s + e) * D + 16 * c];
+        for (int e = 0; e < 8; e++)
+            S[2 * s + e / 4][e % 4] = SUM ? 0.0f : s_in[(size_t)(32 * s + e) * D];
 
-    // what a thread stages: tokens 2p, 2p + 1 (p = p0 + 16 i ...), 8 channels
-    const int ng = tid % (D / 8), p0 = tid / (D / 8);
-    constexpr int PSTEP = 256 / (D / 8);
-    kr_half8 rr[NP][2], kk[NP][2], vv[NP][2];
-    auto fetch = [&](int t0) {
+    // what a thread stages: 8 channels of tokens 2p, 2p + 1
+    const int ng = tid % (D / 8), p = tid / (D / 8);
+    kr_half8 rr[2], kk[2], vv[2];
+    const size_t first = row0 + 2 * p;
+    const kr_half* rp = g.r + first * g.ldr + h * D + 8 * ng;
+    const kr_half* kp = g.k + first * g.ldk + h * D + 8 * ng;
+    const kr_half* vp = g.v + first * g.ldv + h * D + 8 * ng;
+    auto fetch = [&](int t0) {            // in order of t0
         #pragma unroll
-        for (int i = 0; i < NP; i++)
-            #pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const int t = t0 + 2 * (p0 + PSTEP * i) + e;
-                const kr_half8 zero = {0, 0, 0, 0, 0, 0, 0, 0};
-                if (!SUM) rr[i][e] = zero;
-                kk[i][e] = vv[i][e] = zero;
-                if (t < n_tok) {
-                    const size_t row = row0 + t;
-                    const int o = h * D + 8 * ng;
-                    if (!SUM) rr[i][e] = *reinterpret_cast<const kr_half8*>(g.r + row * g.ldr + o);
-                    kk[i][e] = *reinterpret_cast<const kr_half8*>(g.k + row * g.ldk + o);
-                    vv[i][e] = *reinterpret_cast<const kr_half8*>(g.v + row * g.ldv + o);
-                }
+        for (int e = 0; e < 2; e++) {
+            const kr_half8 zero = {0, 0, 0, 0, 0, 0, 0, 0};
+            if (!SUM) rr[e] = zero;
+            kk[e] = vv[e] = zero;
+            if (t0 + 2 * p + e < n_tok) {
+                if (!SUM) rr[e] = *reinterpret_cast<const kr_half8*>(rp + e * g.ldr);
+                kk[e] = *reinterpret_cast<const kr_half8*>(kp + e * g.ldk);
+                vv[e] = *reinterpret_cast<const kr_half8*>(vp + e * g.ldv);
             }
+        }
+        rp += kChunk * g.ldr;
+        kp += kChunk * g.ldk;
+        vp += kChunk * g.ldv;
     };
+    kr_half* yp = g.y + (row0 + l16) * g.ldy + h * D + 16 * wave + 4 * q4;
 
     // decay factors of this lane. P tile (i-tile = wave, rows j): i = 16 wave +
     // l16, j = 16 jt + 4 q4 + r; e^(w(i-j-1)) = e^(w(i-16(jt+1))) e^(w(15-4 q4-r))
@@ -212,7 +258,7 @@ __global__ void __launch_bounds__(256) heads_chunk_kernel(HeadArgs g) {
     if (!SUM) {
         #pragma unroll
         for (int jt = 0; jt < 3; jt++)
-            p_far[jt] = jt < wave ? decay_pow(w2, 16 * (wave - jt - 1) + l16) : 0.0f;
+            p_far[jt] = jt < wave && wave < 4 ? decay_pow(w2, 16 * (wave - jt - 1) + l16) : 0.0f;
         #pragma unroll
         for (int r = 0; r < 4; r++) {
             const int d = l16 - (4 * q4 + r);
@@ -220,7 +266,7 @@ __global__ void __launch_bounds__(256) heads_chunk_kernel(HeadArgs g) {
             p_diag[r] = d > 0 ? decay_pow(w2, d - 1) : d == 0 ? u : 0.0f;
             y_dec[r] = decay_pow(w2, 16 * r + l16);
         }
-        if ((wave & 1) == 0) {            // the half k-step right of the diagonal tile
+        if (wave == 0 || wave == 2) {     // the half k-step right of the diagonal tile
             const int i = 16 * wave + l16, j = 16 * (wave + 1) + 4 * q4;
             kr_half4* ph = reinterpret_cast<kr_half4*>(sh.ph + chan_unit(i, j / 8)) + (j / 4 & 1);
             kr_half4* pl = reinterpret_cast<kr_half4*>(sh.pl + chan_unit(i, j / 8)) + (j / 4 & 1);
@@ -239,155 +285,177 @@ __global__ void __launch_bounds__(256) heads_chunk_kernel(HeadArgs g) {
     fetch(0);
     for (int t0 = 0; t0 < n_tok; t0 += kChunk) {
         const int n = n_tok - t0 < kChunk ? n_tok - t0 : kChunk;
+        // LDS addresses are made anew for each chunk: kept over the loop, they and
+        // the reads moved up to them spill
+        int l16 = lane & 15, q4 = lane >> 4;
+        __asm__ volatile("" : "+v"(l16), "+v"(q4));
         if (n < kChunk) set_v_dec(n);
+        typedef kr_half half2v __attribute__((ext_vector_type(2)));
         #pragma unroll
-        for (int i = 0; i < NP; i++) {
-            const int p = p0 + PSTEP * i;
-            #pragma unroll
-            for (int e = 0; e < 2; e++) {
-                if (!SUM) {
-                    sh.r[tok_unit<D>(2 * p + e, ng)] = rr[i][e];
-                    sh.k[tok_unit<D>(2 * p + e, ng)] = kk[i][e];
-                }
+        for (int e = 0; e < 2; e++) {
+            if (!SUM) {
+                sh.r[tok_unit<D>(2 * p + e, ng)] = rr[e];
+                sh.k[tok_unit<D>(2 * p + e, ng)] = kk[e];
             }
-            typedef kr_half half2v __attribute__((ext_vector_type(2)));
-            #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const int c = chan_unit(8 * ng + e, p / 4) * 4 + p % 4;
-                reinterpret_cast<half2v*>(sh.kt)[c] = half2v{kk[i][0][e], kk[i][1][e]};
-                reinterpret_cast<half2v*>(sh.vt)[c] = half2v{vv[i][0][e], vv[i][1][e]};
-            }
+        }
+        #pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const int c = chan_unit(8 * ng + e, p / 4) * 4 + p % 4;
+            reinterpret_cast<half2v*>(sh.kt)[c] = half2v{kk[0][e], kk[1][e]};
+            reinterpret_cast<half2v*>(sh.vt)[c] = half2v{vv[0][e], vv[1][e]};
         }
         if (t0 + kChunk < n_tok) fetch(t0 + kChunk);
         __syncthreads();
         if (!SUM) {
-            // P' tiles of i-tile `wave`: rows j, columns i
-            kr_half8 ri[KS];
-            #pragma unroll
-            for (int s = 0; s < KS; s++) ri[s] = sh.r[tok_unit<D>(16 * wave + l16, 4 * s + q4)];
-            kr_float4 P[4];
-            float big = 0.0f;
-            #pragma unroll
-            for (int jt = 0; jt < 4; jt++) {
-                if (jt > wave) break;
-                P[jt] = kr_float4{0, 0, 0, 0};
+            if (wave < 4) {
+                // P' tiles of i-tile `wave`: rows j, columns i
+                kr_half8 ri[KS];
                 #pragma unroll
-                for (int s = 0; s < KS; s++)
-                    P[jt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                        sh.k[tok_unit<D>(16 * jt + l16, 4 * s + q4)], ri[s], P[jt], 0, 0, 0);
+                for (int s = 0; s < KS; s++) ri[s] = sh.r[tok_unit<D>(16 * wave + l16, 4 * s + q4)];
+                kr_float4 P[4];
+                float big = 0.0f;
                 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    P[jt][r] *= jt == wave ? p_diag[r] : p_far[jt < 3 ? jt : 0] * p_near[r];
-                    big = fmaxf(big, fabsf(P[jt][r]));
+                for (int jt = 0; jt < 4; jt++) {
+                    P[jt] = kr_float4{0, 0, 0, 0};
+                    if (jt > wave) continue;
+                    #pragma unroll
+                    for (int s = 0; s < KS; s++)
+                        P[jt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                            sh.k[tok_unit<D>(16 * jt + l16, 4 * s + q4)], ri[s], P[jt], 0, 0, 0);
+                    #pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        P[jt][r] *= jt == wave ? p_diag[r] : p_far[jt < 3 ? jt : 0] * p_near[r];
+                        big = fmaxf(big, fabsf(P[jt][r]));
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-            }
-            big = fmaxf(big, kr_xor<16>(big));
-            big = fmaxf(big, kr_xor<32>(big));
-            float up, down;
-            power_scale(big, up, down);
-            const int i = 16 * wave + l16;
-            if (q4 == 0) sh.pdown[i] = down;
-            #pragma unroll
-            for (int jt = 0; jt < 4; jt++) {
-                if (jt > wave) break;
-                kr_half4 hi, lo;
-                #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const float x = P[jt][r] * up;
-                    hi[r] = kr_f16(x);
-                    lo[r] = kr_f16(x - (float)hi[r]);
+                big = fmaxf(big, kr_xor<16>(big));
+                big = fmaxf(big, kr_xor<32>(big));
+                float down = 1.0f;
+                if (!__all(plain_parts(big))) {
+                    float up;
+                    power_scale(big, up, down);
+                    #pragma unroll
+                    for (int jt = 0; jt < 4; jt++) P[jt] *= up;
                 }
-                const int at = chan_unit(i, 2 * jt + q4 / 2);
-                reinterpret_cast<kr_half4*>(sh.ph + at)[q4 & 1] = hi;
-                reinterpret_cast<kr_half4*>(sh.pl + at)[q4 & 1] = lo;
+                const int i = 16 * wave + l16;
+                if (q4 == 0) sh.pdown[i] = down;
+                #pragma unroll
+                for (int jt = 0; jt < 4; jt++) {
+                    if (jt > wave) continue;
+                    kr_half4 hi, lo;
+                    #pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        kr_half a, b;
+                        two_parts(P[jt][r], a, b);
+                        hi[r] = a;
+                        lo[r] = b;
+                    }
+                    const int at = chan_unit(i, 2 * jt + q4 / 2);
+                    reinterpret_cast<kr_half4*>(sh.ph + at)[q4 & 1] = hi;
+                    reinterpret_cast<kr_half4*>(sh.pl + at)[q4 & 1] = lo;
+                }
             }
             __syncthreads();
         }
+        __builtin_amdgcn_sched_barrier(0);
+        kr_half8 vc[2];
         #pragma unroll
-        for (int c = 0; c < MC; c++) {
-            const int m = (D / 4) * wave + 16 * c + l16;
-            kr_half8 vc[2];
+        for (int s = 0; s < 2; s++) vc[s] = sh.vt[chan_unit(m, 4 * s + q4)];
+        if (!SUM) {
+            float big = 0.0f;
             #pragma unroll
-            for (int s = 0; s < 2; s++) vc[s] = sh.vt[chan_unit(m, 4 * s + q4)];
-            if (!SUM) {
-                float big = 0.0f;
+            for (int s = 0; s < 2 * KS; s++)
                 #pragma unroll
-                for (int s = 0; s < 2 * KS; s++)
-                    #pragma unroll
-                    for (int r = 0; r < 4; r++) big = fmaxf(big, fabsf(S[c][s][r]));
-                big = kr_wave_reduce(big, [](float x, float y) { return fmaxf(x, y); });
-                float up, down;
-                power_scale(big, up, down);
-                kr_half8 sh_hi[KS], sh_lo[KS];
+                for (int r = 0; r < 4; r++) big = fmaxf(big, fabsf(S[s][r]));
+            big = kr_wave_reduce(big, [](float x, float y) { return fmaxf(x, y); });
+            float up = 1.0f, down = 1.0f;
+            const bool scaled = !plain_parts(big);
+            if (scaled) power_scale(big, up, down);
+            kr_half8 s_hi[KS], s_lo[KS];
+            auto take_apart = [&](auto with_scale) {
                 #pragma unroll
                 for (int s = 0; s < KS; s++)
                     #pragma unroll
                     for (int e = 0; e < 8; e++) {
-                        const float x = S[c][2 * s + e / 4][e % 4] * up;
-                        sh_hi[s][e] = kr_f16(x);
-                        sh_lo[s][e] = kr_f16(x - (float)sh_hi[s][e]);
+                        const float x = S[2 * s + e / 4][e % 4];
+                        kr_half a, b;
+                        two_parts(decltype(with_scale)::value ? x * up : x, a, b);
+                        s_hi[s][e] = a;
+                        s_lo[s][e] = b;
                     }
-                // y': rows m, columns i
-                #pragma unroll
-                for (int it = 0; it < 4; it++) {
-                    kr_float4 from_s = {0, 0, 0, 0}, inside = {0, 0, 0, 0};
-                    #pragma unroll
-                    for (int s = 0; s < KS; s++) {
-                        const kr_half8 x = sh.r[tok_unit<D>(16 * it + l16, 4 * s + q4)];
-                        from_s = __builtin_amdgcn_mfma_f32_16x16x32_f16(sh_hi[s], x, from_s, 0, 0, 0);
-                        from_s = __builtin_amdgcn_mfma_f32_16x16x32_f16(sh_lo[s], x, from_s, 0, 0, 0);
-                    }
-                    #pragma unroll
-                    for (int s = 0; s < 1 + it / 2; s++) {
-                        const int at = chan_unit(16 * it + l16, 4 * s + q4);
-                        inside = __builtin_amdgcn_mfma_f32_16x16x32_f16(vc[s], sh.ph[at], inside, 0, 0, 0);
-                        inside = __builtin_amdgcn_mfma_f32_16x16x32_f16(vc[s], sh.pl[at], inside, 0, 0, 0);
-                    }
-                    const int i = 16 * it + l16;
-                    const float fs = down * y_dec[it], fp = sh.pdown[i];
-                    kr_half4 y;
-                    #pragma unroll
-                    for (int r = 0; r < 4; r++)
-                        y[r] = kr_f16(__builtin_fmaf(inside[r], fp, from_s[r] * fs));
-                    if (i < n)
-                        *reinterpret_cast<kr_half4*>(g.y + (row0 + t0 + i) * g.ldy + h * D +
-                                                     (D / 4) * wave + 16 * c + 4 * q4) = y;
-                }
-            }
-            // S <- e^(wn) S + k' (e^.. v): v in two parts, scaled by its column
-            float x[16], big = 0.0f;
+            };
+            if (scaled) take_apart(std::integral_constant<bool, true>());
+            else take_apart(std::integral_constant<bool, false>());
+            __builtin_amdgcn_sched_barrier(0);
+            // y': rows m, columns i
             #pragma unroll
-            for (int i = 0; i < 16; i++) {
-                x[i] = (float)vc[i / 8][i % 8] * v_dec[i];
-                big = fmaxf(big, fabsf(x[i]));
+            for (int it = 0; it < 4; it++) {
+                kr_float4 from_s = {0, 0, 0, 0}, inside = {0, 0, 0, 0};
+                #pragma unroll
+                for (int s = 0; s < KS; s++) {
+                    const kr_half8 x = sh.r[tok_unit<D>(16 * it + l16, 4 * s + q4)];
+                    from_s = __builtin_amdgcn_mfma_f32_16x16x32_f16(s_hi[s], x, from_s, 0, 0, 0);
+                    from_s = __builtin_amdgcn_mfma_f32_16x16x32_f16(s_lo[s], x, from_s, 0, 0, 0);
+                }
+                #pragma unroll
+                for (int s = 0; s < 1 + it / 2; s++) {
+                    const int at = chan_unit(16 * it + l16, 4 * s + q4);
+                    inside = __builtin_amdgcn_mfma_f32_16x16x32_f16(vc[s], sh.ph[at], inside, 0, 0, 0);
+                    inside = __builtin_amdgcn_mfma_f32_16x16x32_f16(vc[s], sh.pl[at], inside, 0, 0, 0);
+                }
+                const int i = 16 * it + l16;
+                const float fs = down * y_dec[it], fp = sh.pdown[i];
+                kr_half4 y;
+                #pragma unroll
+                for (int r = 0; r < 4; r++) y[r] = kr_f16(__builtin_fmaf(inside[r], fp, from_s[r] * fs));
+                if (i < n)
+                    *reinterpret_cast<kr_half4*>(yp + 16 * it * g.ldy) = y;
+                __builtin_amdgcn_sched_barrier(0);
             }
-            big = fmaxf(big, kr_xor<16>(big));
-            big = fmaxf(big, kr_xor<32>(big));
-            float up, down;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        yp += kChunk * g.ldy;
+        // S <- e^(wn) S + k' (e^.. v): v in two parts, scaled by its column where it
+        // has to be
+        float x[16], big = 0.0f;
+        #pragma unroll
+        for (int i = 0; i < 16; i++) {
+            x[i] = (float)vc[i / 8][i % 8] * v_dec[i];
+            big = fmaxf(big, fabsf(x[i]));
+        }
+        big = fmaxf(big, kr_xor<16>(big));
+        big = fmaxf(big, kr_xor<32>(big));
+        float down = 1.0f;
+        if (!__all(plain_parts(big))) {
+            float up;
             power_scale(big, up, down);
-            kr_half8 hi[2], lo[2];
             #pragma unroll
-            for (int i = 0; i < 16; i++) {
-                const float z = x[i] * up;
-                hi[i / 8][i % 8] = kr_f16(z);
-                lo[i / 8][i % 8] = kr_f16(z - (float)hi[i / 8][i % 8]);
-            }
-            const float keep = decay_pow(w2, n);
+            for (int i = 0; i < 16; i++) x[i] *= up;
+        }
+        kr_half8 hi[2], lo[2];
+        #pragma unroll
+        for (int i = 0; i < 16; i++) {
+            kr_half a, b;
+            two_parts(x[i], a, b);
+            hi[i / 8][i % 8] = a;
+            lo[i / 8][i % 8] = b;
+        }
+        const float keep = decay_pow(w2, n);
+        #pragma unroll
+        for (int st = 0; st < 2 * KS; st++) {
+            // row l16 of the tile is channel 32 (st / 2) + 8 (l16 / 4) + 4 (st % 2) + l16 % 4
+            const int ch = 32 * (st / 2) + 8 * (l16 >> 2) + 4 * (st % 2) + (l16 & 3);
+            kr_float4 add = {0, 0, 0, 0};
             #pragma unroll
-            for (int st = 0; st < 2 * KS; st++) {
-                // row l16 of the tile is channel 32 (st / 2) + 8 (l16 / 4) + 4 (st % 2) + l16 % 4
-                const int ch = 32 * (st / 2) + 8 * (l16 >> 2) + 4 * (st % 2) + (l16 & 3);
-                kr_float4 add = {0, 0, 0, 0};
-                #pragma unroll
-                for (int s = 0; s < 2; s++) {
-                    const kr_half8 kc = sh.kt[chan_unit(ch, 4 * s + q4)];
-                    add = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, hi[s], add, 0, 0, 0);
-                    add = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, lo[s], add, 0, 0, 0);
-                }
-                #pragma unroll
-                for (int r = 0; r < 4; r++)
-                    S[c][st][r] = __builtin_fmaf(add[r], down, keep * S[c][st][r]);
+            for (int s = 0; s < 2; s++) {
+                const kr_half8 kc = sh.kt[chan_unit(ch, 4 * s + q4)];
+                add = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, hi[s], add, 0, 0, 0);
+                add = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, lo[s], add, 0, 0, 0);
             }
+            #pragma unroll
+            for (int r = 0; r < 4; r++) S[st][r] = __builtin_fmaf(add[r], down, keep * S[st][r]);
+            if (st % 2) __builtin_amdgcn_sched_barrier(0);
         }
         __syncthreads();
     }
@@ -399,15 +467,12 @@ __global__ void __launch_bounds__(256) heads_chunk_kernel(HeadArgs g) {
     if (s_out) {
         s_out += state_at;
         #pragma unroll
-        for (int c = 0; c < MC; c++)
+        for (int s = 0; s < KS; s++)
             #pragma unroll
-            for (int s = 0; s < KS; s++)
-                #pragma unroll
-                for (int e = 0; e < 8; e++)
-                    s_out[(size_t)(32 * s + e) * D + 16 * c] = S[c][2 * s + e / 4][e % 4];
+            for (int e = 0; e < 8; e++) s_out[(size_t)(32 * s + e) * D] = S[2 * s + e / 4][e % 4];
     }
     if (!SUM)
-        for (int i = n_tok * (D / 8) + tid; i < (t_end - t_begin) * (D / 8); i += 256)
+        for (int i = n_tok * (D / 8) + tid; i < (t_end - t_begin) * (D / 8); i += 4 * D)
             *reinterpret_cast<kr_half8*>(g.y + (row0 + i / (D / 8)) * g.ldy + h * D + 8 * (i % (D / 8))) =
                 kr_half8{0, 0, 0, 0, 0, 0, 0, 0};
 }
@@ -425,21 +490,36 @@ __global__ void __launch_bounds__(256) heads_join_kernel(HeadArgs g) {
     kr_float4* seg = reinterpret_cast<kr_float4*>(g.seg_state) + at;
     kr_float4 s = reinterpret_cast<const kr_float4*>(g.state)[at];
     seg[0] = s;
-    for (int i = 1; i < g.segments; i++) {
-        const int before = (i - 1) * g.seg_tokens;
-        const int n = live < before ? 0 : live - before < g.seg_tokens ? live - before : g.seg_tokens;
-        const float keep = decay_pow(w2, n);
-        const kr_float4 add = seg[i * slot];
+    constexpr int kAhead = 8;             // or every step waits for memory
+    for (int i0 = 1; i0 < g.segments; i0 += kAhead) {
+        kr_float4 add[kAhead];
         #pragma unroll
-        for (int r = 0; r < 4; r++) s[r] = __builtin_fmaf(keep, s[r], add[r]);
-        seg[i * slot] = s;
+        for (int j = 0; j < kAhead; j++)
+            if (i0 + j < g.segments) add[j] = seg[(i0 + j) * slot];
+        #pragma unroll
+        for (int j = 0; j < kAhead; j++) {
+            const int i = i0 + j;
+            if (i >= g.segments) break;
+            const int before = (i - 1) * g.seg_tokens;
+            const int n = live < before ? 0 : live - before < g.seg_tokens ? live - before : g.seg_tokens;
+            const float keep = decay_pow(w2, n);
+            #pragma unroll
+            for (int r = 0; r < 4; r++) s[r] = __builtin_fmaf(keep, s[r], add[j][r]);
+            seg[i * slot] = s;
+        }
     }
 }
 
-// Tokens up to which the chunked form is the recurrent one, too.
-constexpr int kStepTokens = 16;
-// Workgroups that a time split aims for, and the fewest tokens of a segment.
-constexpr int kSplitGroups = 512, kSplitTokens = 128;
+// Tokens up to which the chunked form is the recurrent one, too. us, recurrent /
+// chunked, 12 heads of 64: 8 tokens of 1 stream 6.1 / 6.7, of 64 13.4 / 13.2, of 512
+// 64 / 62; 16 tokens 9.5 / 6.8, 20.7 / 13.2, 112 / 64.
+constexpr int kStepTokens = 8;
+// Workgroups that a time split aims for, and the fewest tokens of a segment. A split
+// reads k and v twice and costs two launches. us, aiming for 256 / 512 / 1024: 32 x 512
+// x 12 heads of 64 37.7 / 45.7 / 51.8, 16 x 1024 53 / 52 / 55, 16 x 1024 x 6 of 128 78 /
+// 86 / 92; segments of 64 / 128 / 256 tokens: 1 x 256 x 12 12.6 / 15.9 / 15.3, 1 x 1777 x
+// 8 of 128 28.6 / 31.7 / 42.2, 1 x 4096 x 12 26.5 / 26.5 / 29.2.
+constexpr int kSplitGroups = 256, kSplitTokens = 64;
 
 void split_time(long long heads, int T, int& tokens, int& segments) {
     long long n = (kSplitGroups + heads - 1) / heads;
@@ -455,13 +535,13 @@ int launch(HeadArgs& g, bool chunked, hipStream_t s) {
     if (!chunked || g.T <= kStepTokens) {
         heads_step_kernel<D><<<heads, 4 * D, 0, s>>>(g);
     } else if (g.segments == 1) {
-        heads_chunk_kernel<D, false><<<heads, 256, 0, s>>>(g);
+        heads_chunk_kernel<D, false><<<heads, 4 * D, 0, s>>>(g);
     } else {
-        heads_chunk_kernel<D, true><<<dim3(heads, g.segments - 1), 256, 0, s>>>(g);
+        heads_chunk_kernel<D, true><<<dim3(heads, g.segments - 1), 4 * D, 0, s>>>(g);
         KR_LAUNCHED();
         heads_join_kernel<D><<<heads * (D * D / 1024), 256, 0, s>>>(g);
         KR_LAUNCHED();
-        heads_chunk_kernel<D, false><<<dim3(heads, g.segments), 256, 0, s>>>(g);
+        heads_chunk_kernel<D, false><<<dim3(heads, g.segments), 4 * D, 0, s>>>(g);
     }
     KR_LAUNCHED();
     return KR_OK;

@@ -67,9 +67,9 @@ def test_recurrent(B, T, H, D):
     check(*make(B, T, H, D, B + T + H), chunked=False)
 
 
-# around one and two chunks, and around the lengths where the time axis splits;
-# many heads (no split) and few
-@pytest.mark.parametrize("B,T,H,D", [(1, 17, 1, 64), (2, 63, 2, 64), (1, 64, 3, 64), (3, 65, 4, 64),
+# the last length of the recurrent form, around one and two chunks, and around the
+# lengths where the time axis splits; many heads (no split) and few
+@pytest.mark.parametrize("B,T,H,D", [(2, 8, 3, 64), (2, 9, 3, 64), (1, 17, 1, 64), (2, 63, 2, 64), (1, 64, 3, 64), (3, 65, 4, 64),
                                      (1, 127, 2, 128), (2, 128, 1, 128), (1, 129, 2, 64), (1, 257, 2, 128),
                                      (1, 640, 1, 64), (50, 200, 12, 64), (40, 130, 16, 64), (70, 70, 8, 128),
                                      (1, 1000, 12, 64), (1, 1000, 4, 128)])
@@ -78,7 +78,8 @@ def test_chunked(B, T, H, D):
 
 
 @pytest.mark.parametrize("chunked", [False, True])
-@pytest.mark.parametrize("B,T,H,D", [(7, 150, 2, 64), (9, 400, 1, 128), (130, 90, 4, 64), (6, 3, 2, 64)])
+@pytest.mark.parametrize("B,T,H,D", [(7, 150, 2, 64), (9, 400, 1, 128), (130, 90, 4, 64), (6, 3, 2, 64),
+                                     (300, 70, 1, 64), (257, 40, 2, 128)])
 def test_ragged_streams(B, T, H, D, chunked):
     """Lengths of none, one, a chunk, all and out of range; NaN in the padding."""
     args = make(B, T, H, D, B + T)
