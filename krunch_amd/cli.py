@@ -6,6 +6,8 @@ files.
                                         [--tokenizer PATH] [--w8a8]
     python -m krunch_amd.cli decompress [--in PATH] [--out PATH] [--weights PATH]
                                         [--tokenizer PATH]
+    python -m krunch_amd.cli estimate   [--in PATH] [--out PATH] [--weights PATH]
+                                        [--tokenizer PATH] [--w8a8]
 
 `--in`/`--out` default to stdin/stdout ("-" also means them), as in the
 reference (cli.py:121-134). The model is an RWKV-4 checkpoint (`--weights`
@@ -14,12 +16,15 @@ synthetic RWKV-4-169M-shaped model (seed 0). The tokenizer is a `tokenizers`
 JSON (`--tokenizer` or $KRUNCH_TOKENIZER), else the byte tokenizer. Compress
 writes header + entries for all chunks in one batched call (cli.py:49-70);
 decompress picks the fp16 or int8 codec from the blob's model_id and checks
-codec, CRC32 and length as the reference does (cli.py:73-118). Errors go to
+codec, CRC32 and length as the reference does (cli.py:73-118). Estimate (no
+counterpart) runs the model without the coder and writes one JSON line: the
+input's bytes, the estimated blob's and their ratio. Errors go to
 stderr with exit status 1; logs go to stderr so stdout carries only data.
 """
 from __future__ import annotations
 
 import argparse
+import json
 import logging
 import os
 import sys
@@ -80,10 +85,19 @@ def cmd_decompress(args, load: Callable = _load_engine) -> None:
     logger.info("decompress %d -> %d bytes", len(blob), len(raw))
 
 
+def cmd_estimate(args, load: Callable = _load_engine) -> None:
+    raw = _read_input(args.input)
+    weights, tokenizer = _model_paths(args)
+    size = load(weights, tokenizer, bool(args.w8a8)).estimate(raw)
+    line = {"bytes": len(raw), "estimate": size, "ratio": size / len(raw) if raw else 0.0}
+    _write_output(args.output, (json.dumps(line) + "\n").encode())
+
+
 def build_parser() -> argparse.ArgumentParser:
     ap = argparse.ArgumentParser(prog="krunch", description="Krunch neural compression (MI355X)")
     sub = ap.add_subparsers(dest="cmd", required=True)
-    for name, hlp in (("compress", "Compress bytes"), ("decompress", "Decompress a .krunch blob")):
+    for name, hlp in (("compress", "Compress bytes"), ("decompress", "Decompress a .krunch blob"),
+                      ("estimate", "Estimate the size compress would come to")):
         p = sub.add_parser(name, help=hlp)
         p.add_argument("--in", dest="input", help="input file (default: stdin)")
         p.add_argument("--out", dest="output", help="output file (default: stdout)")
@@ -91,7 +105,7 @@ def build_parser() -> argparse.ArgumentParser:
                                          "default $KRUNCH_WEIGHTS, else the synthetic model")
         p.add_argument("--tokenizer", help="tokenizers JSON; default $KRUNCH_TOKENIZER, "
                                            "else the byte tokenizer")
-        if name == "compress":
+        if name != "decompress":
             p.add_argument("--w8a8", action="store_true",
                            help="int8 codec (model_id 2); decompress detects it from the blob")
     return ap
@@ -102,10 +116,8 @@ def main(argv: Optional[Sequence[str]] = None, load: Callable = _load_engine) ->
                         stream=sys.stderr)
     args = build_parser().parse_args(argv)
     try:
-        if args.cmd == "compress":
-            cmd_compress(args, load)
-        else:
-            cmd_decompress(args, load)
+        {"compress": cmd_compress, "decompress": cmd_decompress,
+         "estimate": cmd_estimate}[args.cmd](args, load)
     except (ValueError, OSError) as e:
         print(f"krunch: {e}", file=sys.stderr)
         return 1

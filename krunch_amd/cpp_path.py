@@ -10,7 +10,8 @@ are bit-identical per row (one GEMM reduction order, shared elementwise
 code), which is what makes compress/decompress round trips byte-exact.
 
 Additions: `forward_packed_batched` runs B chunks x T tokens in one call
-(the reference op already accepts [B,T,C], layer_cpp.cpp:469-474).
+(the reference op already accepts [B,T,C], layer_cpp.cpp:469-474);
+`score_packed_batched` scores B texts without a coder.
 """
 from __future__ import annotations
 
@@ -151,6 +152,61 @@ def forward_stepped_batched(weights: dict, last_tokens, state: State) -> torch.T
 
 def forward_stepped(weights: dict, last_token: int, state: State) -> torch.Tensor:
     return forward_stepped_batched(weights, [int(last_token)], state).reshape(-1)
+
+
+# Rows whose logits score_packed_batched holds at a time (824 MB at the 169M
+# shape), the engine's head block.
+SCORE_ROWS = 8192
+
+
+def score_packed_batched(weights: dict, input_ids, target_ids, state: State, n_top: int = 0,
+                         head_rows: int = SCORE_ROWS):
+    """What the model says of given next tokens, without a coder: input_ids and
+    target_ids [B, T] (-1: none, its logprob is 0) -> logprob and entropy fp32
+    [B, T], in nats, and the n_top most likely tokens, top_logprob and
+    top_token [B, T, n_top] (krunch_ac_hip.token_scores); state (B streams)
+    carried. The layers run as in forward_packed_batched, the head and the
+    scores in blocks of head_rows rows, so no [B * T, V] logits are held."""
+    P: Prepared = weights["prepared"]
+    ids, tgt = _ids(input_ids, P.device), _ids(target_ids, P.device)
+    if ids.dim() != 2 or ids.shape != tgt.shape:
+        raise ValueError(f"input_ids and target_ids must be [B, T], got {tuple(ids.shape)} and "
+                         f"{tuple(tgt.shape)}")
+    B, T = ids.shape
+    assert state.B == B, f"state holds {state.B} streams, input has {B}"
+    _check_ids(ids, P.V)
+    if tgt.numel() and (int(tgt.min()) < -1 or int(tgt.max()) >= P.V):
+        raise ValueError(f"target id out of range [-1, {P.V})")
+    return _score_window(weights, ids, tgt, state, n_top, head_rows)
+
+
+def _score_window(weights, ids, tgt, state, n_top, head_rows):
+    """score_packed_batched on checked device ids."""
+    from krunch_amd import krunch_ac_hip
+    P: Prepared = weights["prepared"]
+    B, T = ids.shape
+    M = B * T
+    x = torch.empty((M, P.C), dtype=torch.float16, device=P.device)
+    s = _lib.stream_ptr()
+    if M:
+        _lib.call("kr_embed", P.ptr, ids.data_ptr(), M, x.data_ptr(), s)
+        ws, nbytes = workspace(weights, M)
+        _lib.call("kr_forward_layers", P.ptr, x.data_ptr(), B, T, state.ptr, ws.data_ptr(), nbytes, s)
+    rows = max(1, min(M, head_rows))
+    xn = torch.empty(((rows + 15) // 16 * 16, P.C), dtype=torch.float16, device=P.device)
+    ld = logits_ld(P.V)
+    logits = torch.empty((rows, ld), dtype=torch.float16, device=P.device)
+    tgt = tgt.reshape(-1)
+    parts = []
+    for r0 in range(0, M, rows):
+        n = min(rows, M - r0)
+        _lib.call("kr_head_logits_rows16", P.ptr, x[r0:].data_ptr(), n, xn.data_ptr(),
+                  logits.data_ptr(), ld, s)
+        parts.append(krunch_ac_hip.token_scores(logits[:n, :P.V], tgt[r0:r0 + n], n_top))
+    if not parts:
+        parts = [krunch_ac_hip.token_scores(logits[:0, :P.V], tgt, n_top)]
+    cols = [p[0] if len(p) == 1 else torch.cat(p) for p in zip(*parts)]
+    return tuple(c.view(B, T, *c.shape[1:]) for c in cols)
 
 
 _STEP_GRAPHS: dict = {}

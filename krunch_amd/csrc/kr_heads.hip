@@ -16,8 +16,6 @@
 #include "kr_wave.h"
 #include "krunch_hip.h"
 
-#include <type_traits>
-
 namespace {
 
 constexpr float kLog2e = 0x1.715476p+0f;
@@ -132,11 +130,9 @@ __global__ void __launch_bounds__(4 * D) heads_step_kernel(HeadArgs g) {
 // Bound: with many heads, the VALU work of taking values apart (about 500
 // instructions a chunk and wave beside 50 products) and the three barriers, with 3
 // workgroups a CU for D = 64 and one for 128; with few heads, latency. Measured on
-// MI355X, heads of 64: 256 x 1024 tokens x 12 heads 400 us (1.71 GB, 4.3 TB/s), 128
-// streams of 256..1024 161 us (619 MB, 3.8 TB/s; 172 in the order they come), 1 x 4096
-// 25.5; heads of 128: 128 x 1024 x 6 272 us (3.3 TB/s), 1 x 1777 x 8 27. With the
-// scaling always done, without the registers' limit (2 workgroups a CU): 256 x 1024
-// 412 and 430.
+// MI355X, heads of 64: 256 x 1024 tokens x 12 heads 401 us (1.71 GB, 4.3 TB/s), 128
+// streams of 256..1024 163 us (640 MB, 3.9 TB/s; 173 in the order they come), 1 x 4096
+// 25; heads of 128: 128 x 1024 x 6 288 us (3.1 TB/s), 1 x 1777 x 8 28.
 // ---------------------------------------------------------------------------
 
 // Powers of two that bring a largest value x to 2^13..2^14, and back. Zero and
@@ -148,14 +144,9 @@ __device__ __forceinline__ void power_scale(float x, float& up, float& down) {
     down = __uint_as_float((uint32_t)(e - 13) << 23);
 }
 
-// Whether values up to `big` can be taken apart as they are: in fp16's range, and
-// their low parts' spacing (2^-24) at most 2^-21 of it. Zeros can, too.
-__device__ __forceinline__ bool plain_parts(float big) {
-    return big == 0.0f || (big >= 0.125f && big <= 32768.0f);
-}
-// x as a high and a low fp16 part. (Without kr_f16's barrier: hi is the rounding of
-// x whichever way it is made, x being exact or already fp32.)
+// x as a high and a low fp16 part.
 __device__ __forceinline__ void two_parts(float x, kr_half& hi, kr_half& lo) {
+    __asm__("" : "+v"(x));       // or x is made twice, in 7 spilled registers (400 -> 473 us)
     hi = (kr_half)x;
     lo = (kr_half)(x - (float)hi);
 }
@@ -331,13 +322,8 @@ __global__ void __launch_bounds__(4 * D, D == 64 ? 3 : 2) heads_chunk_kernel(Hea
                 }
                 big = fmaxf(big, kr_xor<16>(big));
                 big = fmaxf(big, kr_xor<32>(big));
-                float down = 1.0f;
-                if (!__all(plain_parts(big))) {
-                    float up;
-                    power_scale(big, up, down);
-                    #pragma unroll
-                    for (int jt = 0; jt < 4; jt++) P[jt] *= up;
-                }
+                float up, down;
+                power_scale(big, up, down);
                 const int i = 16 * wave + l16;
                 if (q4 == 0) sh.pdown[i] = down;
                 #pragma unroll
@@ -347,7 +333,7 @@ __global__ void __launch_bounds__(4 * D, D == 64 ? 3 : 2) heads_chunk_kernel(Hea
                     #pragma unroll
                     for (int r = 0; r < 4; r++) {
                         kr_half a, b;
-                        two_parts(P[jt][r], a, b);
+                        two_parts(P[jt][r] * up, a, b);
                         hi[r] = a;
                         lo[r] = b;
                     }
@@ -369,24 +355,18 @@ __global__ void __launch_bounds__(4 * D, D == 64 ? 3 : 2) heads_chunk_kernel(Hea
                 #pragma unroll
                 for (int r = 0; r < 4; r++) big = fmaxf(big, fabsf(S[s][r]));
             big = kr_wave_reduce(big, [](float x, float y) { return fmaxf(x, y); });
-            float up = 1.0f, down = 1.0f;
-            const bool scaled = !plain_parts(big);
-            if (scaled) power_scale(big, up, down);
+            float up, down;
+            power_scale(big, up, down);
             kr_half8 s_hi[KS], s_lo[KS];
-            auto take_apart = [&](auto with_scale) {
+            #pragma unroll
+            for (int s = 0; s < KS; s++)
                 #pragma unroll
-                for (int s = 0; s < KS; s++)
-                    #pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const float x = S[2 * s + e / 4][e % 4];
-                        kr_half a, b;
-                        two_parts(decltype(with_scale)::value ? x * up : x, a, b);
-                        s_hi[s][e] = a;
-                        s_lo[s][e] = b;
-                    }
-            };
-            if (scaled) take_apart(std::integral_constant<bool, true>());
-            else take_apart(std::integral_constant<bool, false>());
+                for (int e = 0; e < 8; e++) {
+                    kr_half a, b;
+                    two_parts(S[2 * s + e / 4][e % 4] * up, a, b);
+                    s_hi[s][e] = a;
+                    s_lo[s][e] = b;
+                }
             __builtin_amdgcn_sched_barrier(0);
             // y': rows m, columns i
             #pragma unroll
@@ -416,8 +396,7 @@ __global__ void __launch_bounds__(4 * D, D == 64 ? 3 : 2) heads_chunk_kernel(Hea
         }
         __builtin_amdgcn_sched_barrier(0);
         yp += kChunk * g.ldy;
-        // S <- e^(wn) S + k' (e^.. v): v in two parts, scaled by its column where it
-        // has to be
+        // S <- e^(wn) S + k' (e^.. v): v in two parts, scaled by its column
         float x[16], big = 0.0f;
         #pragma unroll
         for (int i = 0; i < 16; i++) {
@@ -426,18 +405,13 @@ __global__ void __launch_bounds__(4 * D, D == 64 ? 3 : 2) heads_chunk_kernel(Hea
         }
         big = fmaxf(big, kr_xor<16>(big));
         big = fmaxf(big, kr_xor<32>(big));
-        float down = 1.0f;
-        if (!__all(plain_parts(big))) {
-            float up;
-            power_scale(big, up, down);
-            #pragma unroll
-            for (int i = 0; i < 16; i++) x[i] *= up;
-        }
+        float up, down;
+        power_scale(big, up, down);
         kr_half8 hi[2], lo[2];
         #pragma unroll
         for (int i = 0; i < 16; i++) {
             kr_half a, b;
-            two_parts(x[i], a, b);
+            two_parts(x[i] * up, a, b);
             hi[i / 8][i % 8] = a;
             lo[i / 8][i % 8] = b;
         }

@@ -16,13 +16,17 @@ Byte-level methods tokenize with a `tokenizers` JSON when one is loaded,
 else with the byte tokenizer (krunch_amd/tokenizer.py); `compress` /
 `decompress` write and read the `.krunch` container (cli.py:49-118,
 chunking.py) with CRC32, length and codec checks.
+
+Without a counterpart: `score_tokens_batched` gives each token's log
+probability, the entropies and the most likely tokens, `estimate` the size
+that `compress` would come to, both from the forward alone.
 """
 from __future__ import annotations
 
 import os
 import struct
 import zlib
-from typing import List, Optional, Sequence, Tuple
+from typing import List, NamedTuple, Optional, Sequence, Tuple
 
 import numpy as np
 import torch
@@ -146,6 +150,24 @@ def plan_windows(lens: np.ndarray, window: int) -> List[Tuple[int, int, int]]:
         plan.append((cuts[prev[j]], cuts[j], alive[prev[j]]))
         j = prev[j]
     return plan[::-1]
+
+
+class TokenScores(NamedTuple):
+    """Scores of one stream of n tokens, in nats (krunch_ac_hip.token_scores)."""
+    logprob: np.ndarray        # float32 [n], of each token given those before it
+    entropy: np.ndarray        # float32 [n]
+    top_logprob: np.ndarray    # float32 [n, n_top]
+    top_token: np.ndarray      # int32 [n, n_top]
+
+
+def coder_bits(logprob: np.ndarray, V: int) -> float:
+    """Bits the coder spends on tokens of these log probabilities: a token of
+    probability p has floor(p (2^24 - V)) + 1 of the CDF's 2^24 counts (the most
+    likely token of a row also what these leave of 2^24, which is not counted
+    here)."""
+    total = 1 << CDF_PRECISION
+    counts = np.floor(np.exp(logprob.astype(np.float64)) * (total - V)) + 1
+    return float((CDF_PRECISION - np.log2(counts)).sum())
 
 
 class InferenceEngine:
@@ -305,6 +327,53 @@ class InferenceEngine:
                       host[b * per_cap:b * per_cap + n].tobytes())
         return res
 
+    # ----------------------------------------------------------------- score
+    def score_tokens_batched(self, token_streams: Sequence[np.ndarray],
+                             n_top: int = 0) -> List[TokenScores]:
+        """Each stream's tokens scored given those before them (BOS first), in
+        the windows that compress_tokens_batched would run, without the coder."""
+        assert self._ready, "call load() first"
+        B = len(token_streams)
+        if B == 0:
+            return []
+        lens = np.array([len(t) for t in token_streams], dtype=np.int64)
+        if (lens < 1).any():
+            raise ValueError("stream has no tokens")
+        cap = compute_compress_batch(B)
+        if B > cap:
+            res: List[TokenScores] = []
+            for i in range(0, B, cap):
+                res += self.score_tokens_batched(token_streams[i:i + cap], n_top)
+            return res
+        W = self._weights
+        P = W["prepared"]
+        order = np.argsort(-lens, kind="stable")      # longest first, as in compress
+        lens = lens[order]
+        tgt = np.full((B, int(lens[0])), -1, dtype=np.int32)
+        for b, i in enumerate(order):
+            tgt[b, :lens[b]] = np.asarray(token_streams[i], dtype=np.int32)
+        live = np.arange(tgt.shape[1]) < lens[:, None]
+        if tgt[live].min() < 0 or tgt.max() >= P.V:
+            raise ValueError(f"token id out of range [0, {P.V})")
+        inp = np.full_like(tgt, BOS_TOKEN)
+        inp[:, 1:] = np.maximum(tgt[:, :-1], 0)
+        tgt_d, inp_d = torch.from_numpy(tgt).to(P.device), torch.from_numpy(inp).to(P.device)
+        state = State(P.n_layer, B, P.C, P.device)
+        parts = []
+        for w0, w1, n in plan_windows(lens, self.window):
+            if n < state.B:
+                state = state.first(n)
+            parts.append(cpp_path._score_window(W, inp_d[:n, w0:w1].contiguous(),
+                                                tgt_d[:n, w0:w1].contiguous(), state, n_top,
+                                                HEAD_ROWS))
+        parts = [[t.cpu().numpy() for t in part] for part in parts]
+        out: List[Optional[TokenScores]] = [None] * B
+        for b, i in enumerate(order):
+            cols = [np.concatenate(c)[:lens[b]] for c in
+                    zip(*([t[b] for t in part] for part in parts if b < len(part[0])))]
+            out[i] = TokenScores(*cols)
+        return out
+
     # ------------------------------------------------------------ decompress
     def decompress_tokens_batched(self, encoded_chunks: Sequence[bytes]) -> List[np.ndarray]:
         """Chunk payloads -> token streams, decoded in lockstep in calls of at
@@ -401,6 +470,24 @@ class InferenceEngine:
         crc = zlib.crc32(raw) & 0xFFFFFFFF
         return encode_header(len(raw), n, crc, model_id=self.model_id,
                              tokenizer_id=self.tokenizer_id) + b"".join(entries)
+
+    def estimate(self, raw: bytes, chunk_size: Optional[int] = None) -> int:
+        """The size of compress(raw)'s blob, from the tokens' scores: header,
+        entries and, per chunk, its mini-header and coder_bits. Within a few
+        parts in a thousand of the blob (the coder's rounding, and the most likely
+        tokens' extra counts)."""
+        self._need_tokenizer()
+        from krunch_amd import chunking
+
+        def payloads(chunks):
+            toks = [self._tokenizer.encode_bytes(c) for c in chunks]
+            V = self._weights["prepared"].V
+            return [bytes(8 + int(-(-coder_bits(s.logprob, V) // 8)))
+                    for s in self.score_tokens_batched(toks)]
+
+        entries, _ = chunking.compress_all(raw, lambda c: payloads([c])[0], neural_batch_fn=payloads,
+                                           chunk_size=chunk_size)
+        return HEADER_SIZE + sum(len(e) for e in entries)
 
     def decompress(self, blob: bytes) -> bytes:
         """.krunch blob -> bytes, all chunks decoded in lockstep; checks the

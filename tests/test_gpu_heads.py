@@ -215,3 +215,26 @@ def test_nothing_to_do_another_stream_and_a_graph(B, T, H):
         torch.cuda.synchronize()
         for i in range(2):
             assert torch.equal(outs[i], eager) and torch.equal(Sg[i], Se)
+
+
+def test_refusals():
+    B, T, H, D = 2, 5, 2, 64
+    r, k, v, w, u, S = make(B, T, H, D, 1)
+    before = S.clone()
+    lens = torch.tensor([1, 2], dtype=torch.int32, device=DEV)
+    wide = torch.zeros(B, T + 1, H, D, dtype=torch.float16, device=DEV)[:, :T]
+    for args in ((r.float(), k, v, w, u, S), (r, k[:1], v, w, u, S), (r, k, v.cpu(), w, u, S), (r[0], k, v, w, u, S),
+                 (r[..., :32], k[..., :32], v[..., :32], w, u, S), (wide, k, v, w, u, S),
+                 (r.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), w, u, S), (r, k, v, w[:1], u, S),
+                 (r, k, v, w, u.double(), S), (r, k, v, w, u, S[:1]), (r, k, v, w, u, S.half()),
+                 (r, k, v, w, u, S.transpose(2, 3)), (r, k, v, w, u, S, lens[:1]), (r, k, v, w, u, S, lens.long()),
+                 (r[:, :1].expand(B, T, H, D), k, v, w, u, S)):
+        with pytest.raises(RuntimeError):
+            ops.wkv_heads(*args)
+    assert torch.equal(S, before)
+
+
+def test_a_long_prompt():
+    """Many segments of the time axis, sums over thousands of tokens."""
+    r, k, v, w, u, S = make(1, 5000, 2, 64, 14)
+    check(r, k, v, w, u, S)

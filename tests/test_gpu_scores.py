@@ -207,3 +207,13 @@ def test_no_rows_another_stream_and_a_graph():
         eager = ops.token_scores(y, tok, 6)
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(eager, out))
+
+
+def test_refusals():
+    x, tok = rand(4, 100, torch.float16, 1)
+    bad = [(x.bfloat16(), tok, 0), (x.t(), tok, 0), (x.reshape(-1), tok, 0), (x[:1].expand(4, 100), tok, 0),
+           (x, tok[:3], 0), (x, tok.long(), 0), (x, tok.cpu(), 0), (x, tok[None], 0), (x, tok, 33), (x, tok, -1),
+           (x[:, :3], tok, 4), (x[:, :0], tok, 0), (x.repeat(2, 1)[::2, ::2], tok, 0)]
+    for args in bad:
+        with pytest.raises(RuntimeError):
+            ops.token_scores(*args)

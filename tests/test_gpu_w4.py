@@ -199,3 +199,37 @@ def test_no_rows_another_stream_and_a_graph():
         eager = ops.det_matmul_w4(y, w)
         torch.cuda.synchronize()
         assert torch.equal(out, eager)
+
+
+def test_refusals():
+    W = make(768, 40, 1).to(DEV)
+    w = ops.quantize_w4(W)
+    x = make(3, 768, 2, 1.0).to(DEV)
+    res = torch.zeros(3, 40, dtype=torch.float16, device=DEV)
+    for args in ((W[:40],), (W.float(),), (W[0],), (W, 16), (W[:, :0],), (W[:, :1].expand(768, 5),)):
+        with pytest.raises(RuntimeError):
+            ops.quantize_w4(*args)
+    W4 = ops.W4
+    for args in ((x.float(), w), (x[0], w), (x[:, :736], w), (x[:, 1:], w), (x[:1].expand(3, 768), w),
+                 (make(3, 1536, 2).to(DEV)[:, ::2], w), (x, w, torch.bfloat16), (x, w, None, "tanh"),
+                 (x, w, torch.float32, "relu2"), (x, w, None, "residual"), (x, w, None, "none", res),
+                 (x, w, None, "gated", res), (x, w, None, "residual", res[:2]), (x, w, None, "residual", res.float()),
+                 (x, W4(w.q[:-1], w.scales, 768, 40, 64)), (x, W4(w.q, w.scales[1:], 768, 40, 64)),
+                 (x, W4(w.q, w.scales, 768, 56, 64)), (x, W4(w.q, w.scales, 768, 40, 32)),
+                 (x, W4(w.q.cpu(), w.scales, 768, 40, 64)), (x, W4(w.q.float(), w.scales, 768, 40, 64))):
+        with pytest.raises(RuntimeError):
+            ops.det_matmul_w4(*args)
+
+
+def test_offsets_past_32_bits():
+    """x rows and out rows that start more than 2^31 elements after the first."""
+    from krunch_amd import _lib
+    K, N, ld = 64, 48, 2 ** 30 + 8
+    w = ops.quantize_w4(make(K, N, 1).to(DEV), 32)
+    x = make(3, K, 2, 1.0).to(DEV)
+    wide = torch.empty(2 * ld + K, dtype=torch.float16, device=DEV).as_strided((3, K), (ld, 1))
+    wide.copy_(x)
+    out = torch.empty(2 * ld + N, dtype=torch.float16, device=DEV).as_strided((3, N), (ld, 1))
+    _lib.call("kr_det_matmul_w4", wide.data_ptr(), ld, 3, K, w.q.data_ptr(), w.scales.data_ptr(), 32, N,
+              out.data_ptr(), ld, 1, None, None, _lib.stream_ptr())
+    assert torch.equal(out.contiguous(), ops.det_matmul_w4(x, w))
