@@ -116,7 +116,7 @@ int kr_softmax_probs(const uint16_t* logits, int N, int V, long long ld, float* 
 
 /* Scores of tokens, for callers that want a text's cost or a model's next
  * tokens without a coder (no reference counterpart): per row of logits (fp16,
- * or fp32 with logits_f32; any row stride ld >= V, any V), in nats,
+ * or fp32 with logits_f32; any row stride ld >= V; V <= 2^30, N <= 2^24), in nats,
  *   logprob[row]  = ln softmax(row)[tokens[row]]; 0 where tokens[row] = -1 (a
  *                   row without a token), NaN for any other id outside 0..V-1;
  *   entropy[row]  = -sum p ln p;
@@ -256,7 +256,7 @@ typedef struct kr_layer_q8 {
  * weight = q * s. kr_quantize_w4 makes them from W [K, N] fp16 (element (k, n)
  * at W[k * ldk + n * ldn], so either orientation): s = fp16(max |w| / 7), q =
  * w / s to the nearest integer, ties to even, at most 7 in size, 0 where s is
- * 0; a group with an infinity or NaN gets a NaN scale. K % 32 == 0, any N.
+ * 0; a group with an infinity or NaN gets a NaN scale. K % 32 == 0, K <= 2^20, any N.
  * q holds kr_w4_bytes(N, K) bytes, 16-byte aligned: blocks of 16 outputs x 128
  * inputs, 1 KB, outputs major; lane l of a block holds four 32-bit words, word
  * c the inputs 32 c + 8 (l / 16) + e of output l % 16 as nibbles q + 8, e = 0,
@@ -270,9 +270,10 @@ int kr_quantize_w4(const uint16_t* W, long long ldk, long long ldn, int N, int K
 /* out = epilogue(x [M, K] @ W) with W in 4 bits; epilogues, res and gate as
  * kr_det_matmul. x rows have stride ldx (a multiple of 8, x 16-byte aligned),
  * out rows any stride ldo >= N. Products q x are exact, their sums and the
- * scaling fp32: c_g = chain of v_mfma_f32_16x16x32_f16 over group g, P =
- * fma(s_g, c_g, P) over the groups of a 512-wide slice of K from zero, acc = P_0
- * + P_1 + ... left to right; so a row has the same bits for any M. */
+ * scaling fp32: c_g = chain of v_mfma_f32_16x16x32_f16 over group g, acc =
+ * fma(s_g, c_g, acc) over the groups in order from zero; so a row has the same
+ * bits for any M. A NaN scale makes its output NaN; infinite scales are not
+ * supported. M <= 2^19. out must not overlap x (out may be res). */
 int kr_det_matmul_w4(const uint16_t* x, long long ldx, int M, int K, const void* q,
                      const uint16_t* scales, int group, int N, void* out, long long ldo, int epilogue,
                      const uint16_t* res, const uint16_t* gate, void* stream);
@@ -398,9 +399,9 @@ int kr_wkv(int B, int T, int C, const float* decay, const float* first, const fl
  * 1: 64 tokens at a time on the matrix units, for prompts: equal to that up to
  * rounding, and in an order that depends on B * H and T (the time axis is split
  * over workgroups where heads are few). A NaN or infinity of a token then also
- * reaches y of up to 63 tokens before it. Calls of at most 8 tokens
- * are the same in both. ws: kr_wkv_heads_workspace_bytes (chunked only, may be
- * 0), 16-byte aligned, as r, k, v, state and y. */
+ * reaches y of up to 63 tokens before it. Calls of at most 8 tokens are the same
+ * in both. y must not overlap r, k or v. ws: kr_wkv_heads_workspace_bytes
+ * (chunked only, may be 0), 16-byte aligned, as r, k, v, state and y. */
 size_t kr_wkv_heads_workspace_bytes(int B, int T, int H, int D);
 int kr_wkv_heads(int B, int T, int H, int D, const uint16_t* r, long long ldr, const uint16_t* k,
                  long long ldk, const uint16_t* v, long long ldv, const float* decay,

@@ -184,6 +184,8 @@ def _score_window(weights, ids, tgt, state, n_top, head_rows):
     """score_packed_batched on checked device ids."""
     from krunch_amd import krunch_ac_hip
     P: Prepared = weights["prepared"]
+    if not 0 <= n_top <= min(krunch_ac_hip.TOP_TOKENS_MAX, P.V):   # before the state moves
+        raise ValueError(f"n_top must be in 0..{min(krunch_ac_hip.TOP_TOKENS_MAX, P.V)}, got {n_top}")
     B, T = ids.shape
     M = B * T
     x = torch.empty((M, P.C), dtype=torch.float16, device=P.device)

@@ -656,8 +656,8 @@ void launch_by_width(const ScoreArgs& g, hipStream_t s) {
 extern "C" int kr_token_scores(const void* logits, int logits_f32, int N, int V, long long ld,
                                const int32_t* tokens, float* logprob, float* entropy, int n_top,
                                float* top_logprob, int32_t* top_token, void* stream) {
-    KR_REQUIRE(N >= 0, "kr_token_scores: N=%d", N);
-    KR_REQUIRE(V >= 1 && ld >= V, "kr_token_scores: V=%d, ld=%lld", V, ld);
+    KR_REQUIRE(N >= 0 && N <= 1 << 24, "kr_token_scores: N=%d must be in 0..%d", N, 1 << 24);
+    KR_REQUIRE(V >= 1 && V <= 1 << 30 && ld >= V, "kr_token_scores: V=%d, ld=%lld", V, ld);
     KR_REQUIRE(n_top >= 0 && n_top <= kMaxTop && n_top <= V,
                "kr_token_scores: n_top=%d must be in 0..%d and at most V=%d", n_top, kMaxTop, V);
     if (N == 0) return KR_OK;

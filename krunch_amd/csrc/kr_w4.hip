@@ -163,9 +163,9 @@ int launch_rows(const W4Args& g, hipStream_t s) {
     // 1024 tiles are a wave for each SIMD without a split
     if (blocks > 1 && tiles < 1024) {
         const int waves = blocks < kMaxSplit ? blocks : kMaxSplit;
-        const int groups = (g.o.K + 32 * GS - 1) / (32 * GS);
         const int a_group = 64 * g.o.M + 32;                       // bytes of LDS
-        const int turns = (groups * a_group + 65535) / 65536;
+        const int most = 65536 / (a_group * (4 / GS));             // blocks at a time
+        const int turns = (blocks + most - 1) / most;
         const int room = (blocks + turns - 1) / turns * (4 / GS);
         w4_rows_kernel<GS, EP, true><<<tiles, 64 * waves, (size_t)room * a_group, s>>>(g, room);
     } else {
@@ -296,10 +296,11 @@ __global__ void __launch_bounds__(64 * kHeldWaves, kHeldWaves / 4) w4_held_kerne
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l16 = lane & 15, q4 = lane >> 4;
-    // workgroups of one range of outputs are 8 apart: on one XCD, whose L2 then
-    // has the weights for all of them
+    // with ranges of outputs in eights, the workgroups of one are 8 apart: on one XCD,
+    // whose L2 then has the weights for all of them
     const int row_tiles = (g.o.M + 16 * MT - 1) / (16 * MT);
-    const int range = blockIdx.x % 8 + blockIdx.x / 8 / row_tiles * 8, m0 = blockIdx.x / 8 % row_tiles * 16 * MT;
+    const int range = ranges % 8 ? blockIdx.x % ranges : blockIdx.x % 8 + blockIdx.x / 8 / row_tiles * 8;
+    const int m0 = (ranges % 8 ? blockIdx.x / ranges : blockIdx.x / 8 % row_tiles) * 16 * MT;
     const int kb_all = (g.o.K + kBlockK - 1) / kBlockK, groups = (g.o.K + 32 * GS - 1) / (32 * GS);
     const int tiles = g.n16 / 16, units = (tiles + NT - 1) / NT;
     for (int i = tid; i < 16 * MT * kb_all * 16; i += 64 * kHeldWaves) {
@@ -316,7 +317,7 @@ __global__ void __launch_bounds__(64 * kHeldWaves, kHeldWaves / 4) w4_held_kerne
     for (int s = 0; s < 4; s++) xl[s] = xs + l16 * 16 + ((4 * s + q4) ^ l16);
     const int step = ranges * kHeldWaves;
     int unit = range + ranges * wave;
-    if (range >= ranges || unit >= units) return;
+    if (unit >= units) return;
 
     // blocks in flight: next_unit, next_kb is the first not yet asked for
     kr_int4 w[kAhead][NT];
@@ -423,11 +424,12 @@ template <int NT, int MT, int GS, int EP, int kAhead, int kHeldWaves>
 int launch_held(const W4Args& g, hipStream_t s) {
     const int row_tiles = (g.o.M + 16 * MT - 1) / (16 * MT);
     const int units = (g.n16 / 16 + NT - 1) / NT;
+    // one workgroup a CU; in eights where that leaves out few of them
+    int ranges = row_tiles < 256 ? 256 / row_tiles : 1;
     const int most = (units + kHeldWaves - 1) / kHeldWaves;
-    int ranges = (256 + row_tiles - 1) / row_tiles;
     if (ranges > most) ranges = most;
-    w4_held_kernel<NT, MT, GS, EP, kAhead, kHeldWaves>
-        <<<(ranges + 7) / 8 * 8 * row_tiles, 64 * kHeldWaves, 0, s>>>(g, ranges);
+    if (16 * (ranges / 8 * 8) >= 15 * ranges) ranges = ranges / 8 * 8;
+    w4_held_kernel<NT, MT, GS, EP, kAhead, kHeldWaves><<<ranges * row_tiles, 64 * kHeldWaves, 0, s>>>(g, ranges);
     KR_LAUNCHED();
     return KR_OK;
 }
@@ -504,7 +506,8 @@ __global__ void __launch_bounds__(256) w4_quantize_kernel(const kr_half* __restr
 
 int check_w4(const char* who, int N, int K, int group) {
     KR_REQUIRE(N >= 1 && N <= (1 << 30), "%s: N=%d", who, N);
-    KR_REQUIRE(K >= 32 && K % 32 == 0 && K <= (1 << 24), "%s: K=%d must be a multiple of 32", who, K);
+    KR_REQUIRE(K >= 32 && K % 32 == 0 && K <= (1 << 20), "%s: K=%d must be a multiple of 32 up to %d", who, K,
+               1 << 20);
     KR_REQUIRE(group == 32 || group == 64 || group == 128, "%s: group=%d must be 32, 64 or 128", who,
                group);
     return KR_OK;

@@ -349,11 +349,12 @@ def det_matmul_w4(x, W: W4, out_dtype=None, epilogue: str = "none", res=None, ga
     epilogue in EPILOGUES_W4 or _refuse(f"epilogue must be one of {sorted(EPILOGUES_W4)}")
     f32 and epilogue != "none" and _refuse("an epilogue's output is float16")
     code = 0 if f32 else EPILOGUES_W4[epilogue]
-    for t, name, need in ((res, "res", code >= 4), (gate, "gate", code == 5)):
-        (t is not None) == need or _refuse(f"epilogue {epilogue} takes {'a' if need else 'no'} {name}")
-        if need:
-            _cuda(t, torch.float16, name)
-            (t.shape == (M, N) and t.get_device() == dev) or _refuse(f"{name} must be [{M}, {N}]")
+    if code >= 4 or res is not None or gate is not None:
+        for t, name, need in ((res, "res", code >= 4), (gate, "gate", code == 5)):
+            (t is not None) == need or _refuse(f"epilogue {epilogue} takes {'a' if need else 'no'} {name}")
+            if need:
+                _cuda(t, torch.float16, name)
+                (t.shape == (M, N) and t.get_device() == dev) or _refuse(f"{name} must be [{M}, {N}]")
     if _elsewhere(x):
         return _on_device_of(x, det_matmul_w4, x, W, out_dtype, epilogue, res, gate)
     out = x.new_empty((M, N), dtype=torch.float32) if f32 else x.new_empty((M, N))

@@ -47,9 +47,14 @@ def test_scores_are_those_of_the_packed_logits(small):
     assert (got[0][1, 40:] == 0).all()
     empty = cpp_path.score_packed_batched(W, ids[:, :0], tgt[:, :0], st, 2)
     assert [tuple(c.shape) for c in empty] == [(B, 0), (B, 0), (B, 0, 2), (B, 0, 2)]
+    before = st.buf.clone()
     for bad in ((ids, tgt[:, 1:]), (ids + V, tgt), (ids, tgt - 2)):
         with pytest.raises(ValueError):
             cpp_path.score_packed_batched(W, *bad, st)
+    for n in (-1, 33):
+        with pytest.raises(ValueError):
+            cpp_path.score_packed_batched(W, ids, tgt, st, n)
+    assert torch.equal(st.buf, before)
 
 
 def test_ragged_streams_over_windows(small):

@@ -95,7 +95,8 @@ def check(x, w, out_dtype=torch.float16):
 @pytest.mark.parametrize("group", [32, 64, 128])
 @pytest.mark.parametrize("M,K,N", [(1, 32, 1), (3, 96, 15), (1, 160, 17), (16, 512, 48), (17, 544, 33),
                                    (1, 768, 768), (32, 768, 100), (33, 1056, 64), (65, 768, 2100),
-                                   (7, 4096, 70), (130, 1024, 1000), (257, 288, 523)])
+                                   (7, 4096, 70), (130, 1024, 1000), (257, 288, 523), (16, 1984, 48),
+                                   (15, 2080, 100), (16, 8192, 20), (3, 5152, 25000)])
 def test_products(M, K, N, group):
     w = ops.quantize_w4(make(K, N, M + K + N).to(DEV), group)
     x = make(M, K, 7 * M + K, 1.0).to(DEV)
@@ -136,6 +137,18 @@ def test_epilogues(M, N):
     got = ops.det_matmul_w4(x, w, epilogue="sigmoid").double()
     ref = torch.sigmoid(h.double())
     assert ((got - ref).abs() <= 2.0 ** -11 * ref * (1 + 2.0 ** -8) + 2.0 ** -25).all()
+
+
+@pytest.mark.parametrize("M,K,N", [(200, 768, 16400), (800, 256, 12333), (1000, 1280, 8200), (333, 1312, 16384),
+                                   (700, 2560, 8192), (5000, 128, 9000), (20000, 96, 1030)])
+def test_many_rows(M, K, N):
+    """Around the lines between tiles and held rows: the rows of a call of 48."""
+    w = ops.quantize_w4(make(K, N, 5).to(DEV), 64)
+    x = make(M, K, 6, 1.0).to(DEV)
+    full = ops.det_matmul_w4(x, w)
+    for m in (0, M // 2, M - 48):
+        assert torch.equal(ops.det_matmul_w4(x[m:m + 48], w), full[m:m + 48]), m
+    check(x[:48], w)
 
 
 def test_all_values_of_a_nibble():

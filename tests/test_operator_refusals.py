@@ -25,7 +25,9 @@ def scores(logits=PTR, f32=0, N=2, V=10, ld=10, tokens=PTR, lp=PTR, h=PTR, top=0
 def test_token_scores():
     assert scores(N=0) == 0 and scores(N=0, logits=None) == 0
     refused(scores(N=-1), "N=-1")
+    refused(scores(N=(1 << 24) + 1), "N=16777217")
     refused(scores(V=0), "V=0")
+    refused(scores(V=(1 << 30) + 1, ld=1 << 31), "V=1073741825")
     refused(scores(ld=9), "ld=9")
     refused(scores(top=-1), "n_top=-1")
     refused(scores(V=100, ld=100, top=33), "n_top=33")
@@ -45,6 +47,7 @@ def w4(x=PTR, ldx=64, M=2, K=64, q=PTR, s=PTR, group=64, N=8, out=PTR, ldo=8, ep
 def test_products():
     assert w4(M=0) == 0
     for kw, text in (({"K": 48, "ldx": 48}, "K=48"), ({"K": 0}, "K=0"), ({"N": 0}, "N=0"), ({"M": -1}, "M=-1"),
+                     ({"K": (1 << 20) + 32, "ldx": 1 << 21}, "K=1048608"),
                      ({"M": 1 << 20}, "M=1048576"), ({"group": 16}, "group=16"), ({"group": 0}, "group=0"),
                      ({"ldx": 56}, "ldx=56"), ({"ldx": 68}, "ldx=68"), ({"ldo": 7}, "ldo=7"), ({"ep": 6}, "epilogue"),
                      ({"ep": -1}, "epilogue"), ({"ep": 4}, "needs res"), ({"ep": 5, "res": PTR}, "needs gate"),
