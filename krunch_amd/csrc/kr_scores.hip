@@ -209,16 +209,16 @@ scores_kernel(ScoreArgs g) {
     // U chunks of the thread from chunk c0 + lane on, TH apart. fp16 rows that start
     // in the middle of a 4-byte word are read by the words around: reads of 16 bytes
     // run at full speed from any 4-byte boundary, and 26% slower over rows of which
-    // half have none (8192 x 50277 held in registers: 165 us, 209).
+    // half have none (8192 x 50277 held in registers: 165 us, 209). The last element
+    // is read by itself: the word that it begins may end behind the row.
     auto read_block = [&](int c0, kr_int4 (&raw)[U], auto odd_row) {
         constexpr bool ODD = decltype(odd_row)::value;
-        int next[U];
+        uint32_t next[U];
         #pragma unroll
         for (int u = 0; u < U; u++) {
-            const int* words =
-                reinterpret_cast<const int*>(x + chunk_start(c0 + u * TH + lane) - (ODD ? 1 : 0));
-            raw[u] = *reinterpret_cast<const int4_any*>(words);
-            if (ODD) next[u] = words[4];
+            const T* at = x + chunk_start(c0 + u * TH + lane);
+            raw[u] = *reinterpret_cast<const int4_any*>(at - (ODD ? 1 : 0));
+            if (ODD) next[u] = reinterpret_cast<const uint16_t*>(at)[7];
         }
         if (ODD) {
             #pragma unroll
@@ -226,7 +226,7 @@ scores_kernel(ScoreArgs g) {
                 #pragma unroll
                 for (int j = 0; j < 4; j++)
                     raw[u][j] = (int)__builtin_amdgcn_alignbit(
-                        (uint32_t)(j < 3 ? raw[u][j + 1] : next[u]), (uint32_t)raw[u][j], 16);
+                        j < 3 ? (uint32_t)raw[u][j + 1] : next[u], (uint32_t)raw[u][j], 16);
         }
         if ((c0 + (U - 1) * TH + 64) * CH > V) {
             #pragma unroll
@@ -272,14 +272,8 @@ scores_kernel(ScoreArgs g) {
     kr_int4 raw[U];
     if constexpr (W == 1) {
         // the whole row is one block of its wave
-        if (V < CH) {
-            #pragma unroll
-            for (int u = 0; u < U; u++) raw[u] = read_short(x, (u * TH + lane) * CH, V);
-        } else if (is_odd) {
-            read_block(0, raw, odd);
-        } else {
-            read_block(0, raw, even);
-        }
+        if (is_odd) read_block(0, raw, odd);
+        else read_block(0, raw, even);
         #pragma unroll
         for (int u = 0; u < U; u++) m = fmaxf(m, chunk_max<T>(raw[u]));
     } else {
@@ -343,7 +337,7 @@ scores_kernel(ScoreArgs g) {
             for (int u = 0; u < U; u++) {
                 if (!__any(chunk_max<T>(raw[u]) >= th)) continue;
                 const vec v = __builtin_bit_cast(vec, raw[u]);
-                const int start = V < CH ? lane * CH : chunk_start(u * TH + lane);
+                const int start = chunk_start(u * TH + lane);
                 #pragma unroll
                 for (int e = 0; e < CH; e++) {
                     const float xe = (float)v[e];
@@ -461,7 +455,7 @@ scores_kernel(ScoreArgs g) {
 // Short rows: 16 lanes have a row, so a wave's reductions and sort serve four. U
 // chunks of 16 bytes per lane, in registers; n_top <= 8, T the n_top-th largest of
 // the 16 lanes' maxima. Rows of one wave may start at different halves of a word, so
-// fp16 is always read as five words and shifted by 0 or 16 bits.
+// fp16 is always read as four words and the last element, shifted by 0 or 16 bits.
 // Bound: issue (the wave's reductions, sort and lists); 16 rows a workgroup.
 constexpr int kShortChunks = 24, kShortList = 64;      // with candidates, and candidates, of a row
 
@@ -492,12 +486,12 @@ __global__ void __launch_bounds__(256, 8) scores_short_kernel(ScoreArgs g) {
         for (int u = 0; u < U; u++) raw[u] = read_short(x, (u * 16 + l) * CH, V);
     } else {
         const int odd = sizeof(T) == 2 ? (int)((uintptr_t)x >> 1 & 1) : 0;
-        int next[U];
+        uint32_t next[U];
         #pragma unroll
         for (int u = 0; u < U; u++) {
-            const int* words = reinterpret_cast<const int*>(x + chunk_start(u) - odd);
-            raw[u] = *reinterpret_cast<const int4_any*>(words);
-            if (sizeof(T) == 2) next[u] = words[3 + odd];
+            const T* at = x + chunk_start(u);
+            raw[u] = *reinterpret_cast<const int4_any*>(at - odd);
+            if (sizeof(T) == 2) next[u] = reinterpret_cast<const uint16_t*>(at)[7];
         }
         #pragma unroll
         for (int u = 0; u < U; u++) {
@@ -505,7 +499,7 @@ __global__ void __launch_bounds__(256, 8) scores_short_kernel(ScoreArgs g) {
                 #pragma unroll
                 for (int j = 0; j < 4; j++)
                     raw[u][j] = (int)__builtin_amdgcn_alignbit(
-                        (uint32_t)(j < 3 ? raw[u][j + 1] : next[u]), (uint32_t)raw[u][j], 16 * odd);
+                        j < 3 ? (uint32_t)raw[u][j + 1] : next[u], (uint32_t)raw[u][j], 16 * odd);
             }
             if ((u + 1) * 16 * CH > V) raw[u] = without_first<T>(raw[u], (u * 16 + l) * CH - chunk_start(u));
         }
@@ -569,7 +563,6 @@ __global__ void __launch_bounds__(256, 8) scores_short_kernel(ScoreArgs g) {
         }
         row_sync<1>();
         const int chunks = hits[slot];
-        int kept = 0;
         if (chunks <= kShortChunks) {
             for (int i = l; i < chunks * CH; i += 16) {
                 const float v = (float)reinterpret_cast<const T*>(hit_chunk[slot])[i];
@@ -592,11 +585,10 @@ __global__ void __launch_bounds__(256, 8) scores_short_kernel(ScoreArgs g) {
                 if (rank < g.n_top) best[slot][rank] = k;
             }
             row_sync<1>();
-            kept = g.n_top;
         } else {
             // one after the other, each the largest below the one before
             uint64_t last = ~0ull;
-            for (; kept < g.n_top; kept++) {
+            for (int kept = 0; kept < g.n_top; kept++) {
                 uint64_t k = 0;
                 #pragma unroll 1
                 for (int i = l; i < V; i += 16) {
@@ -639,12 +631,20 @@ void launch(const ScoreArgs& g, hipStream_t s) {
     else scores_kernel<T, W, U, false><<<grid, threads, 0, s>>>(g);
 }
 
+// Threads by the length of a row, which alone (with n_top) also fixes its order of
+// sums. us on MI355X:
+//   to 512, n_top <= 8: 16 lanes a row. 100000 x 256 fp32, 3 top 22, by a wave 55;
+//     fp16, 8 top 26 and 67. More top tokens need the wave's 64 maxima.
+//   to 64 CH: a wave with one chunk a lane, here for n_top > 8 only: 100000 x 256
+//     fp16, 20 top 95, with four 127; 100000 x 512 93 and 126.
+//   to 256 CH: a wave with four chunks a lane, the row in registers.
+//   to 1024 CH, 4096 CH and above: 2, 4 and 8 waves that walk the row.
 template <typename T>
 void launch_by_width(const ScoreArgs& g, hipStream_t s) {
     constexpr int CH = Chunk<T>::n;
     if (g.V <= 256 && g.n_top <= 8) launch_short<T, 16 / CH>(g, s);
     else if (g.V <= 512 && g.n_top <= 8) launch_short<T, 32 / CH>(g, s);
-    else if (g.V <= 64 * CH) launch<T, 1, 1>(g, s);
+    else if (g.V <= 64 * CH) scores_kernel<T, 1, 1, true><<<(g.N - 1) / 4 + 1, 256, 0, s>>>(g);
     else if (g.V <= 256 * CH) launch<T, 1, 4>(g, s);
     else if (g.V <= 1024 * CH) launch<T, 2, 4>(g, s);
     else if (g.V <= 4096 * CH) launch<T, 4, 4>(g, s);
