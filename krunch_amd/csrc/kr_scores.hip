@@ -15,9 +15,10 @@
 // maxima, has at least n_top elements >= T and few more where the logits are
 // spread over the groups (64: lanes, so 8 neighbouring tokens, then every 512th).
 // Threads with a maximum >= T, few, are listed and their chunks read again (from
-// the L2; a row of one wave has them in registers), and each element >= T counts how many are before it (larger, or
-// equal with a lower index): that is its rank. A row with more of them than there
-// is room for (long ties) takes its n_top largest one by one instead.
+// the L2; a row of one wave has them in registers), and each element >= T counts
+// how many are before it (larger, or equal with a lower index): that is its rank. A
+// row with more of them than there is room for (long ties) takes its n_top largest
+// one by one instead.
 #include "kr_common.h"
 #include "kr_wave.h"
 #include "krunch_hip.h"
@@ -182,6 +183,10 @@ __device__ __forceinline__ void row_sync() {
 
 // W waves per row, U chunks of 16 bytes per thread at a time; four rows a workgroup
 // with W = 1, else one.
+// Bound: memory with many rows (8192 x 50277 fp16 149 us, with 8 top 155: 5.5 and 5.3
+// TB/s, fp32 270: 6.1; holding rows in registers and sums made anew after the
+// maximum 165, one row per 16 waves 156); latency with few: one row of 50277 6.0 us, 8.1 with
+// 8 top, of which 3.6 is any launch's; a further 2 us are T, the list and the ranks.
 template <typename T, int W, int U, bool TOP>
 __global__ void __launch_bounds__(W > 1 ? 64 * W : 256, 8)
 scores_kernel(ScoreArgs g) {
@@ -456,7 +461,8 @@ scores_kernel(ScoreArgs g) {
 // chunks of 16 bytes per lane, in registers; n_top <= 8, T the n_top-th largest of
 // the 16 lanes' maxima. Rows of one wave may start at different halves of a word, so
 // fp16 is always read as four words and the last element, shifted by 0 or 16 bits.
-// Bound: issue (the wave's reductions, sort and lists); 16 rows a workgroup.
+// Bound: memory without top tokens (100000 x 512 fp32 36.6 us, 5.6 TB/s), issue with
+// them (3 top of 256 fp16: 12.6 us without, 22.5); 16 rows a workgroup.
 constexpr int kShortChunks = 24, kShortList = 64;      // with candidates, and candidates, of a row
 
 template <typename T, int U, bool TOP>
@@ -637,14 +643,19 @@ void launch(const ScoreArgs& g, hipStream_t s) {
 //     fp16, 8 top 26 and 67. More top tokens need the wave's 64 maxima.
 //   to 64 CH: a wave with one chunk a lane, here for n_top > 8 only: 100000 x 256
 //     fp16, 20 top 95, with four 127; 100000 x 512 93 and 126.
-//   to 256 CH: a wave with four chunks a lane, the row in registers.
-//   to 1024 CH, 4096 CH and above: 2, 4 and 8 waves that walk the row.
+//   to 128 CH, 256 CH: a wave with two, four chunks a lane, the row in registers.
+//     30000 x 1000 fp16 16.9 with two, 22.4 with four, 40 by two waves that walk it.
+//   to 1024 CH, 4096 CH and above: 2, 4 and 8 waves that walk the row. 2 / 4 / 8:
+//     10000 x 4000 fp16 18.0 / 29.4 / 52.2, 8000 x 8000 26.8 / 25.8 / 45.8, 4000 x 16000
+//     27.9 / 27.6 / 25.0, 8192 x 50277 154 / 147 / 140 (16 waves: 156), 300 x 50277
+//     20.3 / 12.9 / 11.9; fp32 8000 x 8000 47.5 / 46.4 / 41.7.
 template <typename T>
 void launch_by_width(const ScoreArgs& g, hipStream_t s) {
     constexpr int CH = Chunk<T>::n;
     if (g.V <= 256 && g.n_top <= 8) launch_short<T, 16 / CH>(g, s);
     else if (g.V <= 512 && g.n_top <= 8) launch_short<T, 32 / CH>(g, s);
     else if (g.V <= 64 * CH) scores_kernel<T, 1, 1, true><<<(g.N - 1) / 4 + 1, 256, 0, s>>>(g);
+    else if (g.V <= 128 * CH) launch<T, 1, 2>(g, s);
     else if (g.V <= 256 * CH) launch<T, 1, 4>(g, s);
     else if (g.V <= 1024 * CH) launch<T, 2, 4>(g, s);
     else if (g.V <= 4096 * CH) launch<T, 4, 4>(g, s);

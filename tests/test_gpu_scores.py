@@ -45,10 +45,11 @@ def plain(x, tokens, k):
 def check(x, tokens, k):
     lp, h, tl, tt = (a.cpu().numpy() for a in ops.token_scores(x, tokens, k))
     rlp, rh, rtl, rtt = plain(x, tokens, k)
-    # fp32 throughout. ln s: a thread's chain of at most 64 additions per
-    # segment, then 6 levels in the wave and 16 waves, and the exponents' last
-    # bits, under 128 * 2^-24 in all; x - m and the difference are rounded at
-    # their own size, at most 2^-22 of it together.
+    # fp32 throughout. ln s: a thread's chain of V / 512 additions (V / 64 below
+    # 2049, at most 64 otherwise up to V = 32768), 6 levels in the wave, 8 waves,
+    # and the exponents' last bits, under 128 * 2^-24 in all; at V = 151937, where
+    # the chain has 297, that takes the additions' errors to differ in sign. x - m
+    # and the difference are rounded at their own size, at most 2^-22 of it together.
     tol = lambda r: 2.0 ** -17 + 2.0 ** -22 * np.abs(np.where(np.isfinite(r), r, 0))
     for got, ref in ((lp, rlp), (tl, rtl)):
         assert np.array_equal(np.isnan(got), np.isnan(ref))
