@@ -287,6 +287,14 @@ int launch_tile(const W4Args& g, hipStream_t s) {
 // Rows held: a workgroup has all of K of 16 MT rows in LDS, zeros past K, and its
 // waves take units of 16 NT outputs one after another, each on its own: no barrier
 // after the rows are in. Weights come kAhead blocks ahead into registers.
+// Bound with 64 rows: the VALU's 3.6 operations a product (2 to unpack, shared by four
+// row tiles, 1 to scale) beside a matrix unit at 30%, the waits of three waves a SIMD
+// (43% of their time) and the last units of a range, which leave waves idle. Measured on
+// MI355X, 512 x 768 x 50277 at groups of 32 / 64 / 128: 76 / 62 / 49 us (0.81 PF/s at 128; the
+// rows of x held by 8 waves 53, through LDS a tile at a time 76), 2000 rows 250 / 204 /
+// 192. Rows of 50277 fp16 start anywhere in a line: 50272 takes 45 us. Stores without
+// bounds, with a quarter of the operations, change nothing (50).
+// Bound with 16 rows: latency, about 4.5 us beside what the weights take.
 constexpr int kHeldUnits = 163840 / 16;      // all of a CU's LDS: one workgroup each
 
 template <int NT, int MT, int GS, int EP, int kAhead, int kHeldWaves>
@@ -399,6 +407,8 @@ __global__ void __launch_bounds__(64 * kHeldWaves, kHeldWaves / 4) w4_held_kerne
                             #pragma unroll
                             for (int t = 0; t < MT; t++) y[i][t][r] = __builtin_fmaf(f, c[i][t][r], y[i][t][r]);
                         }
+                    // or the next group's x comes early and registers spill (2000 rows 220 us)
+                    if (GS == 2) __builtin_amdgcn_sched_barrier(0);
                 }
             }
         }
