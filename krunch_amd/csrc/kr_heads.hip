@@ -464,7 +464,7 @@ __global__ void __launch_bounds__(256) heads_join_kernel(HeadArgs g) {
     kr_float4* seg = reinterpret_cast<kr_float4*>(g.seg_state) + at;
     kr_float4 s = reinterpret_cast<const kr_float4*>(g.state)[at];
     seg[0] = s;
-    constexpr int kAhead = 8;             // or every step waits for memory
+    constexpr int kAhead = 8;             // or every step waits for memory (16: the same time)
     for (int i0 = 1; i0 < g.segments; i0 += kAhead) {
         kr_float4 add[kAhead];
         #pragma unroll
