@@ -238,3 +238,30 @@ def test_a_long_prompt():
     """Many segments of the time axis, sums over thousands of tokens."""
     r, k, v, w, u, S = make(1, 5000, 2, 64, 14)
     check(r, k, v, w, u, S)
+
+
+@pytest.mark.parametrize("chunked", [False, True])
+def test_offsets_past_32_bits(chunked):
+    """Token strides of 2^27 elements, and states of more than 2^31."""
+    B, T, H, D, ld = 1, 20, 2, 64, 1 << 27
+    r, k, v, w, u, S = make(B, T, H, D, 9)
+    wide = torch.empty(T * ld, dtype=torch.float16, device=DEV)
+    views = []
+    for i, x in enumerate((r, k, v)):
+        views.append(wide.as_strided((B, T, H, D), (T * ld, ld, D, 1), ld - (3 - i) * H * D))
+        views[-1].copy_(x)
+    S2 = S.clone()
+    assert torch.equal(ops.wkv_heads(*views, w, u, S2, chunked=chunked), ops.wkv_heads(r, k, v, w, u, S, chunked=chunked))
+    assert torch.equal(S, S2)
+    del wide, views
+    B, T, H, D = 8200, 9, 16, 128
+    r, k, v, w, u, S = make(2, T, H, D, 10)
+    big = torch.zeros(B, H, D, D, device=DEV)
+    assert big.numel() > 2 ** 31
+    big[-2:] = S
+    many = [torch.zeros(B, T, H, D, dtype=torch.float16, device=DEV) for _ in range(3)]
+    for m, x in zip(many, (r, k, v)):
+        m[-2:] = x
+    y = ops.wkv_heads(*many, w, u, big, chunked=chunked)
+    assert torch.equal(y[-2:], ops.wkv_heads(r, k, v, w, u, S, chunked=chunked))
+    assert torch.equal(big[-2:], S) and not y[:-2].any() and not big[:-2].any()
