@@ -185,7 +185,7 @@ def _on_device_of(t, op, *args):
 
 
 def _elsewhere(t):
-    return t.get_device() != torch.cuda.current_device()
+    return not _lib.is_current(t.get_device())
 
 
 TOP_TOKENS_MAX = 32

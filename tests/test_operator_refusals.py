@@ -124,7 +124,7 @@ def test_the_launch_goes_to_the_tensors_device(monkeypatch):
     t = torch.zeros(3)
     assert ops._on_device_of(t, lambda a, b: seen.append("run") or a + b, 1, 2) == 3
     assert seen == [t.device, "in", "run", "out"]
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    monkeypatch.setattr(_lib, "_get_device", lambda: 1)
     assert ops._elsewhere(t)             # a host tensor's index is -1
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: -1)
+    monkeypatch.setattr(_lib, "_get_device", lambda: -1)
     assert not ops._elsewhere(t)
