@@ -446,15 +446,15 @@ int launch_held(const W4Args& g, hipStream_t s) {
 
 // Kernel by the work there is, us on MI355X at groups of 32 / 64 / 128:
 //   up to 16 rows, fewer than 1536 tiles of 16 outputs: rows, else held (16 x 16).
-//     1 x 768 x 16384 rows 4.9 / 5.1 / 4.5, held 8.0 / 6.5 / 5.9; 1 x 768 x 32768
-//     9.5 / 10.2 / 8.8 and 8.2 / 6.9 / 6.3; 16 x 768 x 50277 16.5 / 16.7 / 15.6 and
-//     10.0 / 8.8 / 8.4.
+//     1 x 768 x 16384 rows 5.2 / 5.5 / 4.7, held 8.5 / 7.0 / 6.4; 1 x 768 x 32768
+//     9.6 / 10.3 / 8.6 and 8.8 / 7.4 / 6.8; 16 x 768 x 50277 17.1 / 17.1 / 15.9 and
+//     11.1 / 9.7 / 9.2.
 //   more rows: held with 64 rows, else with 32, where that gives each of the 12
 //     waves of 256 workgroups a unit of 32 outputs; else tiles. 512 x 768 x 16384
-//     (4096 units) 24.3 / 20.0 / 17.5, tiles 36 / 30 / 28; 512 x 768 x 8192 (2048
-//     units of 64 rows, 4096 of 32) held 64 18.7 / 16.2 / 14.4, held 32 15.3 / 12.5
-//     / 11.3, tiles 20 / 17 / 16; 128 x 768 x 16384 (2048 of 32) held 32 12.3 / 10.2
-//     / 9.3, tiles 11.1 / 9.3 / 9.2.
+//     (4096 units of 64 rows) held 64 26.3 / 20.4 / 18.2, held 32 29.1 / 22.5 / 20.2,
+//     tiles 34.7 / 29.5 / 25.7; 512 x 768 x 8192 (2048 units of 64 rows, 4096 of 32) held
+//     64 19.4 / 16.4 / 15.0, held 32 15.5 / 12.6 / 12.0, tiles 18.7 / 16.4 / 14.7; 128 x
+//     768 x 16384 (2048 of 32) held 32 13.1 / 11.4 / 10.7, tiles 11.4 / 10.0 / 9.2.
 template <int GS, int EP>
 int launch_by_rows(const W4Args& g, hipStream_t s) {
     if (g.o.M <= 16) {
