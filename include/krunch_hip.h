@@ -398,8 +398,13 @@ int kr_wkv(int B, int T, int C, const float* decay, const float* first, const fl
  * token in fp32; T tokens in one call have the bits of T calls of one. chunked =
  * 1: 64 tokens at a time on the matrix units, for prompts: equal to that up to
  * rounding, and in an order that depends on B * H and T (the time axis is split
- * over workgroups where heads are few). A NaN or infinity of a token then also
- * reaches y of up to 63 tokens before it. Calls of at most 8 tokens are the same
+ * over workgroups where heads are few); rounding is 2^-22 of a value that enters
+ * the matrix units (a state element, a weight r k' between two tokens, a decayed v)
+ * and 2^-38 of the largest one of its value channel's state column, its
+ * token's weights or its channel's v of the 64 tokens. A NaN or infinity of a token
+ * then also reaches y of up to 63 tokens before it, and an infinite state
+ * element makes y of its value channel infinite or NaN; other channels of the
+ * state keep their values and their y. Calls of at most 8 tokens are the same
  * in both. y must not overlap r, k or v. ws: kr_wkv_heads_workspace_bytes
  * (chunked only, may be 0), 16-byte aligned, as r, k, v, state and y. */
 size_t kr_wkv_heads_workspace_bytes(int B, int T, int H, int D);

@@ -11,7 +11,7 @@
 // r, k, v enter the matrix units as they are; the three fp32 quantities that do
 // too, (r k) e^.., e^.. v and S, go in as two fp16 parts, high and low, scaled by
 // a power of two to 2^14: 22 bits of each value, and 2^-38 of the largest
-// one of a row (r k), a column (v) or 16 columns (S).
+// one of a row (r k) or of a column (v, S).
 #include "kr_common.h"
 #include "kr_wave.h"
 #include "krunch_hip.h"
@@ -349,12 +349,14 @@ __global__ void __launch_bounds__(4 * D, D == 64 ? 3 : 2) heads_chunk_kernel(Hea
         #pragma unroll
         for (int s = 0; s < 2; s++) vc[s] = sh.vt[chan_unit(m, 4 * s + q4)];
         if (!SUM) {
+            // a scale for each column, so that an infinite or a huge one changes no other
             float big = 0.0f;
             #pragma unroll
             for (int s = 0; s < 2 * KS; s++)
                 #pragma unroll
                 for (int r = 0; r < 4; r++) big = fmaxf(big, fabsf(S[s][r]));
-            big = kr_wave_reduce(big, [](float x, float y) { return fmaxf(x, y); });
+            big = fmaxf(big, kr_xor<16>(big));
+            big = fmaxf(big, kr_xor<32>(big));
             float up, down;
             power_scale(big, up, down);
             kr_half8 s_hi[KS], s_lo[KS];
@@ -367,6 +369,9 @@ __global__ void __launch_bounds__(4 * D, D == 64 ? 3 : 2) heads_chunk_kernel(Hea
                     s_hi[s][e] = a;
                     s_lo[s][e] = b;
                 }
+            kr_float4 down_m;              // of the rows m that this lane has of y'
+            #pragma unroll
+            for (int r = 0; r < 4; r++) down_m[r] = __shfl(down, 4 * q4 + r);
             __builtin_amdgcn_sched_barrier(0);
             // y': rows m, columns i
             #pragma unroll
@@ -385,10 +390,10 @@ __global__ void __launch_bounds__(4 * D, D == 64 ? 3 : 2) heads_chunk_kernel(Hea
                     inside = __builtin_amdgcn_mfma_f32_16x16x32_f16(vc[s], sh.pl[at], inside, 0, 0, 0);
                 }
                 const int i = 16 * it + l16;
-                const float fs = down * y_dec[it], fp = sh.pdown[i];
+                const float fp = sh.pdown[i];
                 kr_half4 y;
                 #pragma unroll
-                for (int r = 0; r < 4; r++) y[r] = kr_f16(__builtin_fmaf(inside[r], fp, from_s[r] * fs));
+                for (int r = 0; r < 4; r++) y[r] = kr_f16(__builtin_fmaf(inside[r], fp, from_s[r] * (down_m[r] * y_dec[it])));
                 if (i < n)
                     *reinterpret_cast<kr_half4*>(yp + 16 * it * g.ldy) = y;
                 __builtin_amdgcn_sched_barrier(0);

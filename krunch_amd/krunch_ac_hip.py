@@ -370,8 +370,10 @@ def wkv_heads(r, k, v, decay, first, state, lens=None, chunked: bool = True):
     (u) fp32 [H], state fp32 [B, H, D, D] updated in place; returns y fp16
     [B, T, H, D]. lens int32 [B]: each stream's tokens (its state stops there, later
     rows of y are 0). chunked=True (prompts, scoring) takes 64 tokens at a time on
-    the matrix units; chunked=False, and calls of at most 8 tokens, go token by
-    token, and T tokens then have the bits of T calls, as a codec's two directions need."""
+    the matrix units: equal up to rounding for finite inputs (a NaN or infinity of a
+    token also reaches y of up to 63 tokens before it); chunked=False, and calls of
+    at most 8 tokens, go token by token, and T tokens then have the bits of T calls,
+    as a codec's two directions need."""
     r.dim() == 4 or _refuse("r must be [B, T, H, D]")
     shape = r.shape
     B, T, H, D = shape
