@@ -126,7 +126,9 @@ int kr_softmax_probs(const uint16_t* logits, int N, int V, long long ld, float* 
  * A logit of -inf is a masked token: probability 0, never among the top ones
  * (missing ones are -1 with -inf). A row of only masked tokens has logprob
  * -inf and entropy 0; a row with a NaN or +inf has NaN everywhere and top
- * tokens -1. Sums are fp32 in an order that does not depend on N. These are
+ * tokens -1. Sums are fp32 in an order that does not depend on N; ln of a row's
+ * sum is within 2^-17 whatever V, and a row that keeps rising adds 2^-22 for each
+ * time that a thread's running maximum does (V / 8192 times at most). These are
  * the softmax's own probabilities: the coder's integer CDF adds a floor of one
  * count per token and rounds to 2^-cdf_precision. */
 int kr_token_scores(const void* logits, int logits_f32, int N, int V, long long ld,

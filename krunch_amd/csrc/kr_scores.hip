@@ -7,7 +7,10 @@
 // One pass over memory: a thread keeps a running maximum and the two sums relative
 // to it, rescaled where a block of its chunks has a larger one; the threads' are
 // joined at the row's end. Sums are fp32, in an order given by the element's index
-// alone, so a row's results do not depend on N or on where the row lies.
+// alone, so a row's results do not depend on N or on where the row lies. A block of
+// at most 32 terms is summed by itself, and a thread's blocks with their rounding
+// errors carried along, so the error does not grow with V: in one chain, equal
+// logits of V = 2^24 came out 5e-4 off.
 // Exponentials are 2^(x log2 e - m log2 e): for fp16 one fused multiply-add and the
 // hardware's exp2, sums being relative to the rounded m log2 e.
 //
@@ -171,6 +174,16 @@ __device__ __forceinline__ kr_int4 without_first(kr_int4 v, int d) {
     return v;
 }
 
+// sum + x, and what the addition rounded off to low: exactly where |sum| >= |x|.
+// Elsewhere (x has the sum's sign, or the size of a rounding) the sum more than
+// doubles, so what those additions lose, half a last place each, comes to one last
+// place of the final sum in all. 8 operations a block: 8192 x 50277 143.1 -> 143.5 us.
+__device__ __forceinline__ void add_carried(float& sum, float& low, float x) {
+    const float t = sum + x;
+    low += x - (t - sum);
+    sum = t;
+}
+
 // A barrier of the row's threads: the workgroup's, or the wave's own order.
 template <int W>
 __device__ __forceinline__ void row_sync() {
@@ -248,7 +261,9 @@ scores_kernel(ScoreArgs g) {
     // (fp32: the maximum itself, whose log2 e multiple may overflow)
     float m = -INFINITY, ref = 0.0f, s = 0.0f, q = 0.0f;
     auto reference = [](float top) { return top == -INFINITY ? 0.0f : CH == 8 ? top * kLog2e : top; };
+    float s_low = 0.0f, q_low = 0.0f;     // what the additions of blocks rounded off
     auto add = [&](const kr_int4 (&raw)[U]) {
+        float sb = 0.0f, qb = 0.0f;
         #pragma unroll
         for (int u = 0; u < U; u++) {
             const vec v = __builtin_bit_cast(vec, raw[u]);
@@ -258,9 +273,16 @@ scores_kernel(ScoreArgs g) {
                 if constexpr (CH == 8) a = __builtin_fmaf((float)v[e], kLog2e, -ref);
                 else a = ((float)v[e] - ref) * kLog2e;
                 const float ex = __builtin_amdgcn_exp2f(a);
-                s += ex;
-                q = __builtin_fmaf(ex, fmaxf(a, -1000.0f), q);   // e^-inf * -inf = 0
+                sb += ex;
+                qb = __builtin_fmaf(ex, fmaxf(a, -1000.0f), qb);   // e^-inf * -inf = 0
             }
+        }
+        if constexpr (W == 1) {
+            s = sb;
+            q = qb;
+        } else {
+            add_carried(s, s_low, sb);
+            add_carried(q, q_low, qb);
         }
     };
     // s and q relative to `to`, which is not below ref; with m = -inf, nothing is
@@ -271,6 +293,8 @@ scores_kernel(ScoreArgs g) {
             const float f = __builtin_amdgcn_exp2f(d);
             q = f * __builtin_fmaf(d, s, q);
             s = f * s;
+            q_low = f * __builtin_fmaf(d, s_low, q_low);
+            s_low = f * s_low;
         }
         ref = to;
     };
@@ -314,6 +338,8 @@ scores_kernel(ScoreArgs g) {
         add(raw);
     } else {
         rescale(reference(M));
+        s += s_low;
+        q += q_low;
     }
     s = kr_wave_reduce(s, [](float a, float b) { return a + b; });
     q = kr_wave_reduce(q, [](float a, float b) { return a + b; });
