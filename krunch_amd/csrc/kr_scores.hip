@@ -465,6 +465,8 @@ scores_kernel(ScoreArgs g) {
     if (lane == 0) {
         float lp = (x_token - base) - ln_s;
         float h = __logf(s) - kLn2 * (q / s);
+        lp = lp > 0.0f ? 0.0f : lp;           // a rounding of a token of probability 1
+        h = h < 0.0f ? 0.0f : h;
         if (s == 0.0f) {
             lp = -INFINITY;
             h = 0.0f;
@@ -478,7 +480,8 @@ scores_kernel(ScoreArgs g) {
         const bool good = s == s, there = good && lane < kept;
         const uint64_t k = there ? sh.top[lane] : 0;
         const size_t o = (size_t)row * g.n_top + lane;
-        g.top_logprob[o] = there ? (key_value(k) - base) - ln_s : good ? -INFINITY : NAN;
+        const float lp = (key_value(k) - base) - ln_s;
+        g.top_logprob[o] = there ? (lp > 0.0f ? 0.0f : lp) : good ? -INFINITY : NAN;
         g.top_token[o] = there ? (int32_t)key_index(k) : -1;
     }
 }
@@ -570,6 +573,8 @@ __global__ void __launch_bounds__(256, 8) scores_short_kernel(ScoreArgs g) {
     if (there && l == 0) {
         float lp = (x_token - base) - ln_s;
         float h = log_s - kLn2 * (q / s);
+        lp = lp > 0.0f ? 0.0f : lp;           // a rounding of a token of probability 1
+        h = h < 0.0f ? 0.0f : h;
         if (s == 0.0f) {
             lp = -INFINITY;
             h = 0.0f;
@@ -642,7 +647,8 @@ __global__ void __launch_bounds__(256, 8) scores_short_kernel(ScoreArgs g) {
             const bool good = s == s;
             const uint64_t k = good ? best[slot][l] : 0;
             const size_t o = (size_t)row * g.n_top + l;
-            g.top_logprob[o] = k ? (key_value(k) - base) - ln_s : good ? -INFINITY : NAN;
+            const float lp = (key_value(k) - base) - ln_s;
+            g.top_logprob[o] = k ? (lp > 0.0f ? 0.0f : lp) : good ? -INFINITY : NAN;
             g.top_token[o] = k ? (int32_t)key_index(k) : -1;
         }
     }

@@ -1,5 +1,5 @@
-"""Scores of tokens: widths on both sides of the lines between its kernels, and
-sums over very wide rows."""
+"""Scores of tokens: widths on both sides of the lines between its kernels, sums
+over very wide rows, and signs (no probability above 1, no entropy below 0)."""
 import pytest
 import torch
 
@@ -7,6 +7,7 @@ from krunch_amd import krunch_ac_hip as ops
 from tests.test_gpu_scores import check, rand
 
 pytestmark = pytest.mark.gpu
+DEV = "cuda"
 
 
 # chunks are of 8 fp16 or 4 fp32 logits: 256 and 512 logits, and 128, 256, 1024 and
@@ -45,3 +46,20 @@ def test_a_rising_row(dtype):
     want = logp.gather(1, tok.long().cpu()[:, None])[:, 0]
     assert ((lp - want).abs() <= 2.0 ** -15 + 2.0 ** -22 * want.abs()).all()
     assert ((h + (logp.exp() * logp).sum(1)).abs() <= 2.0 ** -14 + 2.0 ** -18 * h).all()
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("V", [1, 100, 300, 700, 2000, 6000, 50277])
+def test_no_probability_above_one_and_no_entropy_below_zero(dtype, V):
+    """Rows of one token of probability 1, by masks or by distance, at many values."""
+    N = 400
+    g = torch.Generator().manual_seed(V)
+    top = (40 * torch.randn(N, generator=g)).to(dtype).to(DEV)
+    x = torch.full((N, V), -float("inf"), dtype=dtype, device=DEV)
+    at = torch.randint(0, V, (N,), generator=g).to(DEV)
+    rows = torch.arange(N, device=DEV)
+    x[N // 2:] = -30000.0
+    x[rows, at] = top
+    lp, h, tl, tt = ops.token_scores(x, at.to(torch.int32), min(V, 3))
+    assert (lp <= 0).all() and (tl <= 0).all() and (h >= 0).all()
+    assert (lp >= -2.0 ** -17).all() and (h <= 2.0 ** -16).all() and torch.equal(tt[:, 0], at.to(torch.int32))
+    check(x, at.to(torch.int32), min(V, 3))
