@@ -44,7 +44,9 @@ template <> struct Chunk<float> {
     typedef kr_float4 vec;
 };
 
-typedef kr_int4 int4_any __attribute__((aligned(4)));
+// 16 bytes of a row: rows, and the last chunk of a row, start at any element.
+typedef kr_int4 int4_any __attribute__((aligned(2)));
+static_assert(alignof(int4_any) <= alignof(kr_half), "chunks start at any element");
 
 struct ScoreArgs {
     const void* logits;
