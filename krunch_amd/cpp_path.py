@@ -155,15 +155,16 @@ def score_packed_batched(weights: dict, input_ids, target_ids, state: State, n_t
     carried. The layers run as in forward_packed_batched, the head and the
     scores in blocks of head_rows rows, so no [B * T, V] logits are held."""
     P: Prepared = weights["prepared"]
-    ids, tgt = _ids(input_ids, P.device), _ids(target_ids, P.device)
+    ids, tgt = (torch.as_tensor(t, device=P.device) for t in (input_ids, target_ids))
     if ids.dim() != 2 or ids.shape != tgt.shape:
         raise ValueError(f"input_ids and target_ids must be [B, T], got {tuple(ids.shape)} and "
                          f"{tuple(tgt.shape)}")
     B, T = ids.shape
     assert state.B == B, f"state holds {state.B} streams, input has {B}"
-    _check_ids(ids, P.V)
+    _check_ids(ids, P.V)                  # both before they are narrowed to 32 bits
     if tgt.numel() and (int(tgt.min()) < -1 or int(tgt.max()) >= P.V):
         raise ValueError(f"target id out of range [-1, {P.V})")
+    ids, tgt = _ids(ids, P.device), _ids(tgt, P.device)
     return _score_window(weights, ids, tgt, state, n_top, head_rows)
 
 

@@ -351,10 +351,10 @@ class InferenceEngine:
         lens = lens[order]
         tgt = np.full((B, int(lens[0])), -1, dtype=np.int32)
         for b, i in enumerate(order):
-            tgt[b, :lens[b]] = np.asarray(token_streams[i], dtype=np.int32)
-        live = np.arange(tgt.shape[1]) < lens[:, None]
-        if tgt[live].min() < 0 or tgt.max() >= P.V:
-            raise ValueError(f"token id out of range [0, {P.V})")
+            t = np.asarray(token_streams[i])
+            if t.min() < 0 or t.max() >= P.V:         # before it is narrowed to 32 bits
+                raise ValueError(f"token id out of range [0, {P.V})")
+            tgt[b, :lens[b]] = t
         inp = np.full_like(tgt, BOS_TOKEN)
         inp[:, 1:] = np.maximum(tgt[:, :-1], 0)
         tgt_d, inp_d = torch.from_numpy(tgt).to(P.device), torch.from_numpy(inp).to(P.device)
