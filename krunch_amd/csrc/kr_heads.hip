@@ -54,8 +54,10 @@ __device__ __forceinline__ int stream_tokens(const HeadArgs& g, int b) {
 // l the columns 4 (l % 4) .. + 3 of rows D/16 (l / 4) .. + D/16 - 1, so y is
 // summed over a lane's rows and then over 16 lanes, with no LDS.
 // Bound, for one token: the state, read and written once. Measured on MI355X, heads
-// of 64: 512 streams x 12 heads 37 us (203 MB, 5.4 TB/s; a copy runs at 5.1), one
-// stream 3.0; a further token about 0.4 us at one stream, 0.9 at 64.
+// of 64: 512 streams x 12 heads 38 us (203 MB, 5.4 TB/s; a copy runs at 5.1), one
+// stream 3.0. For many: at few streams a token's chain (1 x 256 tokens 118 us, 64 x 256
+// 251: 0.5 and 1.0 us a token), at many the VALU (512 x 64 tokens 400 us, 6.2 a token; the
+// bytes would take 78).
 // ---------------------------------------------------------------------------
 template <int D>
 __global__ void __launch_bounds__(4 * D) heads_step_kernel(HeadArgs g) {
@@ -130,9 +132,9 @@ __global__ void __launch_bounds__(4 * D) heads_step_kernel(HeadArgs g) {
 // Bound: with many heads, the VALU work of taking values apart (about 500
 // instructions a chunk and wave beside 50 products) and the three barriers, with 3
 // workgroups a CU for D = 64 and one for 128; with few heads, latency. Measured on
-// MI355X, heads of 64: 256 x 1024 tokens x 12 heads 401 us (1.71 GB, 4.3 TB/s), 128
-// streams of 256..1024 163 us (640 MB, 3.9 TB/s; 173 in the order they come), 1 x 4096
-// 25; heads of 128: 128 x 1024 x 6 288 us (3.1 TB/s), 1 x 1777 x 8 28.
+// MI355X, heads of 64: 256 x 1024 tokens x 12 heads 393 us (1.71 GB, 4.4 TB/s), 128
+// streams of 256..1024 155 us (640 MB, 4.1 TB/s; 10 more in the order they come), 1 x
+// 4096 24; heads of 128: 128 x 1024 x 6 278 us (3.2 TB/s), 1 x 1777 x 8 28.
 // ---------------------------------------------------------------------------
 
 // Powers of two that bring a largest value x to 2^13..2^14, and back. Zero and

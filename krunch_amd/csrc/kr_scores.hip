@@ -198,10 +198,10 @@ __device__ __forceinline__ void row_sync() {
 
 // W waves per row, U chunks of 16 bytes per thread at a time; four rows a workgroup
 // with W = 1, else one.
-// Bound: memory with many rows (8192 x 50277 fp16 149 us, with 8 top 155: 5.5 and 5.3
+// Bound: memory with many rows (8192 x 50277 fp16 143 us, with 8 top 153: 5.8 and 5.4
 // TB/s, fp32 270: 6.1; holding rows in registers and sums made anew after the
-// maximum 165, one row per 16 waves 156); latency with few: one row of 50277 6.0 us, 8.1 with
-// 8 top, of which 3.6 is any launch's; a further 2 us are T, the list and the ranks.
+// maximum 165, one row per 16 waves 194); latency with few: one row of 50277 with 5 top
+// 7.7 us, of which 3.6 is any launch's and 2 are T, the list and the ranks.
 template <typename T, int W, int U, bool TOP>
 __global__ void __launch_bounds__(W > 1 ? 64 * W : 256, 8)
 scores_kernel(ScoreArgs g) {
@@ -680,9 +680,10 @@ void launch(const ScoreArgs& g, hipStream_t s) {
 //   to 128 CH, 256 CH: a wave with two, four chunks a lane, the row in registers.
 //     30000 x 1000 fp16 16.9 with two, 22.4 with four, 40 by two waves that walk it.
 //   to 1024 CH, 4096 CH and above: 2, 4 and 8 waves that walk the row. 2 / 4 / 8:
-//     10000 x 4000 fp16 18.0 / 29.4 / 52.2, 8000 x 8000 26.8 / 25.8 / 45.8, 4000 x 16000
-//     27.9 / 27.6 / 25.0, 8192 x 50277 154 / 147 / 140 (16 waves: 156), 300 x 50277
-//     20.3 / 12.9 / 11.9; fp32 8000 x 8000 47.5 / 46.4 / 41.7.
+//     10000 x 4000 fp16 17.1 / 28.3 / 52.0, 8000 x 8000 26.2 / 25.4 / 45.7, 4000 x 16000
+//     28.3 / 28.0 / 24.9, 8192 x 50277 153 / 149 / 143 (16 waves: 194), 300 x 50277
+//     20.5 / 13.1 / 12.1; fp32 8000 x 8000 48.8 / 47.5 / 42.5, 8192 x 50277 282 / 274 /
+//     269.
 template <typename T>
 void launch_by_width(const ScoreArgs& g, hipStream_t s) {
     constexpr int CH = Chunk<T>::n;

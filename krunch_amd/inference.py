@@ -473,9 +473,11 @@ class InferenceEngine:
 
     def estimate(self, raw: bytes, chunk_size: Optional[int] = None) -> int:
         """The size of compress(raw)'s blob, from the tokens' scores: header,
-        entries and, per chunk, its mini-header and coder_bits. Within a few
-        parts in a thousand of the blob (the coder's rounding, and the most likely
-        tokens' extra counts)."""
+        entries and, per chunk, its mini-header and coder_bits. Near the blob's,
+        and mostly a little above it: the coder rounds, a stream ends in whole bytes,
+        and a row's most likely token has up to V of the 2^24 counts more than
+        coder_bits gives it, so a text that takes it again and again in flat rows
+        (p not far above V / 2^24) costs less than estimated."""
         self._need_tokenizer()
         from krunch_amd import chunking
 
