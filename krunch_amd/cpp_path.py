@@ -156,6 +156,8 @@ def score_packed_batched(weights: dict, input_ids, target_ids, state: State, n_t
     scores in blocks of head_rows rows, so no [B * T, V] logits are held."""
     P: Prepared = weights["prepared"]
     ids, tgt = (torch.as_tensor(t, device=P.device) for t in (input_ids, target_ids))
+    # unsigned types have no min and max
+    ids, tgt = (t if t.dtype == torch.int32 else t.to(torch.int64) for t in (ids, tgt))
     if ids.dim() != 2 or ids.shape != tgt.shape:
         raise ValueError(f"input_ids and target_ids must be [B, T], got {tuple(ids.shape)} and "
                          f"{tuple(tgt.shape)}")

@@ -31,3 +31,16 @@ def test_packed(bad):
             cpp_path.score_packed_batched(W, t, good, st)
         with pytest.raises(ValueError, match="target id out of range"):
             cpp_path.score_packed_batched(W, good, t, st)
+
+
+@pytest.mark.parametrize("dtype", [np.uint8, np.uint16, np.uint32, np.int16, np.int64])
+def test_types(dtype):
+    eng = InferenceEngine()
+    eng._weights, eng._ready = W, True
+    bad, good = np.array([[1, V]], dtype=dtype), np.array([[1, V - 1]], dtype=dtype)
+    with pytest.raises(ValueError, match="token id out of range"):
+        eng.score_tokens_batched([bad[0]])
+    with pytest.raises(ValueError, match="token id out of range"):
+        cpp_path.score_packed_batched(W, bad, good, SimpleNamespace(B=1))
+    with pytest.raises(ValueError, match="target id out of range"):
+        cpp_path.score_packed_batched(W, good, bad, SimpleNamespace(B=1))
