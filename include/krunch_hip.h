@@ -276,7 +276,8 @@ int kr_quantize_w4(const uint16_t* W, long long ldk, long long ldn, int N, int K
  * fma(s_g, c_g, acc) over the groups in order from zero; so a row has the same
  * bits for any M. A NaN scale makes its output NaN; infinite scales are not
  * supported. With many rows the fp16 products are the faster ones: 768 x 50277 from
- * about 100 rows on at groups of 32, 190 at 64, 260 at 128. M <= 2^19. out must not overlap x (out may be res). */
+ * about 100 rows on at groups of 32, 190 at 64, 260 at 128. M <= 2^19. out must
+ * not overlap x (out may be res). */
 int kr_det_matmul_w4(const uint16_t* x, long long ldx, int M, int K, const void* q,
                      const uint16_t* scales, int group, int N, void* out, long long ldo, int epilogue,
                      const uint16_t* res, const uint16_t* gate, void* stream);

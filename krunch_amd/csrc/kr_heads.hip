@@ -395,7 +395,8 @@ __global__ void __launch_bounds__(4 * D, D == 64 ? 3 : 2) heads_chunk_kernel(Hea
                 const float fp = sh.pdown[i];
                 kr_half4 y;
                 #pragma unroll
-                for (int r = 0; r < 4; r++) y[r] = kr_f16(__builtin_fmaf(inside[r], fp, from_s[r] * (down_m[r] * y_dec[it])));
+                for (int r = 0; r < 4; r++)
+                    y[r] = kr_f16(__builtin_fmaf(inside[r], fp, from_s[r] * (down_m[r] * y_dec[it])));
                 if (i < n)
                     *reinterpret_cast<kr_half4*>(yp + 16 * it * g.ldy) = y;
                 __builtin_amdgcn_sched_barrier(0);
