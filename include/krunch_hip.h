@@ -135,6 +135,38 @@ int kr_token_scores(const void* logits, int logits_f32, int N, int V, long long 
                     const int32_t* tokens, float* logprob, float* entropy, int n_top,
                     float* top_logprob, int32_t* top_token, void* stream);
 
+/* Cross entropy of a head in pieces of the vocabulary, without its logits (no
+ * reference counterpart; beside kr_token_scores, which reads logits): x fp16
+ * [N, C] and W fp16 [V, C] by row strides ldx, ldw (multiples of 8, below 2^21; x
+ * and W 16-byte aligned; C a multiple of 64 up to 16384; N, V <= 2^24):
+ *   z = x W' (exact products, fp32 sums, not rounded to fp16 as logits are)
+ *   lse[n]  = ln sum_v e^z[n][v];   loss[n] = lse[n] - z[n][targets[n]]
+ * in nats; loss is 0 where targets[n] = -1 and NaN for any other id outside
+ * 0..V-1; a row with a NaN or +inf in z is NaN. The order of a row's sums depends on
+ * N <= 128 or not. ws: kr_head_loss_workspace_bytes, 256-byte aligned (8 bytes a row
+ * and 128 columns of the vocabulary).
+ *
+ * kr_head_loss_backward, from the same inputs, the lse of the forward call and
+ * dloss fp32 [N]:
+ *   dz[n][v] = dloss[n] (e^(z[n][v] - lse[n]) - [v = targets[n]])
+ *   dx = dz W [N, C],  dW = dz' x [V, C], contiguous, 16-byte aligned, fp16 or
+ * (out_f32) fp32; dx or dW may be NULL. Rows with target -1 or dloss 0 have no
+ * gradient, whatever x, lse and dloss hold there; other ids outside 0..V-1 give
+ * NaN. dz is rounded to fp16 on a scale where the largest finite |dloss| is
+ * 2^14..2^15, so relative to that row's gradient: 2^-11 of each dz above
+ * 2^-28 of the largest |dloss|, 2^-39 of the largest |dloss| below. Sums are
+ * fp32 in an order that depends on the sizes alone. ws:
+ * kr_head_loss_backward_workspace_bytes (dx, dw: which of them is wanted), 256-byte
+ * aligned: at most 256 MB of dz at once (256 columns at least) and fp32 partial
+ * sums. Outputs must not overlap inputs. */
+size_t kr_head_loss_workspace_bytes(int N, int C, int V);
+int kr_head_loss(const uint16_t* x, long long ldx, int N, int C, const uint16_t* W, long long ldw, int V,
+                 const int32_t* targets, float* loss, float* lse, void* ws, size_t ws_bytes, void* stream);
+size_t kr_head_loss_backward_workspace_bytes(int N, int C, int V, int dx, int dw);
+int kr_head_loss_backward(const uint16_t* x, long long ldx, int N, int C, const uint16_t* W, long long ldw,
+                          int V, const int32_t* targets, const float* lse, const float* dloss, int out_f32,
+                          void* dx, void* dW, void* ws, size_t ws_bytes, void* stream);
+
 /* Fused compress stage: per row only the interval of symbols[row],
  * pairs[row] = (cdf[sym], cdf[sym+1]) — replaces det_softmax_cdf + cumsum +
  * the coder's two reads (cpp_path.py:499-500, encode_kernel.cu:110-111). */

@@ -1,0 +1,659 @@
+// Softmax cross entropy of a head [V, C] over a large vocabulary, and its
+// gradients, without [N, V] logits in memory.
+//
+//   z = x W';  lse_n = ln sum_v e^(z_nv);  loss_n = lse_n - z_n,target
+//   dz_nv = dloss_n (e^(z_nv - lse_n) - [v is n's target]);  dx = dz W;  dW = dz' x
+//
+// Forward: tiles of z stay in registers and leave as a maximum and a sum per row
+// and 128 columns, which a second kernel joins. Backward: a piece of the vocabulary
+// at a time, z again, dz of the piece as fp16 in the workspace, and both products
+// that read it in one launch.
+//
+// dz enters the matrix units as fp16 (11 bits, as x and W have): it is kept times a
+// power of two that brings the largest |dloss| to 2^14..2^15, so that
+// probabilities down to 2^-28 of that keep all their bits. Sums are fp32.
+#include <algorithm>
+
+#include "kr_common.h"
+#include "kr_wave.h"
+#include "krunch_hip.h"
+
+namespace {
+
+constexpr float kLog2e = 0x1.715476p+0f, kLn2 = 0x1.62e430p-1f;
+constexpr int kPart = 128;            // columns of a partial maximum and sum
+typedef short short4v __attribute__((__vector_size__(8)));
+typedef __attribute__((address_space(3))) short4v lds_short4;
+
+struct LossArgs {
+    const kr_half* x;
+    const kr_half* W;                 // [V, C], at the piece's first row
+    long long ldx, ldw;
+    const int32_t* targets;
+    const float* lse;                 // GRAD
+    const float* dloss;
+    const float* scale;               // [2] up, down
+    float2* part;                     // LOSS: [parts][N] maximum, sum
+    float* hit;                       // LOSS: [N] the target's z
+    kr_half* G;                       // GRAD: [rows][ldg] dz of the piece
+    long long ldg;
+    int N, C, V;                      // V: the piece's columns
+    int v0, v_all;                    // the piece's first column, the vocabulary
+    int rows;                         // GRAD: N rounded up to 64, the rows of G
+};
+
+__device__ __forceinline__ void copy16(const void* base, unsigned off, unsigned lds) {
+    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :: "s"(lds), "v"(off), "s"(base) : "memory", "m0");
+}
+__device__ __forceinline__ unsigned lds_address(const void* p) {
+    return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
+}
+
+// LDS place, in 16-byte units, of unit kc (8 k) of row r of an operand whose rows
+// lie along k: a copy instruction moves 8 whole 128-byte lines, and 8 rows' units of
+// one kc lie on different banks.
+__device__ __forceinline__ int row_unit(int r, int kc) { return 8 * r + (kc ^ ((r >> 1) & 7)); }
+
+// Tile of the launch's virtual workgroup vb: an eighth of a grouped order for each XCD.
+__device__ __forceinline__ bool tile_of(int gy, int gx, int vb, int group_m, int& m_t, int& n_t) {
+    const int T = gx * gy, per = (T + 7) / 8;
+    const int t = (vb & 7) * per + (vb >> 3);
+    if (t >= T || (vb >> 3) >= per) return false;
+    const int in_group = group_m * gx;
+    const int first_m = (t / in_group) * group_m;
+    const int gm = min(gy - first_m, group_m);
+    const int r = t % in_group;
+    m_t = first_m + r % gm;
+    n_t = r / gm;
+    return true;
+}
+
+// ---------------------------------------------------------------------------
+// z = x W' in tiles of (64 WM) x (128 WN), a wave for each 64 x 128. Steps of 64 k
+// through two LDS stages, copied asynchronously one step ahead, into the next tile.
+// The matrix unit gets W' x', so a lane has 4 columns of a row; W's rows go in
+// in an order that makes them 8 consecutive columns over two tiles.
+// ---------------------------------------------------------------------------
+template <int WM, int WN, bool GRAD>
+__global__ void __launch_bounds__(64 * WM * WN, 1) logits_kernel(LossArgs g, int n_virtual, int group_m) {
+    constexpr int BM = 64 * WM, BN = 128 * WN, WAVES = WM * WN;
+    constexpr int COPIES = (BM + BN) / 8 / WAVES;
+    static_assert((BM + BN) / 8 % WAVES == 0, "copies");
+    constexpr int STAGE = (BM + BN) * 8;                  // 16-byte units
+    __shared__ __attribute__((aligned(1024))) kr_half8 ring[2 * STAGE];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave / WN, wn = wave % WN;
+    const int lr = lane & 15, lq = lane >> 4;
+    const int gy = ((GRAD ? g.rows : g.N) + BM - 1) / BM, gx = (g.V + BN - 1) / BN;
+    const int KS = g.C / 64;
+    const unsigned ring_base = lds_address(ring);
+    auto issue = [&](int m_t, int n_t, int ks, int q) {
+        const kr_half* xa = g.x + (long long)m_t * BM * g.ldx;
+        const kr_half* wa = g.W + (long long)n_t * BN * g.ldw;
+        const unsigned so = ring_base + (unsigned)((q & 1) * STAGE * 16);
+        #pragma unroll
+        for (int i = 0; i < COPIES; i++) {
+            const int j = wave * COPIES + i;              // 8 rows of the stage
+            const bool a = j < BM / 8;
+            const int row = 8 * (a ? j : j - BM / 8) + (lane >> 3);
+            const int last = a ? g.N - 1 - m_t * BM : g.V - 1 - n_t * BN;
+            const int kc = (lane & 7) ^ ((row >> 1) & 7);
+            const unsigned off = (unsigned)max(min(row, last), 0) * (unsigned)(2 * (a ? g.ldx : g.ldw)) +
+                                 (unsigned)(16 * kc + 128 * ks);
+            copy16(a ? xa : wa, off, so + 1024u * (unsigned)j);
+        }
+    };
+    int vb = blockIdx.x, m_t, n_t;
+    if (!tile_of(gy, gx, vb, group_m, m_t, n_t)) return;
+    int q = 0;
+    issue(m_t, n_t, 0, 0);
+    while (true) {
+        int nm_t = 0, nn_t = 0;
+        const bool has_next =
+            vb + (int)gridDim.x < n_virtual && tile_of(gy, gx, vb + (int)gridDim.x, group_m, nm_t, nn_t);
+        kr_float4 acc[4][8];
+        #pragma unroll
+        for (int i = 0; i < 4; i++)
+            #pragma unroll
+            for (int t = 0; t < 8; t++) acc[i][t] = kr_float4{0, 0, 0, 0};
+        #pragma unroll 1
+        for (int ks = 0; ks < KS; ks++, q++) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();   // every wave's copies of step q are in; step q-1's stage is free
+            if (ks + 1 < KS) issue(m_t, n_t, ks + 1, q + 1);
+            else if (has_next) issue(nm_t, nn_t, 0, q + 1);
+            const kr_half8* As = ring + (q & 1) * STAGE;
+            const kr_half8* Ws = As + BM * 8;
+            #pragma unroll
+            for (int kb = 0; kb < 2; kb++) {
+                kr_half8 a[4];
+                #pragma unroll
+                for (int i = 0; i < 4; i++) a[i] = As[row_unit(64 * wm + 16 * i + lr, 4 * kb + lq)];
+                #pragma unroll
+                for (int th = 0; th < 2; th++) {
+                    __builtin_amdgcn_sched_barrier(0);    // four W fragments at a time (registers)
+                    kr_half8 w[4];
+                    #pragma unroll
+                    for (int t = 0; t < 4; t++) {
+                        const int row = 128 * wn + 32 * (2 * th + t / 2) + 8 * (lr >> 2) + 4 * (t & 1) + (lr & 3);
+                        w[t] = Ws[row_unit(row, 4 * kb + lq)];
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                    #pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        #pragma unroll
+                        for (int t = 0; t < 4; t++)
+                            acc[i][4 * th + t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                w[t], a[i], acc[i][4 * th + t], 0, 0, 0);
+                }
+            }
+        }
+        // lane: row 64 wm + 16 i + lr; acc[i][t][r] column 128 wn + 32 (t / 2) + 8 lq + 4 (t % 2) + r
+        const int c0 = n_t * BN + 128 * wn + 8 * lq;
+        #pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int m = m_t * BM + 64 * wm + 16 * i + lr;
+            const int target = m < g.N ? g.targets[m] : -1;
+            const int tc = target - g.v0;                 // the target's column of the piece
+            if constexpr (!GRAD) {
+                float big = -INFINITY, zt = 0.0f;
+                #pragma unroll
+                for (int t = 0; t < 8; t++)
+                    #pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const int c = c0 + 32 * (t / 2) + 4 * (t & 1) + r;
+                        const float z = c < g.V ? acc[i][t][r] : -INFINITY;
+                        acc[i][t][r] = z;
+                        zt = c == tc ? z : zt;
+                        big = fmaxf(big, z);
+                    }
+                big = fmaxf(big, kr_xor<16>(big));
+                big = fmaxf(big, kr_xor<32>(big));
+                const float base = big == -INFINITY ? 0.0f : big;
+                float sum = 0.0f;
+                #pragma unroll
+                for (int t = 0; t < 8; t++) {
+                    float s = 0.0f;
+                    #pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        s += __builtin_amdgcn_exp2f((acc[i][t][r] - base) * kLog2e);
+                    sum += s;
+                }
+                sum += kr_xor<16>(sum);
+                sum += kr_xor<32>(sum);
+                const int d = tc - c0;
+                if (m < g.N) {
+                    if (target >= 0 && tc < g.V && d >= 0 && d < 128 && (d & 31) < 8) g.hit[m] = zt;
+                    if (lq == 0 && n_t * BN + 128 * wn < g.V)
+                        g.part[(size_t)(n_t * WN + wn) * g.N + m] = float2{big, sum};
+                }
+            } else {
+                float f = 0.0f, lse = 0.0f;
+                if (target != -1 && m < g.N) {
+                    f = (unsigned)target < (unsigned)g.v_all ? g.dloss[m] * g.scale[0] : NAN;
+                    lse = g.lse[m];
+                }
+                kr_half* out = g.G + (size_t)m * g.ldg + c0;
+                #pragma unroll
+                for (int p = 0; p < 4; p++) {
+                    kr_half8 v;
+                    #pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const int c = c0 + 32 * p + e;
+                        float z = __builtin_amdgcn_exp2f((acc[i][2 * p + e / 4][e % 4] - lse) * kLog2e);
+                        if (c == tc) z -= 1.0f;
+                        z *= f;
+                        v[e] = kr_f16(f == 0.0f || c >= g.V ? 0.0f : z);
+                    }
+                    if (m < g.rows && c0 + 32 * p < (int)g.ldg) *reinterpret_cast<kr_half8*>(out + 32 * p) = v;
+                }
+            }
+        }
+        if (!has_next) break;
+        vb += gridDim.x;
+        m_t = nm_t;
+        n_t = nn_t;
+    }
+}
+
+// Parts of a row -> lse and loss; 16 rows x 16 parts at a time.
+__global__ void __launch_bounds__(256) loss_join_kernel(const float2* part, const float* hit, int N, int parts,
+                                                        int V, const int32_t* targets, float* loss, float* lse) {
+    __shared__ float big_of[16][16], sum_of[16][16];
+    const int r = threadIdx.x & 15, p0 = threadIdx.x >> 4;
+    const int m = blockIdx.x * 16 + r;
+    float big = -INFINITY, sum = 0.0f;
+    if (m < N)
+        for (int p = p0; p < parts; p += 16) {
+            const float2 v = part[(size_t)p * N + m];
+            const float to = fmaxf(big, v.x), base = to == -INFINITY ? 0.0f : to;
+            sum = sum * __builtin_amdgcn_exp2f((big - base) * kLog2e) +
+                  v.y * __builtin_amdgcn_exp2f((v.x - base) * kLog2e);
+            big = to;
+        }
+    big_of[p0][r] = big;
+    sum_of[p0][r] = sum;
+    __syncthreads();
+    if (threadIdx.x >= 16 || m >= N) return;
+    big = -INFINITY;
+    for (int p = 0; p < 16; p++) big = fmaxf(big, big_of[p][r]);
+    const float base = big == -INFINITY ? 0.0f : big;
+    sum = 0.0f;
+    for (int p = 0; p < 16; p++) sum += sum_of[p][r] * __builtin_amdgcn_exp2f((big_of[p][r] - base) * kLog2e);
+    const float ln_sum = __builtin_amdgcn_logf(sum) * kLn2;
+    const int target = targets[m];
+    lse[m] = base + ln_sum;
+    loss[m] = target == -1 ? 0.0f : (unsigned)target < (unsigned)V ? (base - hit[m]) + ln_sum : NAN;
+}
+
+// ---------------------------------------------------------------------------
+// Backward: the power of two of dz, and x with the rows that have no gradient as
+// zeros (whatever they hold), rounded up to 64 rows.
+// ---------------------------------------------------------------------------
+__global__ void __launch_bounds__(1024) grad_scale_kernel(const int32_t* targets, const float* dloss, int N,
+                                                          float* scale) {
+    __shared__ float part[16];
+    float big = 0.0f;
+    for (int i = threadIdx.x; i < N; i += 1024) {
+        const float a = fabsf(dloss[i]);
+        if (targets[i] != -1 && a < INFINITY) big = fmaxf(big, a);
+    }
+    big = kr_wave_reduce(big, [](float a, float b) { return fmaxf(a, b); });
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = big;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 16; i++) big = fmaxf(big, part[i]);
+        int e = (int)(__float_as_uint(big) >> 23);        // 2^(e - 127) <= big
+        e = e < 15 ? 15 : e;
+        scale[0] = __uint_as_float((uint32_t)(268 - e) << 23);     // 2^(141 - e)
+        scale[1] = __uint_as_float((uint32_t)(e - 14) << 23);
+    }
+}
+
+__global__ void __launch_bounds__(256) live_rows_kernel(const kr_half* x, long long ldx, int N, int C, int rows,
+                                                        const int32_t* targets, const float* dloss, kr_half* out) {
+    const int per = C / 8;
+    const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (at >= (long long)rows * per) return;
+    const int m = (int)(at / per), c = 8 * (int)(at % per);
+    kr_half8 v = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (m < N && targets[m] != -1 && dloss[m] != 0.0f)
+        v = *reinterpret_cast<const kr_half8*>(x + (size_t)m * ldx + c);
+    *reinterpret_cast<kr_half8*>(out + (size_t)m * C + c) = v;
+}
+
+// ---------------------------------------------------------------------------
+// dW += dz' x and dx += dz W of one piece, in tiles of 256 x 256, 8 waves of
+// 64 x 128, steps of 64 k through two stages. Operands whose rows lie across k (W and
+// x as B, dz' as A) are staged as they lie, 64 k x 256 columns, and read by the LDS's
+// transposing reads: 16 lanes get 4 k of 16 columns.
+// ---------------------------------------------------------------------------
+struct ProdArgs {
+    const kr_half* G;                 // [rows][ldg]
+    long long ldg;
+    const kr_half* x;                 // [rows][C]
+    const kr_half* W;                 // [V, C] of the piece
+    long long ldw;
+    const float* scale;
+    float* dx_part;                   // [dx_splits][rows][C]
+    float* dw_part;                   // [dw_splits][V][C], dw_splits > 1
+    void* dW;                         // [V][C] of the piece, dw_splits 1
+    int f32;                          // dW's type
+    int rows, C, V, first;            // first: dx_part is written, not added to
+    int dx_splits, dw_splits;
+    int dw_items, dx_items;
+};
+
+constexpr int kProdStage = 512 * 8;   // 16-byte units: 32 KB of A, 32 of B
+
+// Columns that lie across k: LDS place, in bytes, of (k, 16-column tile, this lane's
+// 4 columns) with the tile XORed by a value of k's bits 0, 1 and 3, so that the 32
+// lanes of half a read are on different banks.
+__device__ __forceinline__ unsigned across(int tile, int lane) {
+    const int lr = lane & 15, lq = lane >> 4;
+    const int sw = (lr >> 2) | ((lq & 1) << 2);
+    return (unsigned)((8 * lq + (lr >> 2)) * 512 + 32 * (tile ^ sw) + 8 * (lr & 3));
+}
+__device__ __forceinline__ kr_half8 read_across(unsigned at) {
+    typedef kr_half half4v __attribute__((ext_vector_type(4)));
+    const half4v lo = __builtin_bit_cast(half4v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(uintptr_t)at));
+    const half4v hi =
+        __builtin_bit_cast(half4v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(uintptr_t)(at + 2048)));
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+template <bool DW>
+__device__ __forceinline__ void product_tile(const ProdArgs& g, kr_half8* ring, int item) {
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave >> 1, wn = wave & 1;
+    const int lr = lane & 15, lq = lane >> 4;
+    const int gx = (g.C + 255) / 256;
+    const int splits = DW ? g.dw_splits : g.dx_splits;
+    const int n_t = item % gx, m_t = item / gx / splits, split = item / gx % splits;
+    const int M = DW ? g.V : g.rows;
+    const int steps = DW ? g.rows / 64 : (g.V + 63) / 64;
+    const int ks0 = (int)((long long)steps * split / splits), ks1 = (int)((long long)steps * (split + 1) / splits);
+    const unsigned ring_base = lds_address(ring);
+    const int m0 = m_t * 256, n0 = n_t * 256;
+    // A: dW reads G across (columns m0.., always inside ldg), dx along
+    const kr_half* a_base = DW ? g.G + m0 : g.G + (size_t)m0 * g.ldg;
+    const kr_half* b_base = (DW ? g.x : g.W) + n0;
+    const long long ldb = DW ? g.C : g.ldw;
+    auto issue = [&](int ks, int q) {
+        const unsigned so = ring_base + (unsigned)((q & 1) * kProdStage * 16);
+        if (wave < 4 && !DW) {
+            #pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int row = 8 * (wave * 8 + i) + (lane >> 3);
+                const int kc = (lane & 7) ^ ((row >> 1) & 7);
+                const unsigned off = (unsigned)min(row, M - 1 - m0) * (unsigned)(2 * g.ldg) +
+                                     (unsigned)(16 * kc + 128 * ks);
+                copy16(a_base, off, so + 1024u * (unsigned)(wave * 8 + i));
+            }
+        } else {
+            const bool a = DW && wave < 4;
+            const kr_half* base = a ? a_base + (long long)ks * 64 * g.ldg : b_base + (long long)ks * 64 * ldb;
+            const long long ld = a ? g.ldg : ldb;
+            // B's k past the piece: the last row, against zeros of G
+            const int last = !DW && !a ? g.V - 1 - 64 * ks : 63;
+            const int cols = a ? (int)g.ldg - m0 : g.C - n0;
+            #pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int k = 2 * ((wave & 3) * 8 + i) + (lane >> 5);
+                const int sw = 2 * ((k & 3) | ((k >> 1) & 4));
+                const int col = 8 * ((lane & 31) ^ sw);
+                const unsigned off = (unsigned)min(k, last) * (unsigned)(2 * ld) + (unsigned)(col < cols ? 2 * col : 0);
+                copy16(base, off, so + 1024u * (unsigned)(wave * 8 + i));
+            }
+        }
+    };
+    kr_float4 acc[4][8];
+    #pragma unroll
+    for (int i = 0; i < 4; i++)
+        #pragma unroll
+        for (int t = 0; t < 8; t++) acc[i][t] = kr_float4{0, 0, 0, 0};
+    unsigned a_at[4], b_at[8];
+    #pragma unroll
+    for (int i = 0; i < 4; i++) a_at[i] = across(4 * wm + i, lane);
+    #pragma unroll
+    for (int t = 0; t < 8; t++) b_at[t] = across(8 * wn + t, lane) + 32768u;
+    if (ks0 < ks1) issue(ks0, 0);
+    #pragma unroll 1
+    for (int ks = ks0, q = 0; ks < ks1; ks++, q++) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (ks + 1 < ks1) issue(ks + 1, q + 1);
+        const kr_half8* As = ring + (q & 1) * kProdStage;
+        const unsigned so = ring_base + (unsigned)((q & 1) * kProdStage * 16);
+        #pragma unroll
+        for (int kb = 0; kb < 2; kb++) {
+            kr_half8 a[4];
+            #pragma unroll
+            for (int i = 0; i < 4; i++)
+                a[i] = DW ? read_across(so + a_at[i] + 16384u * kb) : As[row_unit(64 * wm + 16 * i + lr, 4 * kb + lq)];
+            #pragma unroll
+            for (int th = 0; th < 2; th++) {
+                __builtin_amdgcn_sched_barrier(0);
+                kr_half8 b[4];
+                #pragma unroll
+                for (int t = 0; t < 4; t++) b[t] = read_across(so + b_at[4 * th + t] + 16384u * kb);
+                __builtin_amdgcn_sched_barrier(0);
+                #pragma unroll
+                for (int i = 0; i < 4; i++)
+                    #pragma unroll
+                    for (int t = 0; t < 4; t++)
+                        acc[i][4 * th + t] =
+                            __builtin_amdgcn_mfma_f32_16x16x32_f16(b[t], a[i], acc[i][4 * th + t], 0, 0, 0);
+            }
+        }
+    }
+    const float down = g.scale[1];
+    #pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int m = m0 + 64 * wm + 16 * i + lr;
+        if (m >= M) continue;
+        #pragma unroll
+        for (int t = 0; t < 8; t++) {
+            const int n = n0 + 128 * wn + 16 * t + 4 * lq;
+            if (n >= g.C) continue;
+            kr_float4 v = acc[i][t];
+            if (!DW || splits > 1) {
+                float* part = DW ? g.dw_part : g.dx_part;
+                kr_float4* o = reinterpret_cast<kr_float4*>(part + ((size_t)split * M + m) * g.C + n);
+                if (!DW && !g.first) v += *o;
+                *o = v;
+            } else {
+                v *= down;
+                const size_t o = (size_t)m * g.C + n;
+                if (g.f32) *reinterpret_cast<kr_float4*>(static_cast<float*>(g.dW) + o) = v;
+                else
+                    *reinterpret_cast<kr_half4*>(static_cast<kr_half*>(g.dW) + o) =
+                        kr_half4{kr_f16(v[0]), kr_f16(v[1]), kr_f16(v[2]), kr_f16(v[3])};
+            }
+        }
+    }
+}
+
+__global__ void __launch_bounds__(512, 1) grad_products_kernel(ProdArgs g) {
+    __shared__ __attribute__((aligned(1024))) kr_half8 ring[2 * kProdStage];
+    // an eighth of the items for each XCD, dW's before dx's
+    int b = blockIdx.x;
+    if (b < g.dw_items) {
+        const int per = (g.dw_items + 7) / 8, full = g.dw_items % 8 ? g.dw_items % 8 : 8;
+        const int xcd = b & 7, i = b >> 3;
+        const int item = xcd < full ? xcd * per + i : full * per + (xcd - full) * (per - 1) + i;
+        product_tile<true>(g, ring, item);
+    } else {
+        b -= g.dw_items;
+        const int per = (g.dx_items + 7) / 8, full = g.dx_items % 8 ? g.dx_items % 8 : 8;
+        const int xcd = b & 7, i = b >> 3;
+        const int item = xcd < full ? xcd * per + i : full * per + (xcd - full) * (per - 1) + i;
+        product_tile<false>(g, ring, item);
+    }
+}
+
+// Sum of the splits of n outputs, in their order.
+__global__ void __launch_bounds__(256) grad_sum_kernel(const float* part, long long stride, int splits, long long n,
+                                                       const float* scale, int f32, void* out) {
+    const long long at = 4 * ((long long)blockIdx.x * 256 + threadIdx.x);
+    if (at >= n) return;
+    kr_float4 v = *reinterpret_cast<const kr_float4*>(part + at);
+    for (int s = 1; s < splits; s++) v += *reinterpret_cast<const kr_float4*>(part + s * stride + at);
+    v *= scale[1];
+    if (f32) *reinterpret_cast<kr_float4*>(static_cast<float*>(out) + at) = v;
+    else
+        *reinterpret_cast<kr_half4*>(static_cast<kr_half*>(out) + at) =
+            kr_half4{kr_f16(v[0]), kr_f16(v[1]), kr_f16(v[2]), kr_f16(v[3])};
+}
+
+template <int WM, int WN, bool GRAD>
+int launch_logits(const LossArgs& g, hipStream_t s) {
+    const int gy = ((GRAD ? g.rows : g.N) + 64 * WM - 1) / (64 * WM), gx = (g.V + 128 * WN - 1) / (128 * WN);
+    const int n_virtual = (int)(((long long)gx * gy + 7) / 8 * 8);
+    const int at_once = 256 * (WM * WN >= 8 ? 1 : 2);
+    const int grid = n_virtual < at_once ? n_virtual : at_once;
+    // about 1.25 MB of x to a group of row tiles, as an L2 holds beside W's
+    const int group_m = (int)std::min<long long>(8, std::max<long long>(1, (5ll << 18) / (64 * WM * 2ll * g.C)));
+    logits_kernel<WM, WN, GRAD><<<grid, 64 * WM * WN, 0, s>>>(g, n_virtual, group_m);
+    KR_LAUNCHED();
+    return KR_OK;
+}
+
+template <bool GRAD>
+int logits(const LossArgs& g, hipStream_t s) {
+    return g.N > 128 ? launch_logits<4, 2, GRAD>(g, s) : launch_logits<1, 1, GRAD>(g, s);
+}
+
+bool shape_ok(int N, int C, int V) {
+    return N >= 0 && N <= 1 << 24 && C >= 64 && C % 64 == 0 && C <= 1 << 14 && V >= 1 && V <= 1 << 24;
+}
+
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+
+// How a backward call is cut: pieces of the vocabulary whose dz takes at most
+// 256 MB, and the products' splits.
+struct GradPlan {
+    int rows, piece, pieces, dx_splits, dw_splits;
+    size_t scale, x, G, dx_part, dw_part, total;      // offsets in the workspace
+};
+
+GradPlan grad_plan(int N, int C, int V, bool dx, bool dw) {
+    GradPlan p{};
+    p.rows = (N + 63) / 64 * 64;
+    const long long most = std::max<long long>(256, (128ll << 20) / p.rows / 256 * 256);
+    p.pieces = (int)((V + most - 1) / most);
+    p.piece = ((V + p.pieces - 1) / p.pieces + 255) / 256 * 256;
+    p.pieces = (V + p.piece - 1) / p.piece;
+    const int gx = (C + 255) / 256;
+    const int dx_steps = p.piece / 64, dw_steps = p.rows / 64;
+    const long long dx_tiles = (long long)(p.rows + 255) / 256 * gx, dw_tiles = (long long)p.piece / 256 * gx;
+    const long long total = (dx ? dx_tiles * dx_steps : 0) + (dw ? dw_tiles * dw_steps : 0);
+    const long long each = std::max<long long>(8, total / 1024);
+    p.dx_splits = (int)std::max<long long>(1, std::min<long long>(64, dx_steps / each));
+    p.dw_splits = dw_tiles >= 128 ? 1 : (int)std::max<long long>(1, std::min<long long>(64, dw_steps / each));
+    size_t at = 256;
+    p.x = at;
+    at += up256((size_t)p.rows * C * 2);
+    p.G = at;
+    at += up256((size_t)p.rows * p.piece * 2);
+    p.dx_part = at;
+    if (dx) at += up256((size_t)p.dx_splits * p.rows * C * 4);
+    p.dw_part = at;
+    if (dw && p.dw_splits > 1) at += up256((size_t)p.dw_splits * std::min(V, p.piece) * C * 4);
+    p.total = at;
+    return p;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t kr_head_loss_workspace_bytes(int N, int C, int V) {
+    if (!shape_ok(N, C, V) || N == 0) return 0;
+    return up256((size_t)N * 4) + (size_t)((V + kPart - 1) / kPart) * N * sizeof(float2);
+}
+
+int kr_head_loss(const uint16_t* x, long long ldx, int N, int C, const uint16_t* W, long long ldw, int V,
+                 const int32_t* targets, float* loss, float* lse, void* ws, size_t ws_bytes, void* stream) {
+    KR_REQUIRE(shape_ok(N, C, V), "kr_head_loss: bad shape N=%d C=%d V=%d (C a multiple of 64 up to 16384, N and V up to 2^24)",
+               N, C, V);
+    KR_REQUIRE(ldx >= C && ldw >= C && (ldx | ldw) % 8 == 0 && (ldx | ldw) < 1 << 21,
+               "kr_head_loss: row strides must be multiples of 8, at least C = %d and below 2^21", C);
+    if (N == 0) return KR_OK;
+    KR_REQUIRE(x && W && targets && loss && lse, "kr_head_loss: null pointer");
+    KR_REQUIRE((((uintptr_t)x | (uintptr_t)W) & 15) == 0, "kr_head_loss: x and W must be 16-byte aligned");
+    const size_t need = kr_head_loss_workspace_bytes(N, C, V);
+    KR_REQUIRE(ws && ws_bytes >= need && ((uintptr_t)ws & 255) == 0,
+               "kr_head_loss: workspace of %zu bytes, %zu needed (256-byte aligned)", ws_bytes, need);
+    LossArgs g{};
+    g.x = reinterpret_cast<const kr_half*>(x);
+    g.W = reinterpret_cast<const kr_half*>(W);
+    g.ldx = ldx;
+    g.ldw = ldw;
+    g.targets = targets;
+    g.hit = static_cast<float*>(ws);
+    g.part = reinterpret_cast<float2*>(static_cast<char*>(ws) + up256((size_t)N * 4));
+    g.N = N;
+    g.C = C;
+    g.V = g.v_all = V;
+    const hipStream_t s = kr_stream(stream);
+    const int rc = logits<false>(g, s);
+    if (rc != KR_OK) return rc;
+    loss_join_kernel<<<(N + 15) / 16, 256, 0, s>>>(g.part, g.hit, N, (V + kPart - 1) / kPart, V, targets, loss, lse);
+    KR_LAUNCHED();
+    return KR_OK;
+}
+
+size_t kr_head_loss_backward_workspace_bytes(int N, int C, int V, int dx, int dw) {
+    if (!shape_ok(N, C, V) || N == 0) return 0;
+    return grad_plan(N, C, V, dx != 0, dw != 0).total;
+}
+
+int kr_head_loss_backward(const uint16_t* x, long long ldx, int N, int C, const uint16_t* W, long long ldw, int V,
+                          const int32_t* targets, const float* lse, const float* dloss, int out_f32, void* dx,
+                          void* dW, void* ws, size_t ws_bytes, void* stream) {
+    KR_REQUIRE(shape_ok(N, C, V),
+               "kr_head_loss_backward: bad shape N=%d C=%d V=%d (C a multiple of 64 up to 16384, N and V up to 2^24)",
+               N, C, V);
+    KR_REQUIRE(N >= 1, "kr_head_loss_backward: no rows");
+    KR_REQUIRE(ldx >= C && ldw >= C && (ldx | ldw) % 8 == 0 && (ldx | ldw) < 1 << 21,
+               "kr_head_loss_backward: row strides must be multiples of 8, at least C = %d and below 2^21", C);
+    KR_REQUIRE(x && W && targets && lse && dloss && (dx || dW), "kr_head_loss_backward: null pointer");
+    KR_REQUIRE((((uintptr_t)x | (uintptr_t)W | (uintptr_t)dx | (uintptr_t)dW) & 15) == 0,
+               "kr_head_loss_backward: x, W, dx and dW must be 16-byte aligned");
+    const GradPlan p = grad_plan(N, C, V, dx != nullptr, dW != nullptr);
+    KR_REQUIRE(ws && ws_bytes >= p.total && ((uintptr_t)ws & 255) == 0,
+               "kr_head_loss_backward: workspace of %zu bytes, %zu needed (256-byte aligned)", ws_bytes, p.total);
+    char* base = static_cast<char*>(ws);
+    float* scale = reinterpret_cast<float*>(base);
+    kr_half* live = reinterpret_cast<kr_half*>(base + p.x);
+    const kr_half* xh = reinterpret_cast<const kr_half*>(x);
+    const hipStream_t s = kr_stream(stream);
+    grad_scale_kernel<<<1, 1024, 0, s>>>(targets, dloss, N, scale);
+    KR_LAUNCHED();
+    if (dW) {
+        const long long units = (long long)p.rows * (C / 8);
+        live_rows_kernel<<<(unsigned)((units + 255) / 256), 256, 0, s>>>(xh, ldx, N, C, p.rows, targets, dloss, live);
+        KR_LAUNCHED();
+    }
+    LossArgs g{};
+    g.x = xh;
+    g.ldx = ldx;
+    g.ldw = ldw;
+    g.targets = targets;
+    g.lse = lse;
+    g.dloss = dloss;
+    g.scale = scale;
+    g.G = reinterpret_cast<kr_half*>(base + p.G);
+    g.ldg = p.piece;
+    g.N = N;
+    g.C = C;
+    g.v_all = V;
+    g.rows = p.rows;
+    ProdArgs d{};
+    d.G = g.G;
+    d.ldg = g.ldg;
+    d.x = live;
+    d.ldw = ldw;
+    d.scale = scale;
+    d.dx_part = reinterpret_cast<float*>(base + p.dx_part);
+    d.dw_part = reinterpret_cast<float*>(base + p.dw_part);
+    d.f32 = out_f32 != 0;
+    d.rows = p.rows;
+    d.C = C;
+    d.dx_splits = p.dx_splits;
+    d.dw_splits = p.dw_splits;
+    const int gx = (C + 255) / 256;
+    for (int i = 0; i < p.pieces; i++) {
+        const int v0 = i * p.piece, nv = std::min(V - v0, p.piece);
+        g.W = d.W = reinterpret_cast<const kr_half*>(W) + (size_t)v0 * ldw;
+        g.V = d.V = nv;
+        g.v0 = v0;
+        const int rc = logits<true>(g, s);
+        if (rc != KR_OK) return rc;
+        d.first = i == 0;
+        d.dW = dW ? static_cast<char*>(dW) + (size_t)v0 * C * (out_f32 ? 4 : 2) : nullptr;
+        d.dw_items = dW ? (nv + 255) / 256 * gx * p.dw_splits : 0;
+        d.dx_items = dx ? (p.rows + 255) / 256 * gx * p.dx_splits : 0;
+        grad_products_kernel<<<d.dw_items + d.dx_items, 512, 0, s>>>(d);
+        KR_LAUNCHED();
+        if (dW && p.dw_splits > 1) {
+            const long long n = (long long)nv * C;
+            grad_sum_kernel<<<(unsigned)((n / 4 + 255) / 256), 256, 0, s>>>(d.dw_part, n, p.dw_splits, n, scale, out_f32,
+                                                                           d.dW);
+            KR_LAUNCHED();
+        }
+    }
+    if (dx) {
+        const long long n = (long long)N * C;
+        grad_sum_kernel<<<(unsigned)((n / 4 + 255) / 256), 256, 0, s>>>(d.dx_part, (long long)p.rows * C, p.dx_splits, n,
+                                                                       scale, out_f32, dx);
+        KR_LAUNCHED();
+    }
+    return KR_OK;
+}
+
+}  // extern "C"

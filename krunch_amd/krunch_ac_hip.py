@@ -230,6 +230,88 @@ def token_scores(logits, tokens, n_top: int = 0):
     return logprob, entropy, top_logprob, top_token
 
 
+def _head_rows(t, name, C):
+    """Row stride of a [rows, C] fp16 operand of a head."""
+    (t.is_cuda and t.dtype is torch.float16 and t.dim() == 2) or _refuse(
+        f"{name} must be a 2-dimensional float16 device tensor")
+    t.shape[1] == C or _refuse(f"{name} has {t.shape[1]} columns, the head {C}")
+    ld, step = t.stride()
+    if t.shape[0] <= 1:
+        ld = C
+    (step == 1 and C <= ld < 1 << 21 and ld % 8 == 0 and t.data_ptr() % 16 == 0) or _refuse(
+        f"{name} rows must be contiguous, 16-byte aligned and not overlap, their stride below 2^21")
+    return ld
+
+
+def _head_vector(t, dtype, name, N, dev):
+    (t.is_cuda and t.dtype is dtype and t.is_contiguous() and t.shape == (N,) and t.get_device() == dev) or _refuse(
+        f"{name} must be a contiguous {dtype} device tensor [N] = [{N}] on x's device")
+
+
+def _head_shapes(x, W, targets):
+    W.dim() == 2 or _refuse("W must be [V, C]")
+    V, C = W.shape
+    (V >= 1 and 64 <= C <= 16384 and C % 64 == 0) or _refuse(
+        f"W must be [V, C] with C a multiple of 64 up to 16384, got {tuple(W.shape)}")
+    ldx, ldw = _head_rows(x, "x", C), _head_rows(W, "W", C)
+    N = x.shape[0]
+    max(N, V) <= 1 << 24 or _refuse("N and V must be at most 2^24")
+    dev = x.get_device()
+    W.get_device() == dev or _refuse("x and W must be on one device")
+    _head_vector(targets, torch.int32, "targets", N, dev)
+    return N, C, V, ldx, ldw
+
+
+def head_loss(x, W, targets):
+    """Cross entropy in nats of the next tokens under a head, without its logits:
+    x fp16 [N, C] (what the head reads, normalised), W fp16 [V, C] (as a prepared
+    model keeps its head; rows of both may be strided), targets int32 [N] -> (loss
+    [N], lse [N]) fp32 with z = x @ W.T, lse = logsumexp(z), loss = lse -
+    z[target]. A target of -1 is none (loss 0); other ids outside 0..V-1 give NaN.
+    C must be a multiple of 64. z stays in fp32, so a loss differs from
+    token_scores' of fp16 logits by their rounding. No autograd:
+    head_loss_backward takes lse and gives the gradients."""
+    N, C, V, ldx, ldw = _head_shapes(x, W, targets)
+    if _elsewhere(x):
+        return _on_device_of(x, head_loss, x, W, targets)
+    loss = torch.empty_like(targets, dtype=torch.float32)
+    lse = torch.empty_like(loss)
+    nbytes = _lib.lib().kr_head_loss_workspace_bytes(N, C, V)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    _lib.call("kr_head_loss", x.data_ptr(), ldx, N, C, W.data_ptr(), ldw, V, targets.data_ptr(),
+              loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), nbytes, _lib.stream_ptr())
+    return loss, lse
+
+
+def head_loss_backward(x, W, targets, lse, dloss, out_dtype=None, dx: bool = True, dW: bool = True):
+    """Gradients of head_loss: x, W, targets as there, its lse, and dloss fp32 [N]
+    (the gradient of each loss) -> (dx [N, C], dW [V, C]), fp16 or fp32 by
+    out_dtype, None for one that is not wanted. Rows with target -1 or dloss 0 have
+    no gradient. The gradient of the logits is rounded to fp16 relative to the
+    largest |dloss|; sums are fp32. For fp16 outputs dloss may carry a loss scale."""
+    N, C, V, ldx, ldw = _head_shapes(x, W, targets)
+    dev = x.get_device()
+    _head_vector(lse, torch.float32, "lse", N, dev)
+    _head_vector(dloss, torch.float32, "dloss", N, dev)
+    f32 = out_dtype is torch.float32
+    f32 or out_dtype in (None, torch.float16) or _refuse(f"out_dtype must be float16 or float32, got {out_dtype}")
+    if _elsewhere(x):
+        return _on_device_of(x, head_loss_backward, x, W, targets, lse, dloss, out_dtype, dx, dW)
+    dtype = torch.float32 if f32 else torch.float16
+    gx = x.new_empty((N, C), dtype=dtype) if dx else None
+    gw = x.new_empty((V, C), dtype=dtype) if dW else None
+    if N == 0:
+        return gx, None if gw is None else gw.zero_()
+    if not (dx or dW):
+        return None, None
+    nbytes = _lib.lib().kr_head_loss_backward_workspace_bytes(N, C, V, 1 if dx else 0, 1 if dW else 0)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    _lib.call("kr_head_loss_backward", x.data_ptr(), ldx, N, C, W.data_ptr(), ldw, V, targets.data_ptr(),
+              lse.data_ptr(), dloss.data_ptr(), f32, _lib.ptr(gx), _lib.ptr(gw), ws.data_ptr(), nbytes,
+              _lib.stream_ptr())
+    return gx, gw
+
+
 # ---------------------------------------------------------------------------
 # matmul / layer ops (layer_cpp.cpp)
 # ---------------------------------------------------------------------------
