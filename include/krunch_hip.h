@@ -449,6 +449,48 @@ int kr_wkv_heads(int B, int T, int H, int D, const uint16_t* r, long long ldr, c
                  const float* first, const int32_t* lens, float* state, uint16_t* y, long long ldy,
                  int chunked, void* ws, size_t ws_bytes, void* stream);
 
+/* The gated delta rule (no reference counterpart; beside kr_wkv_heads, for models
+ * whose keys replace what they had stored): q, k, v fp16 [B, T, H, D] by token strides
+ * ldq, ldk, ldv (elements, multiples of 8; streams follow at T tokens), log_decay (g)
+ * and beta fp32 [B, T, H] by token strides ldg, ldb, state fp32 [B, H, D, D] (key
+ * channel major) updated in place, y fp16 by ldy:
+ *   S <- e^g S;  u = beta (v_t - k_t S);  S <- S + k_t' u;  y_t = q_t S
+ * g above 0 counts as 0, below -10000 (-inf too) is no memory. D is 64 or 128. lens
+ * (nullable = T) gives each stream's tokens, clamped to 0..T: its state stops there and
+ * its later rows of y are zeros, whatever the inputs hold there. chunked = 0: token by
+ * token in fp32; T tokens in one call have the bits of T calls of one. chunked = 1:
+ * 64 tokens at a time on the matrix units, for prompts: equal to that up to rounding
+ * (2^-22 of a value that enters the matrix units: a state element, a weight between two
+ * tokens, what a token writes; and 2^-38 of the largest one of its column or row); a
+ * NaN or infinity of a token then also reaches y of up to 63 tokens before it. Calls of
+ * at most 8 tokens are the same in both. Keys of length 1 and beta in 0..1 keep the
+ * recurrence stable; others are computed, too. y must not overlap q, k or v. ws:
+ * kr_gated_delta_workspace_bytes (chunked only, may be 0), 16-byte aligned, as q, k, v,
+ * state and y. */
+size_t kr_gated_delta_workspace_bytes(int B, int T, int H, int D);
+int kr_gated_delta(int B, int T, int H, int D, const uint16_t* q, long long ldq, const uint16_t* k,
+                   long long ldk, const uint16_t* v, long long ldv, const float* log_decay, long long ldg,
+                   const float* beta, long long ldb, const int32_t* lens, float* state, uint16_t* y,
+                   long long ldy, int chunked, void* ws, size_t ws_bytes, void* stream);
+
+/* Gradients of kr_gated_delta (chunked): its inputs, with state as it was before the
+ * call; dy fp16 [B, T, H, D] by ldy, and dstate fp32 [B, H, D, D], the gradient of the
+ * state after the call (NULL: zeros). Writes dq, dk, dv fp16 [B, T, H, D], dlog_decay and
+ * dbeta fp32 [B, T, H], all contiguous, and dstate0 fp32 [B, H, D, D], the gradient
+ * of state. Tokens past lens have gradient 0, as a log_decay above 0 or below -10000
+ * has. Values rounded as in the forward pass, sums fp32. T <= 4194240. ws:
+ * kr_gated_delta_backward_workspace_bytes (for each head and 64 tokens two states and two
+ * rows of D fp32 values a token: 8 D (D + 64) bytes), 256-byte aligned; it must not
+ * overlap anything, nor outputs the inputs. Everything but log_decay, beta, lens and
+ * their gradients is 16-byte aligned. */
+size_t kr_gated_delta_backward_workspace_bytes(int B, int T, int H, int D);
+int kr_gated_delta_backward(int B, int T, int H, int D, const uint16_t* q, long long ldq, const uint16_t* k,
+                            long long ldk, const uint16_t* v, long long ldv, const float* log_decay,
+                            long long ldg, const float* beta, long long ldb, const int32_t* lens,
+                            const float* state, const uint16_t* dy, long long ldy, const float* dstate,
+                            uint16_t* dq, uint16_t* dk, uint16_t* dv, float* dlog_decay, float* dbeta,
+                            float* dstate0, void* ws, size_t ws_bytes, void* stream);
+
 /* All layers over x [B*T, C] (cpp_path.forward_packed_window's layer loop,
  * :155-160; forward_stepped_batched's with T = 1, :451-456). */
 int kr_forward_layers(const kr_model_weights* m, void* x, int B, int T, void* state, void* ws,

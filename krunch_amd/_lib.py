@@ -89,6 +89,11 @@ _SIGS = {
     "kr_head_loss": ([P, LL, I, I, P, LL, I, P, P, P, P, SZ, P], I),
     "kr_head_loss_backward_workspace_bytes": ([I, I, I, I, I], SZ),
     "kr_head_loss_backward": ([P, LL, I, I, P, LL, I, P, P, P, I, P, P, P, SZ, P], I),
+    "kr_gated_delta_workspace_bytes": ([I, I, I, I], SZ),
+    "kr_gated_delta": ([I, I, I, I, P, LL, P, LL, P, LL, P, LL, P, LL, P, P, P, LL, I, P, SZ, P], I),
+    "kr_gated_delta_backward_workspace_bytes": ([I, I, I, I], SZ),
+    "kr_gated_delta_backward": ([I, I, I, I, P, LL, P, LL, P, LL, P, LL, P, LL, P, P, P, LL, P, P, P, P, P, P, P,
+                                 P, SZ, P], I),
     "kr_wkv_heads_workspace_bytes": ([I, I, I, I], SZ),
     "kr_wkv_heads": ([I, I, I, I, P, LL, P, LL, P, LL, P, P, P, P, P, LL, I, P, SZ, P], I),
     "kr_phase_profile": ([I], I),

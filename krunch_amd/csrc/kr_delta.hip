@@ -1,0 +1,1462 @@
+// The gated delta rule: a matrix state [D, D] per head of D = 64 or 128 channels, a
+// decay and a write strength per token and head.
+//
+//   S <- e^g S;  u = beta (v - k S);  S <- S + k' u;  y = q S          (g <= 0)
+//
+// Two forms. The recurrent one runs token by token in fp32. The chunked one takes
+// 64 tokens at a time: with a_i the sum of g to token i of the chunk and
+//   A_ij = e^(a_i - a_j) k_i k_j' (j < i),  P_ij = e^(a_i - a_j) q_i k_j' (j <= i)
+// what the tokens find different from the state, r = v - e^a k S - A u with u = beta r,
+// is the solution of a triangular system, and
+//   y = e^a q S + P u;   S <- e^a_end S + sum_j k_j' (e^(a_end - a_j) u_j).
+// For a block of tokens r = X - N (beta X) with N = A (1 + beta A)^-1, strictly
+// lower triangular: no division by beta, exact where beta is 0. N of 16 x 16
+// blocks comes from forward substitution (powers of beta A would cancel where keys repeat), of
+// 32 x 32 from two products; the two halves of a chunk are solved in turn.
+//
+// q, k, v enter the matrix units (v_mfma_f32_16x16x32_f16) as they are; fp32 values
+// that do too, S, P, N, A and columns of beta X and u, go in as two fp16 parts, high
+// and low, scaled by a power of two to 2^14: 22 bits of each value, and 2^-38 of
+// the largest one of a row (P, N, A) or of a column (S, beta X, u).
+#include "kr_common.h"
+#include "kr_wave.h"
+#include "krunch_hip.h"
+
+namespace {
+
+constexpr int kChunk = 64;
+
+struct DeltaArgs {
+    const kr_half* q;
+    const kr_half* k;
+    const kr_half* v;
+    long long ldq, ldk, ldv;      // elements between tokens; a head's D are contiguous
+    const float* gate;            // log decays, [B, T] by ldg, heads contiguous
+    const float* beta;
+    long long ldg, ldb;
+    const int32_t* lens;          // [B] tokens of each stream (null: T)
+    float* state;                 // [B, H, D, D]
+    kr_half* y;                   // [B, T, H, D] by ldy
+    long long ldy;
+    float* before;                // STATES: [chunks + 1][heads][D][D], the state before each chunk
+    float* diff;                  // STATES: [chunks][heads][64][D], r
+    int B, T, H;
+};
+
+__device__ __forceinline__ int stream_tokens(const int32_t* lens, int b, int T) {
+    if (!lens) return T;
+    const int n = lens[b];
+    return n < 0 ? 0 : n < T ? n : T;
+}
+
+// log2 of a decay, sums of 64 of which stay finite: g above 0 counts as 0, below
+// -10000 as that (both e^g are 0), NaN stays.
+__device__ __forceinline__ double gate_log2(float g) {
+    g = g > 0.0f ? 0.0f : g < -10000.0f ? -10000.0f : g;
+    return (double)g * 0x1.71547652b82fep+0;
+}
+
+// ---------------------------------------------------------------------------
+// Recurrent form. A wave has 16 columns of a head's state in registers: lane l the
+// columns 4 (l % 4) .. + 3 of rows D/16 (l / 4) .. + D/16 - 1. k S, q S and k q' are
+// summed together over a lane's rows and then over 16 lanes: y = q S + (q k') u.
+// ---------------------------------------------------------------------------
+template <int D>
+__global__ void __launch_bounds__(4 * D) delta_step_kernel(DeltaArgs g) {
+    constexpr int R = D / 16;
+    typedef kr_half rows_t __attribute__((ext_vector_type(R)));
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int h = blockIdx.x % g.H, b = blockIdx.x / g.H;
+    const int m0 = 16 * wave + 4 * (lane & 3), n0 = R * (lane >> 2);
+    const int T = stream_tokens(g.lens, b, g.T);
+    float* st = g.state + ((size_t)blockIdx.x * D + n0) * D + m0;
+    const size_t row0 = (size_t)b * g.T;
+    const kr_half* qp = g.q + row0 * g.ldq + h * D + n0;
+    const kr_half* kp = g.k + row0 * g.ldk + h * D + n0;
+    const kr_half* vp = g.v + row0 * g.ldv + h * D + m0;
+    const float* gp = g.gate + row0 * g.ldg + h;
+    const float* bp = g.beta + row0 * g.ldb + h;
+    kr_half* yp = g.y + row0 * g.ldy + h * D + m0;
+    if (T > 0) {
+        kr_float4 S[R];
+        #pragma unroll
+        for (int i = 0; i < R; i++) S[i] = *reinterpret_cast<const kr_float4*>(st + i * D);
+        rows_t qn = *reinterpret_cast<const rows_t*>(qp), kn = *reinterpret_cast<const rows_t*>(kp);
+        kr_half4 vn = *reinterpret_cast<const kr_half4*>(vp);
+        float gn = *gp, bn = *bp;
+        for (int t = 0; t < T; t++) {
+            const rows_t qt = qn, kt = kn;
+            const kr_half4 vt = vn;
+            const float f = __builtin_amdgcn_exp2f((float)gate_log2(gn)), beta = bn;
+            if (t + 1 < T) {
+                qp += g.ldq;
+                kp += g.ldk;
+                vp += g.ldv;
+                gp += g.ldg;
+                bp += g.ldb;
+                qn = *reinterpret_cast<const rows_t*>(qp);
+                kn = *reinterpret_cast<const rows_t*>(kp);
+                vn = *reinterpret_cast<const kr_half4*>(vp);
+                gn = *gp;
+                bn = *bp;
+            }
+            kr_float4 kS = {0, 0, 0, 0}, qS = {0, 0, 0, 0};
+            float kq = 0.0f;
+            #pragma unroll
+            for (int i = 0; i < R; i++) {
+                kq = __builtin_fmaf((float)kt[i], (float)qt[i], kq);
+                #pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    S[i][c] *= f;
+                    kS[c] = __builtin_fmaf((float)kt[i], S[i][c], kS[c]);
+                    qS[c] = __builtin_fmaf((float)qt[i], S[i][c], qS[c]);
+                }
+            }
+            kq += kr_xor<4>(kq);
+            kq += kr_xor<8>(kq);
+            kq += kr_xor<16>(kq);
+            kq += kr_xor<32>(kq);
+            kr_half4 y;
+            #pragma unroll
+            for (int c = 0; c < 4; c++) {
+                kS[c] += kr_xor<4>(kS[c]);
+                qS[c] += kr_xor<4>(qS[c]);
+                kS[c] += kr_xor<8>(kS[c]);
+                qS[c] += kr_xor<8>(qS[c]);
+                kS[c] += kr_xor<16>(kS[c]);
+                qS[c] += kr_xor<16>(qS[c]);
+                kS[c] += kr_xor<32>(kS[c]);
+                qS[c] += kr_xor<32>(qS[c]);
+                const float u = beta * ((float)vt[c] - kS[c]);
+                #pragma unroll
+                for (int i = 0; i < R; i++) S[i][c] = __builtin_fmaf((float)kt[i], u, S[i][c]);
+                y[c] = kr_f16(__builtin_fmaf(kq, u, qS[c]));
+            }
+            if (lane < 4) *reinterpret_cast<kr_half4*>(yp) = y;
+            yp += g.ldy;
+        }
+        #pragma unroll
+        for (int i = 0; i < R; i++) *reinterpret_cast<kr_float4*>(st + i * D) = S[i];
+    }
+    if (lane < 4)
+        for (int t = T; t < g.T; t++, yp += g.ldy)
+            *reinterpret_cast<kr_half4*>(yp) = kr_half4{0, 0, 0, 0};
+}
+
+// ---------------------------------------------------------------------------
+// Parts of the chunked kernels.
+// ---------------------------------------------------------------------------
+
+// Powers of two that bring a largest value x to 2^13..2^14, and back. Zero and
+// values under 2^-113 count as 2^-113; infinities and NaN pass through.
+__device__ __forceinline__ void power_scale(float x, float& up, float& down) {
+    int e = (int)(__float_as_uint(x) >> 23);
+    e = e < 14 ? 14 : e;
+    up = __uint_as_float((uint32_t)(267 - e) << 23);
+    down = __uint_as_float((uint32_t)(e - 13) << 23);
+}
+
+// x as a high and a low fp16 part.
+__device__ __forceinline__ void two_parts(float x, kr_half& hi, kr_half& lo) {
+    __asm__("" : "+v"(x));
+    hi = (kr_half)x;
+    lo = (kr_half)(x - (float)hi);
+}
+
+__device__ __forceinline__ float max_of_quarters(float x) {       // over lanes l % 16
+    x = fmaxf(x, kr_xor<16>(x));
+    return fmaxf(x, kr_xor<32>(x));
+}
+
+// 8 values of a column or row that 4 lanes (l / 16) hold, in two parts.
+struct Parts8 {
+    kr_half8 hi, lo;
+};
+__device__ __forceinline__ float largest8(const float (&x)[8], float big = 0.0f) {
+    #pragma unroll
+    for (int e = 0; e < 8; e++) big = fmaxf(big, fabsf(x[e]));
+    return big;
+}
+__device__ __forceinline__ Parts8 parts8(const float (&x)[8], float up) {
+    Parts8 p;
+    #pragma unroll
+    for (int e = 0; e < 8; e++) {
+        kr_half a, b;
+        two_parts(x[e] * up, a, b);
+        p.hi[e] = a;
+        p.lo[e] = b;
+    }
+    return p;
+}
+__device__ __forceinline__ Parts8 scaled8(const float (&x)[8], float& down) {
+    float up;
+    power_scale(max_of_quarters(largest8(x)), up, down);
+    return parts8(x, up);
+}
+
+__device__ __forceinline__ kr_float4 mfma(kr_half8 a, kr_half8 b, kr_float4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+// a (two parts) times b (two parts), without low x low.
+__device__ __forceinline__ kr_float4 mfma3(kr_half8 ah, kr_half8 al, const Parts8& b, kr_float4 c) {
+    c = mfma(al, b.hi, c);
+    c = mfma(ah, b.lo, c);
+    return mfma(ah, b.hi, c);
+}
+
+// LDS tiles in 16-byte units. Of tokens [64][D]: unit c of token t. Of pairs
+// [64][64]: unit c (8 columns) of row i. The XORs keep the 8 lanes of a 16-byte access
+// on different banks.
+template <int D>
+__device__ __forceinline__ int tok_unit(int t, int c) { return t * (D / 8) + (c ^ (t & (D / 8 - 1))); }
+__device__ __forceinline__ int pair_unit(int i, int c) { return i * 8 + (c ^ ((i ^ (i >> 3)) & 7)); }
+
+// Transposing reads of a token tile: 8 tokens (32 s + 8 (l / 16) ..) of 16 channels,
+// one a lane. channels16: channel 16 tile + l % 16. channels_state: the channel of
+// row l % 16 of state tile st, 32 (st / 2) + 8 (l % 16 / 4) + 4 (st % 2) + l % 4.
+typedef short short4v __attribute__((__vector_size__(8)));
+typedef __attribute__((address_space(3))) short4v lds_short4;
+template <int D>
+__device__ __forceinline__ kr_half8 read_tokens(const kr_half8* tile, int s, int unit, int half, int lane) {
+    typedef kr_half half4v __attribute__((ext_vector_type(4)));
+    const int t = 32 * s + 8 * (lane >> 4) + ((lane & 15) >> 2);
+    const unsigned base = (unsigned)(uintptr_t)(__attribute__((address_space(3))) const char*)tile + 8 * half;
+    const unsigned at0 = base + 16 * tok_unit<D>(t, unit), at1 = base + 16 * tok_unit<D>(t + 4, unit);
+    const half4v a = __builtin_bit_cast(half4v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(uintptr_t)at0));
+    const half4v b = __builtin_bit_cast(half4v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(uintptr_t)at1));
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+template <int D>
+__device__ __forceinline__ kr_half8 channels16(const kr_half8* tile, int s, int t16, int lane) {
+    return read_tokens<D>(tile, s, 2 * t16 + ((lane & 3) >> 1), lane & 1, lane);
+}
+template <int D>
+__device__ __forceinline__ kr_half8 channels_state(const kr_half8* tile, int s, int st, int lane) {
+    return read_tokens<D>(tile, s, 4 * (st >> 1) + (lane & 3), st & 1, lane);
+}
+
+// Per chunk: sums of log2 decays, and what follows from them.
+struct Gates {
+    double a[kChunk];
+    float e0[kChunk], e1[kChunk], beta[kChunk];   // e^a, e^(a_end - a), write strengths
+    float all;                                    // e^a_end
+};
+// By one wave, lane = token.
+__device__ __forceinline__ void make_gates(Gates& o, float gate, float beta, int lane) {
+    double a = gate_log2(gate);
+    #pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const double b = __shfl_up(a, d);
+        if (lane >= d) a += b;
+    }
+    const double end = __shfl(a, 63);
+    o.a[lane] = a;
+    o.e0[lane] = __builtin_amdgcn_exp2f((float)a);
+    o.e1[lane] = __builtin_amdgcn_exp2f((float)(end - a));
+    o.beta[lane] = beta;
+    if (lane == 63) o.all = __builtin_amdgcn_exp2f((float)end);
+}
+
+// The triangular matrices of a chunk as operands: rows i, units of 8 j. M holds N
+// of the chunk's two halves in its diagonal 32 x 32 blocks and A below them. With
+// TRANSPOSED, rows are j and units i, of all three.
+struct Pairs {
+    kr_half8 ph[kChunk * 8], pl[kChunk * 8];
+    kr_half8 mh[kChunk * 8], ml[kChunk * 8];
+    float p_down[kChunk], n_down[kChunk], a_down[kChunk];
+    float work[2][32 * 33];       // fp32 A, then N, of the two halves
+};
+
+__device__ __forceinline__ void store_parts4(kr_half8* hi, kr_half8* lo, int row, int col, kr_float4 x, float up) {
+    kr_half4 h, l;
+    #pragma unroll
+    for (int r = 0; r < 4; r++) {
+        kr_half a, b;
+        two_parts(x[r] * up, a, b);
+        h[r] = a;
+        l[r] = b;
+    }
+    const int at = pair_unit(row, col / 8);
+    reinterpret_cast<kr_half4*>(hi + at)[col / 4 & 1] = h;
+    reinterpret_cast<kr_half4*>(lo + at)[col / 4 & 1] = l;
+}
+
+// P (or P') of 16 rows by one wave, w = 0..3.
+template <int D, bool TRANSPOSED>
+__device__ __forceinline__ void make_p(Pairs& o, const kr_half8* q, const kr_half8* k, const Gates& gates, int w,
+                                       int lane) {
+    constexpr int KS = D / 32;
+    const int l16 = lane & 15, q4 = lane >> 4, row = 16 * w + l16;
+    kr_half8 mine[KS];
+    #pragma unroll
+    for (int s = 0; s < KS; s++) mine[s] = (TRANSPOSED ? k : q)[tok_unit<D>(row, 4 * s + q4)];
+    const double a = gates.a[row];
+    kr_float4 P[4];
+    float big = 0.0f;
+    #pragma unroll
+    for (int ct = 0; ct < 4; ct++) {
+        P[ct] = kr_float4{0, 0, 0, 0};
+        if (TRANSPOSED ? ct < w : ct > w) continue;
+        #pragma unroll
+        for (int s = 0; s < KS; s++)
+            P[ct] = mfma((TRANSPOSED ? q : k)[tok_unit<D>(16 * ct + l16, 4 * s + q4)], mine[s], P[ct]);
+        #pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const int col = 16 * ct + 4 * q4 + r;
+            const double d = TRANSPOSED ? gates.a[col] - a : a - gates.a[col];
+            const bool on = TRANSPOSED ? col >= row : col <= row;
+            P[ct][r] = on ? P[ct][r] * __builtin_amdgcn_exp2f((float)d) : 0.0f;
+            big = fmaxf(big, fabsf(P[ct][r]));
+        }
+    }
+    float up, down;
+    power_scale(max_of_quarters(big), up, down);
+    if (q4 == 0) o.p_down[row] = down;
+    #pragma unroll
+    for (int ct = 0; ct < 4; ct++) {
+        // tiles of zeros inside a k-step of 32 are written, too
+        if (TRANSPOSED ? ct / 2 < w / 2 : ct / 2 > w / 2) continue;
+        store_parts4(o.ph, o.pl, row, 16 * ct + 4 * q4, P[ct], up);
+    }
+}
+
+// A of 16 rows by one wave: the half's own part as fp32, the part below as operand.
+template <int D, bool TRANSPOSED>
+__device__ __forceinline__ void make_a(Pairs& o, const kr_half8* k, const Gates& gates, int w, int lane) {
+    constexpr int KS = D / 32;
+    const int l16 = lane & 15, q4 = lane >> 4, row = 16 * w + l16;
+    kr_half8 mine[KS];
+    #pragma unroll
+    for (int s = 0; s < KS; s++) mine[s] = k[tok_unit<D>(row, 4 * s + q4)];
+    const double a = gates.a[row];
+    // the half's own: rows i, columns j
+    float* work = o.work[w / 2] + (row & 31) * 33;
+    #pragma unroll
+    for (int ct = 0; ct < 2; ct++) {
+        if (ct > (w & 1)) continue;
+        kr_float4 A = {0, 0, 0, 0};
+        #pragma unroll
+        for (int s = 0; s < KS; s++) A = mfma(k[tok_unit<D>(32 * (w / 2) + 16 * ct + l16, 4 * s + q4)], mine[s], A);
+        #pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const int col = 16 * ct + 4 * q4 + r;
+            const float e = __builtin_amdgcn_exp2f((float)(a - gates.a[32 * (w / 2) + col]));
+            work[col] = col < (row & 31) ? A[r] * e : 0.0f;
+        }
+    }
+    // below: rows 32.. against columns 0..31, or transposed
+    if (TRANSPOSED ? w < 2 : w >= 2) {
+        const int c0 = TRANSPOSED ? 32 : 0;
+        kr_float4 A[2];
+        float big = 0.0f;
+        #pragma unroll
+        for (int ct = 0; ct < 2; ct++) {
+            A[ct] = kr_float4{0, 0, 0, 0};
+            #pragma unroll
+            for (int s = 0; s < KS; s++) A[ct] = mfma(k[tok_unit<D>(c0 + 16 * ct + l16, 4 * s + q4)], mine[s], A[ct]);
+            #pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const double b = gates.a[c0 + 16 * ct + 4 * q4 + r];
+                A[ct][r] *= __builtin_amdgcn_exp2f((float)(TRANSPOSED ? b - a : a - b));
+                big = fmaxf(big, fabsf(A[ct][r]));
+            }
+        }
+        float up, down;
+        power_scale(max_of_quarters(big), up, down);
+        if (q4 == 0) o.a_down[row] = down;
+        #pragma unroll
+        for (int ct = 0; ct < 2; ct++) store_parts4(o.mh, o.ml, row, c0 + 16 * ct + 4 * q4, A[ct], up);
+    }
+}
+
+// N of the 16 x 16 diagonal block w, in place of A, by the wave that wrote it: row
+// by row, N_t = A_t - sum_j A_tj (beta_j N_j); lane = column.
+__device__ __forceinline__ void solve_16(Pairs& o, const Gates& gates, int w, int lane) {
+    const int l16 = lane & 15, q4 = lane >> 4;
+    float* block = o.work[w / 2] + 16 * (w & 1) * 34;
+    const float* beta = gates.beta + 16 * w;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    float N[16], bN[16];
+    #pragma unroll
+    for (int t = 0; t < 16; t++) {
+        float x = block[33 * t + l16];
+        #pragma unroll
+        for (int j = 0; j < t; j++) x = __builtin_fmaf(-block[33 * t + j], bN[j], x);
+        N[t] = x;
+        bN[t] = beta[t] * x;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    #pragma unroll
+    for (int t = 0; t < 16; t++)
+        if (t / 4 == q4) block[33 * t + l16] = N[t];
+}
+
+// The 16 x 16 block below, by one wave for each half: with Y = A10 - A10 (beta N00),
+// N10 = Y - N11 (beta Y).
+__device__ __forceinline__ void solve_32(Pairs& o, const Gates& gates, int half, int lane) {
+    const int l16 = lane & 15, q4 = lane >> 4;
+    float* work = o.work[half];
+    const float* beta = gates.beta + 32 * half;
+    kr_float4 Y;
+    #pragma unroll
+    for (int r = 0; r < 4; r++) Y[r] = work[33 * (16 + 4 * q4 + r) + l16];
+    #pragma unroll
+    for (int s = 0; s < 4; s++) {
+        const int j = 4 * q4 + s;
+        Y = __builtin_amdgcn_mfma_f32_16x16x4f32(-work[33 * (16 + l16) + j], beta[j] * work[33 * j + l16], Y, 0, 0, 0);
+    }
+    kr_float4 N = Y;
+    #pragma unroll
+    for (int s = 0; s < 4; s++) {
+        const int j = 16 + 4 * q4 + s;
+        N = __builtin_amdgcn_mfma_f32_16x16x4f32(-work[33 * (16 + l16) + j], beta[j] * Y[s], N, 0, 0, 0);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    #pragma unroll
+    for (int r = 0; r < 4; r++) work[33 * (16 + 4 * q4 + r) + l16] = N[r];
+}
+
+// 16 rows of N of a half (columns for TRANSPOSED) as operands, by one wave.
+template <bool TRANSPOSED>
+__device__ __forceinline__ void store_n(Pairs& o, int w, int lane) {
+    const int l16 = lane & 15, q4 = lane >> 4, row = 16 * w + l16;
+    const float* work = o.work[w / 2];
+    float x[8];
+    #pragma unroll
+    for (int e = 0; e < 8; e++) {
+        const int i = TRANSPOSED ? 8 * q4 + e : row & 31, j = TRANSPOSED ? row & 31 : 8 * q4 + e;
+        x[e] = j < i ? work[33 * i + j] : 0.0f;
+    }
+    float down;
+    const Parts8 p = scaled8(x, down);
+    if (q4 == 0) o.n_down[row] = down;
+    const int at = pair_unit(row, 4 * (w / 2) + q4);
+    o.mh[at] = p.hi;
+    o.ml[at] = p.lo;
+}
+
+// All of them, by the workgroup's 4 or 8 waves; tokens and gates are in LDS, and the
+// matrices are when it returns.
+template <int D, bool TRANSPOSED, bool WITH_P>
+__device__ __forceinline__ void make_pairs(Pairs& o, const kr_half8* q, const kr_half8* k, const Gates& gates, int wave,
+                                           int lane) {
+    if (wave < 4) {
+        make_a<D, TRANSPOSED>(o, k, gates, wave, lane);
+        solve_16(o, gates, wave, lane);
+    }
+    if (WITH_P && (D == 64 || wave >= 4)) make_p<D, TRANSPOSED>(o, q, k, gates, wave & 3, lane);
+    __syncthreads();
+    if (wave < 4 && (wave & 1)) solve_32(o, gates, wave / 2, lane);
+    __syncthreads();
+    if (wave < 4) store_n<TRANSPOSED>(o, wave, lane);
+    __syncthreads();
+}
+
+// Which stream this workgroup has: longest first, so that no long one is left for the end.
+template <int THREADS>
+__device__ __forceinline__ int ranked_stream(const int32_t* lens, int B, int T, int b, int* tmp) {
+    const int tid = threadIdx.x;
+    if (!lens || B > THREADS) return b;
+    if (tid < B) tmp[tid] = stream_tokens(lens, tid, T);
+    __syncthreads();
+    int rank = 0;
+    if (tid < B) {
+        const int mine = tmp[tid];
+        #pragma unroll 8
+        for (int j = 0; j < B; j++) rank += tmp[j] > mine || (tmp[j] == mine && j < tid);
+        if (rank == b) tmp[THREADS] = tid;
+    }
+    __syncthreads();
+    b = __builtin_amdgcn_readfirstlane(tmp[THREADS]);
+    __syncthreads();
+    return b;
+}
+
+template <int D>
+struct DeltaShared {
+    kr_half8 q[kChunk * D / 8], k[kChunk * D / 8], v[kChunk * D / 8];      // by tokens
+    Pairs pairs;
+    Gates gates[2];
+};
+
+// ---------------------------------------------------------------------------
+// Chunked form, forward: a workgroup has one head of one stream and walks its
+// chunks, a wave for each 16 columns of the state, which stays in the wave's
+// registers as the matrix unit leaves it: as such it is the operand of k S and q S,
+// and what they leave is the operand of the next product. STATES: the states before
+// the chunks and the differences r, for the backward pass, and no y.
+// ---------------------------------------------------------------------------
+template <int D, bool STATES>
+__global__ void __launch_bounds__(4 * D, 2) delta_chunk_kernel(DeltaArgs g) {
+    constexpr int KS = D / 32;            // k-steps over the channels
+    __shared__ DeltaShared<D> sh;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l16 = lane & 15, q4 = lane >> 4;
+    const int heads = gridDim.x, h = blockIdx.x % g.H;
+    const int b = ranked_stream<4 * D>(g.lens, g.B, g.T, blockIdx.x / g.H, reinterpret_cast<int*>(&sh.pairs));
+    const int head = b * g.H + h;
+    const int n_tok = stream_tokens(g.lens, b, g.T);
+    const size_t row0 = (size_t)b * g.T;
+
+    // state: column m = 16 wave + l16; S[2s], S[2s + 1] hold rows 32 s + 8 q4 + r and
+    // + 4, so that the pair is the operand of k-step s
+    kr_float4 S[2 * KS];
+    const int m = 16 * wave + l16;
+    const size_t state_at = (size_t)(8 * q4) * D + m;
+    const float* s_in = g.state + (size_t)head * D * D + state_at;
+    #pragma unroll
+    for (int s = 0; s < KS; s++)
+        #pragma unroll
+        for (int e = 0; e < 8; e++) S[2 * s + e / 4][e % 4] = s_in[(size_t)(32 * s + e) * D];
+
+    // what a thread stages: 8 channels of tokens 2p, 2p + 1
+    const int ng = tid % (D / 8), p = tid / (D / 8);
+    kr_half8 qq[2], kk[2], vv[2];
+    const size_t first = row0 + 2 * p;
+    const kr_half* qp = g.q + first * g.ldq + h * D + 8 * ng;
+    const kr_half* kp = g.k + first * g.ldk + h * D + 8 * ng;
+    const kr_half* vp = g.v + first * g.ldv + h * D + 8 * ng;
+    const float* gp = g.gate + (row0 + lane) * g.ldg + h;
+    const float* bp = g.beta + (row0 + lane) * g.ldb + h;
+    float gate = 0.0f, beta = 0.0f;
+    auto fetch = [&](int t0) {            // in order of t0
+        #pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const kr_half8 zero = {0, 0, 0, 0, 0, 0, 0, 0};
+            qq[e] = kk[e] = vv[e] = zero;
+            if (t0 + 2 * p + e < n_tok) {
+                if (!STATES) qq[e] = *reinterpret_cast<const kr_half8*>(qp + e * g.ldq);
+                kk[e] = *reinterpret_cast<const kr_half8*>(kp + e * g.ldk);
+                vv[e] = *reinterpret_cast<const kr_half8*>(vp + e * g.ldv);
+            }
+        }
+        qp += kChunk * g.ldq;
+        kp += kChunk * g.ldk;
+        vp += kChunk * g.ldv;
+    };
+    auto fetch_gates = [&](int t0) {
+        const bool on = t0 + lane < n_tok;
+        gate = on ? *gp : 0.0f;
+        beta = on ? *bp : 0.0f;
+        gp += kChunk * g.ldg;
+        bp += kChunk * g.ldb;
+    };
+    kr_half* yp = g.y + (row0 + l16) * g.ldy + h * D + 16 * wave + 4 * q4;
+
+    fetch(0);
+    if (wave == 0) {
+        fetch_gates(0);
+        make_gates(sh.gates[0], gate, beta, lane);
+        fetch_gates(kChunk);
+    }
+    for (int t0 = 0, c = 0; t0 < n_tok; t0 += kChunk, c++) {
+        const int n = n_tok - t0 < kChunk ? n_tok - t0 : kChunk;
+        #pragma unroll
+        for (int e = 0; e < 2; e++) {
+            if (!STATES) sh.q[tok_unit<D>(2 * p + e, ng)] = qq[e];
+            sh.k[tok_unit<D>(2 * p + e, ng)] = kk[e];
+            sh.v[tok_unit<D>(2 * p + e, ng)] = vv[e];
+        }
+        const Gates& gates = sh.gates[c & 1];
+        if (t0 + kChunk < n_tok) fetch(t0 + kChunk);
+        if constexpr (STATES) {
+            float* out = g.before + ((size_t)c * heads + head) * D * D + state_at;
+            #pragma unroll
+            for (int s = 0; s < KS; s++)
+                #pragma unroll
+                for (int e = 0; e < 8; e++) out[(size_t)(32 * s + e) * D] = S[2 * s + e / 4][e % 4];
+        }
+        __syncthreads();
+        make_pairs<D, false, !STATES>(sh.pairs, sh.q, sh.k, gates, wave, lane);
+        if (wave == 0 && t0 + kChunk < n_tok) {
+            make_gates(sh.gates[(c + 1) & 1], gate, beta, lane);
+            fetch_gates(t0 + 2 * kChunk);
+        }
+
+        // the state's parts, with a scale for each column
+        float big = 0.0f, up, down;
+        #pragma unroll
+        for (int s = 0; s < 2 * KS; s++)
+            #pragma unroll
+            for (int r = 0; r < 4; r++) big = fmaxf(big, fabsf(S[s][r]));
+        power_scale(max_of_quarters(big), up, down);
+        Parts8 sp[KS];
+        #pragma unroll
+        for (int s = 0; s < KS; s++)
+            #pragma unroll
+            for (int e = 0; e < 8; e++) {
+                kr_half x, y;
+                two_parts(S[2 * s + e / 4][e % 4] * up, x, y);
+                sp[s].hi[e] = x;
+                sp[s].lo[e] = y;
+            }
+
+        // X = v - e^a k S, rows t = 32 s + 8 q4 + e, column m
+        float X[2][8];
+        #pragma unroll
+        for (int s = 0; s < 2; s++) {
+            const kr_half8 vc = channels16<D>(sh.v, s, wave, lane);
+            #pragma unroll
+            for (int hf = 0; hf < 2; hf++) {
+                const int t = 32 * s + 8 * (l16 >> 2) + 4 * hf + (l16 & 3);
+                kr_float4 z = {0, 0, 0, 0};
+                #pragma unroll
+                for (int kst = 0; kst < KS; kst++) {
+                    const kr_half8 x = sh.k[tok_unit<D>(t, 4 * kst + q4)];
+                    z = mfma(x, sp[kst].hi, z);
+                    z = mfma(x, sp[kst].lo, z);
+                }
+                const kr_float4 e0 = *reinterpret_cast<const kr_float4*>(gates.e0 + 32 * s + 8 * q4 + 4 * hf);
+                #pragma unroll
+                for (int r = 0; r < 4; r++) X[s][4 * hf + r] = (float)vc[4 * hf + r] - (e0[r] * down) * z[r];
+            }
+        }
+        // u of the first half, then of the second
+        Parts8 up8[2];
+        float u_down[2], U[2][8];
+        #pragma unroll
+        for (int s = 0; s < 2; s++) {
+            float bt[8], x[8], x_down;
+            #pragma unroll
+            for (int e = 0; e < 8; e++) bt[e] = gates.beta[32 * s + 8 * q4 + e];
+            const int t = 32 * s + 8 * (l16 >> 2) + (l16 & 3);
+            if (s == 1) {
+                #pragma unroll
+                for (int hf = 0; hf < 2; hf++) {
+                    const int at = pair_unit(t + 4 * hf, q4);
+                    const kr_float4 z = mfma3(sh.pairs.mh[at], sh.pairs.ml[at], up8[0], kr_float4{0, 0, 0, 0});
+                    const kr_float4 f = *reinterpret_cast<const kr_float4*>(sh.pairs.a_down + 32 + 8 * q4 + 4 * hf);
+                    #pragma unroll
+                    for (int r = 0; r < 4; r++) X[1][4 * hf + r] -= (f[r] * u_down[0]) * z[r];
+                }
+            }
+            #pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = bt[e] * X[s][e];
+            const Parts8 xp = scaled8(x, x_down);
+            #pragma unroll
+            for (int hf = 0; hf < 2; hf++) {
+                const int at = pair_unit(t + 4 * hf, 4 * s + q4);
+                const kr_float4 z = mfma3(sh.pairs.mh[at], sh.pairs.ml[at], xp, kr_float4{0, 0, 0, 0});
+                const kr_float4 f = *reinterpret_cast<const kr_float4*>(sh.pairs.n_down + 32 * s + 8 * q4 + 4 * hf);
+                #pragma unroll
+                for (int r = 0; r < 4; r++) X[s][4 * hf + r] -= (f[r] * x_down) * z[r];
+            }
+            #pragma unroll
+            for (int e = 0; e < 8; e++) U[s][e] = bt[e] * X[s][e];
+            up8[s] = scaled8(U[s], u_down[s]);
+        }
+        if constexpr (STATES) {
+            float* out = g.diff + (((size_t)c * heads + head) * kChunk + 8 * q4) * D + m;
+            #pragma unroll
+            for (int s = 0; s < 2; s++)
+                #pragma unroll
+                for (int e = 0; e < 8; e++) out[(size_t)(32 * s + e) * D] = X[s][e];
+        } else {
+            // y': rows m, columns i
+            kr_float4 down_m, u0_m, u1_m;      // of the rows m that this lane has of y'
+            #pragma unroll
+            for (int r = 0; r < 4; r++) {
+                down_m[r] = __shfl(down, 4 * q4 + r);
+                u0_m[r] = __shfl(u_down[0], 4 * q4 + r);
+                u1_m[r] = __shfl(u_down[1], 4 * q4 + r);
+            }
+            #pragma unroll
+            for (int it = 0; it < 4; it++) {
+                const int i = 16 * it + l16;
+                kr_float4 from_s = {0, 0, 0, 0}, in0 = {0, 0, 0, 0}, in1 = {0, 0, 0, 0};
+                #pragma unroll
+                for (int s = 0; s < KS; s++) {
+                    const kr_half8 x = sh.q[tok_unit<D>(i, 4 * s + q4)];
+                    from_s = mfma(sp[s].hi, x, from_s);
+                    from_s = mfma(sp[s].lo, x, from_s);
+                }
+                const int at = pair_unit(i, q4);
+                in0 = mfma(up8[0].lo, sh.pairs.ph[at], in0);
+                in0 = mfma(up8[0].hi, sh.pairs.pl[at], in0);
+                in0 = mfma(up8[0].hi, sh.pairs.ph[at], in0);
+                if (it >= 2) {
+                    const int at1 = pair_unit(i, 4 + q4);
+                    in1 = mfma(up8[1].lo, sh.pairs.ph[at1], in1);
+                    in1 = mfma(up8[1].hi, sh.pairs.pl[at1], in1);
+                    in1 = mfma(up8[1].hi, sh.pairs.ph[at1], in1);
+                }
+                const float pd = sh.pairs.p_down[i], e0 = gates.e0[i];
+                kr_half4 y;
+                #pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    float x = from_s[r] * (down_m[r] * e0);
+                    x = __builtin_fmaf(in0[r], pd * u0_m[r], x);
+                    if (it >= 2) x = __builtin_fmaf(in1[r], pd * u1_m[r], x);
+                    y[r] = kr_f16(x);
+                }
+                if (i < n) *reinterpret_cast<kr_half4*>(yp + 16 * it * g.ldy) = y;
+            }
+            yp += kChunk * g.ldy;
+        }
+        // S <- e^a_end S + k' (e^(a_end - a) u)
+        float x[2][8];
+        #pragma unroll
+        for (int s = 0; s < 2; s++)
+            #pragma unroll
+            for (int e = 0; e < 8; e++) x[s][e] = gates.e1[32 * s + 8 * q4 + e] * U[s][e];
+        float x_up, x_down;
+        power_scale(max_of_quarters(largest8(x[1], largest8(x[0]))), x_up, x_down);
+        const Parts8 xp[2] = {parts8(x[0], x_up), parts8(x[1], x_up)};
+        const float all = gates.all;
+        #pragma unroll
+        for (int st = 0; st < 2 * KS; st++) {
+            kr_float4 add = {0, 0, 0, 0};
+            #pragma unroll
+            for (int s = 0; s < 2; s++) {
+                const kr_half8 kc = channels_state<D>(sh.k, s, st, lane);
+                add = mfma(kc, xp[s].lo, add);
+                add = mfma(kc, xp[s].hi, add);
+            }
+            #pragma unroll
+            for (int r = 0; r < 4; r++) S[st][r] = __builtin_fmaf(add[r], x_down, all * S[st][r]);
+        }
+        __syncthreads();
+    }
+
+    float* s_out = STATES ? g.before + ((size_t)((n_tok + kChunk - 1) / kChunk) * heads + head) * D * D
+                          : g.state + (size_t)head * D * D;
+    s_out += state_at;
+    #pragma unroll
+    for (int s = 0; s < KS; s++)
+        #pragma unroll
+        for (int e = 0; e < 8; e++) s_out[(size_t)(32 * s + e) * D] = S[2 * s + e / 4][e % 4];
+    if (!STATES)
+        for (int i = n_tok * (D / 8) + tid; i < g.T * (D / 8); i += 4 * D)
+            *reinterpret_cast<kr_half8*>(g.y + (row0 + i / (D / 8)) * g.ldy + h * D + 8 * (i % (D / 8))) =
+                kr_half8{0, 0, 0, 0, 0, 0, 0, 0};
+}
+
+// ---------------------------------------------------------------------------
+// Backward. With D the gradient of the state behind a chunk, from the last chunk to
+// the first and again a wave for each 16 columns:
+//   du = P' dy + e^(a_end - a) k D;   w = du - A' dX with dX = beta w (solved as r is,
+//   with the transposed N and the halves in the other order);
+//   D <- e^a_end D + (e^a q)' dy - (e^a k)' dX.
+// It leaves D behind each chunk and w, from which, with the states and r of a forward
+// pass, all chunks at once get the rest:
+//   dv = dX;  dbeta = w r;  MP_ij = e^(a_i - a_j) dy_i u_j' (j <= i);
+//   MA_ij = -e^(a_i - a_j) dX_i u_j' (j < i);  dq = e^a dy S' + MP k;
+//   dk of the reading key = -e^a dX S' + MA k;
+//   dk of the writing key = MP' q + MA' k + e^(a_end - a) u D';
+//   da = q dq + k dk_read - k dk_write, and at the chunk's end sum D S_behind;
+//   dg_i = sum of da from i to the chunk's end.
+// ---------------------------------------------------------------------------
+struct BackArgs {
+    const kr_half* q;
+    const kr_half* k;
+    const kr_half* dy;
+    long long ldq, ldk, ldy;
+    const float* gate;
+    const float* beta;
+    long long ldg, ldb;
+    const int32_t* lens;
+    const float* dstate;          // null: zeros
+    float* dstate0;
+    float* behind;                // [chunks][heads][D][D]
+    float* w;                     // [chunks][heads][64][D]
+    const float* before;          // of the forward pass: states, r
+    const float* diff;
+    kr_half* dq;                  // [B, T, H, D]
+    kr_half* dk;
+    kr_half* dv;
+    float* dgate;                 // [B, T, H]
+    float* dbeta;
+    int B, T, H;
+};
+
+template <int D>
+__global__ void __launch_bounds__(4 * D, 2) delta_back_kernel(BackArgs g) {
+    constexpr int KS = D / 32;
+    __shared__ DeltaShared<D> sh;         // dy in v's place
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l16 = lane & 15, q4 = lane >> 4;
+    const int heads = gridDim.x, h = blockIdx.x % g.H;
+    const int b = ranked_stream<4 * D>(g.lens, g.B, g.T, blockIdx.x / g.H, reinterpret_cast<int*>(&sh.pairs));
+    const int head = b * g.H + h;
+    const int n_tok = stream_tokens(g.lens, b, g.T);
+    const int chunks = (n_tok + kChunk - 1) / kChunk;
+    const size_t row0 = (size_t)b * g.T;
+
+    kr_float4 S[2 * KS];                  // D, laid out as the forward pass's state
+    const int m = 16 * wave + l16;
+    const size_t state_at = (size_t)(8 * q4) * D + m;
+    #pragma unroll
+    for (int s = 0; s < KS; s++)
+        #pragma unroll
+        for (int e = 0; e < 8; e++)
+            S[2 * s + e / 4][e % 4] =
+                g.dstate ? g.dstate[(size_t)head * D * D + state_at + (size_t)(32 * s + e) * D] : 0.0f;
+
+    const int ng = tid % (D / 8), p = tid / (D / 8);
+    kr_half8 qq[2], kk[2], vv[2];
+    auto fetch = [&](int t0) {
+        #pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const kr_half8 zero = {0, 0, 0, 0, 0, 0, 0, 0};
+            qq[e] = kk[e] = vv[e] = zero;
+            const int t = t0 + 2 * p + e;
+            if (t < n_tok) {
+                const size_t row = row0 + t;
+                qq[e] = *reinterpret_cast<const kr_half8*>(g.q + row * g.ldq + h * D + 8 * ng);
+                kk[e] = *reinterpret_cast<const kr_half8*>(g.k + row * g.ldk + h * D + 8 * ng);
+                vv[e] = *reinterpret_cast<const kr_half8*>(g.dy + row * g.ldy + h * D + 8 * ng);
+            }
+        }
+    };
+    float gate = 0.0f, beta = 0.0f;
+    auto fetch_gates = [&](int t0) {
+        const bool on = t0 >= 0 && t0 + lane < n_tok;
+        gate = on ? g.gate[(row0 + t0 + lane) * g.ldg + h] : 0.0f;
+        beta = on ? g.beta[(row0 + t0 + lane) * g.ldb + h] : 0.0f;
+    };
+    if (chunks > 0) {
+        fetch((chunks - 1) * kChunk);
+        if (wave == 0) {
+            fetch_gates((chunks - 1) * kChunk);
+            make_gates(sh.gates[(chunks - 1) & 1], gate, beta, lane);
+            fetch_gates((chunks - 2) * kChunk);
+        }
+    }
+    for (int c = chunks - 1; c >= 0; c--) {
+        #pragma unroll
+        for (int e = 0; e < 2; e++) {
+            sh.q[tok_unit<D>(2 * p + e, ng)] = qq[e];
+            sh.k[tok_unit<D>(2 * p + e, ng)] = kk[e];
+            sh.v[tok_unit<D>(2 * p + e, ng)] = vv[e];
+        }
+        const Gates& gates = sh.gates[c & 1];
+        if (c > 0) fetch((c - 1) * kChunk);
+        {
+            float* out = g.behind + ((size_t)c * heads + head) * D * D + state_at;
+            #pragma unroll
+            for (int s = 0; s < KS; s++)
+                #pragma unroll
+                for (int e = 0; e < 8; e++) out[(size_t)(32 * s + e) * D] = S[2 * s + e / 4][e % 4];
+        }
+        __syncthreads();
+        make_pairs<D, true, true>(sh.pairs, sh.q, sh.k, gates, wave, lane);
+        if (wave == 0 && c > 0) {
+            make_gates(sh.gates[(c - 1) & 1], gate, beta, lane);
+            fetch_gates((c - 2) * kChunk);
+        }
+        float big = 0.0f, up, down;
+        #pragma unroll
+        for (int s = 0; s < 2 * KS; s++)
+            #pragma unroll
+            for (int r = 0; r < 4; r++) big = fmaxf(big, fabsf(S[s][r]));
+        power_scale(max_of_quarters(big), up, down);
+        Parts8 sp[KS];
+        #pragma unroll
+        for (int s = 0; s < KS; s++)
+            #pragma unroll
+            for (int e = 0; e < 8; e++) {
+                kr_half x, y;
+                two_parts(S[2 * s + e / 4][e % 4] * up, x, y);
+                sp[s].hi[e] = x;
+                sp[s].lo[e] = y;
+            }
+        // du, rows t = 32 s + 8 q4 + e, column m
+        float X[2][8];
+        const kr_half8 dyc[2] = {channels16<D>(sh.v, 0, wave, lane), channels16<D>(sh.v, 1, wave, lane)};
+        #pragma unroll
+        for (int s = 0; s < 2; s++)
+            #pragma unroll
+            for (int hf = 0; hf < 2; hf++) {
+                const int t = 32 * s + 8 * (l16 >> 2) + 4 * hf + (l16 & 3);
+                kr_float4 z = {0, 0, 0, 0}, in = {0, 0, 0, 0};
+                #pragma unroll
+                for (int kst = 0; kst < KS; kst++) {
+                    const kr_half8 x = sh.k[tok_unit<D>(t, 4 * kst + q4)];
+                    z = mfma(x, sp[kst].lo, z);
+                    z = mfma(x, sp[kst].hi, z);
+                }
+                #pragma unroll
+                for (int is = s; is < 2; is++) {
+                    const int at = pair_unit(t, 4 * is + q4);
+                    in = mfma(sh.pairs.pl[at], dyc[is], in);
+                    in = mfma(sh.pairs.ph[at], dyc[is], in);
+                }
+                const kr_float4 e1 = *reinterpret_cast<const kr_float4*>(gates.e1 + 32 * s + 8 * q4 + 4 * hf);
+                const kr_float4 f = *reinterpret_cast<const kr_float4*>(sh.pairs.p_down + 32 * s + 8 * q4 + 4 * hf);
+                #pragma unroll
+                for (int r = 0; r < 4; r++) X[s][4 * hf + r] = __builtin_fmaf(e1[r] * down, z[r], f[r] * in[r]);
+            }
+        // w of the second half, then of the first
+        Parts8 dx1;
+        float dx1_down = 0.0f, dX[2][8];
+        #pragma unroll
+        for (int s = 1; s >= 0; s--) {
+            float bt[8], x[8], x_down;
+            #pragma unroll
+            for (int e = 0; e < 8; e++) bt[e] = gates.beta[32 * s + 8 * q4 + e];
+            const int t = 32 * s + 8 * (l16 >> 2) + (l16 & 3);
+            if (s == 0) {
+                #pragma unroll
+                for (int hf = 0; hf < 2; hf++) {
+                    const int at = pair_unit(t + 4 * hf, 4 + q4);
+                    const kr_float4 z = mfma3(sh.pairs.mh[at], sh.pairs.ml[at], dx1, kr_float4{0, 0, 0, 0});
+                    const kr_float4 f = *reinterpret_cast<const kr_float4*>(sh.pairs.a_down + 8 * q4 + 4 * hf);
+                    #pragma unroll
+                    for (int r = 0; r < 4; r++) X[0][4 * hf + r] -= (f[r] * dx1_down) * z[r];
+                }
+            }
+            #pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = bt[e] * X[s][e];
+            const Parts8 xp = scaled8(x, x_down);
+            #pragma unroll
+            for (int hf = 0; hf < 2; hf++) {
+                const int at = pair_unit(t + 4 * hf, 4 * s + q4);
+                const kr_float4 z = mfma3(sh.pairs.mh[at], sh.pairs.ml[at], xp, kr_float4{0, 0, 0, 0});
+                const kr_float4 f = *reinterpret_cast<const kr_float4*>(sh.pairs.n_down + 32 * s + 8 * q4 + 4 * hf);
+                #pragma unroll
+                for (int r = 0; r < 4; r++) X[s][4 * hf + r] -= (f[r] * x_down) * z[r];
+            }
+            #pragma unroll
+            for (int e = 0; e < 8; e++) dX[s][e] = bt[e] * X[s][e];
+            if (s == 1) dx1 = scaled8(dX[1], dx1_down);
+        }
+        {
+            float* out = g.w + (((size_t)c * heads + head) * kChunk + 8 * q4) * D + m;
+            #pragma unroll
+            for (int s = 0; s < 2; s++)
+                #pragma unroll
+                for (int e = 0; e < 8; e++) out[(size_t)(32 * s + e) * D] = X[s][e];
+        }
+        // D <- e^a_end D + q' (e^a dy) - k' (e^a dX)
+        float yx[2][8];
+        #pragma unroll
+        for (int s = 0; s < 2; s++)
+            #pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float e0 = gates.e0[32 * s + 8 * q4 + e];
+                yx[s][e] = e0 * (float)dyc[s][e];
+                dX[s][e] *= -e0;
+            }
+        float y_up, y_down, x_up, x_down;
+        power_scale(max_of_quarters(largest8(yx[1], largest8(yx[0]))), y_up, y_down);
+        power_scale(max_of_quarters(largest8(dX[1], largest8(dX[0]))), x_up, x_down);
+        const Parts8 yp[2] = {parts8(yx[0], y_up), parts8(yx[1], y_up)};
+        const Parts8 xp[2] = {parts8(dX[0], x_up), parts8(dX[1], x_up)};
+        const float all = gates.all;
+        #pragma unroll
+        for (int st = 0; st < 2 * KS; st++) {
+            kr_float4 from_y = {0, 0, 0, 0}, from_x = {0, 0, 0, 0};
+            #pragma unroll
+            for (int s = 0; s < 2; s++) {
+                const kr_half8 qc = channels_state<D>(sh.q, s, st, lane), kc = channels_state<D>(sh.k, s, st, lane);
+                from_y = mfma(qc, yp[s].lo, from_y);
+                from_y = mfma(qc, yp[s].hi, from_y);
+                from_x = mfma(kc, xp[s].lo, from_x);
+                from_x = mfma(kc, xp[s].hi, from_x);
+            }
+            #pragma unroll
+            for (int r = 0; r < 4; r++)
+                S[st][r] = __builtin_fmaf(from_x[r], x_down, __builtin_fmaf(from_y[r], y_down, all * S[st][r]));
+        }
+        __syncthreads();
+    }
+    float* out = g.dstate0 + (size_t)head * D * D + state_at;
+    #pragma unroll
+    for (int s = 0; s < KS; s++)
+        #pragma unroll
+        for (int e = 0; e < 8; e++) out[(size_t)(32 * s + e) * D] = S[2 * s + e / 4][e % 4];
+}
+
+// A workgroup of 4 waves for each head and chunk, a wave for 16 tokens, as those that
+// read and as those that write. 64 rows of S, then of D, are in LDS at a time.
+template <int D>
+struct GradShared {
+    kr_half8 q[kChunk * D / 8], k[kChunk * D / 8], dy[kChunk * D / 8];             // by tokens
+    kr_half8 uh[kChunk * D / 8], ul[kChunk * D / 8], xh[kChunk * D / 8], xl[kChunk * D / 8];   // u, dX
+    kr_half8 sh[kChunk * D / 8], sl[kChunk * D / 8];                               // 64 rows of S or D
+    float u_down[kChunk], x_down[kChunk], s_down[kChunk], da[kChunk], dot[4];
+    Gates gates;
+};
+
+// 8 values of a row that D / 8 neighbouring lanes hold, in two parts.
+template <int D>
+__device__ __forceinline__ Parts8 row_parts(const float (&x)[8], float& down) {
+    float big = largest8(x), up;
+    big = fmaxf(big, kr_xor<1>(big));
+    big = fmaxf(big, kr_xor<2>(big));
+    big = fmaxf(big, kr_xor<4>(big));
+    if (D == 128) big = fmaxf(big, kr_xor<8>(big));
+    power_scale(big, up, down);
+    return parts8(x, up);
+}
+
+template <int D>
+__device__ __forceinline__ float row_sum(float x) {
+    x += kr_xor<1>(x);
+    x += kr_xor<2>(x);
+    x += kr_xor<4>(x);
+    if (D == 128) x += kr_xor<8>(x);
+    return x;
+}
+
+template <int D>
+__global__ void __launch_bounds__(256, D == 64 ? 2 : 1) delta_grad_kernel(BackArgs g) {
+    constexpr int KS = D / 32, UNITS = D / 8, PASSES = kChunk * UNITS / 256;
+    __shared__ GradShared<D> sh;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l16 = lane & 15, q4 = lane >> 4;
+    const int heads = gridDim.x, head = blockIdx.x, c = blockIdx.y, b = head / g.H, h = head % g.H;
+    const int t0 = c * kChunk;
+    const int live = stream_tokens(g.lens, b, g.T) - t0, n = live < 0 ? 0 : live < kChunk ? live : kChunk;
+    const int rows = g.T - t0 < kChunk ? g.T - t0 : kChunk;
+    const size_t row0 = (size_t)b * g.T + t0;
+    const long long ldo = (long long)g.H * D;
+    const int unit = tid % UNITS, first = tid / UNITS;     // 8 channels of tokens first + 256 / UNITS i
+    if (n == 0) {
+        const kr_half8 zero = {0, 0, 0, 0, 0, 0, 0, 0};
+        for (int t = first; t < rows; t += 256 / UNITS) {
+            const size_t o = (row0 + t) * ldo + h * D + 8 * unit;
+            *reinterpret_cast<kr_half8*>(g.dq + o) = zero;
+            *reinterpret_cast<kr_half8*>(g.dk + o) = zero;
+            *reinterpret_cast<kr_half8*>(g.dv + o) = zero;
+        }
+        if (tid < rows) g.dgate[(row0 + tid) * g.H + h] = g.dbeta[(row0 + tid) * g.H + h] = 0.0f;
+        return;
+    }
+    if (wave == 0) {
+        const bool on = lane < n;
+        make_gates(sh.gates, on ? g.gate[(row0 + lane) * g.ldg + h] : 0.0f,
+                   on ? g.beta[(row0 + lane) * g.ldb + h] : 0.0f, lane);
+    }
+    const size_t diff_at = ((size_t)c * heads + head) * kChunk * D;
+    #pragma unroll
+    for (int i = 0; i < PASSES; i++) {
+        const int t = first + 256 / UNITS * i;
+        const bool on = t < n;
+        const kr_half8 zero = {0, 0, 0, 0, 0, 0, 0, 0};
+        kr_half8 x = zero, y = zero, z = zero;
+        float beta = 0.0f;
+        if (on) {
+            x = *reinterpret_cast<const kr_half8*>(g.q + (row0 + t) * g.ldq + h * D + 8 * unit);
+            y = *reinterpret_cast<const kr_half8*>(g.k + (row0 + t) * g.ldk + h * D + 8 * unit);
+            z = *reinterpret_cast<const kr_half8*>(g.dy + (row0 + t) * g.ldy + h * D + 8 * unit);
+            beta = g.beta[(row0 + t) * g.ldb + h];
+        }
+        const int at = tok_unit<D>(t, unit);
+        sh.q[at] = x;
+        sh.k[at] = y;
+        sh.dy[at] = z;
+        float r[8], w[8], dot = 0.0f;
+        const kr_float4* rp = reinterpret_cast<const kr_float4*>(g.diff + diff_at + (size_t)t * D + 8 * unit);
+        const kr_float4* wp = reinterpret_cast<const kr_float4*>(g.w + diff_at + (size_t)t * D + 8 * unit);
+        kr_half8 dv;
+        #pragma unroll
+        for (int e = 0; e < 8; e++) {
+            r[e] = rp[e / 4][e % 4];
+            w[e] = wp[e / 4][e % 4];
+            dot = __builtin_fmaf(r[e], w[e], dot);
+            r[e] *= beta;
+            w[e] *= beta;
+            dv[e] = kr_f16(w[e]);
+        }
+        float down;
+        const Parts8 up = row_parts<D>(r, down);
+        sh.uh[at] = up.hi;
+        sh.ul[at] = up.lo;
+        if (unit == 0) sh.u_down[t] = down;
+        const Parts8 xp = row_parts<D>(w, down);
+        sh.xh[at] = xp.hi;
+        sh.xl[at] = xp.lo;
+        dot = row_sum<D>(dot);
+        if (unit == 0) sh.x_down[t] = down;
+        if (t < rows) {
+            *reinterpret_cast<kr_half8*>(g.dv + (row0 + t) * ldo + h * D + 8 * unit) = on ? dv : zero;
+            if (unit == 0) g.dbeta[(row0 + t) * g.H + h] = on ? dot : 0.0f;
+        }
+    }
+    float dot = 0.0f;                     // sum D S_behind
+    auto stage = [&](const float* from, const float* times, int nb) {
+        #pragma unroll
+        for (int i = 0; i < PASSES; i++) {
+            const int r = first + 256 / UNITS * i;
+            const size_t at = (size_t)(64 * nb + r) * D + 8 * unit;
+            const kr_float4* fp = reinterpret_cast<const kr_float4*>(from + at);
+            float x[8], down;
+            #pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = fp[e / 4][e % 4];
+            if (times) {
+                const kr_float4* tp = reinterpret_cast<const kr_float4*>(times + at);
+                #pragma unroll
+                for (int e = 0; e < 8; e++) dot = __builtin_fmaf(x[e], tp[e / 4][e % 4], dot);
+            }
+            const Parts8 p = row_parts<D>(x, down);
+            sh.sh[tok_unit<D>(r, unit)] = p.hi;
+            sh.sl[tok_unit<D>(r, unit)] = p.lo;
+            if (unit == 0) sh.s_down[r] = down;
+        }
+    };
+    const float* before = g.before + ((size_t)c * heads + head) * D * D;
+    const float* after = before + (size_t)heads * D * D;
+    const float* behind = g.behind + ((size_t)c * heads + head) * D * D;
+    stage(before, nullptr, 0);
+    __syncthreads();
+
+    const int mine = 16 * wave + l16;     // this lane's token
+    const double a = sh.gates.a[mine];
+    const float e0 = sh.gates.e0[mine], e1 = sh.gates.e1[mine];
+    const float u_mine = sh.u_down[mine], x_mine = sh.x_down[mine];
+    // this lane's dy and dX as tokens that read, u as tokens that write
+    kr_half8 yv[KS];
+    Parts8 xv[KS], uv[KS];
+    #pragma unroll
+    for (int s = 0; s < KS; s++) {
+        const int at = tok_unit<D>(mine, 4 * s + q4);
+        yv[s] = sh.dy[at];
+        xv[s] = Parts8{sh.xh[at], sh.xl[at]};
+        uv[s] = Parts8{sh.uh[at], sh.ul[at]};
+    }
+    // rows of MP and MA (other tokens j = 32 s + 8 q4 + e), then columns (i = ..)
+    Parts8 mp[2], ma[2], mpt[2], mat[2];
+    float mp_down, ma_down, mpt_down, mat_down;
+    {
+        float P[2][8], A[2][8];
+        #pragma unroll
+        for (int s = 0; s < 2; s++)
+            #pragma unroll
+            for (int hf = 0; hf < 2; hf++) {
+                kr_float4 zp = {0, 0, 0, 0}, za = {0, 0, 0, 0};
+                const int t = 32 * s + 8 * (l16 >> 2) + 4 * hf + (l16 & 3);
+                if (s <= wave / 2) {
+                    #pragma unroll
+                    for (int kst = 0; kst < KS; kst++) {
+                        const int at = tok_unit<D>(t, 4 * kst + q4);
+                        const kr_half8 uh = sh.uh[at], ul = sh.ul[at];
+                        zp = mfma(ul, yv[kst], zp);
+                        zp = mfma(uh, yv[kst], zp);
+                        za = mfma3(uh, ul, xv[kst], za);
+                    }
+                }
+                #pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int j = 32 * s + 8 * q4 + 4 * hf + r;
+                    const float f = sh.u_down[j] * __builtin_amdgcn_exp2f((float)(a - sh.gates.a[j]));
+                    P[s][4 * hf + r] = j <= mine ? zp[r] * f : 0.0f;
+                    A[s][4 * hf + r] = j < mine ? -(za[r] * x_mine) * f : 0.0f;
+                }
+            }
+        float up;
+        power_scale(max_of_quarters(largest8(P[1], largest8(P[0]))), up, mp_down);
+        mp[0] = parts8(P[0], up);
+        mp[1] = parts8(P[1], up);
+        power_scale(max_of_quarters(largest8(A[1], largest8(A[0]))), up, ma_down);
+        ma[0] = parts8(A[0], up);
+        ma[1] = parts8(A[1], up);
+        #pragma unroll
+        for (int s = 0; s < 2; s++)
+            #pragma unroll
+            for (int hf = 0; hf < 2; hf++) {
+                kr_float4 zp = {0, 0, 0, 0}, za = {0, 0, 0, 0};
+                const int t = 32 * s + 8 * (l16 >> 2) + 4 * hf + (l16 & 3);
+                if (s >= wave / 2) {
+                    #pragma unroll
+                    for (int kst = 0; kst < KS; kst++) {
+                        const int at = tok_unit<D>(t, 4 * kst + q4);
+                        const kr_half8 y = sh.dy[at];
+                        zp = mfma(y, uv[kst].lo, zp);
+                        zp = mfma(y, uv[kst].hi, zp);
+                        za = mfma3(sh.xh[at], sh.xl[at], uv[kst], za);
+                    }
+                }
+                #pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int i = 32 * s + 8 * q4 + 4 * hf + r;
+                    const float f = u_mine * __builtin_amdgcn_exp2f((float)(sh.gates.a[i] - a));
+                    P[s][4 * hf + r] = i >= mine ? zp[r] * f : 0.0f;
+                    A[s][4 * hf + r] = i > mine ? -(za[r] * sh.x_down[i]) * f : 0.0f;
+                }
+            }
+        power_scale(max_of_quarters(largest8(P[1], largest8(P[0]))), up, mpt_down);
+        mpt[0] = parts8(P[0], up);
+        mpt[1] = parts8(P[1], up);
+        power_scale(max_of_quarters(largest8(A[1], largest8(A[0]))), up, mat_down);
+        mat[0] = parts8(A[0], up);
+        mat[1] = parts8(A[1], up);
+    }
+    // 64 channels at a time: rows n of 16, this lane's token
+    float da = 0.0f;
+    for (int nb = 0; nb < D / 64; nb++) {
+        if (nb > 0) {
+            __syncthreads();
+            stage(before, nullptr, nb);
+            __syncthreads();
+        }
+        kr_float4 dq[4], read[4], write[4];
+        #pragma unroll
+        for (int nt = 0; nt < 4; nt++) {
+            kr_float4 zq = {0, 0, 0, 0}, zk = {0, 0, 0, 0}, pk = {0, 0, 0, 0}, ak = {0, 0, 0, 0};
+            #pragma unroll
+            for (int s = 0; s < KS; s++) {
+                const int at = tok_unit<D>(16 * nt + l16, 4 * s + q4);
+                const kr_half8 hi = sh.sh[at], lo = sh.sl[at];
+                zq = mfma(lo, yv[s], zq);
+                zq = mfma(hi, yv[s], zq);
+                zk = mfma3(hi, lo, xv[s], zk);
+            }
+            #pragma unroll
+            for (int s = 0; s < 2; s++) {
+                if (s > wave / 2) continue;
+                const kr_half8 kc = channels16<D>(sh.k, s, 4 * nb + nt, lane);
+                pk = mfma(kc, mp[s].lo, pk);
+                pk = mfma(kc, mp[s].hi, pk);
+                ak = mfma(kc, ma[s].lo, ak);
+                ak = mfma(kc, ma[s].hi, ak);
+            }
+            const kr_float4 sd = *reinterpret_cast<const kr_float4*>(sh.s_down + 16 * nt + 4 * q4);
+            #pragma unroll
+            for (int r = 0; r < 4; r++) {
+                dq[nt][r] = __builtin_fmaf(pk[r], mp_down, zq[r] * (sd[r] * e0));
+                read[nt][r] = __builtin_fmaf(ak[r], ma_down, -(zk[r] * x_mine) * (sd[r] * e0));
+            }
+        }
+        __syncthreads();
+        stage(behind, after, nb);
+        __syncthreads();
+        #pragma unroll
+        for (int nt = 0; nt < 4; nt++) {
+            kr_float4 zu = {0, 0, 0, 0}, pq = {0, 0, 0, 0}, ak = {0, 0, 0, 0};
+            #pragma unroll
+            for (int s = 0; s < KS; s++) {
+                const int at = tok_unit<D>(16 * nt + l16, 4 * s + q4);
+                zu = mfma3(sh.sh[at], sh.sl[at], uv[s], zu);
+            }
+            #pragma unroll
+            for (int s = 0; s < 2; s++) {
+                if (s < wave / 2) continue;
+                const kr_half8 qc = channels16<D>(sh.q, s, 4 * nb + nt, lane);
+                const kr_half8 kc = channels16<D>(sh.k, s, 4 * nb + nt, lane);
+                pq = mfma(qc, mpt[s].lo, pq);
+                pq = mfma(qc, mpt[s].hi, pq);
+                ak = mfma(kc, mat[s].lo, ak);
+                ak = mfma(kc, mat[s].hi, ak);
+            }
+            const kr_float4 sd = *reinterpret_cast<const kr_float4*>(sh.s_down + 16 * nt + 4 * q4);
+            #pragma unroll
+            for (int r = 0; r < 4; r++)
+                write[nt][r] = __builtin_fmaf(pq[r], mpt_down,
+                                              __builtin_fmaf(ak[r], mat_down, (zu[r] * u_mine) * (sd[r] * e1)));
+        }
+        #pragma unroll
+        for (int nt = 0; nt < 4; nt++) {
+            const int ch = 64 * nb + 16 * nt + 4 * q4;
+            const int at = tok_unit<D>(mine, ch / 8);
+            const kr_half4 qv = reinterpret_cast<const kr_half4*>(sh.q + at)[ch / 4 & 1];
+            const kr_half4 kv = reinterpret_cast<const kr_half4*>(sh.k + at)[ch / 4 & 1];
+            kr_half4 oq, ok;
+            #pragma unroll
+            for (int r = 0; r < 4; r++) {
+                da = __builtin_fmaf((float)qv[r], dq[nt][r], da);
+                da = __builtin_fmaf((float)kv[r], read[nt][r] - write[nt][r], da);
+                oq[r] = kr_f16(dq[nt][r]);
+                ok[r] = kr_f16(read[nt][r] + write[nt][r]);
+            }
+            if (mine < rows) {
+                const kr_half4 zero = {0, 0, 0, 0};
+                const size_t o = (row0 + mine) * ldo + h * D + ch;
+                *reinterpret_cast<kr_half4*>(g.dq + o) = mine < n ? oq : zero;
+                *reinterpret_cast<kr_half4*>(g.dk + o) = mine < n ? ok : zero;
+            }
+        }
+    }
+    da += kr_xor<16>(da);
+    da += kr_xor<32>(da);
+    dot = kr_wave_reduce(dot, [](float x, float y) { return x + y; });
+    if (q4 == 0) sh.da[mine] = da;
+    if (lane == 0) sh.dot[wave] = dot;
+    __syncthreads();
+    if (wave == 0) {
+        double x = sh.da[lane];
+        if (lane == 63) x += ((double)sh.dot[0] + sh.dot[1]) + ((double)sh.dot[2] + sh.dot[3]);
+        #pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const double y = __shfl_down(x, d);
+            if (lane + d < 64) x += y;
+        }
+        if (lane < rows) {
+            const float gate = lane < n ? g.gate[(row0 + lane) * g.ldg + h] : 0.0f;
+            // a constant where the gate is outside its range
+            g.dgate[(row0 + lane) * g.H + h] = lane >= n || gate > 0.0f || gate < -10000.0f ? 0.0f : (float)x;
+        }
+    }
+}
+
+// Tokens up to which the chunked form is the recurrent one, too.
+constexpr int kStepTokens = 8;
+
+bool shape_ok(int B, int T, int H, int D) {
+    return B >= 0 && T >= 0 && H >= 1 && (D == 64 || D == 128) && (long long)B * H <= 1 << 24 && T <= 1 << 30;
+}
+
+template <int D>
+int launch(const DeltaArgs& g, bool chunked, hipStream_t s) {
+    const int heads = g.B * g.H;
+    if (!chunked || g.T <= kStepTokens) delta_step_kernel<D><<<heads, 4 * D, 0, s>>>(g);
+    else delta_chunk_kernel<D, false><<<heads, 4 * D, 0, s>>>(g);
+    KR_LAUNCHED();
+    return KR_OK;
+}
+
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+
+// The backward pass's workspace: states, r, D and w of all chunks.
+struct BackPlan {
+    size_t before, diff, behind, w, total;
+};
+BackPlan back_plan(int B, int T, int H, int D) {
+    const size_t heads = (size_t)B * H, chunks = (size_t)(T + kChunk - 1) / kChunk;
+    const size_t state = heads * D * D * sizeof(float), rows = heads * kChunk * D * sizeof(float);
+    BackPlan p{};
+    p.diff = p.before + up256((chunks + 1) * state);
+    p.behind = p.diff + up256(chunks * rows);
+    p.w = p.behind + up256(chunks * state);
+    p.total = p.w + up256(chunks * rows);
+    return p;
+}
+
+template <int D>
+int launch_back(const DeltaArgs& f, const BackArgs& g, hipStream_t s) {
+    const int heads = g.B * g.H, chunks = (g.T + kChunk - 1) / kChunk;
+    delta_chunk_kernel<D, true><<<heads, 4 * D, 0, s>>>(f);
+    KR_LAUNCHED();
+    delta_back_kernel<D><<<heads, 4 * D, 0, s>>>(g);
+    KR_LAUNCHED();
+    delta_grad_kernel<D><<<dim3(heads, chunks), 256, 0, s>>>(g);
+    KR_LAUNCHED();
+    return KR_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t kr_gated_delta_workspace_bytes(int B, int T, int H, int D) {
+    (void)B, (void)T, (void)H, (void)D;
+    return 0;
+}
+
+int kr_gated_delta(int B, int T, int H, int D, const uint16_t* q, long long ldq, const uint16_t* k, long long ldk,
+                   const uint16_t* v, long long ldv, const float* log_decay, long long ldg, const float* beta,
+                   long long ldb, const int32_t* lens, float* state, uint16_t* y, long long ldy, int chunked, void* ws,
+                   size_t ws_bytes, void* stream) {
+    KR_REQUIRE(shape_ok(B, T, H, D), "kr_gated_delta: bad shape B=%d T=%d H=%d D=%d (D: 64 or 128)", B, T, H, D);
+    const long long C = (long long)H * D;
+    KR_REQUIRE(ldq >= C && ldk >= C && ldv >= C && ldy >= C && (ldq | ldk | ldv | ldy) % 8 == 0,
+               "kr_gated_delta: token strides must be multiples of 8 and at least H * D = %lld", C);
+    KR_REQUIRE(ldg >= H && ldb >= H, "kr_gated_delta: strides of log_decay and beta must be at least H = %d", H);
+    if (B == 0 || T == 0) return KR_OK;
+    KR_REQUIRE(q && k && v && log_decay && beta && state && y, "kr_gated_delta: null pointer");
+    KR_REQUIRE((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)state | (uintptr_t)y) & 15) == 0,
+               "kr_gated_delta: q, k, v, state and y must be 16-byte aligned");
+    const size_t need = kr_gated_delta_workspace_bytes(B, T, H, D);
+    KR_REQUIRE(need == 0 || (ws && ws_bytes >= need && ((uintptr_t)ws & 15) == 0),
+               "kr_gated_delta: workspace of %zu bytes, %zu needed (16-byte aligned)", ws_bytes, need);
+    DeltaArgs g{};
+    g.q = reinterpret_cast<const kr_half*>(q);
+    g.k = reinterpret_cast<const kr_half*>(k);
+    g.v = reinterpret_cast<const kr_half*>(v);
+    g.ldq = ldq;
+    g.ldk = ldk;
+    g.ldv = ldv;
+    g.gate = log_decay;
+    g.beta = beta;
+    g.ldg = ldg;
+    g.ldb = ldb;
+    g.lens = lens;
+    g.state = state;
+    g.y = reinterpret_cast<kr_half*>(y);
+    g.ldy = ldy;
+    g.B = B;
+    g.T = T;
+    g.H = H;
+    return D == 64 ? launch<64>(g, chunked != 0, kr_stream(stream)) : launch<128>(g, chunked != 0, kr_stream(stream));
+}
+
+size_t kr_gated_delta_backward_workspace_bytes(int B, int T, int H, int D) {
+    if (!shape_ok(B, T, H, D) || B == 0 || T == 0) return 0;
+    return back_plan(B, T, H, D).total;
+}
+
+int kr_gated_delta_backward(int B, int T, int H, int D, const uint16_t* q, long long ldq, const uint16_t* k,
+                            long long ldk, const uint16_t* v, long long ldv, const float* log_decay, long long ldg,
+                            const float* beta, long long ldb, const int32_t* lens, const float* state,
+                            const uint16_t* dy, long long ldy, const float* dstate, uint16_t* dq, uint16_t* dk,
+                            uint16_t* dv, float* dlog_decay, float* dbeta, float* dstate0, void* ws, size_t ws_bytes,
+                            void* stream) {
+    KR_REQUIRE(shape_ok(B, T, H, D) && B > 0 && T > 0 && T <= kChunk * 65535,
+               "kr_gated_delta_backward: bad shape B=%d T=%d H=%d D=%d (D: 64 or 128, T: 1..4194240)", B, T, H, D);
+    const long long C = (long long)H * D;
+    KR_REQUIRE(ldq >= C && ldk >= C && ldv >= C && ldy >= C && (ldq | ldk | ldv | ldy) % 8 == 0,
+               "kr_gated_delta_backward: token strides must be multiples of 8 and at least H * D = %lld", C);
+    KR_REQUIRE(ldg >= H && ldb >= H, "kr_gated_delta_backward: strides of log_decay and beta must be at least H = %d", H);
+    KR_REQUIRE(q && k && v && log_decay && beta && state && dy && dq && dk && dv && dlog_decay && dbeta && dstate0,
+               "kr_gated_delta_backward: null pointer");
+    KR_REQUIRE((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)state | (uintptr_t)dy | (uintptr_t)dstate |
+                 (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv | (uintptr_t)dstate0) & 15) == 0,
+               "kr_gated_delta_backward: all but log_decay, beta, lens and their gradients must be 16-byte aligned");
+    const BackPlan p = back_plan(B, T, H, D);
+    KR_REQUIRE(ws && ws_bytes >= p.total && ((uintptr_t)ws & 255) == 0,
+               "kr_gated_delta_backward: workspace of %zu bytes, %zu needed (256-byte aligned)", ws_bytes, p.total);
+    char* base = static_cast<char*>(ws);
+    DeltaArgs f{};
+    f.q = reinterpret_cast<const kr_half*>(q);
+    f.k = reinterpret_cast<const kr_half*>(k);
+    f.v = reinterpret_cast<const kr_half*>(v);
+    f.ldq = ldq;
+    f.ldk = ldk;
+    f.ldv = ldv;
+    f.gate = log_decay;
+    f.beta = beta;
+    f.ldg = ldg;
+    f.ldb = ldb;
+    f.lens = lens;
+    f.state = const_cast<float*>(state);          // only read where states are kept
+    f.before = reinterpret_cast<float*>(base + p.before);
+    f.diff = reinterpret_cast<float*>(base + p.diff);
+    f.B = B;
+    f.T = T;
+    f.H = H;
+    BackArgs g{};
+    g.q = f.q;
+    g.k = f.k;
+    g.dy = reinterpret_cast<const kr_half*>(dy);
+    g.ldq = ldq;
+    g.ldk = ldk;
+    g.ldy = ldy;
+    g.gate = log_decay;
+    g.beta = beta;
+    g.ldg = ldg;
+    g.ldb = ldb;
+    g.lens = lens;
+    g.dstate = dstate;
+    g.dstate0 = dstate0;
+    g.before = f.before;
+    g.diff = f.diff;
+    g.behind = reinterpret_cast<float*>(base + p.behind);
+    g.w = reinterpret_cast<float*>(base + p.w);
+    g.dq = reinterpret_cast<kr_half*>(dq);
+    g.dk = reinterpret_cast<kr_half*>(dk);
+    g.dv = reinterpret_cast<kr_half*>(dv);
+    g.dgate = dlog_decay;
+    g.dbeta = dbeta;
+    g.B = B;
+    g.T = T;
+    g.H = H;
+    return D == 64 ? launch_back<64>(f, g, kr_stream(stream)) : launch_back<128>(f, g, kr_stream(stream));
+}
+
+}  // extern "C"

@@ -505,6 +505,114 @@ def wkv_heads(r, k, v, decay, first, state, lens=None, chunked: bool = True):
     return y
 
 
+def _delta_tokens(t, name, shape, dev):
+    """Token stride of a [B, T, H, D] fp16 operand."""
+    (t.is_cuda and t.dtype is torch.float16) or _refuse(f"{name} must be a float16 device tensor")
+    (t.shape == shape and t.get_device() == dev) or _refuse(f"{name} must be {tuple(shape)} on q's device")
+    B, T, H, D = shape
+    if B * T == 0:
+        return H * D
+    sb, st, sh, sd = t.stride()
+    if T == 1:
+        st = sb if B > 1 else H * D
+    (sd == 1 and (sh == D or H == 1) and st >= H * D and (sb == T * st or B == 1) and st % 8 == 0
+     and t.data_ptr() % 16 == 0) or _refuse(
+        f"{name}: heads must be contiguous, tokens evenly spaced and 16-byte aligned")
+    return st
+
+
+def _delta_gates(t, name, shape, dev):
+    """Token stride of a [B, T, H] fp32 operand."""
+    B, T, H, _ = shape
+    (t.is_cuda and t.dtype is torch.float32 and t.shape == (B, T, H) and t.get_device() == dev) or _refuse(
+        f"{name} must be a float32 device tensor {(B, T, H)} on q's device")
+    if B * T == 0:
+        return H
+    sb, st, sh = t.stride()
+    if T == 1:
+        st = sb if B > 1 else H
+    ((sh == 1 or H == 1) and st >= H and (sb == T * st or B == 1)) or _refuse(
+        f"{name}: heads must be contiguous and tokens evenly spaced")
+    return st
+
+
+def _delta_state(t, name, shape, dev):
+    B, _, H, D = shape
+    (t.is_cuda and t.dtype is torch.float32 and t.is_contiguous() and t.shape == (B, H, D, D)
+     and t.get_device() == dev and t.data_ptr() % 16 == 0) or _refuse(
+        f"{name} must be a contiguous float32 device tensor {(B, H, D, D)} on q's device, 16-byte aligned")
+
+
+def _delta_args(q, k, v, log_decay, beta, state, lens):
+    q.dim() == 4 or _refuse("q must be [B, T, H, D]")
+    shape = q.shape
+    B, T, H, D = shape
+    (D in (64, 128) and H >= 1) or _refuse(f"q must have heads of 64 or 128 channels, got {tuple(shape)}")
+    dev = q.get_device()
+    ld = [_delta_tokens(t, name, shape, dev) for t, name in ((q, "q"), (k, "k"), (v, "v"))]
+    ld += [_delta_gates(t, name, shape, dev) for t, name in ((log_decay, "log_decay"), (beta, "beta"))]
+    _delta_state(state, "state", shape, dev)
+    lens is None or (lens.is_cuda and lens.dtype is torch.int32 and lens.is_contiguous()
+                     and lens.numel() == B and lens.get_device() == dev) or _refuse(
+        f"lens must be a contiguous int32 device tensor [B] = [{B}] on q's device")
+    return shape, ld
+
+
+def gated_delta(q, k, v, log_decay, beta, state, lens=None, chunked: bool = True):
+    """The gated delta rule, a matrix state per head whose keys replace what they had
+    stored: S <- e^g S; u = beta (v_t - k_t S); S <- S + k_t' u; y_t = q_t S. q, k, v
+    fp16 [B, T, H, D], D 64 or 128, log_decay (g <= 0) and beta fp32 [B, T, H] (heads
+    contiguous; token strides free, so slices of one projection will do), state fp32
+    [B, H, D, D] updated in place; returns y fp16 [B, T, H, D]. Keys are usually
+    normalised by the caller and beta is in 0..1. lens int32 [B]: each stream's tokens (its
+    state stops there, later rows of y are 0). chunked=True (prompts, scoring, training)
+    takes 64 tokens at a time on the matrix units: equal up to rounding for finite inputs;
+    chunked=False, and calls of at most 8 tokens, go token by token, and T tokens then
+    have the bits of T calls. No autograd: gated_delta_backward gives the gradients."""
+    shape, ld = _delta_args(q, k, v, log_decay, beta, state, lens)
+    if _elsewhere(q):
+        return _on_device_of(q, gated_delta, q, k, v, log_decay, beta, state, lens, chunked)
+    B, T, H, D = shape
+    y = q.new_empty(shape)
+    ws, nbytes = None, 0
+    if chunked and T > 1:
+        nbytes = _lib.lib().kr_gated_delta_workspace_bytes(B, T, H, D)
+        if nbytes:
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    _lib.call("kr_gated_delta", B, T, H, D, q.data_ptr(), ld[0], k.data_ptr(), ld[1], v.data_ptr(), ld[2],
+              log_decay.data_ptr(), ld[3], beta.data_ptr(), ld[4], _lib.ptr(lens), state.data_ptr(),
+              y.data_ptr(), H * D, 1 if chunked else 0, _lib.ptr(ws), nbytes, _lib.stream_ptr())
+    return y
+
+
+def gated_delta_backward(q, k, v, log_decay, beta, state, dy, dstate=None, lens=None):
+    """Gradients of gated_delta: its inputs, with state as it was BEFORE the call
+    (which updates it in place), dy fp16 [B, T, H, D] and dstate fp32 [B, H, D, D], the
+    gradient of the state after the call (None: zeros) -> (dq, dk, dv fp16 [B, T, H, D],
+    dlog_decay, dbeta fp32 [B, T, H], dstate fp32 [B, H, D, D] of the state before).
+    Tokens past lens have gradient 0, and so has a log_decay above 0 or below -10000.
+    Its states are computed again: nothing is kept from the forward call."""
+    shape, ld = _delta_args(q, k, v, log_decay, beta, state, lens)
+    dev = q.get_device()
+    ldy = _delta_tokens(dy, "dy", shape, dev)
+    dstate is None or _delta_state(dstate, "dstate", shape, dev)
+    if _elsewhere(q):
+        return _on_device_of(q, gated_delta_backward, q, k, v, log_decay, beta, state, dy, dstate, lens)
+    B, T, H, D = shape
+    dq, dk, dv = (q.new_empty(shape) for _ in range(3))
+    dg, db = (state.new_empty((B, T, H)) for _ in range(2))
+    if B * T == 0:
+        return dq, dk, dv, dg, db, torch.zeros_like(state) if dstate is None else dstate.clone()
+    d0 = torch.empty_like(state)
+    nbytes = _lib.lib().kr_gated_delta_backward_workspace_bytes(B, T, H, D)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    _lib.call("kr_gated_delta_backward", B, T, H, D, q.data_ptr(), ld[0], k.data_ptr(), ld[1], v.data_ptr(),
+              ld[2], log_decay.data_ptr(), ld[3], beta.data_ptr(), ld[4], _lib.ptr(lens), state.data_ptr(),
+              dy.data_ptr(), ldy, _lib.ptr(dstate), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dg.data_ptr(),
+              db.data_ptr(), d0.data_ptr(), ws.data_ptr(), nbytes, _lib.stream_ptr())
+    return dq, dk, dv, dg, db, d0
+
+
 def _layer_struct(x, att_xx, aa, bb, pp, ffn_xx, ln1_w, ln1_b, tm_k, tm_v, tm_r, time_decay,
                   time_first, Kw, Vw, Rw, Ow, ln2_w, ln2_b, ffn_tm_k, ffn_tm_r, ffn_Kw, ffn_Vw,
                   ffn_Rw):
