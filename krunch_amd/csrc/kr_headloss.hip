@@ -21,7 +21,6 @@
 namespace {
 
 constexpr float kLog2e = 0x1.715476p+0f, kLn2 = 0x1.62e430p-1f;
-constexpr int kPart = 128;            // columns of a partial maximum and sum
 typedef short short4v __attribute__((__vector_size__(8)));
 typedef __attribute__((address_space(3))) short4v lds_short4;
 
@@ -43,8 +42,16 @@ struct LossArgs {
 };
 
 __device__ __forceinline__ void copy16(const void* base, unsigned off, unsigned lds) {
+    lds = (unsigned)__builtin_amdgcn_readfirstlane((int)lds);
     asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2"
                  :: "s"(lds), "v"(off), "s"(base) : "memory", "m0");
+}
+// A pointer that all lanes share, as such to the compiler.
+template <typename T>
+__device__ __forceinline__ const T* shared_by_lanes(const T* p) {
+    const uint64_t v = (uint64_t)p;
+    return reinterpret_cast<const T*>((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v) |
+                                      (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32);
 }
 __device__ __forceinline__ unsigned lds_address(const void* p) {
     return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
@@ -70,16 +77,20 @@ __device__ __forceinline__ bool tile_of(int gy, int gx, int vb, int group_m, int
 }
 
 // ---------------------------------------------------------------------------
-// z = x W' in tiles of (64 WM) x (128 WN), a wave for each 64 x 128. Steps of 64 k
-// through two LDS stages, copied asynchronously one step ahead, into the next tile.
-// The matrix unit gets W' x', so a lane has 4 columns of a row; W's rows go in
-// in an order that makes them 8 consecutive columns over two tiles.
+// z = x W' in tiles of (64 WM) x (16 TN WN), a wave for each 64 x 16 TN. Steps of 64 k
+// through two LDS stages, copied asynchronously one step ahead, into the next tile. The
+// matrix unit gets W' x', so a lane has 4 columns of a row; W's rows go in in an
+// order that makes them 8 consecutive columns over two of its tiles.
 // ---------------------------------------------------------------------------
-template <int WM, int WN, bool GRAD>
-__global__ void __launch_bounds__(64 * WM * WN, 1) logits_kernel(LossArgs g, int n_virtual, int group_m) {
-    constexpr int BM = 64 * WM, BN = 128 * WN, WAVES = WM * WN;
+template <int N>
+__device__ __forceinline__ void wait_copies() { asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory"); }
+
+template <int WM, int WN, int TN, bool GRAD>
+__global__ void __launch_bounds__(64 * WM * WN, WM * WN >= 8 ? 1 : 2) logits_kernel(LossArgs g, int n_virtual,
+                                                                                 int group_m) {
+    constexpr int BM = 64 * WM, BN = 16 * TN * WN, WAVES = WM * WN;
     constexpr int COPIES = (BM + BN) / 8 / WAVES;
-    static_assert((BM + BN) / 8 % WAVES == 0, "copies");
+    static_assert((BM + BN) / 8 % WAVES == 0 && TN % 4 == 0, "tile");
     constexpr int STAGE = (BM + BN) * 8;                  // 16-byte units
     __shared__ __attribute__((aligned(1024))) kr_half8 ring[2 * STAGE];
     const int tid = threadIdx.x, lane = tid & 63;
@@ -113,15 +124,15 @@ __global__ void __launch_bounds__(64 * WM * WN, 1) logits_kernel(LossArgs g, int
         int nm_t = 0, nn_t = 0;
         const bool has_next =
             vb + (int)gridDim.x < n_virtual && tile_of(gy, gx, vb + (int)gridDim.x, group_m, nm_t, nn_t);
-        kr_float4 acc[4][8];
+        kr_float4 acc[4][TN];
         #pragma unroll
         for (int i = 0; i < 4; i++)
             #pragma unroll
-            for (int t = 0; t < 8; t++) acc[i][t] = kr_float4{0, 0, 0, 0};
+            for (int t = 0; t < TN; t++) acc[i][t] = kr_float4{0, 0, 0, 0};
         #pragma unroll 1
         for (int ks = 0; ks < KS; ks++, q++) {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();   // every wave's copies of step q are in; step q-1's stage is free
+            wait_copies<0>();
+            __syncthreads();   // every wave's copies are in; the step before is read
             if (ks + 1 < KS) issue(m_t, n_t, ks + 1, q + 1);
             else if (has_next) issue(nm_t, nn_t, 0, q + 1);
             const kr_half8* As = ring + (q & 1) * STAGE;
@@ -132,12 +143,12 @@ __global__ void __launch_bounds__(64 * WM * WN, 1) logits_kernel(LossArgs g, int
                 #pragma unroll
                 for (int i = 0; i < 4; i++) a[i] = As[row_unit(64 * wm + 16 * i + lr, 4 * kb + lq)];
                 #pragma unroll
-                for (int th = 0; th < 2; th++) {
+                for (int th = 0; th < TN / 4; th++) {
                     __builtin_amdgcn_sched_barrier(0);    // four W fragments at a time (registers)
                     kr_half8 w[4];
                     #pragma unroll
                     for (int t = 0; t < 4; t++) {
-                        const int row = 128 * wn + 32 * (2 * th + t / 2) + 8 * (lr >> 2) + 4 * (t & 1) + (lr & 3);
+                        const int row = 16 * TN * wn + 32 * (2 * th + t / 2) + 8 * (lr >> 2) + 4 * (t & 1) + (lr & 3);
                         w[t] = Ws[row_unit(row, 4 * kb + lq)];
                     }
                     __builtin_amdgcn_sched_barrier(0);
@@ -150,63 +161,82 @@ __global__ void __launch_bounds__(64 * WM * WN, 1) logits_kernel(LossArgs g, int
                 }
             }
         }
-        // lane: row 64 wm + 16 i + lr; acc[i][t][r] column 128 wn + 32 (t / 2) + 8 lq + 4 (t % 2) + r
-        const int c0 = n_t * BN + 128 * wn + 8 * lq;
+        // lane: row 64 wm + 16 i + lr; acc[i][t][r] column 16 TN wn + 32 (t / 2) + 8 lq + 4 (t % 2) + r
+        const int first = n_t * BN + 16 * TN * wn, c0 = first + 8 * lq;
+        const bool whole = first + 16 * TN <= g.V;        // no column past the end
         #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int m = m_t * BM + 64 * wm + 16 * i + lr;
             const int target = m < g.N ? g.targets[m] : -1;
-            const int tc = target - g.v0;                 // the target's column of the piece
+            const int d = target - g.v0 - c0;             // the target's column from c0
+            // this lane's part of the row has it (rare)
+            const bool hit = target >= 0 && target - g.v0 < g.V && d >= 0 && d < 16 * TN && (d & 31) < 8;
             if constexpr (!GRAD) {
-                float big = -INFINITY, zt = 0.0f;
-                #pragma unroll
-                for (int t = 0; t < 8; t++)
+                float big = -INFINITY;
+                if (!whole)
                     #pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        const int c = c0 + 32 * (t / 2) + 4 * (t & 1) + r;
-                        const float z = c < g.V ? acc[i][t][r] : -INFINITY;
-                        acc[i][t][r] = z;
-                        zt = c == tc ? z : zt;
-                        big = fmaxf(big, z);
-                    }
+                    for (int t = 0; t < TN; t++)
+                        #pragma unroll
+                        for (int r = 0; r < 4; r++)
+                            if (c0 + 32 * (t / 2) + 4 * (t & 1) + r >= g.V) acc[i][t][r] = -INFINITY;
+                if (hit) {
+                    float zt = 0.0f;
+                    #pragma unroll
+                    for (int t = 0; t < TN; t++)
+                        #pragma unroll
+                        for (int r = 0; r < 4; r++) zt = d == 32 * (t / 2) + 4 * (t & 1) + r ? acc[i][t][r] : zt;
+                    g.hit[m] = zt;
+                }
+                #pragma unroll
+                for (int t = 0; t < TN; t++)
+                    #pragma unroll
+                    for (int r = 0; r < 4; r++) big = fmaxf(big, acc[i][t][r]);
                 big = fmaxf(big, kr_xor<16>(big));
                 big = fmaxf(big, kr_xor<32>(big));
+                // e^(z - big) as 2^(z log2 e - c); the rounding of c is taken back from the sum
                 const float base = big == -INFINITY ? 0.0f : big;
+                const float c = base * kLog2e;
+                const float back = __builtin_amdgcn_exp2f(__builtin_fmaf(-base, kLog2e, c));
                 float sum = 0.0f;
                 #pragma unroll
-                for (int t = 0; t < 8; t++) {
+                for (int t = 0; t < TN; t++) {
                     float s = 0.0f;
                     #pragma unroll
                     for (int r = 0; r < 4; r++)
-                        s += __builtin_amdgcn_exp2f((acc[i][t][r] - base) * kLog2e);
+                        s += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][t][r], kLog2e, -c));
                     sum += s;
                 }
                 sum += kr_xor<16>(sum);
                 sum += kr_xor<32>(sum);
-                const int d = tc - c0;
-                if (m < g.N) {
-                    if (target >= 0 && tc < g.V && d >= 0 && d < 128 && (d & 31) < 8) g.hit[m] = zt;
-                    if (lq == 0 && n_t * BN + 128 * wn < g.V)
-                        g.part[(size_t)(n_t * WN + wn) * g.N + m] = float2{big, sum};
-                }
+                if (m < g.N && lq == 0 && first < g.V)
+                    g.part[(size_t)(n_t * WN + wn) * g.N + m] = float2{big, sum * back};
             } else {
-                float f = 0.0f, lse = 0.0f;
+                // f e^(z - lse) as 2^(z log2 e - c) with f's sign set behind it
+                float f = 0.0f, c = 0.0f;
                 if (target != -1 && m < g.N) {
                     f = (unsigned)target < (unsigned)g.v_all ? g.dloss[m] * g.scale[0] : NAN;
-                    lse = g.lse[m];
+                    c = g.lse[m] * kLog2e - __builtin_amdgcn_logf(fabsf(f));
                 }
+                const float sign = f < 0.0f ? -1.0f : 1.0f;
                 kr_half* out = g.G + (size_t)m * g.ldg + c0;
                 #pragma unroll
-                for (int p = 0; p < 4; p++) {
+                for (int p = 0; p < TN / 2; p++) {
+                    float x[8];
+                    #pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        x[e] = sign * __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][2 * p + e / 4][e % 4], kLog2e, -c));
+                    if (hit && (unsigned)(d - 32 * p) < 8u)
+                        #pragma unroll
+                        for (int e = 0; e < 8; e++)
+                            if (d == 32 * p + e) x[e] -= f;
                     kr_half8 v;
                     #pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const int c = c0 + 32 * p + e;
-                        float z = __builtin_amdgcn_exp2f((acc[i][2 * p + e / 4][e % 4] - lse) * kLog2e);
-                        if (c == tc) z -= 1.0f;
-                        z *= f;
-                        v[e] = kr_f16(f == 0.0f || c >= g.V ? 0.0f : z);
-                    }
+                    for (int e = 0; e < 8; e++) v[e] = (kr_half)x[e];
+                    if (!whole)
+                        #pragma unroll
+                        for (int e = 0; e < 8; e++)
+                            if (c0 + 32 * p + e >= g.V) v[e] = 0;
+                    if (f == 0.0f) v = kr_half8{0, 0, 0, 0, 0, 0, 0, 0};
                     if (m < g.rows && c0 + 32 * p < (int)g.ldg) *reinterpret_cast<kr_half8*>(out + 32 * p) = v;
                 }
             }
@@ -218,30 +248,144 @@ __global__ void __launch_bounds__(64 * WM * WN, 1) logits_kernel(LossArgs g, int
     }
 }
 
-// Parts of a row -> lse and loss; 16 rows x 16 parts at a time.
+// ---------------------------------------------------------------------------
+// The forward pass of up to 16 rows: bound by W. Every wave walks 16-row blocks of W
+// through an LDS ring of its own (steps of 64 k, whole lines, no barriers) beside
+// x in LDS, and keeps a maximum and a sum per row.
+// ---------------------------------------------------------------------------
+constexpr int kFewRows = 16, kFewC = 1536, kFewWaves = 8, kFewStages = 6;
+
+__global__ void __launch_bounds__(64 * kFewWaves, 1) few_rows_kernel(LossArgs g) {
+    __shared__ __attribute__((aligned(1024))) kr_half8 ring[kFewWaves * kFewStages * 128];
+    __shared__ __attribute__((aligned(16))) kr_half8 xs[kFewRows * kFewC / 8];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int lr = lane & 15, lq = lane >> 4;
+    const int KS = g.C / 64, units = g.C / 8, blocks = (g.V + 15) / 16;
+    const int step = gridDim.x * kFewWaves, block0 = blockIdx.x + gridDim.x * wave;
+    const unsigned ring_base = lds_address(ring) + (unsigned)(wave * kFewStages * 2048);
+    int c_block = block0, c_ks = 0, c_stage = 0, ahead = 0;
+    auto copy_step = [&]() {
+        if (c_block >= blocks) return;
+        const kr_half* wa = g.W + (long long)c_block * 16 * g.ldw;
+        #pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const int row = 8 * i + (lane >> 3), kc = (lane & 7) ^ ((row >> 1) & 7);
+            const unsigned off = (unsigned)min(row, g.V - 1 - 16 * c_block) * (unsigned)(2 * g.ldw) +
+                                 (unsigned)(16 * kc + 128 * c_ks);
+            copy16(wa, off, ring_base + (unsigned)(c_stage * 2048 + 1024 * i));
+        }
+        ahead++;
+        c_stage = c_stage + 1 == kFewStages ? 0 : c_stage + 1;
+        if (++c_ks == KS) {
+            c_ks = 0;
+            c_block += step;
+        }
+    };
+    #pragma unroll
+    for (int i = 0; i < kFewStages - 1; i++) copy_step();
+    for (int i = tid; i < kFewRows * units; i += 64 * kFewWaves) {
+        const int n = i / units, u = i % units;
+        kr_half8 v = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (n < g.N) v = *reinterpret_cast<const kr_half8*>(g.x + (size_t)n * g.ldx + 8 * u);
+        xs[n * units + (u ^ (n & 7))] = v;
+    }
+    const int target = lr < g.N ? g.targets[lr] : -1;
+    __syncthreads();
+    float big = -INFINITY, sum = 0.0f;
+    int stage = 0;
+    for (int block = block0; block < blocks; block += step) {
+        kr_float4 z = {0, 0, 0, 0};
+        #pragma unroll 1
+        for (int ks = 0; ks < KS; ks++) {
+            if (ahead >= kFewStages - 1) wait_copies<(kFewStages - 2) * 2>();
+            else wait_copies<0>();
+            ahead--;
+            const kr_half8* Ws = ring + (wave * kFewStages + stage) * 128;
+            stage = stage + 1 == kFewStages ? 0 : stage + 1;
+            #pragma unroll
+            for (int kb = 0; kb < 2; kb++)
+                z = __builtin_amdgcn_mfma_f32_16x16x32_f16(Ws[row_unit(lr, 4 * kb + lq)],
+                                                           xs[lr * units + ((8 * ks + 4 * kb + lq) ^ (lr & 7))], z, 0,
+                                                           0, 0);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");    // the stage is read
+            copy_step();
+        }
+        const int v0 = 16 * block + 4 * lq, d = target - v0;
+        float to = big;
+        #pragma unroll
+        for (int r = 0; r < 4; r++) {
+            if (d == r && v0 + r < g.V) g.hit[lr] = z[r];
+            if (v0 + r >= g.V) z[r] = -INFINITY;
+            to = fmaxf(to, z[r]);
+        }
+        const float base = to == -INFINITY ? 0.0f : to;
+        sum *= __builtin_amdgcn_exp2f((big - base) * kLog2e);
+        #pragma unroll
+        for (int r = 0; r < 4; r++) sum += __builtin_amdgcn_exp2f((z[r] - base) * kLog2e);
+        big = to;
+    }
+    // the 4 x 8 parts of a row
+    __syncthreads();
+    float2* parts = reinterpret_cast<float2*>(xs);
+    parts[(4 * wave + lq) * 16 + lr] = float2{big, sum};
+    __syncthreads();
+    if (tid >= g.N) return;
+    big = -INFINITY;
+    for (int p = 0; p < 4 * kFewWaves; p++) big = fmaxf(big, parts[p * 16 + tid].x);
+    const float base = big == -INFINITY ? 0.0f : big;
+    sum = 0.0f;
+    for (int p = 0; p < 4 * kFewWaves; p++)
+        sum += parts[p * 16 + tid].y * __builtin_amdgcn_exp2f((parts[p * 16 + tid].x - base) * kLog2e);
+    g.part[(size_t)blockIdx.x * g.N + tid] = float2{big, sum};
+}
+
+// Parts of a row -> lse and loss; ROWS rows x 256 / ROWS parts at a time.
+template <int ROWS>
 __global__ void __launch_bounds__(256) loss_join_kernel(const float2* part, const float* hit, int N, int parts,
                                                         int V, const int32_t* targets, float* loss, float* lse) {
-    __shared__ float big_of[16][16], sum_of[16][16];
-    const int r = threadIdx.x & 15, p0 = threadIdx.x >> 4;
-    const int m = blockIdx.x * 16 + r;
+    constexpr int LANES = 256 / ROWS;
+    __shared__ float big_of[LANES][ROWS], sum_of[LANES][ROWS];
+    const int r = threadIdx.x % ROWS, p0 = threadIdx.x / ROWS;
+    const int m = blockIdx.x * ROWS + r;
     float big = -INFINITY, sum = 0.0f;
+    constexpr int kAhead = 8;             // or every step waits for memory
     if (m < N)
-        for (int p = p0; p < parts; p += 16) {
-            const float2 v = part[(size_t)p * N + m];
-            const float to = fmaxf(big, v.x), base = to == -INFINITY ? 0.0f : to;
-            sum = sum * __builtin_amdgcn_exp2f((big - base) * kLog2e) +
-                  v.y * __builtin_amdgcn_exp2f((v.x - base) * kLog2e);
+        for (int p = p0; p < parts; p += kAhead * LANES) {
+            float2 v[kAhead];
+            #pragma unroll
+            for (int i = 0; i < kAhead; i++)
+                v[i] = p + i * LANES < parts ? part[(size_t)(p + i * LANES) * N + m] : float2{-INFINITY, 0.0f};
+            float to = big;
+            #pragma unroll
+            for (int i = 0; i < kAhead; i++) to = fmaxf(to, v[i].x);
+            const float base = to == -INFINITY ? 0.0f : to;
+            sum *= __builtin_amdgcn_exp2f((big - base) * kLog2e);
+            #pragma unroll
+            for (int i = 0; i < kAhead; i++) sum += v[i].y * __builtin_amdgcn_exp2f((v[i].x - base) * kLog2e);
             big = to;
         }
     big_of[p0][r] = big;
     sum_of[p0][r] = sum;
     __syncthreads();
-    if (threadIdx.x >= 16 || m >= N) return;
+    if (ROWS == 1) {                      // 256 parts: first to 4 waves', then together
+        const float most = kr_wave_reduce(big, [](float a, float b) { return fmaxf(a, b); });
+        const float base = most == -INFINITY ? 0.0f : most;
+        sum = kr_wave_reduce(sum * __builtin_amdgcn_exp2f((big - base) * kLog2e), [](float a, float b) { return a + b; });
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) {
+            big_of[threadIdx.x >> 6][0] = most;
+            sum_of[threadIdx.x >> 6][0] = sum;
+        }
+        __syncthreads();
+    }
+    if (threadIdx.x >= ROWS || m >= N) return;
+    constexpr int LEFT = ROWS == 1 ? 4 : LANES;
     big = -INFINITY;
-    for (int p = 0; p < 16; p++) big = fmaxf(big, big_of[p][r]);
+    for (int p = 0; p < LEFT; p++) big = fmaxf(big, big_of[p][r]);
     const float base = big == -INFINITY ? 0.0f : big;
     sum = 0.0f;
-    for (int p = 0; p < 16; p++) sum += sum_of[p][r] * __builtin_amdgcn_exp2f((big_of[p][r] - base) * kLog2e);
+    for (int p = 0; p < LEFT; p++) sum += sum_of[p][r] * __builtin_amdgcn_exp2f((big_of[p][r] - base) * kLog2e);
     const float ln_sum = __builtin_amdgcn_logf(sum) * kLn2;
     const int target = targets[m];
     lse[m] = base + ln_sum;
@@ -249,13 +393,26 @@ __global__ void __launch_bounds__(256) loss_join_kernel(const float2* part, cons
 }
 
 // ---------------------------------------------------------------------------
-// Backward: the power of two of dz, and x with the rows that have no gradient as
-// zeros (whatever they hold), rounded up to 64 rows.
+// Backward: the power of two of dz (the last workgroup), and x with the rows that have
+// no gradient as zeros (whatever they hold), rounded up to 64 rows.
 // ---------------------------------------------------------------------------
-__global__ void __launch_bounds__(1024) grad_scale_kernel(const int32_t* targets, const float* dloss, int N,
-                                                          float* scale) {
+__global__ void __launch_bounds__(1024) grad_prepare_kernel(const kr_half* x, long long ldx, int N, int C, int rows,
+                                                            const int32_t* targets, const float* dloss,
+                                                            float* scale, kr_half* out) {
     __shared__ float part[16];
+    if (blockIdx.x + 1 < gridDim.x) {
+        const int per = C / 8;
+        const long long at = (long long)blockIdx.x * 1024 + threadIdx.x;
+        if (at >= (long long)rows * per) return;
+        const int m = (int)(at / per), c = 8 * (int)(at % per);
+        kr_half8 v = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (m < N && targets[m] != -1 && dloss[m] != 0.0f)
+            v = *reinterpret_cast<const kr_half8*>(x + (size_t)m * ldx + c);
+        *reinterpret_cast<kr_half8*>(out + (size_t)m * C + c) = v;
+        return;
+    }
     float big = 0.0f;
+    #pragma unroll 8
     for (int i = threadIdx.x; i < N; i += 1024) {
         const float a = fabsf(dloss[i]);
         if (targets[i] != -1 && a < INFINITY) big = fmaxf(big, a);
@@ -272,23 +429,11 @@ __global__ void __launch_bounds__(1024) grad_scale_kernel(const int32_t* targets
     }
 }
 
-__global__ void __launch_bounds__(256) live_rows_kernel(const kr_half* x, long long ldx, int N, int C, int rows,
-                                                        const int32_t* targets, const float* dloss, kr_half* out) {
-    const int per = C / 8;
-    const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (at >= (long long)rows * per) return;
-    const int m = (int)(at / per), c = 8 * (int)(at % per);
-    kr_half8 v = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (m < N && targets[m] != -1 && dloss[m] != 0.0f)
-        v = *reinterpret_cast<const kr_half8*>(x + (size_t)m * ldx + c);
-    *reinterpret_cast<kr_half8*>(out + (size_t)m * C + c) = v;
-}
-
 // ---------------------------------------------------------------------------
-// dW += dz' x and dx += dz W of one piece, in tiles of 256 x 256, 8 waves of
-// 64 x 128, steps of 64 k through two stages. Operands whose rows lie across k (W and
-// x as B, dz' as A) are staged as they lie, 64 k x 256 columns, and read by the LDS's
-// transposing reads: 16 lanes get 4 k of 16 columns.
+// dW += dz' x and dx += dz W of one piece, in tiles of (64 WM) x (16 TN WN), a wave for
+// each 64 x 16 TN, steps of 64 k through two stages. Operands whose rows lie across k
+// (W and x as B, dz' as A) are staged as they lie, 64 k x the tile's columns, and
+// read by the LDS's transposing reads: 16 lanes get 4 k of 16 columns.
 // ---------------------------------------------------------------------------
 struct ProdArgs {
     const kr_half* G;                 // [rows][ldg]
@@ -297,162 +442,185 @@ struct ProdArgs {
     const kr_half* W;                 // [V, C] of the piece
     long long ldw;
     const float* scale;
-    float* dx_part;                   // [dx_splits][rows][C]
-    float* dw_part;                   // [dw_splits][V][C], dw_splits > 1
-    void* dW;                         // [V][C] of the piece, dw_splits 1
-    int f32;                          // dW's type
-    int rows, C, V, first;            // first: dx_part is written, not added to
-    int dx_splits, dw_splits;
+    float* dx_part;                   // [dx_splits][rows][C], if not direct
+    float* dw_part;                   // [dw_splits][V][C], if not direct
+    void* dx;                         // [N][C], direct: one split, one piece
+    void* dW;                         // [V][C] of the piece, direct: one split
+    int f32;                          // their type
+    int N, rows, C, V, first;         // first: dx_part is written, not added to
+    int dx_splits, dw_splits, dx_direct;
+    int dw_run;                       // column tiles that an item of dW takes in turn
     int dw_items, dx_items;
 };
 
-constexpr int kProdStage = 512 * 8;   // 16-byte units: 32 KB of A, 32 of B
-
-// Columns that lie across k: LDS place, in bytes, of (k, 16-column tile, this lane's
-// 4 columns) with the tile XORed by a value of k's bits 0, 1 and 3, so that the 32
-// lanes of half a read are on different banks.
+// Columns that lie across k, in an LDS tile of COLS of them: place, in bytes, of this
+// lane's 4 columns of a 16-column tile for k = 8 (l / 16) + (l % 16) / 4, with the tile
+// XORed by a value of k's bits 0, 1 and 3, so that the 32 lanes of half a read are on
+// different banks.
+template <int COLS>
 __device__ __forceinline__ unsigned across(int tile, int lane) {
     const int lr = lane & 15, lq = lane >> 4;
     const int sw = (lr >> 2) | ((lq & 1) << 2);
-    return (unsigned)((8 * lq + (lr >> 2)) * 512 + 32 * (tile ^ sw) + 8 * (lr & 3));
+    return (unsigned)((8 * lq + (lr >> 2)) * 2 * COLS + 32 * (tile ^ sw) + 8 * (lr & 3));
 }
+template <int COLS>
 __device__ __forceinline__ kr_half8 read_across(unsigned at) {
     typedef kr_half half4v __attribute__((ext_vector_type(4)));
     const half4v lo = __builtin_bit_cast(half4v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(uintptr_t)at));
-    const half4v hi =
-        __builtin_bit_cast(half4v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(uintptr_t)(at + 2048)));
+    const half4v hi = __builtin_bit_cast(
+        half4v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(uintptr_t)(at + 8 * COLS)));
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-template <bool DW>
+// Copies of one step of an operand, 64 k x COLS, by half of the workgroup's waves.
+template <int COLS, int COPIES>
+__device__ __forceinline__ void copy_across(const kr_half* base, long long ld, int last, int cols, unsigned to,
+                                            int part, int lane) {
+    constexpr int PER = 512 / COLS, LANES = 64 / PER;     // rows of a copy, lanes of a row
+    base = shared_by_lanes(base);
+    #pragma unroll
+    for (int i = 0; i < COPIES; i++) {
+        const int k = PER * (part * COPIES + i) + lane / LANES;
+        const int sw = 2 * ((k & 3) | ((k >> 1) & 4));
+        const int col = 8 * ((lane % LANES) ^ sw);
+        const unsigned off = (unsigned)min(k, last) * (unsigned)(2 * ld) + (unsigned)(col < cols ? 2 * col : 0);
+        copy16(base, off, to + 1024u * (unsigned)(part * COPIES + i));
+    }
+}
+
+__device__ __forceinline__ void store_out(void* out, size_t at, kr_float4 v, int f32) {
+    if (f32) *reinterpret_cast<kr_float4*>(static_cast<float*>(out) + at) = v;
+    else
+        *reinterpret_cast<kr_half4*>(static_cast<kr_half*>(out) + at) =
+            kr_half4{kr_f16(v[0]), kr_f16(v[1]), kr_f16(v[2]), kr_f16(v[3])};
+}
+
+template <int WM, int WN, int TN, bool DW>
 __device__ __forceinline__ void product_tile(const ProdArgs& g, kr_half8* ring, int item) {
+    constexpr int BM = 64 * WM, BN = 16 * TN * WN, WAVES = WM * WN;
+    static_assert(BM == BN, "half of the waves copy each operand");
+    constexpr int COPIES = BM / 8 / (WAVES / 2), STAGE = (BM + BN) * 8;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wm = wave >> 1, wn = wave & 1;
+    const int wm = wave / WN, wn = wave % WN;
     const int lr = lane & 15, lq = lane >> 4;
-    const int gx = (g.C + 255) / 256;
+    const int gx = (g.C + BN - 1) / BN;
     const int splits = DW ? g.dw_splits : g.dx_splits;
-    const int n_t = item % gx, m_t = item / gx / splits, split = item / gx % splits;
+    const int runs = DW ? (gx + g.dw_run - 1) / g.dw_run : gx;
+    const int n_first = item % runs * (DW ? g.dw_run : 1), n_last = DW ? min(n_first + g.dw_run, gx) : n_first + 1;
+    const int m_t = item / runs / splits, split = item / runs % splits;
     const int M = DW ? g.V : g.rows;
     const int steps = DW ? g.rows / 64 : (g.V + 63) / 64;
     const int ks0 = (int)((long long)steps * split / splits), ks1 = (int)((long long)steps * (split + 1) / splits);
     const unsigned ring_base = lds_address(ring);
-    const int m0 = m_t * 256, n0 = n_t * 256;
+    const int m0 = m_t * BM;
     // A: dW reads G across (columns m0.., always inside ldg), dx along
     const kr_half* a_base = DW ? g.G + m0 : g.G + (size_t)m0 * g.ldg;
-    const kr_half* b_base = (DW ? g.x : g.W) + n0;
+    const kr_half* b_base = DW ? g.x : g.W;
     const long long ldb = DW ? g.C : g.ldw;
-    auto issue = [&](int ks, int q) {
-        const unsigned so = ring_base + (unsigned)((q & 1) * kProdStage * 16);
-        if (wave < 4 && !DW) {
+    auto issue = [&](int n_t, int ks, int q) {
+        const unsigned so = ring_base + (unsigned)((q & 1) * STAGE * 16);
+        const int n0 = n_t * BN;
+        if (wave >= WAVES / 2) {
+            // B's k past the piece: the last row, against zeros of G
+            copy_across<BN, COPIES>(b_base + n0 + (long long)ks * 64 * ldb, ldb, DW ? 63 : g.V - 1 - 64 * ks, g.C - n0,
+                                    so + BM * 128, wave - WAVES / 2, lane);
+        } else if (DW) {
+            copy_across<BM, COPIES>(a_base + (long long)ks * 64 * g.ldg, g.ldg, 63, (int)g.ldg - m0, so, wave, lane);
+        } else {
             #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const int row = 8 * (wave * 8 + i) + (lane >> 3);
+            for (int i = 0; i < COPIES; i++) {
+                const int row = 8 * (wave * COPIES + i) + (lane >> 3);
                 const int kc = (lane & 7) ^ ((row >> 1) & 7);
                 const unsigned off = (unsigned)min(row, M - 1 - m0) * (unsigned)(2 * g.ldg) +
                                      (unsigned)(16 * kc + 128 * ks);
-                copy16(a_base, off, so + 1024u * (unsigned)(wave * 8 + i));
-            }
-        } else {
-            const bool a = DW && wave < 4;
-            const kr_half* base = a ? a_base + (long long)ks * 64 * g.ldg : b_base + (long long)ks * 64 * ldb;
-            const long long ld = a ? g.ldg : ldb;
-            // B's k past the piece: the last row, against zeros of G
-            const int last = !DW && !a ? g.V - 1 - 64 * ks : 63;
-            const int cols = a ? (int)g.ldg - m0 : g.C - n0;
-            #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const int k = 2 * ((wave & 3) * 8 + i) + (lane >> 5);
-                const int sw = 2 * ((k & 3) | ((k >> 1) & 4));
-                const int col = 8 * ((lane & 31) ^ sw);
-                const unsigned off = (unsigned)min(k, last) * (unsigned)(2 * ld) + (unsigned)(col < cols ? 2 * col : 0);
-                copy16(base, off, so + 1024u * (unsigned)(wave * 8 + i));
+                copy16(a_base, off, so + 1024u * (unsigned)(wave * COPIES + i));
             }
         }
     };
-    kr_float4 acc[4][8];
+    unsigned a_at[4], b_at[TN];
     #pragma unroll
-    for (int i = 0; i < 4; i++)
+    for (int i = 0; i < 4; i++) a_at[i] = across<BM>(4 * wm + i, lane);
+    #pragma unroll
+    for (int t = 0; t < TN; t++) b_at[t] = across<BN>(TN * wn + t, lane) + BM * 128u;
+    const float down = g.scale[1];
+    const bool direct = DW ? splits == 1 : g.dx_direct != 0;
+    const int m_end = !DW && direct ? g.N : M;
+    int q = 0;
+    issue(n_first, ks0, 0);
+    for (int n_t = n_first; n_t < n_last; n_t++) {
+        kr_float4 acc[4][TN];
         #pragma unroll
-        for (int t = 0; t < 8; t++) acc[i][t] = kr_float4{0, 0, 0, 0};
-    unsigned a_at[4], b_at[8];
-    #pragma unroll
-    for (int i = 0; i < 4; i++) a_at[i] = across(4 * wm + i, lane);
-    #pragma unroll
-    for (int t = 0; t < 8; t++) b_at[t] = across(8 * wn + t, lane) + 32768u;
-    if (ks0 < ks1) issue(ks0, 0);
-    #pragma unroll 1
-    for (int ks = ks0, q = 0; ks < ks1; ks++, q++) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        if (ks + 1 < ks1) issue(ks + 1, q + 1);
-        const kr_half8* As = ring + (q & 1) * kProdStage;
-        const unsigned so = ring_base + (unsigned)((q & 1) * kProdStage * 16);
-        #pragma unroll
-        for (int kb = 0; kb < 2; kb++) {
-            kr_half8 a[4];
+        for (int i = 0; i < 4; i++)
             #pragma unroll
-            for (int i = 0; i < 4; i++)
-                a[i] = DW ? read_across(so + a_at[i] + 16384u * kb) : As[row_unit(64 * wm + 16 * i + lr, 4 * kb + lq)];
+            for (int t = 0; t < TN; t++) acc[i][t] = kr_float4{0, 0, 0, 0};
+        #pragma unroll 1
+        for (int ks = ks0; ks < ks1; ks++, q++) {
+            wait_copies<0>();
+            __syncthreads();   // every wave's copies are in; the step before is read
+            if (ks + 1 < ks1) issue(n_t, ks + 1, q + 1);
+            else if (n_t + 1 < n_last) issue(n_t + 1, ks0, q + 1);
+            const kr_half8* As = ring + (q & 1) * STAGE;
+            const unsigned so = ring_base + (unsigned)((q & 1) * STAGE * 16);
             #pragma unroll
-            for (int th = 0; th < 2; th++) {
-                __builtin_amdgcn_sched_barrier(0);
-                kr_half8 b[4];
-                #pragma unroll
-                for (int t = 0; t < 4; t++) b[t] = read_across(so + b_at[4 * th + t] + 16384u * kb);
-                __builtin_amdgcn_sched_barrier(0);
+            for (int kb = 0; kb < 2; kb++) {
+                kr_half8 a[4];
                 #pragma unroll
                 for (int i = 0; i < 4; i++)
+                    a[i] = DW ? read_across<BM>(so + a_at[i] + 64u * BM * kb)
+                              : As[row_unit(64 * wm + 16 * i + lr, 4 * kb + lq)];
+                #pragma unroll
+                for (int th = 0; th < TN / 4; th++) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    kr_half8 b[4];
                     #pragma unroll
-                    for (int t = 0; t < 4; t++)
-                        acc[i][4 * th + t] =
-                            __builtin_amdgcn_mfma_f32_16x16x32_f16(b[t], a[i], acc[i][4 * th + t], 0, 0, 0);
+                    for (int t = 0; t < 4; t++) b[t] = read_across<BN>(so + b_at[4 * th + t] + 64u * BN * kb);
+                    __builtin_amdgcn_sched_barrier(0);
+                    #pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        #pragma unroll
+                        for (int t = 0; t < 4; t++)
+                            acc[i][4 * th + t] =
+                                __builtin_amdgcn_mfma_f32_16x16x32_f16(b[t], a[i], acc[i][4 * th + t], 0, 0, 0);
+                }
             }
         }
-    }
-    const float down = g.scale[1];
-    #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int m = m0 + 64 * wm + 16 * i + lr;
-        if (m >= M) continue;
         #pragma unroll
-        for (int t = 0; t < 8; t++) {
-            const int n = n0 + 128 * wn + 16 * t + 4 * lq;
-            if (n >= g.C) continue;
-            kr_float4 v = acc[i][t];
-            if (!DW || splits > 1) {
-                float* part = DW ? g.dw_part : g.dx_part;
-                kr_float4* o = reinterpret_cast<kr_float4*>(part + ((size_t)split * M + m) * g.C + n);
-                if (!DW && !g.first) v += *o;
-                *o = v;
-            } else {
-                v *= down;
-                const size_t o = (size_t)m * g.C + n;
-                if (g.f32) *reinterpret_cast<kr_float4*>(static_cast<float*>(g.dW) + o) = v;
-                else
-                    *reinterpret_cast<kr_half4*>(static_cast<kr_half*>(g.dW) + o) =
-                        kr_half4{kr_f16(v[0]), kr_f16(v[1]), kr_f16(v[2]), kr_f16(v[3])};
+        for (int i = 0; i < 4; i++) {
+            const int m = m0 + 64 * wm + 16 * i + lr;
+            if (m >= m_end) continue;
+            #pragma unroll
+            for (int t = 0; t < TN; t++) {
+                const int n = n_t * BN + 16 * TN * wn + 16 * t + 4 * lq;
+                if (n >= g.C) continue;
+                kr_float4 v = acc[i][t];
+                if (direct) {
+                    store_out(DW ? g.dW : g.dx, (size_t)m * g.C + n, v * down, g.f32);
+                } else {
+                    float* part = DW ? g.dw_part : g.dx_part;
+                    kr_float4* o = reinterpret_cast<kr_float4*>(part + ((size_t)split * M + m) * g.C + n);
+                    if (!DW && !g.first) v += *o;
+                    *o = v;
+                }
             }
         }
     }
 }
 
-__global__ void __launch_bounds__(512, 1) grad_products_kernel(ProdArgs g) {
-    __shared__ __attribute__((aligned(1024))) kr_half8 ring[2 * kProdStage];
-    // an eighth of the items for each XCD, dW's before dx's
-    int b = blockIdx.x;
-    if (b < g.dw_items) {
-        const int per = (g.dw_items + 7) / 8, full = g.dw_items % 8 ? g.dw_items % 8 : 8;
-        const int xcd = b & 7, i = b >> 3;
-        const int item = xcd < full ? xcd * per + i : full * per + (xcd - full) * (per - 1) + i;
-        product_tile<true>(g, ring, item);
-    } else {
-        b -= g.dw_items;
-        const int per = (g.dx_items + 7) / 8, full = g.dx_items % 8 ? g.dx_items % 8 : 8;
-        const int xcd = b & 7, i = b >> 3;
-        const int item = xcd < full ? xcd * per + i : full * per + (xcd - full) * (per - 1) + i;
-        product_tile<false>(g, ring, item);
-    }
+// Item of workgroup b: an eighth of the items in order for each XCD.
+__device__ __forceinline__ int item_of(int b, int items) {
+    const int per = (items + 7) / 8, full = items % 8 ? items % 8 : 8;
+    const int xcd = b & 7, i = b >> 3;
+    return xcd < full ? xcd * per + i : full * per + (xcd - full) * (per - 1) + i;
+}
+
+template <int WM, int WN, int TN>
+__global__ void __launch_bounds__(64 * WM * WN, WM * WN >= 8 ? 1 : 2) grad_products_kernel(ProdArgs g) {
+    __shared__ __attribute__((aligned(1024))) kr_half8 ring[2 * (64 * WM + 16 * TN * WN) * 8];
+    // dW's items before dx's
+    const int b = blockIdx.x;
+    if (b < g.dw_items) product_tile<WM, WN, TN, true>(g, ring, item_of(b, g.dw_items));
+    else product_tile<WM, WN, TN, false>(g, ring, item_of(b - g.dw_items, g.dx_items));
 }
 
 // Sum of the splits of n outputs, in their order.
@@ -460,31 +628,47 @@ __global__ void __launch_bounds__(256) grad_sum_kernel(const float* part, long l
                                                        const float* scale, int f32, void* out) {
     const long long at = 4 * ((long long)blockIdx.x * 256 + threadIdx.x);
     if (at >= n) return;
-    kr_float4 v = *reinterpret_cast<const kr_float4*>(part + at);
-    for (int s = 1; s < splits; s++) v += *reinterpret_cast<const kr_float4*>(part + s * stride + at);
-    v *= scale[1];
-    if (f32) *reinterpret_cast<kr_float4*>(static_cast<float*>(out) + at) = v;
-    else
-        *reinterpret_cast<kr_half4*>(static_cast<kr_half*>(out) + at) =
-            kr_half4{kr_f16(v[0]), kr_f16(v[1]), kr_f16(v[2]), kr_f16(v[3])};
+    kr_float4 v = {0, 0, 0, 0};
+    constexpr int kAhead = 8;             // or every split waits for memory
+    for (int s = 0; s < splits; s += kAhead) {
+        kr_float4 x[kAhead];
+        #pragma unroll
+        for (int i = 0; i < kAhead; i++)
+            x[i] = s + i < splits ? *reinterpret_cast<const kr_float4*>(part + (s + i) * stride + at) : kr_float4{0, 0, 0, 0};
+        #pragma unroll
+        for (int i = 0; i < kAhead; i++) v += x[i];
+    }
+    store_out(out, at, v * scale[1], f32);
 }
 
-template <int WM, int WN, bool GRAD>
+template <int WM, int WN, int TN, bool GRAD>
 int launch_logits(const LossArgs& g, hipStream_t s) {
-    const int gy = ((GRAD ? g.rows : g.N) + 64 * WM - 1) / (64 * WM), gx = (g.V + 128 * WN - 1) / (128 * WN);
-    const int n_virtual = (int)(((long long)gx * gy + 7) / 8 * 8);
+    constexpr int BM = 64 * WM, BN = 16 * TN * WN;
+    const int gy = ((GRAD ? g.rows : g.N) + BM - 1) / BM, gx = (g.V + BN - 1) / BN;
+    const long long tiles = (long long)gx * gy;
+    const int n_virtual = (int)((tiles + 7) / 8 * 8);
     const int at_once = 256 * (WM * WN >= 8 ? 1 : 2);
     const int grid = n_virtual < at_once ? n_virtual : at_once;
     // about 1.25 MB of x to a group of row tiles, as an L2 holds beside W's
-    const int group_m = (int)std::min<long long>(8, std::max<long long>(1, (5ll << 18) / (64 * WM * 2ll * g.C)));
-    logits_kernel<WM, WN, GRAD><<<grid, 64 * WM * WN, 0, s>>>(g, n_virtual, group_m);
+    const int group_m = (int)std::min<long long>(8, std::max<long long>(1, (5ll << 18) / (BM * 2ll * g.C)));
+    logits_kernel<WM, WN, TN, GRAD><<<grid, 64 * WM * WN, 0, s>>>(g, n_virtual, group_m);
     KR_LAUNCHED();
     return KR_OK;
 }
 
+// Which tiles: 256 x 256 once they fill the chip, 128 x 128 below.
+bool big_tiles(int N, int V) { return (long long)((N + 255) / 256) * ((V + 255) / 256) >= 512; }
+
 template <bool GRAD>
-int logits(const LossArgs& g, hipStream_t s) {
-    return g.N > 128 ? launch_logits<4, 2, GRAD>(g, s) : launch_logits<1, 1, GRAD>(g, s);
+int logits(const LossArgs& g, bool big, hipStream_t s) {
+    return big ? launch_logits<4, 2, 8, GRAD>(g, s) : launch_logits<2, 2, 4, GRAD>(g, s);
+}
+
+// Forward: parts of a row, and their count.
+bool few_rows(int N, int C) { return N <= kFewRows && C <= kFewC; }
+int loss_parts(int N, int C, int V) {
+    if (few_rows(N, C)) return std::min(256, (V + 16 * kFewWaves - 1) / (16 * kFewWaves));
+    return big_tiles(N, V) ? (V + 127) / 128 : (V + 63) / 64;
 }
 
 bool shape_ok(int N, int C, int V) {
@@ -494,33 +678,37 @@ bool shape_ok(int N, int C, int V) {
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
 // How a backward call is cut: pieces of the vocabulary whose dz takes at most
-// 256 MB, and the products' splits.
+// 176 MB, and the products' splits.
 struct GradPlan {
-    int rows, piece, pieces, dx_splits, dw_splits;
-    size_t scale, x, G, dx_part, dw_part, total;      // offsets in the workspace
+    int rows, piece, pieces, dx_splits, dw_splits, dw_run;
+    bool big, dx_direct;
+    size_t x, G, dx_part, dw_part, total;             // offsets in the workspace
 };
 
 GradPlan grad_plan(int N, int C, int V, bool dx, bool dw) {
     GradPlan p{};
     p.rows = (N + 63) / 64 * 64;
-    const long long most = std::max<long long>(256, (128ll << 20) / p.rows / 256 * 256);
+    const long long most = std::max<long long>(256, (88ll << 20) / p.rows / 256 * 256);
     p.pieces = (int)((V + most - 1) / most);
     p.piece = ((V + p.pieces - 1) / p.pieces + 255) / 256 * 256;
     p.pieces = (V + p.piece - 1) / p.piece;
-    const int gx = (C + 255) / 256;
-    const int dx_steps = p.piece / 64, dw_steps = p.rows / 64;
-    const long long dx_tiles = (long long)(p.rows + 255) / 256 * gx, dw_tiles = (long long)p.piece / 256 * gx;
+    p.big = big_tiles(N, V) && p.rows >= 1024;
+    const int tile = p.big ? 256 : 128, slots = p.big ? 256 : 512;
+    const int gx = (C + tile - 1) / tile, dx_steps = p.piece / 64, dw_steps = p.rows / 64;
+    const long long dx_tiles = (long long)(p.rows + tile - 1) / tile * gx, dw_tiles = (long long)p.piece / tile * gx;
     const long long total = (dx ? dx_tiles * dx_steps : 0) + (dw ? dw_tiles * dw_steps : 0);
-    const long long each = std::max<long long>(8, total / 1024);
+    const long long each = std::max<long long>(8, total / (3 * slots));
     p.dx_splits = (int)std::max<long long>(1, std::min<long long>(64, dx_steps / each));
-    p.dw_splits = dw_tiles >= 128 ? 1 : (int)std::max<long long>(1, std::min<long long>(64, dw_steps / each));
-    size_t at = 256;
+    p.dw_splits = dw_tiles >= slots / 4 ? 1 : (int)std::max<long long>(1, std::min<long long>(64, dw_steps / each));
+    p.dw_run = dw_steps <= 8 && p.dw_splits == 1 ? gx : 1;
+    p.dx_direct = p.dx_splits == 1 && p.pieces == 1;
+    size_t at = 256;                                  // the scale
     p.x = at;
     at += up256((size_t)p.rows * C * 2);
     p.G = at;
     at += up256((size_t)p.rows * p.piece * 2);
     p.dx_part = at;
-    if (dx) at += up256((size_t)p.dx_splits * p.rows * C * 4);
+    if (dx && !p.dx_direct) at += up256((size_t)p.dx_splits * p.rows * C * 4);
     p.dw_part = at;
     if (dw && p.dw_splits > 1) at += up256((size_t)p.dw_splits * std::min(V, p.piece) * C * 4);
     p.total = at;
@@ -533,7 +721,7 @@ extern "C" {
 
 size_t kr_head_loss_workspace_bytes(int N, int C, int V) {
     if (!shape_ok(N, C, V) || N == 0) return 0;
-    return up256((size_t)N * 4) + (size_t)((V + kPart - 1) / kPart) * N * sizeof(float2);
+    return up256((size_t)N * 4) + (size_t)loss_parts(N, C, V) * N * sizeof(float2);
 }
 
 int kr_head_loss(const uint16_t* x, long long ldx, int N, int C, const uint16_t* W, long long ldw, int V,
@@ -560,9 +748,16 @@ int kr_head_loss(const uint16_t* x, long long ldx, int N, int C, const uint16_t*
     g.C = C;
     g.V = g.v_all = V;
     const hipStream_t s = kr_stream(stream);
-    const int rc = logits<false>(g, s);
-    if (rc != KR_OK) return rc;
-    loss_join_kernel<<<(N + 15) / 16, 256, 0, s>>>(g.part, g.hit, N, (V + kPart - 1) / kPart, V, targets, loss, lse);
+    const int parts = loss_parts(N, C, V);
+    if (few_rows(N, C)) {
+        few_rows_kernel<<<parts, 64 * kFewWaves, 0, s>>>(g);
+        KR_LAUNCHED();
+    } else {
+        const int rc = logits<false>(g, big_tiles(N, V), s);
+        if (rc != KR_OK) return rc;
+    }
+    if (N <= 256) loss_join_kernel<1><<<N, 256, 0, s>>>(g.part, g.hit, N, parts, V, targets, loss, lse);
+    else loss_join_kernel<16><<<(N + 15) / 16, 256, 0, s>>>(g.part, g.hit, N, parts, V, targets, loss, lse);
     KR_LAUNCHED();
     return KR_OK;
 }
@@ -592,13 +787,10 @@ int kr_head_loss_backward(const uint16_t* x, long long ldx, int N, int C, const 
     kr_half* live = reinterpret_cast<kr_half*>(base + p.x);
     const kr_half* xh = reinterpret_cast<const kr_half*>(x);
     const hipStream_t s = kr_stream(stream);
-    grad_scale_kernel<<<1, 1024, 0, s>>>(targets, dloss, N, scale);
+    const long long units = dW ? (long long)p.rows * (C / 8) : 0;
+    grad_prepare_kernel<<<(unsigned)((units + 1023) / 1024 + 1), 1024, 0, s>>>(xh, ldx, N, C, p.rows, targets, dloss,
+                                                                              scale, live);
     KR_LAUNCHED();
-    if (dW) {
-        const long long units = (long long)p.rows * (C / 8);
-        live_rows_kernel<<<(unsigned)((units + 255) / 256), 256, 0, s>>>(xh, ldx, N, C, p.rows, targets, dloss, live);
-        KR_LAUNCHED();
-    }
     LossArgs g{};
     g.x = xh;
     g.ldx = ldx;
@@ -626,19 +818,24 @@ int kr_head_loss_backward(const uint16_t* x, long long ldx, int N, int C, const 
     d.C = C;
     d.dx_splits = p.dx_splits;
     d.dw_splits = p.dw_splits;
-    const int gx = (C + 255) / 256;
+    d.N = N;
+    d.dx = dx;
+    d.dx_direct = p.dx_direct;
+    d.dw_run = p.dw_run;
+    const int tile = p.big ? 256 : 128, gx = (C + tile - 1) / tile;
     for (int i = 0; i < p.pieces; i++) {
         const int v0 = i * p.piece, nv = std::min(V - v0, p.piece);
         g.W = d.W = reinterpret_cast<const kr_half*>(W) + (size_t)v0 * ldw;
         g.V = d.V = nv;
         g.v0 = v0;
-        const int rc = logits<true>(g, s);
+        const int rc = logits<true>(g, p.big, s);
         if (rc != KR_OK) return rc;
         d.first = i == 0;
         d.dW = dW ? static_cast<char*>(dW) + (size_t)v0 * C * (out_f32 ? 4 : 2) : nullptr;
-        d.dw_items = dW ? (nv + 255) / 256 * gx * p.dw_splits : 0;
-        d.dx_items = dx ? (p.rows + 255) / 256 * gx * p.dx_splits : 0;
-        grad_products_kernel<<<d.dw_items + d.dx_items, 512, 0, s>>>(d);
+        d.dw_items = dW ? (nv + tile - 1) / tile * ((gx + p.dw_run - 1) / p.dw_run) * p.dw_splits : 0;
+        d.dx_items = dx ? (p.rows + tile - 1) / tile * gx * p.dx_splits : 0;
+        if (p.big) grad_products_kernel<4, 2, 8><<<d.dw_items + d.dx_items, 512, 0, s>>>(d);
+        else grad_products_kernel<2, 2, 4><<<d.dw_items + d.dx_items, 256, 0, s>>>(d);
         KR_LAUNCHED();
         if (dW && p.dw_splits > 1) {
             const long long n = (long long)nv * C;
@@ -647,7 +844,7 @@ int kr_head_loss_backward(const uint16_t* x, long long ldx, int N, int C, const 
             KR_LAUNCHED();
         }
     }
-    if (dx) {
+    if (dx && !p.dx_direct) {
         const long long n = (long long)N * C;
         grad_sum_kernel<<<(unsigned)((n / 4 + 255) / 256), 256, 0, s>>>(d.dx_part, (long long)p.rows * C, p.dx_splits, n,
                                                                        scale, out_f32, dx);
