@@ -147,6 +147,15 @@ __global__ void __launch_bounds__(4 * D) delta_step_kernel(DeltaArgs g) {
 // Parts of the chunked kernels.
 // ---------------------------------------------------------------------------
 
+// The lane, made anew: LDS addresses that follow from it are not kept over a chunk,
+// where they and the reads moved up to them spill.
+__device__ __forceinline__ int fresh(int lane) {
+    __asm__ volatile("" : "+v"(lane));
+    return lane;
+}
+// Nothing is moved over this, for the same reason.
+__device__ __forceinline__ void phase() { __builtin_amdgcn_sched_barrier(0); }
+
 // Powers of two that bring a largest value x to 2^13..2^14, and back. Zero and
 // values under 2^-113 count as 2^-113; infinities and NaN pass through.
 __device__ __forceinline__ void power_scale(float x, float& up, float& down) {
@@ -236,7 +245,7 @@ __device__ __forceinline__ kr_half8 channels_state(const kr_half8* tile, int s, 
 }
 
 // Per chunk: sums of log2 decays, and what follows from them.
-struct Gates {
+struct alignas(16) Gates {
     double a[kChunk];
     float e0[kChunk], e1[kChunk], beta[kChunk];   // e^a, e^(a_end - a), write strengths
     float all;                                    // e^a_end
@@ -260,11 +269,12 @@ __device__ __forceinline__ void make_gates(Gates& o, float gate, float beta, int
 // The triangular matrices of a chunk as operands: rows i, units of 8 j. M holds N
 // of the chunk's two halves in its diagonal 32 x 32 blocks and A below them. With
 // TRANSPOSED, rows are j and units i, of all three.
+constexpr int kWork = 36;             // floats of a row
 struct Pairs {
     kr_half8 ph[kChunk * 8], pl[kChunk * 8];
     kr_half8 mh[kChunk * 8], ml[kChunk * 8];
     float p_down[kChunk], n_down[kChunk], a_down[kChunk];
-    float work[2][32 * 33];       // fp32 A, then N, of the two halves
+    float work[2][32 * kWork];    // fp32 A, then N, of the two halves
 };
 
 __device__ __forceinline__ void store_parts4(kr_half8* hi, kr_half8* lo, int row, int col, kr_float4 x, float up) {
@@ -286,6 +296,8 @@ template <int D, bool TRANSPOSED>
 __device__ __forceinline__ void make_p(Pairs& o, const kr_half8* q, const kr_half8* k, const Gates& gates, int w,
                                        int lane) {
     constexpr int KS = D / 32;
+    phase();
+    lane = fresh(lane);
     const int l16 = lane & 15, q4 = lane >> 4, row = 16 * w + l16;
     kr_half8 mine[KS];
     #pragma unroll
@@ -293,22 +305,29 @@ __device__ __forceinline__ void make_p(Pairs& o, const kr_half8* q, const kr_hal
     const double a = gates.a[row];
     kr_float4 P[4];
     float big = 0.0f;
+    // all four tiles, though those on one side of the diagonal are not used: their reads
+    // and products are in flight together
     #pragma unroll
     for (int ct = 0; ct < 4; ct++) {
         P[ct] = kr_float4{0, 0, 0, 0};
-        if (TRANSPOSED ? ct < w : ct > w) continue;
         #pragma unroll
         for (int s = 0; s < KS; s++)
             P[ct] = mfma((TRANSPOSED ? q : k)[tok_unit<D>(16 * ct + l16, 4 * s + q4)], mine[s], P[ct]);
-        #pragma unroll
-        for (int r = 0; r < 4; r++) {
-            const int col = 16 * ct + 4 * q4 + r;
-            const double d = TRANSPOSED ? gates.a[col] - a : a - gates.a[col];
-            const bool on = TRANSPOSED ? col >= row : col <= row;
-            P[ct][r] = on ? P[ct][r] * __builtin_amdgcn_exp2f((float)d) : 0.0f;
-            big = fmaxf(big, fabsf(P[ct][r]));
-        }
     }
+    #pragma unroll
+    for (int ct = 0; ct < 4; ct++)
+        if (TRANSPOSED ? ct >= w : ct <= w) {
+            #pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int col = 16 * ct + 4 * q4 + r;
+                const double d = TRANSPOSED ? gates.a[col] - a : a - gates.a[col];
+                const bool on = TRANSPOSED ? col >= row : col <= row;
+                P[ct][r] = on ? P[ct][r] * __builtin_amdgcn_exp2f((float)d) : 0.0f;
+                big = fmaxf(big, fabsf(P[ct][r]));
+            }
+        } else {
+            P[ct] = kr_float4{0, 0, 0, 0};
+        }
     float up, down;
     power_scale(max_of_quarters(big), up, down);
     if (q4 == 0) o.p_down[row] = down;
@@ -324,43 +343,51 @@ __device__ __forceinline__ void make_p(Pairs& o, const kr_half8* q, const kr_hal
 template <int D, bool TRANSPOSED>
 __device__ __forceinline__ void make_a(Pairs& o, const kr_half8* k, const Gates& gates, int w, int lane) {
     constexpr int KS = D / 32;
+    phase();
+    lane = fresh(lane);
     const int l16 = lane & 15, q4 = lane >> 4, row = 16 * w + l16;
     kr_half8 mine[KS];
     #pragma unroll
     for (int s = 0; s < KS; s++) mine[s] = k[tok_unit<D>(row, 4 * s + q4)];
     const double a = gates.a[row];
-    // the half's own: rows i, columns j
-    float* work = o.work[w / 2] + (row & 31) * 33;
+    // the half's own: rows i, columns j (the tile above the diagonal gives zeros)
+    const int half = w / 2;
+    float* work = o.work[half] + (row & 31) * kWork;
+    kr_float4 A[2];
     #pragma unroll
     for (int ct = 0; ct < 2; ct++) {
-        if (ct > (w & 1)) continue;
-        kr_float4 A = {0, 0, 0, 0};
+        A[ct] = kr_float4{0, 0, 0, 0};
         #pragma unroll
-        for (int s = 0; s < KS; s++) A = mfma(k[tok_unit<D>(32 * (w / 2) + 16 * ct + l16, 4 * s + q4)], mine[s], A);
+        for (int s = 0; s < KS; s++) A[ct] = mfma(k[tok_unit<D>(32 * half + 16 * ct + l16, 4 * s + q4)], mine[s], A[ct]);
+    }
+    #pragma unroll
+    for (int ct = 0; ct < 2; ct++) {
         #pragma unroll
         for (int r = 0; r < 4; r++) {
             const int col = 16 * ct + 4 * q4 + r;
-            const float e = __builtin_amdgcn_exp2f((float)(a - gates.a[32 * (w / 2) + col]));
-            work[col] = col < (row & 31) ? A[r] * e : 0.0f;
+            const float e = __builtin_amdgcn_exp2f((float)(a - gates.a[32 * half + col]));
+            A[ct][r] = col < (row & 31) ? A[ct][r] * e : 0.0f;
         }
+        *reinterpret_cast<kr_float4*>(work + 16 * ct + 4 * q4) = A[ct];
     }
     // below: rows 32.. against columns 0..31, or transposed
     if (TRANSPOSED ? w < 2 : w >= 2) {
         const int c0 = TRANSPOSED ? 32 : 0;
-        kr_float4 A[2];
         float big = 0.0f;
         #pragma unroll
         for (int ct = 0; ct < 2; ct++) {
             A[ct] = kr_float4{0, 0, 0, 0};
             #pragma unroll
             for (int s = 0; s < KS; s++) A[ct] = mfma(k[tok_unit<D>(c0 + 16 * ct + l16, 4 * s + q4)], mine[s], A[ct]);
+        }
+        #pragma unroll
+        for (int ct = 0; ct < 2; ct++)
             #pragma unroll
             for (int r = 0; r < 4; r++) {
                 const double b = gates.a[c0 + 16 * ct + 4 * q4 + r];
                 A[ct][r] *= __builtin_amdgcn_exp2f((float)(TRANSPOSED ? b - a : a - b));
                 big = fmaxf(big, fabsf(A[ct][r]));
             }
-        }
         float up, down;
         power_scale(max_of_quarters(big), up, down);
         if (q4 == 0) o.a_down[row] = down;
@@ -369,66 +396,79 @@ __device__ __forceinline__ void make_a(Pairs& o, const kr_half8* k, const Gates&
     }
 }
 
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // N of the 16 x 16 diagonal block w, in place of A, by the wave that wrote it: row
 // by row, N_t = A_t - sum_j A_tj (beta_j N_j); lane = column.
 __device__ __forceinline__ void solve_16(Pairs& o, const Gates& gates, int w, int lane) {
+    phase();
+    lane = fresh(lane);
     const int l16 = lane & 15, q4 = lane >> 4;
-    float* block = o.work[w / 2] + 16 * (w & 1) * 34;
+    float* block = o.work[w / 2] + 16 * (w & 1) * (kWork + 1);
     const float* beta = gates.beta + 16 * w;
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
+    wave_sync();
     float N[16], bN[16];
     #pragma unroll
     for (int t = 0; t < 16; t++) {
-        float x = block[33 * t + l16];
+        float x = block[kWork * t + l16];
         #pragma unroll
-        for (int j = 0; j < t; j++) x = __builtin_fmaf(-block[33 * t + j], bN[j], x);
+        for (int j4 = 0; j4 < t; j4 += 4) {
+            const kr_float4 at = *reinterpret_cast<const kr_float4*>(block + kWork * t + j4);
+            #pragma unroll
+            for (int j = j4; j < j4 + 4 && j < t; j++) x = __builtin_fmaf(-at[j - j4], bN[j], x);
+        }
         N[t] = x;
         bN[t] = beta[t] * x;
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
+    wave_sync();
     #pragma unroll
     for (int t = 0; t < 16; t++)
-        if (t / 4 == q4) block[33 * t + l16] = N[t];
+        if (t / 4 == q4) block[kWork * t + l16] = N[t];
+    wave_sync();
 }
 
 // The 16 x 16 block below, by one wave for each half: with Y = A10 - A10 (beta N00),
 // N10 = Y - N11 (beta Y).
 __device__ __forceinline__ void solve_32(Pairs& o, const Gates& gates, int half, int lane) {
+    phase();
+    lane = fresh(lane);
     const int l16 = lane & 15, q4 = lane >> 4;
     float* work = o.work[half];
     const float* beta = gates.beta + 32 * half;
     kr_float4 Y;
     #pragma unroll
-    for (int r = 0; r < 4; r++) Y[r] = work[33 * (16 + 4 * q4 + r) + l16];
+    for (int r = 0; r < 4; r++) Y[r] = work[kWork * (16 + 4 * q4 + r) + l16];
+    const kr_float4 a10 = *reinterpret_cast<const kr_float4*>(work + kWork * (16 + l16) + 4 * q4);
+    const kr_float4 n11 = *reinterpret_cast<const kr_float4*>(work + kWork * (16 + l16) + 16 + 4 * q4);
+    const kr_float4 b0 = *reinterpret_cast<const kr_float4*>(beta + 4 * q4);
+    const kr_float4 b1 = *reinterpret_cast<const kr_float4*>(beta + 16 + 4 * q4);
     #pragma unroll
-    for (int s = 0; s < 4; s++) {
-        const int j = 4 * q4 + s;
-        Y = __builtin_amdgcn_mfma_f32_16x16x4f32(-work[33 * (16 + l16) + j], beta[j] * work[33 * j + l16], Y, 0, 0, 0);
-    }
+    for (int s = 0; s < 4; s++)
+        Y = __builtin_amdgcn_mfma_f32_16x16x4f32(-a10[s], b0[s] * work[kWork * (4 * q4 + s) + l16], Y, 0, 0, 0);
     kr_float4 N = Y;
     #pragma unroll
-    for (int s = 0; s < 4; s++) {
-        const int j = 16 + 4 * q4 + s;
-        N = __builtin_amdgcn_mfma_f32_16x16x4f32(-work[33 * (16 + l16) + j], beta[j] * Y[s], N, 0, 0, 0);
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
+    for (int s = 0; s < 4; s++) N = __builtin_amdgcn_mfma_f32_16x16x4f32(-n11[s], b1[s] * Y[s], N, 0, 0, 0);
+    wave_sync();
     #pragma unroll
-    for (int r = 0; r < 4; r++) work[33 * (16 + 4 * q4 + r) + l16] = N[r];
+    for (int r = 0; r < 4; r++) work[kWork * (16 + 4 * q4 + r) + l16] = N[r];
+    wave_sync();
 }
 
 // 16 rows of N of a half (columns for TRANSPOSED) as operands, by one wave.
 template <bool TRANSPOSED>
 __device__ __forceinline__ void store_n(Pairs& o, int w, int lane) {
+    phase();
+    lane = fresh(lane);
     const int l16 = lane & 15, q4 = lane >> 4, row = 16 * w + l16;
     const float* work = o.work[w / 2];
     float x[8];
     #pragma unroll
     for (int e = 0; e < 8; e++) {
         const int i = TRANSPOSED ? 8 * q4 + e : row & 31, j = TRANSPOSED ? row & 31 : 8 * q4 + e;
-        x[e] = j < i ? work[33 * i + j] : 0.0f;
+        x[e] = j < i ? work[kWork * i + j] : 0.0f;
     }
     float down;
     const Parts8 p = scaled8(x, down);
@@ -439,19 +479,26 @@ __device__ __forceinline__ void store_n(Pairs& o, int w, int lane) {
 }
 
 // All of them, by the workgroup's 4 or 8 waves; tokens and gates are in LDS, and the
-// matrices are when it returns.
-template <int D, bool TRANSPOSED, bool WITH_P>
+// matrices are when it returns. The 16 rows of a half whose operand does not take the
+// block below (the first ones, transposed the second) are done before the others.
+// next(): what wave 0, which has least of A, does meanwhile.
+template <int D, bool TRANSPOSED, bool WITH_P, typename Next>
 __device__ __forceinline__ void make_pairs(Pairs& o, const kr_half8* q, const kr_half8* k, const Gates& gates, int wave,
-                                           int lane) {
+                                           int lane, Next next) {
+    const bool first = (wave & 1) == (TRANSPOSED ? 1 : 0);
     if (wave < 4) {
         make_a<D, TRANSPOSED>(o, k, gates, wave, lane);
         solve_16(o, gates, wave, lane);
+        if (first) store_n<TRANSPOSED>(o, wave, lane);
     }
-    if (WITH_P && (D == 64 || wave >= 4)) make_p<D, TRANSPOSED>(o, q, k, gates, wave & 3, lane);
+    // P's tiles go against A's: the wave with most of one has least of the other
+    if (WITH_P && (D == 64 || wave >= 4)) make_p<D, TRANSPOSED>(o, q, k, gates, 3 - (wave & 3), lane);
+    if (wave == (D == 64 ? 3 : 0)) next();
     __syncthreads();
-    if (wave < 4 && (wave & 1)) solve_32(o, gates, wave / 2, lane);
-    __syncthreads();
-    if (wave < 4) store_n<TRANSPOSED>(o, wave, lane);
+    if (wave < 4 && !first) {
+        solve_32(o, gates, wave / 2, lane);
+        store_n<TRANSPOSED>(o, wave, lane);
+    }
     __syncthreads();
 }
 
@@ -548,7 +595,7 @@ __global__ void __launch_bounds__(4 * D, 2) delta_chunk_kernel(DeltaArgs g) {
     kr_half* yp = g.y + (row0 + l16) * g.ldy + h * D + 16 * wave + 4 * q4;
 
     fetch(0);
-    if (wave == 0) {
+    if (wave == (D == 64 ? 3 : 0)) {
         fetch_gates(0);
         make_gates(sh.gates[0], gate, beta, lane);
         fetch_gates(kChunk);
@@ -571,13 +618,15 @@ __global__ void __launch_bounds__(4 * D, 2) delta_chunk_kernel(DeltaArgs g) {
                 for (int e = 0; e < 8; e++) out[(size_t)(32 * s + e) * D] = S[2 * s + e / 4][e % 4];
         }
         __syncthreads();
-        make_pairs<D, false, !STATES>(sh.pairs, sh.q, sh.k, gates, wave, lane);
-        if (wave == 0 && t0 + kChunk < n_tok) {
+        make_pairs<D, false, !STATES>(sh.pairs, sh.q, sh.k, gates, wave, lane, [&]() {
+            if (t0 + kChunk >= n_tok) return;
             make_gates(sh.gates[(c + 1) & 1], gate, beta, lane);
             fetch_gates(t0 + 2 * kChunk);
-        }
+        });
 
         // the state's parts, with a scale for each column
+        phase();
+        const int ln = fresh(lane), l16 = ln & 15, q4 = ln >> 4;
         float big = 0.0f, up, down;
         #pragma unroll
         for (int s = 0; s < 2 * KS; s++)
@@ -595,11 +644,12 @@ __global__ void __launch_bounds__(4 * D, 2) delta_chunk_kernel(DeltaArgs g) {
                 sp[s].lo[e] = y;
             }
 
+        phase();
         // X = v - e^a k S, rows t = 32 s + 8 q4 + e, column m
         float X[2][8];
         #pragma unroll
         for (int s = 0; s < 2; s++) {
-            const kr_half8 vc = channels16<D>(sh.v, s, wave, lane);
+            const kr_half8 vc = channels16<D>(sh.v, s, wave, ln);
             #pragma unroll
             for (int hf = 0; hf < 2; hf++) {
                 const int t = 32 * s + 8 * (l16 >> 2) + 4 * hf + (l16 & 3);
@@ -615,40 +665,52 @@ __global__ void __launch_bounds__(4 * D, 2) delta_chunk_kernel(DeltaArgs g) {
                 for (int r = 0; r < 4; r++) X[s][4 * hf + r] = (float)vc[4 * hf + r] - (e0[r] * down) * z[r];
             }
         }
-        // u of the first half, then of the second
-        Parts8 up8[2];
-        float u_down[2], U[2][8];
+        phase();
+        // u of the first half, then of the second; first all operands that they take
+        Parts8 up8[2], n_of[2][2], a_of[2];
+        float u_down[2], U[2][8], bt[2][8];
+        kr_float4 n_f[2][2], a_f[2];
+        #pragma unroll
+        for (int s = 0; s < 2; s++)
+            #pragma unroll
+            for (int hf = 0; hf < 2; hf++) {
+                const int t = 32 * s + 8 * (l16 >> 2) + 4 * hf + (l16 & 3), at = pair_unit(t, 4 * s + q4);
+                n_of[s][hf] = Parts8{sh.pairs.mh[at], sh.pairs.ml[at]};
+                n_f[s][hf] = *reinterpret_cast<const kr_float4*>(sh.pairs.n_down + 32 * s + 8 * q4 + 4 * hf);
+                const kr_float4 b4 = *reinterpret_cast<const kr_float4*>(gates.beta + 32 * s + 8 * q4 + 4 * hf);
+                #pragma unroll
+                for (int r = 0; r < 4; r++) bt[s][4 * hf + r] = b4[r];
+                if (s == 1) {
+                    const int below = pair_unit(t, q4);
+                    a_of[hf] = Parts8{sh.pairs.mh[below], sh.pairs.ml[below]};
+                    a_f[hf] = *reinterpret_cast<const kr_float4*>(sh.pairs.a_down + 32 + 8 * q4 + 4 * hf);
+                }
+            }
         #pragma unroll
         for (int s = 0; s < 2; s++) {
-            float bt[8], x[8], x_down;
-            #pragma unroll
-            for (int e = 0; e < 8; e++) bt[e] = gates.beta[32 * s + 8 * q4 + e];
-            const int t = 32 * s + 8 * (l16 >> 2) + (l16 & 3);
+            float x[8], x_down;
             if (s == 1) {
                 #pragma unroll
                 for (int hf = 0; hf < 2; hf++) {
-                    const int at = pair_unit(t + 4 * hf, q4);
-                    const kr_float4 z = mfma3(sh.pairs.mh[at], sh.pairs.ml[at], up8[0], kr_float4{0, 0, 0, 0});
-                    const kr_float4 f = *reinterpret_cast<const kr_float4*>(sh.pairs.a_down + 32 + 8 * q4 + 4 * hf);
+                    const kr_float4 z = mfma3(a_of[hf].hi, a_of[hf].lo, up8[0], kr_float4{0, 0, 0, 0});
                     #pragma unroll
-                    for (int r = 0; r < 4; r++) X[1][4 * hf + r] -= (f[r] * u_down[0]) * z[r];
+                    for (int r = 0; r < 4; r++) X[1][4 * hf + r] -= (a_f[hf][r] * u_down[0]) * z[r];
                 }
             }
             #pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = bt[e] * X[s][e];
+            for (int e = 0; e < 8; e++) x[e] = bt[s][e] * X[s][e];
             const Parts8 xp = scaled8(x, x_down);
             #pragma unroll
             for (int hf = 0; hf < 2; hf++) {
-                const int at = pair_unit(t + 4 * hf, 4 * s + q4);
-                const kr_float4 z = mfma3(sh.pairs.mh[at], sh.pairs.ml[at], xp, kr_float4{0, 0, 0, 0});
-                const kr_float4 f = *reinterpret_cast<const kr_float4*>(sh.pairs.n_down + 32 * s + 8 * q4 + 4 * hf);
+                const kr_float4 z = mfma3(n_of[s][hf].hi, n_of[s][hf].lo, xp, kr_float4{0, 0, 0, 0});
                 #pragma unroll
-                for (int r = 0; r < 4; r++) X[s][4 * hf + r] -= (f[r] * x_down) * z[r];
+                for (int r = 0; r < 4; r++) X[s][4 * hf + r] -= (n_f[s][hf][r] * x_down) * z[r];
             }
             #pragma unroll
-            for (int e = 0; e < 8; e++) U[s][e] = bt[e] * X[s][e];
+            for (int e = 0; e < 8; e++) U[s][e] = bt[s][e] * X[s][e];
             up8[s] = scaled8(U[s], u_down[s]);
         }
+        phase();
         if constexpr (STATES) {
             float* out = g.diff + (((size_t)c * heads + head) * kChunk + 8 * q4) * D + m;
             #pragma unroll
@@ -666,6 +728,7 @@ __global__ void __launch_bounds__(4 * D, 2) delta_chunk_kernel(DeltaArgs g) {
             }
             #pragma unroll
             for (int it = 0; it < 4; it++) {
+                if (it == 2) phase();
                 const int i = 16 * it + l16;
                 kr_float4 from_s = {0, 0, 0, 0}, in0 = {0, 0, 0, 0}, in1 = {0, 0, 0, 0};
                 #pragma unroll
@@ -697,6 +760,7 @@ __global__ void __launch_bounds__(4 * D, 2) delta_chunk_kernel(DeltaArgs g) {
             }
             yp += kChunk * g.ldy;
         }
+        phase();
         // S <- e^a_end S + k' (e^(a_end - a) u)
         float x[2][8];
         #pragma unroll
@@ -712,12 +776,13 @@ __global__ void __launch_bounds__(4 * D, 2) delta_chunk_kernel(DeltaArgs g) {
             kr_float4 add = {0, 0, 0, 0};
             #pragma unroll
             for (int s = 0; s < 2; s++) {
-                const kr_half8 kc = channels_state<D>(sh.k, s, st, lane);
+                const kr_half8 kc = channels_state<D>(sh.k, s, st, ln);
                 add = mfma(kc, xp[s].lo, add);
                 add = mfma(kc, xp[s].hi, add);
             }
             #pragma unroll
             for (int r = 0; r < 4; r++) S[st][r] = __builtin_fmaf(add[r], x_down, all * S[st][r]);
+            if (st % 2) phase();
         }
         __syncthreads();
     }
@@ -821,7 +886,7 @@ __global__ void __launch_bounds__(4 * D, 2) delta_back_kernel(BackArgs g) {
     };
     if (chunks > 0) {
         fetch((chunks - 1) * kChunk);
-        if (wave == 0) {
+        if (wave == (D == 64 ? 3 : 0)) {
             fetch_gates((chunks - 1) * kChunk);
             make_gates(sh.gates[(chunks - 1) & 1], gate, beta, lane);
             fetch_gates((chunks - 2) * kChunk);
@@ -844,11 +909,13 @@ __global__ void __launch_bounds__(4 * D, 2) delta_back_kernel(BackArgs g) {
                 for (int e = 0; e < 8; e++) out[(size_t)(32 * s + e) * D] = S[2 * s + e / 4][e % 4];
         }
         __syncthreads();
-        make_pairs<D, true, true>(sh.pairs, sh.q, sh.k, gates, wave, lane);
-        if (wave == 0 && c > 0) {
+        make_pairs<D, true, true>(sh.pairs, sh.q, sh.k, gates, wave, lane, [&]() {
+            if (c == 0) return;
             make_gates(sh.gates[(c - 1) & 1], gate, beta, lane);
             fetch_gates((c - 2) * kChunk);
-        }
+        });
+        phase();
+        const int ln = fresh(lane), l16 = ln & 15, q4 = ln >> 4;
         float big = 0.0f, up, down;
         #pragma unroll
         for (int s = 0; s < 2 * KS; s++)
@@ -865,9 +932,10 @@ __global__ void __launch_bounds__(4 * D, 2) delta_back_kernel(BackArgs g) {
                 sp[s].hi[e] = x;
                 sp[s].lo[e] = y;
             }
+        phase();
         // du, rows t = 32 s + 8 q4 + e, column m
         float X[2][8];
-        const kr_half8 dyc[2] = {channels16<D>(sh.v, 0, wave, lane), channels16<D>(sh.v, 1, wave, lane)};
+        const kr_half8 dyc[2] = {channels16<D>(sh.v, 0, wave, ln), channels16<D>(sh.v, 1, wave, ln)};
         #pragma unroll
         for (int s = 0; s < 2; s++)
             #pragma unroll
@@ -891,38 +959,49 @@ __global__ void __launch_bounds__(4 * D, 2) delta_back_kernel(BackArgs g) {
                 #pragma unroll
                 for (int r = 0; r < 4; r++) X[s][4 * hf + r] = __builtin_fmaf(e1[r] * down, z[r], f[r] * in[r]);
             }
-        // w of the second half, then of the first
-        Parts8 dx1;
-        float dx1_down = 0.0f, dX[2][8];
+        phase();
+        // w of the second half, then of the first; first all operands that they take
+        Parts8 dx1, n_of[2][2], a_of[2];
+        float dx1_down = 0.0f, dX[2][8], bt[2][8];
+        kr_float4 n_f[2][2], a_f[2];
+        #pragma unroll
+        for (int s = 0; s < 2; s++)
+            #pragma unroll
+            for (int hf = 0; hf < 2; hf++) {
+                const int t = 32 * s + 8 * (l16 >> 2) + 4 * hf + (l16 & 3), at = pair_unit(t, 4 * s + q4);
+                n_of[s][hf] = Parts8{sh.pairs.mh[at], sh.pairs.ml[at]};
+                n_f[s][hf] = *reinterpret_cast<const kr_float4*>(sh.pairs.n_down + 32 * s + 8 * q4 + 4 * hf);
+                const kr_float4 b4 = *reinterpret_cast<const kr_float4*>(gates.beta + 32 * s + 8 * q4 + 4 * hf);
+                #pragma unroll
+                for (int r = 0; r < 4; r++) bt[s][4 * hf + r] = b4[r];
+                if (s == 0) {
+                    const int above = pair_unit(t, 4 + q4);
+                    a_of[hf] = Parts8{sh.pairs.mh[above], sh.pairs.ml[above]};
+                    a_f[hf] = *reinterpret_cast<const kr_float4*>(sh.pairs.a_down + 8 * q4 + 4 * hf);
+                }
+            }
         #pragma unroll
         for (int s = 1; s >= 0; s--) {
-            float bt[8], x[8], x_down;
-            #pragma unroll
-            for (int e = 0; e < 8; e++) bt[e] = gates.beta[32 * s + 8 * q4 + e];
-            const int t = 32 * s + 8 * (l16 >> 2) + (l16 & 3);
+            float x[8], x_down;
             if (s == 0) {
                 #pragma unroll
                 for (int hf = 0; hf < 2; hf++) {
-                    const int at = pair_unit(t + 4 * hf, 4 + q4);
-                    const kr_float4 z = mfma3(sh.pairs.mh[at], sh.pairs.ml[at], dx1, kr_float4{0, 0, 0, 0});
-                    const kr_float4 f = *reinterpret_cast<const kr_float4*>(sh.pairs.a_down + 8 * q4 + 4 * hf);
+                    const kr_float4 z = mfma3(a_of[hf].hi, a_of[hf].lo, dx1, kr_float4{0, 0, 0, 0});
                     #pragma unroll
-                    for (int r = 0; r < 4; r++) X[0][4 * hf + r] -= (f[r] * dx1_down) * z[r];
+                    for (int r = 0; r < 4; r++) X[0][4 * hf + r] -= (a_f[hf][r] * dx1_down) * z[r];
                 }
             }
             #pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = bt[e] * X[s][e];
+            for (int e = 0; e < 8; e++) x[e] = bt[s][e] * X[s][e];
             const Parts8 xp = scaled8(x, x_down);
             #pragma unroll
             for (int hf = 0; hf < 2; hf++) {
-                const int at = pair_unit(t + 4 * hf, 4 * s + q4);
-                const kr_float4 z = mfma3(sh.pairs.mh[at], sh.pairs.ml[at], xp, kr_float4{0, 0, 0, 0});
-                const kr_float4 f = *reinterpret_cast<const kr_float4*>(sh.pairs.n_down + 32 * s + 8 * q4 + 4 * hf);
+                const kr_float4 z = mfma3(n_of[s][hf].hi, n_of[s][hf].lo, xp, kr_float4{0, 0, 0, 0});
                 #pragma unroll
-                for (int r = 0; r < 4; r++) X[s][4 * hf + r] -= (f[r] * x_down) * z[r];
+                for (int r = 0; r < 4; r++) X[s][4 * hf + r] -= (n_f[s][hf][r] * x_down) * z[r];
             }
             #pragma unroll
-            for (int e = 0; e < 8; e++) dX[s][e] = bt[e] * X[s][e];
+            for (int e = 0; e < 8; e++) dX[s][e] = bt[s][e] * X[s][e];
             if (s == 1) dx1 = scaled8(dX[1], dx1_down);
         }
         {
@@ -932,6 +1011,7 @@ __global__ void __launch_bounds__(4 * D, 2) delta_back_kernel(BackArgs g) {
                 #pragma unroll
                 for (int e = 0; e < 8; e++) out[(size_t)(32 * s + e) * D] = X[s][e];
         }
+        phase();
         // D <- e^a_end D + q' (e^a dy) - k' (e^a dX)
         float yx[2][8];
         #pragma unroll
@@ -953,7 +1033,7 @@ __global__ void __launch_bounds__(4 * D, 2) delta_back_kernel(BackArgs g) {
             kr_float4 from_y = {0, 0, 0, 0}, from_x = {0, 0, 0, 0};
             #pragma unroll
             for (int s = 0; s < 2; s++) {
-                const kr_half8 qc = channels_state<D>(sh.q, s, st, lane), kc = channels_state<D>(sh.k, s, st, lane);
+                const kr_half8 qc = channels_state<D>(sh.q, s, st, ln), kc = channels_state<D>(sh.k, s, st, ln);
                 from_y = mfma(qc, yp[s].lo, from_y);
                 from_y = mfma(qc, yp[s].hi, from_y);
                 from_x = mfma(kc, xp[s].lo, from_x);
@@ -962,6 +1042,7 @@ __global__ void __launch_bounds__(4 * D, 2) delta_back_kernel(BackArgs g) {
             #pragma unroll
             for (int r = 0; r < 4; r++)
                 S[st][r] = __builtin_fmaf(from_x[r], x_down, __builtin_fmaf(from_y[r], y_down, all * S[st][r]));
+            if (st % 2) phase();
         }
         __syncthreads();
     }
