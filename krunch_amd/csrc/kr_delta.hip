@@ -165,11 +165,11 @@ __device__ __forceinline__ void power_scale(float x, float& up, float& down) {
     down = __uint_as_float((uint32_t)(e - 13) << 23);
 }
 
-// x as a high and a low fp16 part.
-__device__ __forceinline__ void two_parts(float x, kr_half& hi, kr_half& lo) {
-    __asm__("" : "+v"(x));
-    hi = (kr_half)x;
-    lo = (kr_half)(x - (float)hi);
+// x up as a high and a low fp16 part (up a power of two: two instructions, since both
+// are an fma rounded to fp16).
+__device__ __forceinline__ void two_parts(float x, float up, kr_half& hi, kr_half& lo) {
+    hi = (kr_half)__builtin_fmaf(x, up, 0.0f);
+    lo = (kr_half)__builtin_fmaf(x, up, -(float)hi);
 }
 
 __device__ __forceinline__ float max_of_quarters(float x) {       // over lanes l % 16
@@ -191,7 +191,7 @@ __device__ __forceinline__ Parts8 parts8(const float (&x)[8], float up) {
     #pragma unroll
     for (int e = 0; e < 8; e++) {
         kr_half a, b;
-        two_parts(x[e] * up, a, b);
+        two_parts(x[e], up, a, b);
         p.hi[e] = a;
         p.lo[e] = b;
     }
@@ -244,10 +244,14 @@ __device__ __forceinline__ kr_half8 channels_state(const kr_half8* tile, int s, 
     return read_tokens<D>(tile, s, 4 * (st >> 1) + (lane & 3), st & 1, lane);
 }
 
-// Per chunk: sums of log2 decays, and what follows from them.
+// Per chunk: sums of log2 decays, and what follows from them. A decay between tokens of
+// two tiles of 16 is one to the later tile's start times one from there, both at most
+// 1: a product instead of an exponential a pair.
 struct alignas(16) Gates {
     double a[kChunk];
     float e0[kChunk], e1[kChunk], beta[kChunk];   // e^a, e^(a_end - a), write strengths
+    float from[kChunk];                           // from the start of the token's tile to it
+    float to[3][kChunk];                          // from the token to the start of tile 1, 2, 3
     float all;                                    // e^a_end
 };
 // By one wave, lane = token.
@@ -258,12 +262,24 @@ __device__ __forceinline__ void make_gates(Gates& o, float gate, float beta, int
         const double b = __shfl_up(a, d);
         if (lane >= d) a += b;
     }
-    const double end = __shfl(a, 63);
+    const double end = __shfl(a, 63), starts[3] = {__shfl(a, 15), __shfl(a, 31), __shfl(a, 47)};
+    const double start = lane < 16 ? 0.0 : lane < 32 ? starts[0] : lane < 48 ? starts[1] : starts[2];
     o.a[lane] = a;
     o.e0[lane] = __builtin_amdgcn_exp2f((float)a);
     o.e1[lane] = __builtin_amdgcn_exp2f((float)(end - a));
     o.beta[lane] = beta;
+    o.from[lane] = __builtin_amdgcn_exp2f((float)(a - start));
+    #pragma unroll
+    for (int i = 0; i < 3; i++) o.to[i][lane] = __builtin_amdgcn_exp2f((float)(starts[i] - a));
     if (lane == 63) o.all = __builtin_amdgcn_exp2f((float)end);
+}
+// e^(a_row - a_col) for 4 columns from `col`, of an earlier tile than row's, w.
+__device__ __forceinline__ kr_float4 decays_to(const Gates& g, int w, float from_row, int col) {
+    return *reinterpret_cast<const kr_float4*>(g.to[w - 1] + col) * from_row;
+}
+// The same for columns of a later tile ct, e^(a_col - a_row).
+__device__ __forceinline__ kr_float4 decays_from(const Gates& g, int ct, int row, int col) {
+    return *reinterpret_cast<const kr_float4*>(g.from + col) * g.to[ct - 1][row];
 }
 
 // The triangular matrices of a chunk as operands: rows i, units of 8 j. M holds N
@@ -282,7 +298,7 @@ __device__ __forceinline__ void store_parts4(kr_half8* hi, kr_half8* lo, int row
     #pragma unroll
     for (int r = 0; r < 4; r++) {
         kr_half a, b;
-        two_parts(x[r] * up, a, b);
+        two_parts(x[r], up, a, b);
         h[r] = a;
         l[r] = b;
     }
@@ -303,6 +319,7 @@ __device__ __forceinline__ void make_p(Pairs& o, const kr_half8* q, const kr_hal
     #pragma unroll
     for (int s = 0; s < KS; s++) mine[s] = (TRANSPOSED ? k : q)[tok_unit<D>(row, 4 * s + q4)];
     const double a = gates.a[row];
+    const float from = gates.from[row];
     kr_float4 P[4];
     float big = 0.0f;
     // all four tiles, though those on one side of the diagonal are not used: their reads
@@ -315,19 +332,23 @@ __device__ __forceinline__ void make_p(Pairs& o, const kr_half8* q, const kr_hal
             P[ct] = mfma((TRANSPOSED ? q : k)[tok_unit<D>(16 * ct + l16, 4 * s + q4)], mine[s], P[ct]);
     }
     #pragma unroll
-    for (int ct = 0; ct < 4; ct++)
-        if (TRANSPOSED ? ct >= w : ct <= w) {
+    for (int ct = 0; ct < 4; ct++) {
+        const int col = 16 * ct + 4 * q4;
+        if (ct == w) {
             #pragma unroll
             for (int r = 0; r < 4; r++) {
-                const int col = 16 * ct + 4 * q4 + r;
-                const double d = TRANSPOSED ? gates.a[col] - a : a - gates.a[col];
-                const bool on = TRANSPOSED ? col >= row : col <= row;
+                const double d = TRANSPOSED ? gates.a[col + r] - a : a - gates.a[col + r];
+                const bool on = TRANSPOSED ? col + r >= row : col + r <= row;
                 P[ct][r] = on ? P[ct][r] * __builtin_amdgcn_exp2f((float)d) : 0.0f;
-                big = fmaxf(big, fabsf(P[ct][r]));
             }
+        } else if (TRANSPOSED ? ct > w : ct < w) {
+            P[ct] *= TRANSPOSED ? decays_from(gates, ct, row, col) : decays_to(gates, w, from, col);
         } else {
             P[ct] = kr_float4{0, 0, 0, 0};
         }
+        #pragma unroll
+        for (int r = 0; r < 4; r++) big = fmaxf(big, fabsf(P[ct][r]));
+    }
     float up, down;
     power_scale(max_of_quarters(big), up, down);
     if (q4 == 0) o.p_down[row] = down;
@@ -360,15 +381,20 @@ __device__ __forceinline__ void make_a(Pairs& o, const kr_half8* k, const Gates&
         #pragma unroll
         for (int s = 0; s < KS; s++) A[ct] = mfma(k[tok_unit<D>(32 * half + 16 * ct + l16, 4 * s + q4)], mine[s], A[ct]);
     }
+    const float from = gates.from[row];
     #pragma unroll
     for (int ct = 0; ct < 2; ct++) {
-        #pragma unroll
-        for (int r = 0; r < 4; r++) {
-            const int col = 16 * ct + 4 * q4 + r;
-            const float e = __builtin_amdgcn_exp2f((float)(a - gates.a[32 * half + col]));
-            A[ct][r] = col < (row & 31) ? A[ct][r] * e : 0.0f;
+        const int col = 32 * half + 16 * ct + 4 * q4;
+        if (ct == (w & 1)) {
+            #pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const float e = __builtin_amdgcn_exp2f((float)(a - gates.a[col + r]));
+                A[ct][r] = col + r < row ? A[ct][r] * e : 0.0f;
+            }
+        } else if (ct == 0) {
+            A[ct] *= decays_to(gates, w, from, col);
         }
-        *reinterpret_cast<kr_float4*>(work + 16 * ct + 4 * q4) = A[ct];
+        if (ct <= (w & 1)) *reinterpret_cast<kr_float4*>(work + 16 * ct + 4 * q4) = A[ct];
     }
     // below: rows 32.. against columns 0..31, or transposed
     if (TRANSPOSED ? w < 2 : w >= 2) {
@@ -381,13 +407,12 @@ __device__ __forceinline__ void make_a(Pairs& o, const kr_half8* k, const Gates&
             for (int s = 0; s < KS; s++) A[ct] = mfma(k[tok_unit<D>(c0 + 16 * ct + l16, 4 * s + q4)], mine[s], A[ct]);
         }
         #pragma unroll
-        for (int ct = 0; ct < 2; ct++)
+        for (int ct = 0; ct < 2; ct++) {
+            const int col = c0 + 16 * ct + 4 * q4;
+            A[ct] *= TRANSPOSED ? decays_from(gates, 2 + ct, row, col) : decays_to(gates, w, from, col);
             #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const double b = gates.a[c0 + 16 * ct + 4 * q4 + r];
-                A[ct][r] *= __builtin_amdgcn_exp2f((float)(TRANSPOSED ? b - a : a - b));
-                big = fmaxf(big, fabsf(A[ct][r]));
-            }
+            for (int r = 0; r < 4; r++) big = fmaxf(big, fabsf(A[ct][r]));
+        }
         float up, down;
         power_scale(max_of_quarters(big), up, down);
         if (q4 == 0) o.a_down[row] = down;
@@ -401,15 +426,14 @@ __device__ __forceinline__ void wave_sync() {
     __builtin_amdgcn_wave_barrier();
 }
 
-// N of the 16 x 16 diagonal block w, in place of A, by the wave that wrote it: row
+// N of the four 16 x 16 diagonal blocks, in place of A, by one wave, 16 lanes each: row
 // by row, N_t = A_t - sum_j A_tj (beta_j N_j); lane = column.
-__device__ __forceinline__ void solve_16(Pairs& o, const Gates& gates, int w, int lane) {
+__device__ __forceinline__ void solve_16(Pairs& o, const Gates& gates, int lane) {
     phase();
     lane = fresh(lane);
-    const int l16 = lane & 15, q4 = lane >> 4;
+    const int l16 = lane & 15, w = lane >> 4;
     float* block = o.work[w / 2] + 16 * (w & 1) * (kWork + 1);
     const float* beta = gates.beta + 16 * w;
-    wave_sync();
     float N[16], bN[16];
     #pragma unroll
     for (int t = 0; t < 16; t++) {
@@ -425,12 +449,11 @@ __device__ __forceinline__ void solve_16(Pairs& o, const Gates& gates, int w, in
     }
     wave_sync();
     #pragma unroll
-    for (int t = 0; t < 16; t++)
-        if (t / 4 == q4) block[kWork * t + l16] = N[t];
+    for (int t = 0; t < 16; t++) block[kWork * t + l16] = N[t];
     wave_sync();
 }
 
-// The 16 x 16 block below, by one wave for each half: with Y = A10 - A10 (beta N00),
+// The 16 x 16 block below in a half, by the same wave: with Y = A10 - A10 (beta N00),
 // N10 = Y - N11 (beta Y).
 __device__ __forceinline__ void solve_32(Pairs& o, const Gates& gates, int half, int lane) {
     phase();
@@ -479,26 +502,27 @@ __device__ __forceinline__ void store_n(Pairs& o, int w, int lane) {
 }
 
 // All of them, by the workgroup's 4 or 8 waves; tokens and gates are in LDS, and the
-// matrices are when it returns. The 16 rows of a half whose operand does not take the
-// block below (the first ones, transposed the second) are done before the others.
-// next(): what wave 0, which has least of A, does meanwhile.
+// matrices are when it returns. One wave solves while the others make P.
+// next(): for one wave meanwhile.
 template <int D, bool TRANSPOSED, bool WITH_P, typename Next>
 __device__ __forceinline__ void make_pairs(Pairs& o, const kr_half8* q, const kr_half8* k, const Gates& gates, int wave,
                                            int lane, Next next) {
-    const bool first = (wave & 1) == (TRANSPOSED ? 1 : 0);
-    if (wave < 4) {
-        make_a<D, TRANSPOSED>(o, k, gates, wave, lane);
-        solve_16(o, gates, wave, lane);
-        if (first) store_n<TRANSPOSED>(o, wave, lane);
-    }
-    // P's tiles go against A's: the wave with most of one has least of the other
-    if (WITH_P && (D == 64 || wave >= 4)) make_p<D, TRANSPOSED>(o, q, k, gates, 3 - (wave & 3), lane);
-    if (wave == (D == 64 ? 3 : 0)) next();
+    if (wave < 4) make_a<D, TRANSPOSED>(o, k, gates, wave, lane);
+    if (D == 128 && WITH_P && wave >= 4) make_p<D, TRANSPOSED>(o, q, k, gates, wave - 4, lane);
     __syncthreads();
-    if (wave < 4 && !first) {
-        solve_32(o, gates, wave / 2, lane);
-        store_n<TRANSPOSED>(o, wave, lane);
+    if (wave == 0) {
+        solve_16(o, gates, lane);
+        solve_32(o, gates, 0, lane);
+        solve_32(o, gates, 1, lane);
     }
+    if (D == 64 && WITH_P && wave > 0) {
+        // 16 rows have one to four tiles: 4, 3, and 2 with 1
+        make_p<D, TRANSPOSED>(o, q, k, gates, TRANSPOSED ? wave - 1 : 4 - wave, lane);
+        if (wave == 3) make_p<D, TRANSPOSED>(o, q, k, gates, TRANSPOSED ? 3 : 0, lane);
+    }
+    if (wave == 2) next();
+    __syncthreads();
+    if (wave < 4) store_n<TRANSPOSED>(o, wave, lane);
     __syncthreads();
 }
 
@@ -595,7 +619,7 @@ __global__ void __launch_bounds__(4 * D, 2) delta_chunk_kernel(DeltaArgs g) {
     kr_half* yp = g.y + (row0 + l16) * g.ldy + h * D + 16 * wave + 4 * q4;
 
     fetch(0);
-    if (wave == (D == 64 ? 3 : 0)) {
+    if (wave == 2) {
         fetch_gates(0);
         make_gates(sh.gates[0], gate, beta, lane);
         fetch_gates(kChunk);
@@ -639,7 +663,7 @@ __global__ void __launch_bounds__(4 * D, 2) delta_chunk_kernel(DeltaArgs g) {
             #pragma unroll
             for (int e = 0; e < 8; e++) {
                 kr_half x, y;
-                two_parts(S[2 * s + e / 4][e % 4] * up, x, y);
+                two_parts(S[2 * s + e / 4][e % 4], up, x, y);
                 sp[s].hi[e] = x;
                 sp[s].lo[e] = y;
             }
@@ -662,7 +686,7 @@ __global__ void __launch_bounds__(4 * D, 2) delta_chunk_kernel(DeltaArgs g) {
                 }
                 const kr_float4 e0 = *reinterpret_cast<const kr_float4*>(gates.e0 + 32 * s + 8 * q4 + 4 * hf);
                 #pragma unroll
-                for (int r = 0; r < 4; r++) X[s][4 * hf + r] = (float)vc[4 * hf + r] - (e0[r] * down) * z[r];
+                for (int r = 0; r < 4; r++) X[s][4 * hf + r] = __builtin_fmaf(-(e0[r] * down), z[r], (float)vc[4 * hf + r]);
             }
         }
         phase();
@@ -694,7 +718,7 @@ __global__ void __launch_bounds__(4 * D, 2) delta_chunk_kernel(DeltaArgs g) {
                 for (int hf = 0; hf < 2; hf++) {
                     const kr_float4 z = mfma3(a_of[hf].hi, a_of[hf].lo, up8[0], kr_float4{0, 0, 0, 0});
                     #pragma unroll
-                    for (int r = 0; r < 4; r++) X[1][4 * hf + r] -= (a_f[hf][r] * u_down[0]) * z[r];
+                    for (int r = 0; r < 4; r++) X[1][4 * hf + r] = __builtin_fmaf(-(a_f[hf][r] * u_down[0]), z[r], X[1][4 * hf + r]);
                 }
             }
             #pragma unroll
@@ -704,7 +728,7 @@ __global__ void __launch_bounds__(4 * D, 2) delta_chunk_kernel(DeltaArgs g) {
             for (int hf = 0; hf < 2; hf++) {
                 const kr_float4 z = mfma3(n_of[s][hf].hi, n_of[s][hf].lo, xp, kr_float4{0, 0, 0, 0});
                 #pragma unroll
-                for (int r = 0; r < 4; r++) X[s][4 * hf + r] -= (n_f[s][hf][r] * x_down) * z[r];
+                for (int r = 0; r < 4; r++) X[s][4 * hf + r] = __builtin_fmaf(-(n_f[s][hf][r] * x_down), z[r], X[s][4 * hf + r]);
             }
             #pragma unroll
             for (int e = 0; e < 8; e++) U[s][e] = bt[s][e] * X[s][e];
@@ -886,7 +910,7 @@ __global__ void __launch_bounds__(4 * D, 2) delta_back_kernel(BackArgs g) {
     };
     if (chunks > 0) {
         fetch((chunks - 1) * kChunk);
-        if (wave == (D == 64 ? 3 : 0)) {
+        if (wave == 2) {
             fetch_gates((chunks - 1) * kChunk);
             make_gates(sh.gates[(chunks - 1) & 1], gate, beta, lane);
             fetch_gates((chunks - 2) * kChunk);
@@ -928,7 +952,7 @@ __global__ void __launch_bounds__(4 * D, 2) delta_back_kernel(BackArgs g) {
             #pragma unroll
             for (int e = 0; e < 8; e++) {
                 kr_half x, y;
-                two_parts(S[2 * s + e / 4][e % 4] * up, x, y);
+                two_parts(S[2 * s + e / 4][e % 4], up, x, y);
                 sp[s].hi[e] = x;
                 sp[s].lo[e] = y;
             }
@@ -988,7 +1012,7 @@ __global__ void __launch_bounds__(4 * D, 2) delta_back_kernel(BackArgs g) {
                 for (int hf = 0; hf < 2; hf++) {
                     const kr_float4 z = mfma3(a_of[hf].hi, a_of[hf].lo, dx1, kr_float4{0, 0, 0, 0});
                     #pragma unroll
-                    for (int r = 0; r < 4; r++) X[0][4 * hf + r] -= (a_f[hf][r] * dx1_down) * z[r];
+                    for (int r = 0; r < 4; r++) X[0][4 * hf + r] = __builtin_fmaf(-(a_f[hf][r] * dx1_down), z[r], X[0][4 * hf + r]);
                 }
             }
             #pragma unroll
@@ -998,7 +1022,7 @@ __global__ void __launch_bounds__(4 * D, 2) delta_back_kernel(BackArgs g) {
             for (int hf = 0; hf < 2; hf++) {
                 const kr_float4 z = mfma3(n_of[s][hf].hi, n_of[s][hf].lo, xp, kr_float4{0, 0, 0, 0});
                 #pragma unroll
-                for (int r = 0; r < 4; r++) X[s][4 * hf + r] -= (n_f[s][hf][r] * x_down) * z[r];
+                for (int r = 0; r < 4; r++) X[s][4 * hf + r] = __builtin_fmaf(-(n_f[s][hf][r] * x_down), z[r], X[s][4 * hf + r]);
             }
             #pragma unroll
             for (int e = 0; e < 8; e++) dX[s][e] = bt[s][e] * X[s][e];
