@@ -40,8 +40,13 @@ struct DeltaArgs {
     long long ldy;
     float* before;                // STATES: [chunks + 1][heads][D][D], the state before each chunk
     float* diff;                  // STATES: [chunks][heads][64][D], r
+    float* sums;                  // SUMS: [segments][heads][D][D] what a segment adds
+    float* maps;                  // SUMS: [segments][heads][D][D] what it makes of a state
+    float* starts;                // [segments][heads][D][D] (time split: the states at the starts)
     int B, T, H;
+    int seg_chunks, segments;     // segments of the time axis (1: none)
 };
+enum { FORWARD, STATES, SUMS };   // what a walk over chunks leaves: y; states and r; sums or maps
 
 __device__ __forceinline__ int stream_tokens(const int32_t* lens, int b, int T) {
     if (!lens) return T;
@@ -554,35 +559,39 @@ struct DeltaShared {
 };
 
 // ---------------------------------------------------------------------------
-// Chunked form, forward: a workgroup has one head of one stream and walks its
-// chunks, a wave for each 16 columns of the state, which stays in the wave's
-// registers as the matrix unit leaves it: as such it is the operand of k S and q S,
-// and what they leave is the operand of the next product. STATES: the states before
-// the chunks and the differences r, for the backward pass, and no y.
+// Chunked form, forward: a workgroup has one head of one stream (or a segment of its
+// time axis) and walks its chunks, a wave for each 16 columns of the state, which
+// stays in the wave's registers as the matrix unit leaves it: as such it is the operand
+// of k S and q S, and what they leave is the operand of the next product. A segment
+// makes map S + sum of the state S at its start: SUMS gives one or the other, as the
+// state that follows from the identity without values, or from zero.
 // ---------------------------------------------------------------------------
-template <int D, bool STATES>
-__global__ void __launch_bounds__(4 * D, 2) delta_chunk_kernel(DeltaArgs g) {
+template <int D, int MODE>
+__device__ __forceinline__ void walk_chunks(const DeltaArgs& g, DeltaShared<D>& sh, int heads, int b, int h, int seg,
+                                            bool map) {
     constexpr int KS = D / 32;            // k-steps over the channels
-    __shared__ DeltaShared<D> sh;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l16 = lane & 15, q4 = lane >> 4;
-    const int heads = gridDim.x, h = blockIdx.x % g.H;
-    const int b = ranked_stream<4 * D>(g.lens, g.B, g.T, blockIdx.x / g.H, reinterpret_cast<int*>(&sh.pairs));
     const int head = b * g.H + h;
-    const int n_tok = stream_tokens(g.lens, b, g.T);
-    const size_t row0 = (size_t)b * g.T;
+    const int c0 = seg * g.seg_chunks, t_begin = c0 * kChunk;
+    const int t_end = g.T - t_begin < g.seg_chunks * kChunk ? g.T : t_begin + g.seg_chunks * kChunk;
+    const int live = stream_tokens(g.lens, b, g.T);
+    const int n_tok = live < t_begin ? 0 : (live < t_end ? live : t_end) - t_begin;
+    const size_t row0 = (size_t)b * g.T + t_begin;
 
     // state: column m = 16 wave + l16; S[2s], S[2s + 1] hold rows 32 s + 8 q4 + r and
     // + 4, so that the pair is the operand of k-step s
     kr_float4 S[2 * KS];
     const int m = 16 * wave + l16;
-    const size_t state_at = (size_t)(8 * q4) * D + m;
-    const float* s_in = g.state + (size_t)head * D * D + state_at;
+    const size_t state_at = (size_t)(8 * q4) * D + m, slot = ((size_t)seg * heads + head) * D * D + state_at;
+    const float* s_in = g.segments > 1 ? g.starts + slot : g.state + (size_t)head * D * D + state_at;
     #pragma unroll
     for (int s = 0; s < KS; s++)
         #pragma unroll
-        for (int e = 0; e < 8; e++) S[2 * s + e / 4][e % 4] = s_in[(size_t)(32 * s + e) * D];
+        for (int e = 0; e < 8; e++)
+            S[2 * s + e / 4][e % 4] = MODE != SUMS ? s_in[(size_t)(32 * s + e) * D]
+                                                   : map && 32 * s + 8 * q4 + e == m ? 1.0f : 0.0f;
 
     // what a thread stages: 8 channels of tokens 2p, 2p + 1
     const int ng = tid % (D / 8), p = tid / (D / 8);
@@ -600,9 +609,9 @@ __global__ void __launch_bounds__(4 * D, 2) delta_chunk_kernel(DeltaArgs g) {
             const kr_half8 zero = {0, 0, 0, 0, 0, 0, 0, 0};
             qq[e] = kk[e] = vv[e] = zero;
             if (t0 + 2 * p + e < n_tok) {
-                if (!STATES) qq[e] = *reinterpret_cast<const kr_half8*>(qp + e * g.ldq);
+                if (MODE == FORWARD) qq[e] = *reinterpret_cast<const kr_half8*>(qp + e * g.ldq);
                 kk[e] = *reinterpret_cast<const kr_half8*>(kp + e * g.ldk);
-                vv[e] = *reinterpret_cast<const kr_half8*>(vp + e * g.ldv);
+                if (!map) vv[e] = *reinterpret_cast<const kr_half8*>(vp + e * g.ldv);
             }
         }
         qp += kChunk * g.ldq;
@@ -628,21 +637,21 @@ __global__ void __launch_bounds__(4 * D, 2) delta_chunk_kernel(DeltaArgs g) {
         const int n = n_tok - t0 < kChunk ? n_tok - t0 : kChunk;
         #pragma unroll
         for (int e = 0; e < 2; e++) {
-            if (!STATES) sh.q[tok_unit<D>(2 * p + e, ng)] = qq[e];
+            if (MODE == FORWARD) sh.q[tok_unit<D>(2 * p + e, ng)] = qq[e];
             sh.k[tok_unit<D>(2 * p + e, ng)] = kk[e];
             sh.v[tok_unit<D>(2 * p + e, ng)] = vv[e];
         }
         const Gates& gates = sh.gates[c & 1];
         if (t0 + kChunk < n_tok) fetch(t0 + kChunk);
-        if constexpr (STATES) {
-            float* out = g.before + ((size_t)c * heads + head) * D * D + state_at;
+        if constexpr (MODE == STATES) {
+            float* out = g.before + ((size_t)(c0 + c) * heads + head) * D * D + state_at;
             #pragma unroll
             for (int s = 0; s < KS; s++)
                 #pragma unroll
                 for (int e = 0; e < 8; e++) out[(size_t)(32 * s + e) * D] = S[2 * s + e / 4][e % 4];
         }
         __syncthreads();
-        make_pairs<D, false, !STATES>(sh.pairs, sh.q, sh.k, gates, wave, lane, [&]() {
+        make_pairs<D, false, MODE == FORWARD>(sh.pairs, sh.q, sh.k, gates, wave, lane, [&]() {
             if (t0 + kChunk >= n_tok) return;
             make_gates(sh.gates[(c + 1) & 1], gate, beta, lane);
             fetch_gates(t0 + 2 * kChunk);
@@ -735,13 +744,14 @@ __global__ void __launch_bounds__(4 * D, 2) delta_chunk_kernel(DeltaArgs g) {
             up8[s] = scaled8(U[s], u_down[s]);
         }
         phase();
-        if constexpr (STATES) {
-            float* out = g.diff + (((size_t)c * heads + head) * kChunk + 8 * q4) * D + m;
+        if constexpr (MODE == STATES) {
+            float* out = g.diff + (((size_t)(c0 + c) * heads + head) * kChunk + 8 * q4) * D + m;
             #pragma unroll
             for (int s = 0; s < 2; s++)
                 #pragma unroll
                 for (int e = 0; e < 8; e++) out[(size_t)(32 * s + e) * D] = X[s][e];
-        } else {
+        }
+        if constexpr (MODE == FORWARD) {
             // y': rows m, columns i
             kr_float4 down_m, u0_m, u1_m;      // of the rows m that this lane has of y'
             #pragma unroll
@@ -811,17 +821,31 @@ __global__ void __launch_bounds__(4 * D, 2) delta_chunk_kernel(DeltaArgs g) {
         __syncthreads();
     }
 
-    float* s_out = STATES ? g.before + ((size_t)((n_tok + kChunk - 1) / kChunk) * heads + head) * D * D
-                          : g.state + (size_t)head * D * D;
-    s_out += state_at;
-    #pragma unroll
-    for (int s = 0; s < KS; s++)
+    float* s_out = nullptr;
+    if (MODE == SUMS) {
+        s_out = (map ? g.maps : g.sums) + slot;
+    } else if (MODE == FORWARD) {
+        if (seg == g.segments - 1) s_out = g.state + (size_t)head * D * D + state_at;
+    } else if ((live > t_begin || seg == 0) && live <= t_end) {       // the stream's end
+        s_out = g.before + ((size_t)((live + kChunk - 1) / kChunk) * heads + head) * D * D + state_at;
+    }
+    if (s_out)
         #pragma unroll
-        for (int e = 0; e < 8; e++) s_out[(size_t)(32 * s + e) * D] = S[2 * s + e / 4][e % 4];
-    if (!STATES)
-        for (int i = n_tok * (D / 8) + tid; i < g.T * (D / 8); i += 4 * D)
+        for (int s = 0; s < KS; s++)
+            #pragma unroll
+            for (int e = 0; e < 8; e++) s_out[(size_t)(32 * s + e) * D] = S[2 * s + e / 4][e % 4];
+    if (MODE == FORWARD)
+        for (long long i = (long long)n_tok * (D / 8) + tid; i < (long long)(t_end - t_begin) * (D / 8); i += 4 * D)
             *reinterpret_cast<kr_half8*>(g.y + (row0 + i / (D / 8)) * g.ldy + h * D + 8 * (i % (D / 8))) =
                 kr_half8{0, 0, 0, 0, 0, 0, 0, 0};
+}
+
+template <int D>
+__global__ void __launch_bounds__(4 * D, 2) delta_chunk_kernel(DeltaArgs g) {
+    __shared__ DeltaShared<D> sh;
+    int b = blockIdx.x / g.H;
+    if (g.segments == 1) b = ranked_stream<4 * D>(g.lens, g.B, g.T, b, reinterpret_cast<int*>(&sh.pairs));
+    walk_chunks<D, FORWARD>(g, sh, gridDim.x, b, blockIdx.x % g.H, blockIdx.y, false);
 }
 
 // ---------------------------------------------------------------------------
@@ -859,32 +883,36 @@ struct BackArgs {
     kr_half* dv;
     float* dgate;                 // [B, T, H]
     float* dbeta;
+    float* sums;                  // [segments][heads][D][D], what a segment adds to D
+    float* ends;                  // [segments][heads][D][D], D behind the segments (time split)
     int B, T, H;
+    int seg_chunks, segments;
 };
 
-template <int D>
-__global__ void __launch_bounds__(4 * D, 2) delta_back_kernel(BackArgs g) {
-    constexpr int KS = D / 32;
-    __shared__ DeltaShared<D> sh;         // dy in v's place
+// SUM: only what a segment adds to D, from zero behind it.
+template <int D, bool SUM>
+__device__ __forceinline__ void walk_back(const BackArgs& g, DeltaShared<D>& sh, int heads, int b, int h, int seg) {
+    constexpr int KS = D / 32;            // dy is in v's place
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l16 = lane & 15, q4 = lane >> 4;
-    const int heads = gridDim.x, h = blockIdx.x % g.H;
-    const int b = ranked_stream<4 * D>(g.lens, g.B, g.T, blockIdx.x / g.H, reinterpret_cast<int*>(&sh.pairs));
     const int head = b * g.H + h;
-    const int n_tok = stream_tokens(g.lens, b, g.T);
+    const int c0 = seg * g.seg_chunks, t_begin = c0 * kChunk;
+    const int t_end = g.T - t_begin < g.seg_chunks * kChunk ? g.T : t_begin + g.seg_chunks * kChunk;
+    const int live = stream_tokens(g.lens, b, g.T);
+    const int n_tok = live < t_begin ? 0 : (live < t_end ? live : t_end) - t_begin;
     const int chunks = (n_tok + kChunk - 1) / kChunk;
-    const size_t row0 = (size_t)b * g.T;
+    const size_t row0 = (size_t)b * g.T + t_begin;
 
     kr_float4 S[2 * KS];                  // D, laid out as the forward pass's state
     const int m = 16 * wave + l16;
-    const size_t state_at = (size_t)(8 * q4) * D + m;
+    const size_t state_at = (size_t)(8 * q4) * D + m, slot = ((size_t)seg * heads + head) * D * D + state_at;
+    const float* d_in = SUM ? nullptr : g.segments > 1 ? g.ends + slot
+                        : g.dstate ? g.dstate + (size_t)head * D * D + state_at : nullptr;
     #pragma unroll
     for (int s = 0; s < KS; s++)
         #pragma unroll
-        for (int e = 0; e < 8; e++)
-            S[2 * s + e / 4][e % 4] =
-                g.dstate ? g.dstate[(size_t)head * D * D + state_at + (size_t)(32 * s + e) * D] : 0.0f;
+        for (int e = 0; e < 8; e++) S[2 * s + e / 4][e % 4] = d_in ? d_in[(size_t)(32 * s + e) * D] : 0.0f;
 
     const int ng = tid % (D / 8), p = tid / (D / 8);
     kr_half8 qq[2], kk[2], vv[2];
@@ -925,8 +953,8 @@ __global__ void __launch_bounds__(4 * D, 2) delta_back_kernel(BackArgs g) {
         }
         const Gates& gates = sh.gates[c & 1];
         if (c > 0) fetch((c - 1) * kChunk);
-        {
-            float* out = g.behind + ((size_t)c * heads + head) * D * D + state_at;
+        if constexpr (!SUM) {
+            float* out = g.behind + ((size_t)(c0 + c) * heads + head) * D * D + state_at;
             #pragma unroll
             for (int s = 0; s < KS; s++)
                 #pragma unroll
@@ -1028,8 +1056,8 @@ __global__ void __launch_bounds__(4 * D, 2) delta_back_kernel(BackArgs g) {
             for (int e = 0; e < 8; e++) dX[s][e] = bt[s][e] * X[s][e];
             if (s == 1) dx1 = scaled8(dX[1], dx1_down);
         }
-        {
-            float* out = g.w + (((size_t)c * heads + head) * kChunk + 8 * q4) * D + m;
+        if constexpr (!SUM) {
+            float* out = g.w + (((size_t)(c0 + c) * heads + head) * kChunk + 8 * q4) * D + m;
             #pragma unroll
             for (int s = 0; s < 2; s++)
                 #pragma unroll
@@ -1070,11 +1098,130 @@ __global__ void __launch_bounds__(4 * D, 2) delta_back_kernel(BackArgs g) {
         }
         __syncthreads();
     }
-    float* out = g.dstate0 + (size_t)head * D * D + state_at;
-    #pragma unroll
-    for (int s = 0; s < KS; s++)
+    float* out = SUM ? g.sums + slot : seg == 0 ? g.dstate0 + (size_t)head * D * D + state_at : nullptr;
+    if (out)
         #pragma unroll
-        for (int e = 0; e < 8; e++) out[(size_t)(32 * s + e) * D] = S[2 * s + e / 4][e % 4];
+        for (int s = 0; s < KS; s++)
+            #pragma unroll
+            for (int e = 0; e < 8; e++) out[(size_t)(32 * s + e) * D] = S[2 * s + e / 4][e % 4];
+}
+
+// The states of a forward pass and D, one beside the other.
+template <int D>
+__global__ void __launch_bounds__(4 * D, 2) delta_both_kernel(DeltaArgs f, BackArgs g) {
+    __shared__ DeltaShared<D> sh;
+    int b = blockIdx.x / g.H;
+    if (g.segments == 1) b = ranked_stream<4 * D>(g.lens, g.B, g.T, b, reinterpret_cast<int*>(&sh.pairs));
+    if (blockIdx.z == 0) walk_chunks<D, STATES>(f, sh, gridDim.x, b, blockIdx.x % g.H, blockIdx.y, false);
+    else walk_back<D, false>(g, sh, gridDim.x, b, blockIdx.x % g.H, blockIdx.y);
+}
+
+// ---------------------------------------------------------------------------
+// Time split, for few heads: what each segment makes of a state, S -> map S + sum, is
+// computed for all segments at once, the states at their starts follow one from
+// the other, and then all segments run. Backward, D -> map' D + sum.
+// z of the sums' launch: 0 sums, 1 maps, 2 D's sums; of the states': 0 forward, 1 back.
+// ---------------------------------------------------------------------------
+template <int D>
+__global__ void __launch_bounds__(4 * D, 2) delta_sums_kernel(DeltaArgs f, BackArgs g) {
+    __shared__ DeltaShared<D> sh;
+    const int seg = blockIdx.y, b = blockIdx.x / f.H, h = blockIdx.x % f.H;
+    if (blockIdx.z < 2) {
+        if (blockIdx.z == 0 && seg == f.segments - 1) return;         // not needed
+        walk_chunks<D, SUMS>(f, sh, gridDim.x, b, h, seg, blockIdx.z == 1);
+    } else if (seg > 0) {
+        walk_back<D, true>(g, sh, gridDim.x, b, h, seg);
+    }
+}
+
+// 16 columns of a head: a wave has 16 rows of every segment's map, read two segments
+// ahead (or every step waits for memory); the column passes through LDS, [m][n] in two
+// buffers.
+template <int D>
+struct JoinPiece {
+    float map[D / 32][8], sum[4];
+};
+template <int D, bool BACK>
+__device__ __forceinline__ void join_segments(const DeltaArgs& f, const float* sums, const float* first, float* out,
+                                              float (&S)[2][16 * (D + 4)], int heads, int head, int m0) {
+    constexpr int KS = D / 32, LD = D + 4;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l16 = lane & 15, q4 = lane >> 4, m = m0 + l16;
+    const int n = f.segments, rows = 16 * wave, live = stream_tokens(f.lens, head / f.H, f.T);
+    const size_t step = (size_t)heads * D * D, at = (size_t)head * D * D;
+    const int sum_at = (rows + 4 * q4) * D + m;           // of 4 rows in a column
+    const int map_at = BACK ? 8 * q4 * D + rows + l16 : (rows + l16) * D + 8 * q4;
+    // step i takes segment seg(i)'s map and sum, and gives the next one's start (or end)
+    auto seg = [&](int i) { return BACK ? n - 1 - i : i; };
+    auto fetch = [&](int i, JoinPiece<D>& o) {            // without a branch, so that waits are counted
+        i = i < n - 2 ? i : n - 2;
+        const float* p = f.maps + at + seg(i) * step + map_at;
+        #pragma unroll
+        for (int s = 0; s < KS; s++)
+            #pragma unroll
+            for (int e = 0; e < 8; e++)
+                o.map[s][e] = BACK ? p[(32 * s + e) * D] : reinterpret_cast<const kr_float4*>(p + 32 * s)[e / 4][e % 4];
+        #pragma unroll
+        for (int r = 0; r < 4; r++) o.sum[r] = sums[at + seg(i) * step + sum_at + r * D];
+    };
+    kr_float4 x;
+    #pragma unroll
+    for (int r = 0; r < 4; r++) x[r] = first ? first[at + sum_at + r * D] : 0.0f;
+    auto take = [&](int i, JoinPiece<D>& o) {
+        float* to = out + at + seg(i) * step + sum_at;
+        #pragma unroll
+        for (int r = 0; r < 4; r++) to[r * D] = x[r];
+        float* col = S[i & 1];
+        *reinterpret_cast<kr_float4*>(col + l16 * LD + rows + 4 * q4) = x;
+        // the map's parts, with a scale for each row
+        Parts8 mp[KS];
+        float big = 0.0f, up, m_down, x_down;
+        #pragma unroll
+        for (int s = 0; s < KS; s++) big = largest8(o.map[s], big);
+        power_scale(max_of_quarters(big), up, m_down);
+        #pragma unroll
+        for (int s = 0; s < KS; s++) mp[s] = parts8(o.map[s], up);
+        const kr_float4 add = {o.sum[0], o.sum[1], o.sum[2], o.sum[3]};
+        fetch(i + 2, o);
+        if (seg(i) * f.seg_chunks * kChunk >= live) return;           // no token: as it is
+        __syncthreads();
+        float c[KS][8];
+        big = 0.0f;
+        #pragma unroll
+        for (int s = 0; s < KS; s++) {
+            const kr_float4* p = reinterpret_cast<const kr_float4*>(col + l16 * LD + 32 * s + 8 * q4);
+            #pragma unroll
+            for (int e = 0; e < 8; e++) c[s][e] = p[e / 4][e % 4];
+            big = largest8(c[s], big);
+        }
+        power_scale(max_of_quarters(big), up, x_down);
+        kr_float4 z = {0, 0, 0, 0};
+        #pragma unroll
+        for (int s = 0; s < KS; s++) z = mfma3(mp[s].hi, mp[s].lo, parts8(c[s], up), z);
+        #pragma unroll
+        for (int r = 0; r < 4; r++) x[r] = __builtin_fmaf(z[r], x_down * __shfl(m_down, 4 * q4 + r), add[r]);
+    };
+    JoinPiece<D> a, b;
+    fetch(0, a);
+    fetch(1, b);
+    int i = 0;
+    for (; i + 2 < n; i += 2) {
+        take(i, a);
+        take(i + 1, b);
+    }
+    if (i < n - 1) take(i, a);
+    float* to = out + at + seg(n - 1) * step + sum_at;
+    #pragma unroll
+    for (int r = 0; r < 4; r++) to[r * D] = x[r];
+}
+
+template <int D>
+__global__ void __launch_bounds__(4 * D) delta_join_kernel(DeltaArgs f, BackArgs g) {
+    __shared__ __attribute__((aligned(16))) float S[2][16 * (D + 4)];
+    const int heads = gridDim.x, head = blockIdx.x, m0 = 16 * blockIdx.y;
+    if (blockIdx.z == 0) join_segments<D, false>(f, f.sums, f.state, f.starts, S, heads, head, m0);
+    else join_segments<D, true>(f, g.sums, g.dstate, g.ends, S, heads, head, m0);
 }
 
 // A workgroup of 4 waves for each head and chunk, a wave for 16 tokens, as those that
@@ -1403,42 +1550,118 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1) delta_grad_kernel(BackAr
 // Tokens up to which the chunked form is the recurrent one, too.
 constexpr int kStepTokens = 8;
 
-bool shape_ok(int B, int T, int H, int D) {
-    return B >= 0 && T >= 0 && H >= 1 && (D == 64 || D == 128) && (long long)B * H <= 1 << 24 && T <= 1 << 30;
-}
-
-template <int D>
-int launch(const DeltaArgs& g, bool chunked, hipStream_t s) {
-    const int heads = g.B * g.H;
-    if (!chunked || g.T <= kStepTokens) delta_step_kernel<D><<<heads, 4 * D, 0, s>>>(g);
-    else delta_chunk_kernel<D, false><<<heads, 4 * D, 0, s>>>(g);
-    KR_LAUNCHED();
-    return KR_OK;
+// Segments of the time axis, by what a call would take: rounds of workgroups (one a CU
+// for D = 128, two for 64) times a segment's chunks, for the sums and for the walk, and
+// the join's steps, a twelfth of a chunk each. A segment has two chunks at least.
+void split_time(long long heads, int T, int D, bool back, int& seg_chunks, int& segments) {
+    const int chunks = (T + kChunk - 1) / kChunk;
+    const long long slots = D == 64 ? 512 : 256;
+    auto rounds = [&](long long n) { return (n + slots - 1) / slots; };
+    const int walks = back ? 2 : 1;
+    seg_chunks = chunks;
+    segments = 1;
+    long long best = 12 * chunks * rounds(walks * heads);
+    for (int n = 2; n <= chunks / 2 && n <= 128 && n * heads <= 2 * slots; n++) {
+        const int c = (chunks + n - 1) / n, used = (chunks + c - 1) / c;
+        const long long cost = 12ll * c * (rounds((back ? 3 : 2) * heads * used) + rounds(walks * heads * used)) + used + 24;
+        if (cost < best) {
+            best = cost;
+            seg_chunks = c;
+            segments = used;
+        }
+    }
 }
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
-// The backward pass's workspace: states, r, D and w of all chunks.
-struct BackPlan {
-    size_t before, diff, behind, w, total;
+// A call's workspace: for the segments of a time split sums, maps and starts (backward
+// sums and ends, too), and for the backward pass states, r, D and w of all chunks.
+struct DeltaPlan {
+    int seg_chunks, segments;
+    size_t sums, maps, starts, back_sums, ends, before, diff, behind, w, total;
 };
-BackPlan back_plan(int B, int T, int H, int D) {
+DeltaPlan delta_plan(int B, int T, int H, int D, bool back) {
     const size_t heads = (size_t)B * H, chunks = (size_t)(T + kChunk - 1) / kChunk;
     const size_t state = heads * D * D * sizeof(float), rows = heads * kChunk * D * sizeof(float);
-    BackPlan p{};
-    p.diff = p.before + up256((chunks + 1) * state);
-    p.behind = p.diff + up256(chunks * rows);
-    p.w = p.behind + up256(chunks * state);
-    p.total = p.w + up256(chunks * rows);
+    DeltaPlan p{};
+    split_time((long long)heads, T, D, back, p.seg_chunks, p.segments);
+    size_t at = 0;
+    auto take = [&](size_t& to, size_t bytes) {
+        to = at;
+        at += up256(bytes);
+    };
+    if (p.segments > 1) {
+        take(p.sums, p.segments * state);
+        take(p.maps, p.segments * state);
+        take(p.starts, p.segments * state);
+        if (back) take(p.back_sums, p.segments * state);
+        if (back) take(p.ends, p.segments * state);
+    }
+    if (back) {
+        take(p.before, (chunks + 1) * state);
+        take(p.diff, chunks * rows);
+        take(p.behind, chunks * state);
+        take(p.w, chunks * rows);
+    }
+    p.total = at;
     return p;
+}
+
+bool shape_ok(int B, int T, int H, int D) {
+    return B >= 0 && T >= 0 && H >= 1 && (D == 64 || D == 128) && (long long)B * H <= 1 << 24 && T <= 1 << 30;
+}
+
+void place(DeltaArgs& f, BackArgs& g, const DeltaPlan& p, char* ws) {
+    auto at = [&](size_t o) { return reinterpret_cast<float*>(ws + o); };
+    f.seg_chunks = g.seg_chunks = p.seg_chunks;
+    f.segments = g.segments = p.segments;
+    f.sums = at(p.sums);
+    f.maps = at(p.maps);
+    f.starts = at(p.starts);
+    g.sums = at(p.back_sums);
+    g.ends = at(p.ends);
+    f.before = at(p.before);
+    f.diff = at(p.diff);
+    g.before = f.before;
+    g.diff = f.diff;
+    g.behind = at(p.behind);
+    g.w = at(p.w);
+}
+
+template <int D>
+int launch_join(const DeltaArgs& f, const BackArgs& g, bool back, hipStream_t s) {
+    const int heads = f.B * f.H;
+    delta_sums_kernel<D><<<dim3(heads, back ? f.segments : f.segments - 1, back ? 3 : 2), 4 * D, 0, s>>>(f, g);
+    KR_LAUNCHED();
+    delta_join_kernel<D><<<dim3(heads, D / 16, back ? 2 : 1), 4 * D, 0, s>>>(f, g);
+    KR_LAUNCHED();
+    return KR_OK;
+}
+
+template <int D>
+int launch(const DeltaArgs& f, const BackArgs& g, bool chunked, hipStream_t s) {
+    const int heads = f.B * f.H;
+    if (!chunked) {
+        delta_step_kernel<D><<<heads, 4 * D, 0, s>>>(f);
+    } else {
+        if (f.segments > 1) {
+            const int rc = launch_join<D>(f, g, false, s);
+            if (rc != KR_OK) return rc;
+        }
+        delta_chunk_kernel<D><<<dim3(heads, f.segments), 4 * D, 0, s>>>(f);
+    }
+    KR_LAUNCHED();
+    return KR_OK;
 }
 
 template <int D>
 int launch_back(const DeltaArgs& f, const BackArgs& g, hipStream_t s) {
     const int heads = g.B * g.H, chunks = (g.T + kChunk - 1) / kChunk;
-    delta_chunk_kernel<D, true><<<heads, 4 * D, 0, s>>>(f);
-    KR_LAUNCHED();
-    delta_back_kernel<D><<<heads, 4 * D, 0, s>>>(g);
+    if (f.segments > 1) {
+        const int rc = launch_join<D>(f, g, true, s);
+        if (rc != KR_OK) return rc;
+    }
+    delta_both_kernel<D><<<dim3(heads, f.segments, 2), 4 * D, 0, s>>>(f, g);
     KR_LAUNCHED();
     delta_grad_kernel<D><<<dim3(heads, chunks), 256, 0, s>>>(g);
     KR_LAUNCHED();
@@ -1450,8 +1673,8 @@ int launch_back(const DeltaArgs& f, const BackArgs& g, hipStream_t s) {
 extern "C" {
 
 size_t kr_gated_delta_workspace_bytes(int B, int T, int H, int D) {
-    (void)B, (void)T, (void)H, (void)D;
-    return 0;
+    if (!shape_ok(B, T, H, D) || B == 0 || T <= kStepTokens) return 0;
+    return delta_plan(B, T, H, D, false).total;
 }
 
 int kr_gated_delta(int B, int T, int H, int D, const uint16_t* q, long long ldq, const uint16_t* k, long long ldk,
@@ -1467,9 +1690,10 @@ int kr_gated_delta(int B, int T, int H, int D, const uint16_t* q, long long ldq,
     KR_REQUIRE(q && k && v && log_decay && beta && state && y, "kr_gated_delta: null pointer");
     KR_REQUIRE((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)state | (uintptr_t)y) & 15) == 0,
                "kr_gated_delta: q, k, v, state and y must be 16-byte aligned");
-    const size_t need = kr_gated_delta_workspace_bytes(B, T, H, D);
-    KR_REQUIRE(need == 0 || (ws && ws_bytes >= need && ((uintptr_t)ws & 15) == 0),
-               "kr_gated_delta: workspace of %zu bytes, %zu needed (16-byte aligned)", ws_bytes, need);
+    const bool chunks = chunked && T > kStepTokens;
+    const DeltaPlan p = chunks ? delta_plan(B, T, H, D, false) : DeltaPlan{};
+    KR_REQUIRE(p.total == 0 || (ws && ws_bytes >= p.total && ((uintptr_t)ws & 15) == 0),
+               "kr_gated_delta: workspace of %zu bytes, %zu needed (16-byte aligned)", ws_bytes, p.total);
     DeltaArgs g{};
     g.q = reinterpret_cast<const kr_half*>(q);
     g.k = reinterpret_cast<const kr_half*>(k);
@@ -1488,12 +1712,14 @@ int kr_gated_delta(int B, int T, int H, int D, const uint16_t* q, long long ldq,
     g.B = B;
     g.T = T;
     g.H = H;
-    return D == 64 ? launch<64>(g, chunked != 0, kr_stream(stream)) : launch<128>(g, chunked != 0, kr_stream(stream));
+    BackArgs none{};
+    place(g, none, p, static_cast<char*>(ws));
+    return D == 64 ? launch<64>(g, none, chunks, kr_stream(stream)) : launch<128>(g, none, chunks, kr_stream(stream));
 }
 
 size_t kr_gated_delta_backward_workspace_bytes(int B, int T, int H, int D) {
     if (!shape_ok(B, T, H, D) || B == 0 || T == 0) return 0;
-    return back_plan(B, T, H, D).total;
+    return delta_plan(B, T, H, D, true).total;
 }
 
 int kr_gated_delta_backward(int B, int T, int H, int D, const uint16_t* q, long long ldq, const uint16_t* k,
@@ -1513,10 +1739,9 @@ int kr_gated_delta_backward(int B, int T, int H, int D, const uint16_t* q, long 
     KR_REQUIRE((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)state | (uintptr_t)dy | (uintptr_t)dstate |
                  (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv | (uintptr_t)dstate0) & 15) == 0,
                "kr_gated_delta_backward: all but log_decay, beta, lens and their gradients must be 16-byte aligned");
-    const BackPlan p = back_plan(B, T, H, D);
+    const DeltaPlan p = delta_plan(B, T, H, D, true);
     KR_REQUIRE(ws && ws_bytes >= p.total && ((uintptr_t)ws & 255) == 0,
                "kr_gated_delta_backward: workspace of %zu bytes, %zu needed (256-byte aligned)", ws_bytes, p.total);
-    char* base = static_cast<char*>(ws);
     DeltaArgs f{};
     f.q = reinterpret_cast<const kr_half*>(q);
     f.k = reinterpret_cast<const kr_half*>(k);
@@ -1530,8 +1755,6 @@ int kr_gated_delta_backward(int B, int T, int H, int D, const uint16_t* q, long 
     f.ldb = ldb;
     f.lens = lens;
     f.state = const_cast<float*>(state);          // only read where states are kept
-    f.before = reinterpret_cast<float*>(base + p.before);
-    f.diff = reinterpret_cast<float*>(base + p.diff);
     f.B = B;
     f.T = T;
     f.H = H;
@@ -1549,10 +1772,7 @@ int kr_gated_delta_backward(int B, int T, int H, int D, const uint16_t* q, long 
     g.lens = lens;
     g.dstate = dstate;
     g.dstate0 = dstate0;
-    g.before = f.before;
-    g.diff = f.diff;
-    g.behind = reinterpret_cast<float*>(base + p.behind);
-    g.w = reinterpret_cast<float*>(base + p.w);
+    place(f, g, p, static_cast<char*>(ws));
     g.dq = reinterpret_cast<kr_half*>(dq);
     g.dk = reinterpret_cast<kr_half*>(dk);
     g.dv = reinterpret_cast<kr_half*>(dv);
