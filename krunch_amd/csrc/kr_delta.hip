@@ -365,65 +365,65 @@ __device__ __forceinline__ void make_p(Pairs& o, const kr_half8* q, const kr_hal
     }
 }
 
-// A of 16 rows by one wave: the half's own part as fp32, the part below as operand.
-template <int D, bool TRANSPOSED>
-__device__ __forceinline__ void make_a(Pairs& o, const kr_half8* k, const Gates& gates, int w, int lane) {
-    constexpr int KS = D / 32;
+// 16 rows of k against 16 others: a tile of k k' with rows `col`.. and columns row..
+template <int D>
+__device__ __forceinline__ kr_float4 key_products(const kr_half8* k, int row0, int col0, int l16, int q4) {
+    kr_float4 A = {0, 0, 0, 0};
+    #pragma unroll
+    for (int s = 0; s < D / 32; s++)
+        A = mfma(k[tok_unit<D>(col0 + l16, 4 * s + q4)], k[tok_unit<D>(row0 + l16, 4 * s + q4)], A);
+    return A;
+}
+
+// The diagonal tile w of A, fp32.
+template <int D>
+__device__ __forceinline__ void make_diagonal(Pairs& o, const kr_half8* k, const Gates& gates, int w, int lane) {
     phase();
     lane = fresh(lane);
-    const int l16 = lane & 15, q4 = lane >> 4, row = 16 * w + l16;
-    kr_half8 mine[KS];
-    #pragma unroll
-    for (int s = 0; s < KS; s++) mine[s] = k[tok_unit<D>(row, 4 * s + q4)];
+    const int l16 = lane & 15, q4 = lane >> 4, row = 16 * w + l16, col = 16 * w + 4 * q4;
+    kr_float4 A = key_products<D>(k, 16 * w, 16 * w, l16, q4);
     const double a = gates.a[row];
-    // the half's own: rows i, columns j (the tile above the diagonal gives zeros)
-    const int half = w / 2;
-    float* work = o.work[half] + (row & 31) * kWork;
+    #pragma unroll
+    for (int r = 0; r < 4; r++) {
+        const float e = __builtin_amdgcn_exp2f((float)(a - gates.a[col + r]));
+        A[r] = col + r < row ? A[r] * e : 0.0f;
+    }
+    *reinterpret_cast<kr_float4*>(o.work[w / 2] + (row & 31) * kWork + (col & 31)) = A;
+}
+
+// The tile below it in a half, fp32.
+template <int D>
+__device__ __forceinline__ void make_half(Pairs& o, const kr_half8* k, const Gates& gates, int half, int lane) {
+    phase();
+    lane = fresh(lane);
+    const int l16 = lane & 15, q4 = lane >> 4, w = 2 * half + 1, row = 16 * w + l16, col = 32 * half + 4 * q4;
+    kr_float4 A = key_products<D>(k, 16 * w, 32 * half, l16, q4);
+    A *= decays_to(gates, w, gates.from[row], col);
+    *reinterpret_cast<kr_float4*>(o.work[half] + (16 + l16) * kWork + 4 * q4) = A;
+}
+
+// 16 rows of the block below the halves (w = 2, 3; transposed its columns, w = 0, 1), as operand.
+template <int D, bool TRANSPOSED>
+__device__ __forceinline__ void make_below(Pairs& o, const kr_half8* k, const Gates& gates, int w, int lane) {
+    phase();
+    lane = fresh(lane);
+    const int l16 = lane & 15, q4 = lane >> 4, row = 16 * w + l16, c0 = TRANSPOSED ? 32 : 0;
     kr_float4 A[2];
+    float big = 0.0f;
+    #pragma unroll
+    for (int ct = 0; ct < 2; ct++) A[ct] = key_products<D>(k, 16 * w, c0 + 16 * ct, l16, q4);
     #pragma unroll
     for (int ct = 0; ct < 2; ct++) {
-        A[ct] = kr_float4{0, 0, 0, 0};
+        const int col = c0 + 16 * ct + 4 * q4;
+        A[ct] *= TRANSPOSED ? decays_from(gates, 2 + ct, row, col) : decays_to(gates, w, gates.from[row], col);
         #pragma unroll
-        for (int s = 0; s < KS; s++) A[ct] = mfma(k[tok_unit<D>(32 * half + 16 * ct + l16, 4 * s + q4)], mine[s], A[ct]);
+        for (int r = 0; r < 4; r++) big = fmaxf(big, fabsf(A[ct][r]));
     }
-    const float from = gates.from[row];
+    float up, down;
+    power_scale(max_of_quarters(big), up, down);
+    if (q4 == 0) o.a_down[row] = down;
     #pragma unroll
-    for (int ct = 0; ct < 2; ct++) {
-        const int col = 32 * half + 16 * ct + 4 * q4;
-        if (ct == (w & 1)) {
-            #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const float e = __builtin_amdgcn_exp2f((float)(a - gates.a[col + r]));
-                A[ct][r] = col + r < row ? A[ct][r] * e : 0.0f;
-            }
-        } else if (ct == 0) {
-            A[ct] *= decays_to(gates, w, from, col);
-        }
-        if (ct <= (w & 1)) *reinterpret_cast<kr_float4*>(work + 16 * ct + 4 * q4) = A[ct];
-    }
-    // below: rows 32.. against columns 0..31, or transposed
-    if (TRANSPOSED ? w < 2 : w >= 2) {
-        const int c0 = TRANSPOSED ? 32 : 0;
-        float big = 0.0f;
-        #pragma unroll
-        for (int ct = 0; ct < 2; ct++) {
-            A[ct] = kr_float4{0, 0, 0, 0};
-            #pragma unroll
-            for (int s = 0; s < KS; s++) A[ct] = mfma(k[tok_unit<D>(c0 + 16 * ct + l16, 4 * s + q4)], mine[s], A[ct]);
-        }
-        #pragma unroll
-        for (int ct = 0; ct < 2; ct++) {
-            const int col = c0 + 16 * ct + 4 * q4;
-            A[ct] *= TRANSPOSED ? decays_from(gates, 2 + ct, row, col) : decays_to(gates, w, from, col);
-            #pragma unroll
-            for (int r = 0; r < 4; r++) big = fmaxf(big, fabsf(A[ct][r]));
-        }
-        float up, down;
-        power_scale(max_of_quarters(big), up, down);
-        if (q4 == 0) o.a_down[row] = down;
-        #pragma unroll
-        for (int ct = 0; ct < 2; ct++) store_parts4(o.mh, o.ml, row, c0 + 16 * ct + 4 * q4, A[ct], up);
-    }
+    for (int ct = 0; ct < 2; ct++) store_parts4(o.mh, o.ml, row, c0 + 16 * ct + 4 * q4, A[ct], up);
 }
 
 __device__ __forceinline__ void wave_sync() {
@@ -458,7 +458,7 @@ __device__ __forceinline__ void solve_16(Pairs& o, const Gates& gates, int lane)
     wave_sync();
 }
 
-// The 16 x 16 block below in a half, by the same wave: with Y = A10 - A10 (beta N00),
+// The 16 x 16 block below in a half, by one wave: with Y = A10 - A10 (beta N00),
 // N10 = Y - N11 (beta Y).
 __device__ __forceinline__ void solve_32(Pairs& o, const Gates& gates, int half, int lane) {
     phase();
@@ -507,27 +507,43 @@ __device__ __forceinline__ void store_n(Pairs& o, int w, int lane) {
 }
 
 // All of them, by the workgroup's 4 or 8 waves; tokens and gates are in LDS, and the
-// matrices are when it returns. One wave solves while the others make P.
-// next(): for one wave meanwhile.
+// matrices are when it returns. One wave solves the diagonal tiles while the others make
+// the rest. next(): for one wave meanwhile.
 template <int D, bool TRANSPOSED, bool WITH_P, typename Next>
 __device__ __forceinline__ void make_pairs(Pairs& o, const kr_half8* q, const kr_half8* k, const Gates& gates, int wave,
                                            int lane, Next next) {
-    if (wave < 4) make_a<D, TRANSPOSED>(o, k, gates, wave, lane);
-    if (D == 128 && WITH_P && wave >= 4) make_p<D, TRANSPOSED>(o, q, k, gates, wave - 4, lane);
+    // rows of P by how many tiles they have, 1 to 4
+    auto p_rows = [](int tiles) { return TRANSPOSED ? 4 - tiles : tiles - 1; };
+    auto make_rows = [&](int w) { make_p<D, TRANSPOSED>(o, q, k, gates, w, lane); };
+    if (wave < 4) make_diagonal<D>(o, k, gates, wave, lane);
+    else if (WITH_P && wave >= 6) make_rows(p_rows(wave - 3));        // 4, 3
     __syncthreads();
     if (wave == 0) {
         solve_16(o, gates, lane);
-        solve_32(o, gates, 0, lane);
-        solve_32(o, gates, 1, lane);
+    } else if (wave == 1) {
+        make_half<D>(o, k, gates, 0, lane);
+        if (D == 64 && WITH_P) make_rows(p_rows(4));
+        else make_half<D>(o, k, gates, 1, lane);
+    } else if (wave == 2) {
+        make_below<D, TRANSPOSED>(o, k, gates, TRANSPOSED ? 0 : 2, lane);
+        if (D == 64 && WITH_P) make_rows(p_rows(3));
+        next();
+    } else if (wave == 3) {
+        make_below<D, TRANSPOSED>(o, k, gates, TRANSPOSED ? 1 : 3, lane);
+        if (D == 64 && WITH_P) {
+            make_half<D>(o, k, gates, 1, lane);
+            make_rows(p_rows(2));
+            make_rows(p_rows(1));
+        }
+    } else if (WITH_P && wave < 6) {
+        make_rows(p_rows(wave - 3));                                  // 1, 2
     }
-    if (D == 64 && WITH_P && wave > 0) {
-        // 16 rows have one to four tiles: 4, 3, and 2 with 1
-        make_p<D, TRANSPOSED>(o, q, k, gates, TRANSPOSED ? wave - 1 : 4 - wave, lane);
-        if (wave == 3) make_p<D, TRANSPOSED>(o, q, k, gates, TRANSPOSED ? 3 : 0, lane);
-    }
-    if (wave == 2) next();
     __syncthreads();
-    if (wave < 4) store_n<TRANSPOSED>(o, wave, lane);
+    if (wave < 4) {
+        // the rows that take the tile below wait for it
+        if ((wave & 1) == (TRANSPOSED ? 0 : 1)) solve_32(o, gates, wave / 2, lane);
+        store_n<TRANSPOSED>(o, wave, lane);
+    }
     __syncthreads();
 }
 
@@ -678,8 +694,20 @@ __device__ __forceinline__ void walk_chunks(const DeltaArgs& g, DeltaShared<D>& 
             }
 
         phase();
-        // X = v - e^a k S, rows t = 32 s + 8 q4 + e, column m
+        // X = v - e^a k S, rows t = 32 s + 8 q4 + e, column m; q S, rows m, columns i
         float X[2][8];
+        kr_float4 from_s[4];
+        if constexpr (MODE == FORWARD)
+            #pragma unroll
+            for (int it = 0; it < 4; it++) {
+                from_s[it] = kr_float4{0, 0, 0, 0};
+                #pragma unroll
+                for (int s = 0; s < KS; s++) {
+                    const kr_half8 x = sh.q[tok_unit<D>(16 * it + l16, 4 * s + q4)];
+                    from_s[it] = mfma(sp[s].hi, x, from_s[it]);
+                    from_s[it] = mfma(sp[s].lo, x, from_s[it]);
+                }
+            }
         #pragma unroll
         for (int s = 0; s < 2; s++) {
             const kr_half8 vc = channels16<D>(sh.v, s, wave, ln);
@@ -764,13 +792,7 @@ __device__ __forceinline__ void walk_chunks(const DeltaArgs& g, DeltaShared<D>& 
             for (int it = 0; it < 4; it++) {
                 if (it == 2) phase();
                 const int i = 16 * it + l16;
-                kr_float4 from_s = {0, 0, 0, 0}, in0 = {0, 0, 0, 0}, in1 = {0, 0, 0, 0};
-                #pragma unroll
-                for (int s = 0; s < KS; s++) {
-                    const kr_half8 x = sh.q[tok_unit<D>(i, 4 * s + q4)];
-                    from_s = mfma(sp[s].hi, x, from_s);
-                    from_s = mfma(sp[s].lo, x, from_s);
-                }
+                kr_float4 in0 = {0, 0, 0, 0}, in1 = {0, 0, 0, 0};
                 const int at = pair_unit(i, q4);
                 in0 = mfma(up8[0].lo, sh.pairs.ph[at], in0);
                 in0 = mfma(up8[0].hi, sh.pairs.pl[at], in0);
@@ -785,7 +807,7 @@ __device__ __forceinline__ void walk_chunks(const DeltaArgs& g, DeltaShared<D>& 
                 kr_half4 y;
                 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    float x = from_s[r] * (down_m[r] * e0);
+                    float x = from_s[it][r] * (down_m[r] * e0);
                     x = __builtin_fmaf(in0[r], pd * u0_m[r], x);
                     if (it >= 2) x = __builtin_fmaf(in1[r], pd * u1_m[r], x);
                     y[r] = kr_f16(x);
