@@ -36,6 +36,7 @@ struct LossArgs {
     float* hit;                       // LOSS: [N] the target's z
     kr_half* G;                       // GRAD: [rows][ldg] dz of the piece
     long long ldg;
+    float* left;                      // GRAD: [N] what fp16 leaves of the target's dz
     int N, C, V;                      // V: the piece's columns
     int v0, v_all;                    // the piece's first column, the vocabulary
     int rows;                         // GRAD: N rounded up to 64, the rows of G
@@ -228,7 +229,10 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN >= 8 ? 1 : 2) logits_ker
                     if (hit && (unsigned)(d - 32 * p) < 8u)
                         #pragma unroll
                         for (int e = 0; e < 8; e++)
-                            if (d == 32 * p + e) x[e] -= f;
+                            if (d == 32 * p + e) {
+                                x[e] -= f;
+                                g.left[m] = f == 0.0f ? 0.0f : x[e] - (float)(kr_half)x[e];
+                            }
                     kr_half8 v;
                     #pragma unroll
                     for (int e = 0; e < 8; e++) v[e] = (kr_half)x[e];
@@ -412,10 +416,18 @@ __global__ void __launch_bounds__(1024) grad_prepare_kernel(const kr_half* x, lo
         return;
     }
     float big = 0.0f;
-    #pragma unroll 8
-    for (int i = threadIdx.x; i < N; i += 1024) {
-        const float a = fabsf(dloss[i]);
-        if (targets[i] != -1 && a < INFINITY) big = fmaxf(big, a);
+    for (int i0 = threadIdx.x; i0 < N; i0 += 8 * 1024) {
+        float a[8];
+        int t[8];
+        #pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const int i = min(i0 + 1024 * j, N - 1);
+            a[j] = fabsf(dloss[i]);
+            t[j] = targets[i];
+        }
+        #pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (t[j] != -1 && a[j] < INFINITY) big = fmaxf(big, a[j]);
     }
     big = kr_wave_reduce(big, [](float a, float b) { return fmaxf(a, b); });
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = big;
@@ -442,6 +454,10 @@ struct ProdArgs {
     const kr_half* W;                 // [V, C] of the piece
     long long ldw;
     const float* scale;
+    const kr_half* W_all;             // [V, C]
+    const int32_t* targets;
+    const float* left;
+    int v_all;
     float* dx_part;                   // [dx_splits][rows][C], if not direct
     float* dw_part;                   // [dw_splits][V][C], if not direct
     void* dx;                         // [N][C], direct: one split, one piece
@@ -487,6 +503,26 @@ __device__ __forceinline__ void copy_across(const kr_half* base, long long ld, i
         copy16(base, off, to + 1024u * (unsigned)(part * COPIES + i));
     }
 }
+
+// What fp16 left of the target's dz (one value, but of most of a row's dx: 4.2e-4 of it
+// without this, 2.2e-4 with) times its row of W.
+struct TargetRest {
+    const kr_half* w;
+    float left;
+    __device__ TargetRest(const kr_half* W, long long ldw, int V, const int32_t* targets, const float* rest, int m) {
+        const int t = targets[m];
+        const bool on = (unsigned)t < (unsigned)V;
+        w = W + (on ? (size_t)t * ldw : 0);
+        left = on ? rest[m] : 0.0f;
+    }
+    __device__ kr_half4 row(int n) const { return *reinterpret_cast<const kr_half4*>(w + n); }
+    __device__ kr_float4 times(kr_half4 x) const {       // 0 where there is none, whatever W has
+        kr_float4 v;
+        #pragma unroll
+        for (int r = 0; r < 4; r++) v[r] = left == 0.0f ? 0.0f : left * (float)x[r];
+        return v;
+    }
+};
 
 __device__ __forceinline__ void store_out(void* out, size_t at, kr_float4 v, int f32) {
     if (f32) *reinterpret_cast<kr_float4*>(static_cast<float*>(out) + at) = v;
@@ -587,15 +623,26 @@ __device__ __forceinline__ void product_tile(const ProdArgs& g, kr_half8* ring, 
         }
         #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const int m = m0 + 64 * wm + 16 * i + lr;
+            const int m = m0 + 64 * wm + 16 * i + lr, c0 = n_t * BN + 16 * TN * wn + 4 * lq;
             if (m >= m_end) continue;
+            if (!DW && direct) {
+                const TargetRest rest(g.W_all, g.ldw, g.v_all, g.targets, g.left, m);
+                kr_half4 w[TN];
+                #pragma unroll
+                for (int t = 0; t < TN; t++) w[t] = rest.row(c0 + 16 * t < g.C ? c0 + 16 * t : 0);
+                #pragma unroll
+                for (int t = 0; t < TN; t++)
+                    if (c0 + 16 * t < g.C)
+                        store_out(g.dx, (size_t)m * g.C + c0 + 16 * t, (acc[i][t] + rest.times(w[t])) * down, g.f32);
+                continue;
+            }
             #pragma unroll
             for (int t = 0; t < TN; t++) {
-                const int n = n_t * BN + 16 * TN * wn + 16 * t + 4 * lq;
+                const int n = c0 + 16 * t;
                 if (n >= g.C) continue;
                 kr_float4 v = acc[i][t];
                 if (direct) {
-                    store_out(DW ? g.dW : g.dx, (size_t)m * g.C + n, v * down, g.f32);
+                    store_out(g.dW, (size_t)m * g.C + n, v * down, g.f32);
                 } else {
                     float* part = DW ? g.dw_part : g.dx_part;
                     kr_float4* o = reinterpret_cast<kr_float4*>(part + ((size_t)split * M + m) * g.C + n);
@@ -623,9 +670,11 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN >= 8 ? 1 : 2) grad_produ
     else product_tile<WM, WN, TN, false>(g, ring, item_of(b - g.dw_items, g.dx_items));
 }
 
-// Sum of the splits of n outputs, in their order.
+// Sum of the splits of n outputs, in their order; of dx (W not null), with the targets' rest.
 __global__ void __launch_bounds__(256) grad_sum_kernel(const float* part, long long stride, int splits, long long n,
-                                                       const float* scale, int f32, void* out) {
+                                                       const float* scale, int f32, void* out, const kr_half* W,
+                                                       long long ldw, int V, const int32_t* targets,
+                                                       const float* left, int C) {
     const long long at = 4 * ((long long)blockIdx.x * 256 + threadIdx.x);
     if (at >= n) return;
     kr_float4 v = {0, 0, 0, 0};
@@ -637,6 +686,10 @@ __global__ void __launch_bounds__(256) grad_sum_kernel(const float* part, long l
             x[i] = s + i < splits ? *reinterpret_cast<const kr_float4*>(part + (s + i) * stride + at) : kr_float4{0, 0, 0, 0};
         #pragma unroll
         for (int i = 0; i < kAhead; i++) v += x[i];
+    }
+    if (W) {
+        const TargetRest rest(W, ldw, V, targets, left, (int)(at / C));
+        v += rest.times(rest.row((int)(at % C)));
     }
     store_out(out, at, v * scale[1], f32);
 }
@@ -682,7 +735,7 @@ size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 struct GradPlan {
     int rows, piece, pieces, dx_splits, dw_splits, dw_run;
     bool big, dx_direct;
-    size_t x, G, dx_part, dw_part, total;             // offsets in the workspace
+    size_t left, x, G, dx_part, dw_part, total;             // offsets in the workspace
 };
 
 GradPlan grad_plan(int N, int C, int V, bool dx, bool dw) {
@@ -703,6 +756,8 @@ GradPlan grad_plan(int N, int C, int V, bool dx, bool dw) {
     p.dw_run = dw_steps <= 8 && p.dw_splits == 1 ? gx : 1;
     p.dx_direct = p.dx_splits == 1 && p.pieces == 1;
     size_t at = 256;                                  // the scale
+    p.left = at;
+    at += up256((size_t)p.rows * 4);
     p.x = at;
     at += up256((size_t)p.rows * C * 2);
     p.G = at;
@@ -800,6 +855,7 @@ int kr_head_loss_backward(const uint16_t* x, long long ldx, int N, int C, const 
     g.dloss = dloss;
     g.scale = scale;
     g.G = reinterpret_cast<kr_half*>(base + p.G);
+    g.left = reinterpret_cast<float*>(base + p.left);
     g.ldg = p.piece;
     g.N = N;
     g.C = C;
@@ -809,6 +865,10 @@ int kr_head_loss_backward(const uint16_t* x, long long ldx, int N, int C, const 
     d.G = g.G;
     d.ldg = g.ldg;
     d.x = live;
+    d.W_all = g.W = reinterpret_cast<const kr_half*>(W);
+    d.targets = targets;
+    d.left = g.left;
+    d.v_all = V;
     d.ldw = ldw;
     d.scale = scale;
     d.dx_part = reinterpret_cast<float*>(base + p.dx_part);
@@ -839,15 +899,16 @@ int kr_head_loss_backward(const uint16_t* x, long long ldx, int N, int C, const 
         KR_LAUNCHED();
         if (dW && p.dw_splits > 1) {
             const long long n = (long long)nv * C;
-            grad_sum_kernel<<<(unsigned)((n / 4 + 255) / 256), 256, 0, s>>>(d.dw_part, n, p.dw_splits, n, scale, out_f32,
-                                                                           d.dW);
+            grad_sum_kernel<<<(unsigned)((n / 4 + 255) / 256), 256, 0, s>>>(d.dw_part, n, p.dw_splits, n, scale, out_f32, d.dW,
+                                                                           nullptr, 0, 0, nullptr, nullptr, C);
             KR_LAUNCHED();
         }
     }
     if (dx && !p.dx_direct) {
         const long long n = (long long)N * C;
         grad_sum_kernel<<<(unsigned)((n / 4 + 255) / 256), 256, 0, s>>>(d.dx_part, (long long)p.rows * C, p.dx_splits, n,
-                                                                       scale, out_f32, dx);
+                                                                       scale, out_f32, dx, d.W_all, ldw, V, targets,
+                                                                       d.left, C);
         KR_LAUNCHED();
     }
     return KR_OK;
