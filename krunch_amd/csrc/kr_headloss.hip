@@ -709,8 +709,12 @@ int launch_logits(const LossArgs& g, hipStream_t s) {
     return KR_OK;
 }
 
-// Which tiles: 256 x 256 once they fill the chip, 128 x 128 below.
-bool big_tiles(int N, int V) { return (long long)((N + 255) / 256) * ((V + 255) / 256) >= 512; }
+// Which tiles. us, 128 x 128 / 256 x 256, width 768: losses over 50277 columns of 128
+// rows 23 / 32, 256 39 / 32, 1024 104 / 104, 4096 372 / 314; over 4096 columns of 2048 rows
+// (128 large tiles) 20 / 29, 8192 64 / 56.
+bool big_tiles(int N, int V) {
+    return N > 128 && (long long)((N + 255) / 256) * ((V + 255) / 256) >= 192;
+}
 
 template <bool GRAD>
 int logits(const LossArgs& g, bool big, hipStream_t s) {
@@ -734,7 +738,7 @@ size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 // 176 MB, and the products' splits.
 struct GradPlan {
     int rows, piece, pieces, dx_splits, dw_splits, dw_run;
-    bool big, dx_direct;
+    bool big, big_products, dx_direct;
     size_t left, x, G, dx_part, dw_part, total;             // offsets in the workspace
 };
 
@@ -745,8 +749,12 @@ GradPlan grad_plan(int N, int C, int V, bool dx, bool dw) {
     p.pieces = (int)((V + most - 1) / most);
     p.piece = ((V + p.pieces - 1) / p.pieces + 255) / 256 * 256;
     p.pieces = (V + p.piece - 1) / p.piece;
-    p.big = big_tiles(N, V) && p.rows >= 1024;
-    const int tile = p.big ? 256 : 128, slots = p.big ? 256 : 512;
+    p.big = big_tiles(N, V);
+    // us for gradients, 128 x 128 / 256 x 256 tiles in the products: 8192 x 768 x 50277 2084 /
+    // 2014, 512 wide 1463 / 1596, 4096 x 256 wide 510 / 581, 16384 x 768 x 16384 (66 tiles of dW
+    // a piece) 1410 / 1666, 4096 x 1024 x 4096 (64) 134 / 167
+    p.big_products = p.big && C > 512 && (p.piece / 256) * ((C + 255) / 256) >= 100;
+    const int tile = p.big_products ? 256 : 128, slots = p.big_products ? 256 : 512;
     const int gx = (C + tile - 1) / tile, dx_steps = p.piece / 64, dw_steps = p.rows / 64;
     const long long dx_tiles = (long long)(p.rows + tile - 1) / tile * gx, dw_tiles = (long long)p.piece / tile * gx;
     const long long total = (dx ? dx_tiles * dx_steps : 0) + (dw ? dw_tiles * dw_steps : 0);
@@ -882,7 +890,7 @@ int kr_head_loss_backward(const uint16_t* x, long long ldx, int N, int C, const 
     d.dx = dx;
     d.dx_direct = p.dx_direct;
     d.dw_run = p.dw_run;
-    const int tile = p.big ? 256 : 128, gx = (C + tile - 1) / tile;
+    const int tile = p.big_products ? 256 : 128, gx = (C + tile - 1) / tile;
     for (int i = 0; i < p.pieces; i++) {
         const int v0 = i * p.piece, nv = std::min(V - v0, p.piece);
         g.W = d.W = reinterpret_cast<const kr_half*>(W) + (size_t)v0 * ldw;
@@ -894,7 +902,7 @@ int kr_head_loss_backward(const uint16_t* x, long long ldx, int N, int C, const 
         d.dW = dW ? static_cast<char*>(dW) + (size_t)v0 * C * (out_f32 ? 4 : 2) : nullptr;
         d.dw_items = dW ? (nv + tile - 1) / tile * ((gx + p.dw_run - 1) / p.dw_run) * p.dw_splits : 0;
         d.dx_items = dx ? (p.rows + tile - 1) / tile * gx * p.dx_splits : 0;
-        if (p.big) grad_products_kernel<4, 2, 8><<<d.dw_items + d.dx_items, 512, 0, s>>>(d);
+        if (p.big_products) grad_products_kernel<4, 2, 8><<<d.dw_items + d.dx_items, 512, 0, s>>>(d);
         else grad_products_kernel<2, 2, 4><<<d.dw_items + d.dx_items, 256, 0, s>>>(d);
         KR_LAUNCHED();
         if (dW && p.dw_splits > 1) {
