@@ -138,13 +138,13 @@ int kr_token_scores(const void* logits, int logits_f32, int N, int V, long long 
 /* Cross entropy of a head in pieces of the vocabulary, without its logits (no
  * reference counterpart; beside kr_token_scores, which reads logits): x fp16
  * [N, C] and W fp16 [V, C] by row strides ldx, ldw (multiples of 8, below 2^21; x
- * and W 16-byte aligned; C a multiple of 64 up to 16384; N, V <= 2^24):
+ * and W 16-byte aligned; C a multiple of 64 up to 16384; N, V <= 2^24, N V <= 2^44):
  *   z = x W' (exact products, fp32 sums, not rounded to fp16 as logits are)
  *   lse[n]  = ln sum_v e^z[n][v];   loss[n] = lse[n] - z[n][targets[n]]
  * in nats; loss is 0 where targets[n] = -1 and NaN for any other id outside
- * 0..V-1; a row with a NaN or +inf in z is NaN. The order of a row's sums depends on
- * N <= 128 or not. ws: kr_head_loss_workspace_bytes, 256-byte aligned (8 bytes a row
- * and 128 columns of the vocabulary).
+ * 0..V-1; a row with a NaN or +inf in z is NaN. Sums are fp32; the order of a row's
+ * depends on N and V (z itself does not). ws: kr_head_loss_workspace_bytes, 256-byte
+ * aligned (at most 8 bytes for a row and 64 columns, of up to 65536 rows at a time).
  *
  * kr_head_loss_backward, from the same inputs, the lse of the forward call and
  * dloss fp32 [N]:
@@ -153,12 +153,12 @@ int kr_token_scores(const void* logits, int logits_f32, int N, int V, long long 
  * (out_f32) fp32; dx or dW may be NULL. Rows with target -1 or dloss 0 have no
  * gradient, whatever x, lse and dloss hold there; other ids outside 0..V-1 give
  * NaN. dz is rounded to fp16 on a scale where the largest finite |dloss| is
- * 2^14..2^15, so relative to that row's gradient: 2^-11 of each dz above
- * 2^-28 of the largest |dloss|, 2^-39 of the largest |dloss| below. Sums are
- * fp32 in an order that depends on the sizes alone. ws:
+ * 2^14..2^15: by 2^-11 of each dz above 2^-28 of the largest |dloss|, by 2^-39 of
+ * the largest |dloss| below; in dx, what that leaves of the target's dz is added back.
+ * Sums are fp32 in an order that depends on the sizes alone. ws:
  * kr_head_loss_backward_workspace_bytes (dx, dw: which of them is wanted), 256-byte
- * aligned: at most 256 MB of dz at once (256 columns at least) and fp32 partial
- * sums. Outputs must not overlap inputs. */
+ * aligned: at most 176 MB of dz at once (256 columns at least), a copy of x and fp32
+ * partial sums. Outputs must not overlap inputs. */
 size_t kr_head_loss_workspace_bytes(int N, int C, int V);
 int kr_head_loss(const uint16_t* x, long long ldx, int N, int C, const uint16_t* W, long long ldw, int V,
                  const int32_t* targets, float* loss, float* lse, void* ws, size_t ws_bytes, void* stream);
@@ -461,8 +461,9 @@ int kr_wkv_heads(int B, int T, int H, int D, const uint16_t* r, long long ldr, c
  * token in fp32; T tokens in one call have the bits of T calls of one. chunked = 1:
  * 64 tokens at a time on the matrix units, for prompts: equal to that up to rounding
  * (2^-22 of a value that enters the matrix units: a state element, a weight between two
- * tokens, what a token writes; and 2^-38 of the largest one of its column or row); a
- * NaN or infinity of a token then also reaches y of up to 63 tokens before it. Calls of
+ * tokens, what a token writes; and 2^-38 of the largest one of its column or row), in
+ * an order that depends on B * H and T (the time axis is split over workgroups where
+ * heads are few); a NaN or infinity of a token then also reaches y of up to 63 tokens before it. Calls of
  * at most 8 tokens are the same in both. Keys of length 1 and beta in 0..1 keep the
  * recurrence stable; others are computed, too. y must not overlap q, k or v. ws:
  * kr_gated_delta_workspace_bytes (chunked only, may be 0), 16-byte aligned, as q, k, v,
@@ -478,7 +479,9 @@ int kr_gated_delta(int B, int T, int H, int D, const uint16_t* q, long long ldq,
  * state after the call (NULL: zeros). Writes dq, dk, dv fp16 [B, T, H, D], dlog_decay and
  * dbeta fp32 [B, T, H], all contiguous, and dstate0 fp32 [B, H, D, D], the gradient
  * of state. Tokens past lens have gradient 0, as a log_decay above 0 or below -10000
- * has. Values rounded as in the forward pass, sums fp32. T <= 4194240. ws:
+ * has. Values rounded as in the forward pass, sums fp32; dlog_decay is a difference of
+ * sums over a chunk's tokens, so its error is relative to those, not to a small
+ * gradient behind a strong decay. T <= 4194240. ws:
  * kr_gated_delta_backward_workspace_bytes (for each head and 64 tokens two states and two
  * rows of D fp32 values a token: 8 D (D + 64) bytes), 256-byte aligned; it must not
  * overlap anything, nor outputs the inputs. Everything but log_decay, beta, lens and

@@ -1579,13 +1579,13 @@ void split_time(long long heads, int T, int D, bool back, int& seg_chunks, int& 
     const int chunks = (T + kChunk - 1) / kChunk;
     const long long slots = D == 64 ? 512 : 256;
     auto rounds = [&](long long n) { return (n + slots - 1) / slots; };
-    const int walks = back ? 2 : 1;
+    const int walks = back ? 2 : 1, step = D == 64 ? 2 : 3;
     seg_chunks = chunks;
     segments = 1;
     long long best = 12 * chunks * rounds(walks * heads);
     for (int n = 2; n <= chunks / 2 && n <= 128 && n * heads <= 2 * slots; n++) {
         const int c = (chunks + n - 1) / n, used = (chunks + c - 1) / c;
-        const long long cost = 12ll * c * (rounds((back ? 3 : 2) * heads * used) + rounds(walks * heads * used)) + used + 24;
+        const long long cost = 12ll * c * (rounds((back ? 3 : 2) * heads * used) + rounds(walks * heads * used)) + step * used + 24;
         if (cost < best) {
             best = cost;
             seg_chunks = c;

@@ -729,8 +729,10 @@ int loss_parts(int N, int C, int V) {
 }
 
 bool shape_ok(int N, int C, int V) {
-    return N >= 0 && N <= 1 << 24 && C >= 64 && C % 64 == 0 && C <= 1 << 14 && V >= 1 && V <= 1 << 24;
+    return N >= 0 && N <= 1 << 24 && C >= 64 && C % 64 == 0 && C <= 1 << 14 && V >= 1 && V <= 1 << 24 &&
+           (long long)N * V <= 1ll << 44;             // a launch's tiles stay below 2^31
 }
+constexpr int kLossRows = 1 << 16;                    // of a forward launch: bounds its parts
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
@@ -784,12 +786,14 @@ extern "C" {
 
 size_t kr_head_loss_workspace_bytes(int N, int C, int V) {
     if (!shape_ok(N, C, V) || N == 0) return 0;
-    return up256((size_t)N * 4) + (size_t)loss_parts(N, C, V) * N * sizeof(float2);
+    const int rows = std::min(N, kLossRows), last = (N - 1) % kLossRows + 1;
+    const size_t parts = std::max((size_t)loss_parts(rows, C, V) * rows, (size_t)loss_parts(last, C, V) * last);
+    return up256((size_t)rows * 4) + parts * sizeof(float2);
 }
 
 int kr_head_loss(const uint16_t* x, long long ldx, int N, int C, const uint16_t* W, long long ldw, int V,
                  const int32_t* targets, float* loss, float* lse, void* ws, size_t ws_bytes, void* stream) {
-    KR_REQUIRE(shape_ok(N, C, V), "kr_head_loss: bad shape N=%d C=%d V=%d (C a multiple of 64 up to 16384, N and V up to 2^24)",
+    KR_REQUIRE(shape_ok(N, C, V), "kr_head_loss: bad shape N=%d C=%d V=%d (C a multiple of 64 up to 16384, N and V up to 2^24, N * V up to 2^44)",
                N, C, V);
     KR_REQUIRE(ldx >= C && ldw >= C && (ldx | ldw) % 8 == 0 && (ldx | ldw) < 1 << 21,
                "kr_head_loss: row strides must be multiples of 8, at least C = %d and below 2^21", C);
@@ -800,28 +804,32 @@ int kr_head_loss(const uint16_t* x, long long ldx, int N, int C, const uint16_t*
     KR_REQUIRE(ws && ws_bytes >= need && ((uintptr_t)ws & 255) == 0,
                "kr_head_loss: workspace of %zu bytes, %zu needed (256-byte aligned)", ws_bytes, need);
     LossArgs g{};
-    g.x = reinterpret_cast<const kr_half*>(x);
     g.W = reinterpret_cast<const kr_half*>(W);
     g.ldx = ldx;
     g.ldw = ldw;
-    g.targets = targets;
     g.hit = static_cast<float*>(ws);
-    g.part = reinterpret_cast<float2*>(static_cast<char*>(ws) + up256((size_t)N * 4));
-    g.N = N;
+    g.part = reinterpret_cast<float2*>(static_cast<char*>(ws) + up256((size_t)std::min(N, kLossRows) * 4));
     g.C = C;
     g.V = g.v_all = V;
     const hipStream_t s = kr_stream(stream);
-    const int parts = loss_parts(N, C, V);
-    if (few_rows(N, C)) {
-        few_rows_kernel<<<parts, 64 * kFewWaves, 0, s>>>(g);
+    for (int r0 = 0; r0 < N; r0 += kLossRows) {
+        const int n = std::min(N - r0, kLossRows), parts = loss_parts(n, C, V);
+        g.x = reinterpret_cast<const kr_half*>(x) + (size_t)r0 * ldx;
+        g.targets = targets + r0;
+        g.N = n;
+        if (few_rows(n, C)) {
+            few_rows_kernel<<<parts, 64 * kFewWaves, 0, s>>>(g);
+            KR_LAUNCHED();
+        } else {
+            const int rc = logits<false>(g, big_tiles(n, V), s);
+            if (rc != KR_OK) return rc;
+        }
+        if (n <= 256)
+            loss_join_kernel<1><<<n, 256, 0, s>>>(g.part, g.hit, n, parts, V, g.targets, loss + r0, lse + r0);
+        else
+            loss_join_kernel<16><<<(n + 15) / 16, 256, 0, s>>>(g.part, g.hit, n, parts, V, g.targets, loss + r0, lse + r0);
         KR_LAUNCHED();
-    } else {
-        const int rc = logits<false>(g, big_tiles(N, V), s);
-        if (rc != KR_OK) return rc;
     }
-    if (N <= 256) loss_join_kernel<1><<<N, 256, 0, s>>>(g.part, g.hit, N, parts, V, targets, loss, lse);
-    else loss_join_kernel<16><<<(N + 15) / 16, 256, 0, s>>>(g.part, g.hit, N, parts, V, targets, loss, lse);
-    KR_LAUNCHED();
     return KR_OK;
 }
 
@@ -834,7 +842,7 @@ int kr_head_loss_backward(const uint16_t* x, long long ldx, int N, int C, const 
                           const int32_t* targets, const float* lse, const float* dloss, int out_f32, void* dx,
                           void* dW, void* ws, size_t ws_bytes, void* stream) {
     KR_REQUIRE(shape_ok(N, C, V),
-               "kr_head_loss_backward: bad shape N=%d C=%d V=%d (C a multiple of 64 up to 16384, N and V up to 2^24)",
+               "kr_head_loss_backward: bad shape N=%d C=%d V=%d (C a multiple of 64 up to 16384, N and V up to 2^24, N * V up to 2^44)",
                N, C, V);
     KR_REQUIRE(N >= 1, "kr_head_loss_backward: no rows");
     KR_REQUIRE(ldx >= C && ldw >= C && (ldx | ldw) % 8 == 0 && (ldx | ldw) < 1 << 21,

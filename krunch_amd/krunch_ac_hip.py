@@ -255,7 +255,7 @@ def _head_shapes(x, W, targets):
         f"W must be [V, C] with C a multiple of 64 up to 16384, got {tuple(W.shape)}")
     ldx, ldw = _head_rows(x, "x", C), _head_rows(W, "W", C)
     N = x.shape[0]
-    max(N, V) <= 1 << 24 or _refuse("N and V must be at most 2^24")
+    (max(N, V) <= 1 << 24 and N * V <= 1 << 44) or _refuse("N and V must be at most 2^24, N * V at most 2^44")
     dev = x.get_device()
     W.get_device() == dev or _refuse("x and W must be on one device")
     _head_vector(targets, torch.int32, "targets", N, dev)
@@ -602,7 +602,7 @@ def gated_delta_backward(q, k, v, log_decay, beta, state, dy, dstate=None, lens=
     dq, dk, dv = (q.new_empty(shape) for _ in range(3))
     dg, db = (state.new_empty((B, T, H)) for _ in range(2))
     if B * T == 0:
-        return dq, dk, dv, dg, db, torch.zeros_like(state) if dstate is None else dstate.clone()
+        return dq, dk, dv, dg, db, torch.zeros_like(state) if dstate is None else dstate.detach().clone()
     d0 = torch.empty_like(state)
     nbytes = _lib.lib().kr_gated_delta_backward_workspace_bytes(B, T, H, D)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)

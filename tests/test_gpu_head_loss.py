@@ -108,7 +108,8 @@ def test_sizes(N, C, V):
     check_grads(x, W, t, w)
 
 
-@pytest.mark.parametrize("N,C,V", [(8192, 64, 20000), (5000, 128, 50277), (70000, 64, 300), (300, 64, 200001)])
+@pytest.mark.parametrize("N,C,V", [(8192, 64, 20000), (5000, 128, 50277), (70000, 64, 300), (65541, 64, 130),
+                                   (300, 64, 200001)])
 def test_pieces_and_splits(N, C, V):
     x, W, t, w = make(N, C, V, 5)
     check_loss(x, W, t)
