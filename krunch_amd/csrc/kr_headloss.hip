@@ -63,6 +63,10 @@ __device__ __forceinline__ unsigned lds_address(const void* p) {
 // one kc lie on different banks.
 __device__ __forceinline__ int row_unit(int r, int kc) { return 8 * r + (kc ^ ((r >> 1) & 7)); }
 
+// The same for W of a tile, 16 of whose rows are read as 8 a + b, a and b 0..3 (or 4 more).
+__device__ __forceinline__ int w_swap(int r) { return ((r >> 1) & 1) | ((r >> 2) & 6); }
+__device__ __forceinline__ int w_unit(int r, int kc) { return 8 * r + (kc ^ w_swap(r)); }
+
 // Tile of the launch's virtual workgroup vb: an eighth of a grouped order for each XCD.
 __device__ __forceinline__ bool tile_of(int gy, int gx, int vb, int group_m, int& m_t, int& n_t) {
     const int T = gx * gy, per = (T + 7) / 8;
@@ -111,7 +115,7 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN >= 8 ? 1 : 2) logits_ker
             const bool a = j < BM / 8;
             const int row = 8 * (a ? j : j - BM / 8) + (lane >> 3);
             const int last = a ? g.N - 1 - m_t * BM : g.V - 1 - n_t * BN;
-            const int kc = (lane & 7) ^ ((row >> 1) & 7);
+            const int kc = (lane & 7) ^ (a ? (row >> 1) & 7 : w_swap(row));
             const unsigned off = (unsigned)max(min(row, last), 0) * (unsigned)(2 * (a ? g.ldx : g.ldw)) +
                                  (unsigned)(16 * kc + 128 * ks);
             copy16(a ? xa : wa, off, so + 1024u * (unsigned)j);
@@ -150,7 +154,7 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN >= 8 ? 1 : 2) logits_ker
                     #pragma unroll
                     for (int t = 0; t < 4; t++) {
                         const int row = 16 * TN * wn + 32 * (2 * th + t / 2) + 8 * (lr >> 2) + 4 * (t & 1) + (lr & 3);
-                        w[t] = Ws[row_unit(row, 4 * kb + lq)];
+                        w[t] = Ws[w_unit(row, 4 * kb + lq)];
                     }
                     __builtin_amdgcn_sched_barrier(0);
                     #pragma unroll
