@@ -65,6 +65,9 @@ __device__ __forceinline__ double gate_log2(float g) {
 // Recurrent form. A wave has 16 columns of a head's state in registers: lane l the
 // columns 4 (l % 4) .. + 3 of rows D/16 (l / 4) .. + D/16 - 1. k S, q S and k q' are
 // summed together over a lane's rows and then over 16 lanes: y = q S + (q k') u.
+// Bound, for one token: the state, read and written once. Measured on MI355X, heads of
+// 64: 512 streams x 12 heads 32 us (203 MB, 6.3 TB/s), one stream 3.2 (a call 11, the
+// host's). For many: a token's chain, 0.7 us.
 // ---------------------------------------------------------------------------
 template <int D>
 __global__ void __launch_bounds__(4 * D) delta_step_kernel(DeltaArgs g) {
@@ -581,6 +584,11 @@ struct DeltaShared {
 // of k S and q S, and what they leave is the operand of the next product. A segment
 // makes map S + sum of the state S at its start: SUMS gives one or the other, as the
 // state that follows from the identity without values, or from zero.
+// Bound: instructions issued, about 2,100 a chunk and wave (1,400 of them VALU, a third
+// for taking values apart and scales), with 8 waves a CU: 72 KB of LDS a workgroup for D =
+// 64, 96 for 128, allow no more; a wave alone issues one about every 8 cycles. Measured on
+// MI355X, heads of 64: 128 streams of 256..1024 tokens x 12 heads 263-287 us (640 MB: 125 at
+// a copy's rate; VALU 60% busy, matrix units 16%); a chunk alone 8 us, for D = 128 10.
 // ---------------------------------------------------------------------------
 template <int D, int MODE>
 __device__ __forceinline__ void walk_chunks(const DeltaArgs& g, DeltaShared<D>& sh, int heads, int b, int h, int seg,
@@ -1143,6 +1151,9 @@ __global__ void __launch_bounds__(4 * D, 2) delta_both_kernel(DeltaArgs f, BackA
 // computed for all segments at once, the states at their starts follow one from
 // the other, and then all segments run. Backward, D -> map' D + sum.
 // z of the sums' launch: 0 sums, 1 maps, 2 D's sums; of the states': 0 forward, 1 back.
+// Three times the work, side by side: 1 x 1777 x 8 heads of 128 274 -> 78 us (14 segments:
+// sums 20, join 38, walk 24), gradients of 1 x 2000 x 12 of 64 394 -> 84 (29, 12, 29, and
+// 22 for the chunks' gradients).
 // ---------------------------------------------------------------------------
 template <int D>
 __global__ void __launch_bounds__(4 * D, 2) delta_sums_kernel(DeltaArgs f, BackArgs g) {
@@ -1158,7 +1169,8 @@ __global__ void __launch_bounds__(4 * D, 2) delta_sums_kernel(DeltaArgs f, BackA
 
 // 16 columns of a head: a wave has 16 rows of every segment's map, read two segments
 // ahead (or every step waits for memory); the column passes through LDS, [m][n] in two
-// buffers.
+// buffers. Bound by a step's chain: 1.2 us for D = 64, 2.9 for 128 (values taken apart by
+// 8 waves on one CU, a barrier, 12 products).
 template <int D>
 struct JoinPiece {
     float map[D / 32][8], sum[4];
@@ -1248,6 +1260,10 @@ __global__ void __launch_bounds__(4 * D) delta_join_kernel(DeltaArgs f, BackArgs
 
 // A workgroup of 4 waves for each head and chunk, a wave for 16 tokens, as those that
 // read and as those that write. 64 rows of S, then of D, are in LDS at a time.
+// Bound: waits for memory with 8 waves a CU (77 KB of LDS a workgroup): a chunk's 130 KB
+// are loaded, then computed on. Measured on MI355X, 48 streams of 256..1024 x 12 heads of
+// 64: 278 us (0.55 GB, 2 TB/s; VALU 38% busy), the walks before it 243 (0.53 GB). Eight waves
+// a workgroup, four for each side, spill at 128 registers: 634.
 template <int D>
 struct GradShared {
     kr_half8 q[kChunk * D / 8], k[kChunk * D / 8], dy[kChunk * D / 8];             // by tokens
@@ -1569,12 +1585,16 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1) delta_grad_kernel(BackAr
     }
 }
 
-// Tokens up to which the chunked form is the recurrent one, too.
+// Tokens up to which the chunked form is the recurrent one, too. us, recurrent / chunked, 12
+// heads of 64: 8 tokens of 1 stream 12.8 / 12.9, of 64 16 / 20, of 512 88 / 117; 12 tokens 13.4 /
+// 13.6, 22 / 20, 123 / 116; 6 heads of 128: 8 tokens 12.4 / 12.7, 24 / 28, 111 / 153.
 constexpr int kStepTokens = 8;
 
 // Segments of the time axis, by what a call would take: rounds of workgroups (one a CU
 // for D = 128, two for 64) times a segment's chunks, for the sums and for the walk, and
-// the join's steps, a twelfth of a chunk each. A segment has two chunks at least.
+// the join's steps, two or three twelfths of a chunk. A segment has two chunks at least.
+// us, one walk / split: 12 heads of 64, 1 x 1024 99 / 38, 1 x 4096 386 / 75, 4 x 1024 100 /
+// 59, 8 x 1024 101 / 96; 8 heads of 128 147 / 63, 584 / 122, 151 / 93, 152 / 138.
 void split_time(long long heads, int T, int D, bool back, int& seg_chunks, int& segments) {
     const int chunks = (T + kChunk - 1) / kChunk;
     const long long slots = D == 64 ? 512 : 256;
