@@ -87,9 +87,9 @@ __device__ __forceinline__ bool tile_of(int gy, int gx, int vb, int group_m, int
 // through two LDS stages, copied asynchronously one step ahead, into the next tile. The
 // matrix unit gets W' x', so a lane has 4 columns of a row; W's rows go in in an
 // order that makes them 8 consecutive columns over two of its tiles.
-// Bound, at 256 x 256: LDS reads (192 KB a step beside 64 KB written) and matrix
-// instructions, about 2,050 cycles of each a step, and the epilogue that neither
-// overlaps (an exponential each). Measured on MI355X, 8192 x 768 x 50277: losses 577 us
+// Bound, at 256 x 256: the copies, one step ahead (a step takes 4,400 cycles, its matrix
+// instructions 2,050, LDS reads 770), and the epilogue that nothing overlaps (an
+// exponential each). Measured on MI355X, 8192 x 768 x 50277: losses 577 us
 // (1.10 PF/s; a library's product of the same sizes 703, 8192^3 at 1.16), dz 155 us for
 // 10240 columns (0.83 PF/s, 168 MB stored). A bank conflict in every read of W cost 40 us of
 // the losses, a cursor over tiles that allows more stages 25. At 128 x 128, two workgroups
@@ -463,7 +463,7 @@ __global__ void __launch_bounds__(1024) grad_prepare_kernel(const kr_half* x, lo
 // Bound: copies (one step ahead) and the last round of workgroups: dW's tiles of a piece
 // take all N rows each, dx's splits fill up behind them. Measured on MI355X, a piece of
 // 10240 columns of 8192 x 768 x 50277: 282 us for both products (0.90 PF/s; a library's of
-// these sizes 0.77 dW, 1.04 dx). Pieces: dz of 176 MB at most stays in the memory-side
+// these sizes 0.77 dW, 1.04 dx); steps of 32 k, three ahead, 292. Pieces: dz of 176 MB at most stays in the memory-side
 // cache; 224, 288 and 420 MB 2045, 2062 and 1937 us for the call, 176 2037.
 // ---------------------------------------------------------------------------
 struct ProdArgs {
