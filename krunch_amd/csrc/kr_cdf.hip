@@ -27,6 +27,7 @@
 #include <vector>
 #include <algorithm>
 
+#include "kr_copy.h"
 #include "kr_math.h"
 #include "kr_rc_device.h"
 #include "kr_rowops.h"
@@ -398,14 +399,6 @@ __device__ __forceinline__ int scaled_floor(float p, float scale) {
     else return (int)floorf(__fmul_rn(p, scale));
 }
 
-// 16-byte asynchronous copy global -> LDS: lane l writes LDS byte address
-// lds + 16 l. The compiler does not count it: readers wait with an explicit
-// s_waitcnt vmcnt(0) and a barrier.
-__device__ __forceinline__ void lds_copy16(const void* src, unsigned lds) {
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off"
-                 :: "s"(lds), "v"(src) : "memory", "m0");
-}
-
 // stage_row's layout for a 16-byte-aligned row whose last chunk of 8 lies
 // inside its allocation (row stride a multiple of 8): chunk c at 16-byte unit
 // c + c / 16, so unit 17 s + t holds chunk 16 s + t for t < 16 and unit
@@ -422,7 +415,7 @@ __device__ __forceinline__ void stage_row_async(const kr_half* rp, int V, unsign
         const int u = 64 * q + lane;
         const int s = (u * 61681) >> 20;                    // u / 17 for u < 20000
         const int c = min(16 * s + min(u - 17 * s, 15), nch - 1);
-        lds_copy16(rp + 8 * c, stage_lds + 1024u * (unsigned)q);
+        kr_copy16(rp + 8 * c, stage_lds + 1024u * (unsigned)q);
     }
 }
 

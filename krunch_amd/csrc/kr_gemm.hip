@@ -24,6 +24,7 @@
 #include <climits>
 #include <type_traits>
 
+#include "kr_copy.h"
 #include "kr_gemm.h"
 #include "kr_gemm_epilogue.h"
 #include "kr_math.h"
@@ -232,13 +233,6 @@ constexpr int kBigRows = 384;
 constexpr int kBigStage = kBigRows * 8;          // 16-byte units per stage (48 KB)
 
 
-// 16-byte asynchronous copy global -> LDS: lane l writes LDS byte address
-// lds + 16 l. Invisible to the compiler's wait-count tracking (see above).
-__device__ __forceinline__ void big_copy(const void* src, unsigned lds) {
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off"
-                 :: "s"(lds), "v"(src) : "memory", "m0");
-}
-
 // Tile t of the launch (the dealing of tile_of, for a launch of `grid`
 // virtual blocks, in groups of group_m row tiles): false past the last tile.
 template <int BM>
@@ -318,7 +312,7 @@ __global__ void __launch_bounds__(512, 1) gemm_big_kernel(kr_gemm_args g, int n_
     auto issue = [&](const char* (&src)[6], int ks, int q) {
         const unsigned so = (unsigned)((q % 3) * kBigStage * 16);
         #pragma unroll
-        for (int i = 0; i < 6; i++) big_copy(src[i] + (size_t)ks * 128, dst[i] + so);
+        for (int i = 0; i < 6; i++) kr_copy16(src[i] + (size_t)ks * 128, dst[i] + so);
     };
 
     int vb = blockIdx.x, m_t, n_t;
@@ -726,7 +720,7 @@ __global__ void __launch_bounds__(256, 1) gemm_head_small_kernel(
             Wf + ((size_t)(b0 + j) * KB + (size_t)wave * CPW) * 512 + lane * 8);
         const unsigned dst = ring_base + (unsigned)(((j % kHeadStages) * KB + wave * CPW) * 1024);
         #pragma unroll
-        for (int u = 0; u < CPW; u++) big_copy(src + u * 1024, dst + u * 1024);
+        for (int u = 0; u < CPW; u++) kr_copy16(src + u * 1024, dst + u * 1024);
     };
     #pragma unroll
     for (int j = 0; j < kHeadStages - 1; j++)

@@ -5,6 +5,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "kr_copy.h"
 #include "kr_gemm.h"
 
 namespace {
@@ -41,12 +42,6 @@ constexpr int kStages = 6;
 
 typedef kr_half4 kr_half4_any __attribute__((aligned(2)));   // any row stride: global memory takes it
 
-// 16-byte asynchronous copy global -> LDS (lane l writes lds + 16 l),
-// invisible to the compiler's wait counts.
-__device__ __forceinline__ void head_copy(const void* src, unsigned lds) {
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off"
-                 :: "s"(lds), "v"(src) : "memory", "m0");
-}
 template <int N>
 __device__ __forceinline__ void wait_vm() {
     asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory");
@@ -92,7 +87,7 @@ __global__ void __launch_bounds__(256, 1) gemm_head_rows_kernel(
             Wf + ((size_t)(b0 + j) * KB + (size_t)wave * CPW) * 512 + lane * 8);
         const unsigned dst = ring_base + (unsigned)(((j % kStages) * KB + wave * CPW) * 1024);
         #pragma unroll
-        for (int u = 0; u < CPW; u++) head_copy(src + u * 1024, dst + u * 1024);
+        for (int u = 0; u < CPW; u++) kr_copy16(src + u * 1024, dst + u * 1024);
     };
     #pragma unroll
     for (int j = 0; j < kStages - 1; j++)

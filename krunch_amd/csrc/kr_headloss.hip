@@ -16,6 +16,7 @@
 #include <algorithm>
 
 #include "kr_common.h"
+#include "kr_copy.h"
 #include "kr_wave.h"
 #include "krunch_hip.h"
 
@@ -44,9 +45,7 @@ struct LossArgs {
 };
 
 __device__ __forceinline__ void copy16(const void* base, unsigned off, unsigned lds) {
-    lds = (unsigned)__builtin_amdgcn_readfirstlane((int)lds);
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2"
-                 :: "s"(lds), "v"(off), "s"(base) : "memory", "m0");
+    kr_copy16(base, off, (unsigned)__builtin_amdgcn_readfirstlane((int)lds));
 }
 // A pointer that all lanes share, as such to the compiler.
 template <typename T>

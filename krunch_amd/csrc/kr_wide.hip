@@ -3,6 +3,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "kr_copy.h"
 #include "kr_gemm.h"
 #include "kr_gemm_epilogue.h"
 #include "kr_math.h"
@@ -32,11 +33,6 @@
 namespace {
 
 constexpr int kWideStageUnits = 512 * 8;      // 16-byte units per 64 KB stage
-
-__device__ __forceinline__ void wide_copy(const void* base, unsigned off, unsigned lds) {
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2"
-                 :: "s"(lds), "v"(off), "s"(base) : "memory", "m0");
-}
 
 __device__ __forceinline__ bool wide_tile(int M, int N, int vb, int group_m, int& m_t, int& n_t) {
     const int gy = (M + 255) / 256, gx = (N + 255) / 256;
@@ -79,7 +75,7 @@ __global__ void __launch_bounds__(512, 1) gemm_wide_kernel(kr_gemm_args g, int n
             const int ckc = (lane & 7) ^ ((crow >> 1) & 7);
             const unsigned off = (unsigned)((long long)min(r0 + crow, lim - 1) * ld16 * 2) +
                                  (unsigned)(ckc * 16 + ks * 128);
-            wide_copy(base, off, so + (unsigned)((wave * 8 + i) * 1024));
+            kr_copy16(base, off, so + (unsigned)((wave * 8 + i) * 1024));
         }
     };
     int vb = blockIdx.x, m_t, n_t;
