@@ -12,8 +12,9 @@ __device__ __forceinline__ void kr_copy16(const void* src, unsigned lds) {
                  :: "s"(lds), "v"(src) : "memory", "m0");
 }
 
-// From an address that all lanes share and a byte offset a lane.
+// From an address that all lanes share and a byte offset a lane. The address may come
+// from a v_readfirstlane just before: five wait states until the copy reads it.
 __device__ __forceinline__ void kr_copy16(const void* base, unsigned off, unsigned lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2"
                  :: "s"(lds), "v"(off), "s"(base) : "memory", "m0");
 }
