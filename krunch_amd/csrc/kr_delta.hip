@@ -1169,8 +1169,9 @@ __global__ void __launch_bounds__(4 * D, 2) delta_sums_kernel(DeltaArgs f, BackA
 
 // 16 columns of a head: a wave has 16 rows of every segment's map, read two segments
 // ahead (or every step waits for memory); the column passes through LDS, [m][n] in two
-// buffers. Bound by a step's chain: 1.2 us for D = 64, 2.9 for 128 (values taken apart by
-// 8 waves on one CU, a barrier, 12 products).
+// buffers, with a barrier a step that uses them: a stream's segments with tokens follow
+// one another, and steps of those without touch neither. Bound by a step's chain: 1.2 us
+// for D = 64, 2.9 for 128 (values taken apart by 8 waves on one CU, a barrier, 12 products).
 template <int D>
 struct JoinPiece {
     float map[D / 32][8], sum[4];
@@ -1206,6 +1207,10 @@ __device__ __forceinline__ void join_segments(const DeltaArgs& f, const float* s
         float* to = out + at + seg(i) * step + sum_at;
         #pragma unroll
         for (int r = 0; r < 4; r++) to[r * D] = x[r];
+        if (seg(i) * f.seg_chunks * kChunk >= live) {     // no token: x stays, and so does LDS,
+            fetch(i + 2, o);                              // which slower waves may still read
+            return;
+        }
         float* col = S[i & 1];
         *reinterpret_cast<kr_float4*>(col + l16 * LD + rows + 4 * q4) = x;
         // the map's parts, with a scale for each row
@@ -1218,7 +1223,6 @@ __device__ __forceinline__ void join_segments(const DeltaArgs& f, const float* s
         for (int s = 0; s < KS; s++) mp[s] = parts8(o.map[s], up);
         const kr_float4 add = {o.sum[0], o.sum[1], o.sum[2], o.sum[3]};
         fetch(i + 2, o);
-        if (seg(i) * f.seg_chunks * kChunk >= live) return;           // no token: as it is
         __syncthreads();
         float c[KS][8];
         big = 0.0f;
