@@ -601,7 +601,8 @@ __device__ __forceinline__ void product_tile(const ProdArgs& g, kr_half8* ring, 
     const bool direct = DW ? splits == 1 : g.dx_direct != 0;
     const int m_end = !DW && direct ? g.N : M;
     int q = 0;
-    issue(n_first, ks0, 0);
+    // a short last piece has fewer steps than dx's splits: one without steps only adds zeros
+    if (ks0 < ks1) issue(n_first, ks0, 0);
     for (int n_t = n_first; n_t < n_last; n_t++) {
         kr_float4 acc[4][TN];
         #pragma unroll

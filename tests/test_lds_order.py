@@ -15,3 +15,12 @@ def test_a_join_step_that_ends_early_leaves_lds_alone():
     writes = [m.start() for m in re.finditer(r"\(col \+|S\[i & 1\]\s*\[", step)]
     assert writes and early < barrier
     assert all(w > early for w in writes)
+
+
+def test_a_split_without_steps_copies_nothing():
+    """The loop over a split's steps is what waits for its copies: the first one is issued
+    only where a step follows, or a workgroup ends with copies to its LDS on the way."""
+    text = open(os.path.join(CSRC, "kr_headloss.hip")).read()
+    body = text[text.index("void product_tile("):text.index("grad_products_kernel(")]
+    first = [x.strip() for x in body.split("\n") if "issue(n_first, ks0, 0)" in x]
+    assert first == ["if (ks0 < ks1) issue(n_first, ks0, 0);"]
