@@ -154,7 +154,8 @@ int kr_token_scores(const void* logits, int logits_f32, int N, int V, long long 
  * gradient, whatever x, lse and dloss hold there; other ids outside 0..V-1 give
  * NaN. dz is rounded to fp16 on a scale where the largest finite |dloss| is
  * 2^14..2^15: by 2^-11 of each dz above 2^-28 of the largest |dloss|, by 2^-39 of
- * the largest |dloss| below; in dx, what that leaves of the target's dz is added back.
+ * the largest |dloss| below; what that leaves of the target's dz is added back, in dx
+ * and in dW, so that some 3e-5 to 9e-5 of their 2-norm is left, in fp32 outputs too.
  * Sums are fp32 in an order that depends on the sizes alone. ws:
  * kr_head_loss_backward_workspace_bytes (dx, dw: which of them is wanted), 256-byte
  * aligned: at most 176 MB of dz at once (256 columns at least), a copy of x and fp32

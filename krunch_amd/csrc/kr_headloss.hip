@@ -482,6 +482,7 @@ struct ProdArgs {
     void* dW;                         // [V][C] of the piece, direct: one split
     int f32;                          // their type
     int N, rows, C, V, first;         // first: dx_part is written, not added to
+    int v0;                           // the piece's first column
     int dx_splits, dw_splits, dx_direct;
     int dw_run;                       // column tiles that an item of dW takes in turn
     int dw_items, dx_items;
@@ -523,7 +524,7 @@ __device__ __forceinline__ void copy_across(const kr_half* base, long long ld, i
 }
 
 // What fp16 left of the target's dz (one value, but of most of a row's dx: 4.2e-4 of it
-// without this, 2.2e-4 with) times its row of W.
+// without this, 2.2e-4 with) times its row of W; its row of x goes into dW (TargetRows).
 struct TargetRest {
     const kr_half* w;
     float left;
@@ -549,8 +550,73 @@ __device__ __forceinline__ void store_out(void* out, size_t at, kr_float4 v, int
             kr_half4{kr_f16(v[0]), kr_f16(v[1]), kr_f16(v[2]), kr_f16(v[3])};
 }
 
+// The rows n of a range whose target is one of `columns` from v0, and what fp16 left of
+// its dz, in their order, some kHits at a time: a tile of dW takes them after its other
+// rows, 64 a step. Of dW's 2-norm the rest is 2.1e-4 on average, as the rounding of an
+// fp16 output is, and 3.9e-4 where all dloss are just above a power of two; without it
+// 6e-5 is left, the other dz's. All waves look through all rows and write the same list, so
+// that none waits for another. Measured on MI355X, gradients with / without: 8192 x 768 x 50277
+// 2069 / 2053 us, 20000 x 256 x 256 (half of all rows in every tile) 44.8 / 41.8, 97 x 1024 x
+// 50277 122.6 / 112.6 (three barriers and a step in a quarter of the tiles, which have two).
+constexpr int kHits = 1024, kLooked = 8 * 64;
+struct TargetRows {
+    int2* list;                       // n; column | fp16 rest << 16
+    int end, v0, columns;
+    int at, count;                    // the next row to look at, entries of the list
+
+    __device__ void fill(const int32_t* targets, const float* left, int lane) {
+        count = 0;
+        while (at < end && count <= kHits - kLooked) {
+            int column[8];
+            float rest[8];
+            #pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int n = min(at + 64 * j + lane, end - 1);
+                column[j] = targets[n] - v0;
+                rest[j] = left[n];
+            }
+            #pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int n = at + 64 * j + lane;
+                const bool on = n < end && (unsigned)column[j] < (unsigned)columns && rest[j] != 0.0f;
+                const uint64_t all = __ballot(on);
+                if (on)
+                    list[count + __popcll(all & ((1ull << lane) - 1))] =
+                        int2{n, column[j] | (int)__builtin_bit_cast(uint16_t, (kr_half)rest[j]) << 16};
+                count += __popcll(all);
+            }
+            at += kLooked;
+        }
+    }
+};
+
+// A stage of 64 of them: A zeros but for the rests, B their rows of x. Past the list's end
+// the last row again, against zeros.
+template <int BM, int BN, int WAVES>
+__device__ __forceinline__ void target_step(const TargetRows& r, int e0, const kr_half* x, int ldx, int cols,
+                                            kr_half8* stage, unsigned at, int tid, int wave, int lane) {
+    constexpr int PER = 512 / BN, LANES = 64 / PER, COPIES = BN / 8 / WAVES;
+    auto swap = [](int k) { return 2 * ((k & 3) | ((k >> 1) & 4)); };       // as copy_across has it
+    #pragma unroll
+    for (int i = 0; i < COPIES; i++) {
+        const int k = PER * (wave * COPIES + i) + lane / LANES;
+        const int col = 8 * ((lane % LANES) ^ swap(k));
+        const kr_half* src = x + (size_t)r.list[min(e0 + k, r.count - 1)].x * ldx + (col < cols ? col : 0);
+        kr_copy16(src, (unsigned)__builtin_amdgcn_readfirstlane((int)(at + BM * 128u + 1024u * (wave * COPIES + i))));
+    }
+    #pragma unroll
+    for (int i = 0; i < BM / 8 / WAVES; i++) stage[64 * WAVES * i + tid] = kr_half8{0, 0, 0, 0, 0, 0, 0, 0};
+    __syncthreads();
+    if (tid < 64 && e0 + tid < r.count) {
+        const int v = r.list[e0 + tid].y, column = v & 0xffff;
+        reinterpret_cast<uint16_t*>(stage + tid * (BM / 8) + ((column / 8) ^ swap(tid)))[column % 8] = (uint16_t)(v >> 16);
+    }
+    wait_copies<0>();
+    __syncthreads();
+}
+
 template <int WM, int WN, int TN, bool DW>
-__device__ __forceinline__ void product_tile(const ProdArgs& g, kr_half8* ring, int item) {
+__device__ __forceinline__ void product_tile(const ProdArgs& g, kr_half8* ring, int2* hits, int item) {
     constexpr int BM = 64 * WM, BN = 16 * TN * WN, WAVES = WM * WN;
     static_assert(BM == BN, "half of the waves copy each operand");
     constexpr int COPIES = BM / 8 / (WAVES / 2), STAGE = (BM + BN) * 8;
@@ -603,20 +669,17 @@ __device__ __forceinline__ void product_tile(const ProdArgs& g, kr_half8* ring, 
     int q = 0;
     // a short last piece has fewer steps than dx's splits: one without steps only adds zeros
     if (ks0 < ks1) issue(n_first, ks0, 0);
+    TargetRows rows{hits, min(64 * ks1, g.N), g.v0 + m0, min(BM, g.V - m0), 64 * ks0, 0};
+    if (DW) rows.fill(g.targets, g.left, lane);
     for (int n_t = n_first; n_t < n_last; n_t++) {
         kr_float4 acc[4][TN];
         #pragma unroll
         for (int i = 0; i < 4; i++)
             #pragma unroll
             for (int t = 0; t < TN; t++) acc[i][t] = kr_float4{0, 0, 0, 0};
-        #pragma unroll 1
-        for (int ks = ks0; ks < ks1; ks++, q++) {
-            wait_copies<0>();
-            __syncthreads();   // every wave's copies are in; the step before is read
-            if (ks + 1 < ks1) issue(n_t, ks + 1, q + 1);
-            else if (n_t + 1 < n_last) issue(n_t + 1, ks0, q + 1);
-            const kr_half8* As = ring + (q & 1) * STAGE;
-            const unsigned so = ring_base + (unsigned)((q & 1) * STAGE * 16);
+        auto multiply = [&](int stage) {
+            const kr_half8* As = ring + stage * STAGE;
+            const unsigned so = ring_base + (unsigned)(stage * STAGE * 16);
             #pragma unroll
             for (int kb = 0; kb < 2; kb++) {
                 kr_half8 a[4];
@@ -638,6 +701,29 @@ __device__ __forceinline__ void product_tile(const ProdArgs& g, kr_half8* ring, 
                             acc[i][4 * th + t] =
                                 __builtin_amdgcn_mfma_f32_16x16x32_f16(b[t], a[i], acc[i][4 * th + t], 0, 0, 0);
                 }
+            }
+        };
+        #pragma unroll 1
+        for (int ks = ks0; ks < ks1; ks++, q++) {
+            wait_copies<0>();
+            __syncthreads();   // every wave's copies are in; the step before is read
+            if (ks + 1 < ks1) issue(n_t, ks + 1, q + 1);
+            else if (n_t + 1 < n_last) issue(n_t + 1, ks0, q + 1);
+            multiply(q & 1);
+        }
+        if constexpr (DW) {
+            // the targets' rests, 64 rows of x a step, in the stage read last
+            const int stage = (q + 1) & 1, n0 = n_t * BN;
+            while (true) {                    // a run of column tiles has one list (dw_run)
+                #pragma unroll 1
+                for (int e0 = 0; e0 < rows.count; e0 += 64) {
+                    __syncthreads();   // the stage is read
+                    target_step<BM, BN, WAVES>(rows, e0, g.x + n0, g.C, g.C - n0, ring + stage * STAGE,
+                                               ring_base + (unsigned)(stage * STAGE * 16), tid, wave, lane);
+                    multiply(stage);
+                }
+                if (rows.at >= rows.end) break;
+                rows.fill(g.targets, g.left, lane);
             }
         }
         #pragma unroll
@@ -683,10 +769,11 @@ __device__ __forceinline__ int item_of(int b, int items) {
 template <int WM, int WN, int TN>
 __global__ void __launch_bounds__(64 * WM * WN, WM * WN >= 8 ? 1 : 2) grad_products_kernel(ProdArgs g) {
     __shared__ __attribute__((aligned(1024))) kr_half8 ring[2 * (64 * WM + 16 * TN * WN) * 8];
+    __shared__ int2 hits[kHits];
     // dW's items before dx's
     const int b = blockIdx.x;
-    if (b < g.dw_items) product_tile<WM, WN, TN, true>(g, ring, item_of(b, g.dw_items));
-    else product_tile<WM, WN, TN, false>(g, ring, item_of(b - g.dw_items, g.dx_items));
+    if (b < g.dw_items) product_tile<WM, WN, TN, true>(g, ring, hits, item_of(b, g.dw_items));
+    else product_tile<WM, WN, TN, false>(g, ring, hits, item_of(b - g.dw_items, g.dx_items));
 }
 
 // Sum of the splits of n outputs, in their order; of dx (W not null), with the targets' rest.
@@ -782,7 +869,7 @@ GradPlan grad_plan(int N, int C, int V, bool dx, bool dw) {
     const long long each = std::max<long long>(8, total / (3 * slots));
     p.dx_splits = (int)std::max<long long>(1, std::min<long long>(64, dx_steps / each));
     p.dw_splits = dw_tiles >= slots / 4 ? 1 : (int)std::max<long long>(1, std::min<long long>(64, dw_steps / each));
-    p.dw_run = dw_steps <= 8 && p.dw_splits == 1 ? gx : 1;
+    p.dw_run = 64 * dw_steps <= kLooked && p.dw_splits == 1 ? gx : 1;
     p.dx_direct = p.dx_splits == 1 && p.pieces == 1;
     size_t at = 256;                                  // the scale
     p.left = at;
@@ -922,7 +1009,7 @@ int kr_head_loss_backward(const uint16_t* x, long long ldx, int N, int C, const 
         const int v0 = i * p.piece, nv = std::min(V - v0, p.piece);
         g.W = d.W = reinterpret_cast<const kr_half*>(W) + (size_t)v0 * ldw;
         g.V = d.V = nv;
-        g.v0 = v0;
+        g.v0 = d.v0 = v0;
         const int rc = logits<true>(g, p.big, s);
         if (rc != KR_OK) return rc;
         d.first = i == 0;

@@ -288,7 +288,8 @@ def head_loss_backward(x, W, targets, lse, dloss, out_dtype=None, dx: bool = Tru
     (the gradient of each loss) -> (dx [N, C], dW [V, C]), fp16 or fp32 by
     out_dtype, None for one that is not wanted. Rows with target -1 or dloss 0 have
     no gradient. The gradient of the logits is rounded to fp16 relative to the
-    largest |dloss|; sums are fp32. For fp16 outputs dloss may carry a loss scale."""
+    largest |dloss|, but for the target's; sums are fp32. For fp16 outputs dloss may
+    carry a loss scale."""
     N, C, V, ldx, ldw = _head_shapes(x, W, targets)
     dev = x.get_device()
     _head_vector(lse, torch.float32, "lse", N, dev)
