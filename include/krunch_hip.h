@@ -152,14 +152,15 @@ int kr_token_scores(const void* logits, int logits_f32, int N, int V, long long 
  *   dx = dz W [N, C],  dW = dz' x [V, C], contiguous, 16-byte aligned, fp16 or
  * (out_f32) fp32; dx or dW may be NULL. Rows with target -1 or dloss 0 have no
  * gradient, whatever x, lse and dloss hold there; other ids outside 0..V-1 give
- * NaN. dz is rounded to fp16 on a scale where the largest finite |dloss| is
- * 2^14..2^15: by 2^-11 of each dz above 2^-28 of the largest |dloss|, by 2^-39 of
- * the largest |dloss| below; what that leaves of the target's dz is added back, in dx
- * and in dW, so that some 3e-5 to 9e-5 of their 2-norm is left, in fp32 outputs too.
+ * NaN. For fp16 outputs dz is rounded to fp16 on a scale where the largest finite
+ * |dloss| is 2^14..2^15: by 2^-11 of each dz above 2^-28 of the largest |dloss|, by
+ * 2^-39 of the largest |dloss| below; what that leaves of the target's dz is added
+ * back, in dx and in dW. For fp32 outputs dz has a second such part: 2^-22 of each, and
+ * products of twice the length.
  * Sums are fp32 in an order that depends on the sizes alone. ws:
  * kr_head_loss_backward_workspace_bytes (dx, dw: which of them is wanted), 256-byte
- * aligned: at most 176 MB of dz at once (256 columns at least), a copy of x and fp32
- * partial sums. Outputs must not overlap inputs. */
+ * aligned, enough for both output types: at most 176 MB of dz at once (256 columns at
+ * least), a copy of x and fp32 partial sums. Outputs must not overlap inputs. */
 size_t kr_head_loss_workspace_bytes(int N, int C, int V);
 int kr_head_loss(const uint16_t* x, long long ldx, int N, int C, const uint16_t* W, long long ldw, int V,
                  const int32_t* targets, float* loss, float* lse, void* ws, size_t ws_bytes, void* stream);

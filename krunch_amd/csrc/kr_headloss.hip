@@ -12,7 +12,11 @@
 //
 // dz enters the matrix units as fp16 (11 bits, as x and W have): it is kept times a
 // power of two that brings the largest |dloss| to 2^14..2^15, so that
-// probabilities down to 2^-28 of that keep all their bits. Sums are fp32.
+// probabilities down to 2^-28 of that keep all their bits; what is left of a target's is
+// added back, and an fp16 output's own rounding is nearly all of its error. For fp32
+// outputs dz is kept in two such parts, 22 bits (7e-7 of dx and dW in 2-norm; with one part
+// 3e-5 and 6e-5), and the products have twice the steps: 8192 x 768 x 50277 3,665 us,
+// fp16 2,070. Sums are fp32.
 #include <algorithm>
 
 #include "kr_common.h"
@@ -37,6 +41,7 @@ struct LossArgs {
     float2* part;                     // LOSS: [parts][N] maximum, sum
     float* hit;                       // LOSS: [N] the target's z
     kr_half* G;                       // GRAD: [rows][ldg] dz of the piece
+    kr_half* G_low;                   // GRAD: what fp16 leaves of them (null: not kept)
     long long ldg;
     float* left;                      // GRAD: [N] what fp16 leaves of the target's dz
     int N, C, V;                      // V: the piece's columns
@@ -243,17 +248,25 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN >= 8 ? 1 : 2) logits_ker
                         for (int e = 0; e < 8; e++)
                             if (d == 32 * p + e) {
                                 x[e] -= f;
-                                g.left[m] = f == 0.0f ? 0.0f : x[e] - (float)(kr_half)x[e];
+                                g.left[m] = f == 0.0f || g.G_low ? 0.0f : x[e] - (float)(kr_half)x[e];
                             }
-                    kr_half8 v;
-                    #pragma unroll
-                    for (int e = 0; e < 8; e++) v[e] = (kr_half)x[e];
                     if (!whole)
                         #pragma unroll
                         for (int e = 0; e < 8; e++)
-                            if (c0 + 32 * p + e >= g.V) v[e] = 0;
-                    if (f == 0.0f) v = kr_half8{0, 0, 0, 0, 0, 0, 0, 0};
-                    if (m < g.rows && c0 + 32 * p < (int)g.ldg) *reinterpret_cast<kr_half8*>(out + 32 * p) = v;
+                            if (c0 + 32 * p + e >= g.V) x[e] = 0.0f;
+                    if (f == 0.0f)
+                        #pragma unroll
+                        for (int e = 0; e < 8; e++) x[e] = 0.0f;
+                    kr_half8 v;
+                    #pragma unroll
+                    for (int e = 0; e < 8; e++) v[e] = (kr_half)x[e];
+                    const bool on = m < g.rows && c0 + 32 * p < (int)g.ldg;
+                    if (on) *reinterpret_cast<kr_half8*>(out + 32 * p) = v;
+                    if (on && g.G_low) {
+                        #pragma unroll
+                        for (int e = 0; e < 8; e++) v[e] = (kr_half)(x[e] - (float)v[e]);
+                        *reinterpret_cast<kr_half8*>(g.G_low + (out - g.G) + 32 * p) = v;
+                    }
                 }
             }
         }
@@ -468,6 +481,7 @@ __global__ void __launch_bounds__(1024) grad_prepare_kernel(const kr_half* x, lo
 struct ProdArgs {
     const kr_half* G;                 // [rows][ldg]
     long long ldg;
+    int parts;                        // 2: and what fp16 left of it, behind
     const kr_half* x;                 // [rows][C]
     const kr_half* W;                 // [V, C] of the piece
     long long ldw;
@@ -630,7 +644,8 @@ __device__ __forceinline__ void product_tile(const ProdArgs& g, kr_half8* ring, 
     const int n_first = item % runs * (DW ? g.dw_run : 1), n_last = DW ? min(n_first + g.dw_run, gx) : n_first + 1;
     const int m_t = item / runs / splits, split = item / runs % splits;
     const int M = DW ? g.V : g.rows;
-    const int steps = DW ? g.rows / 64 : (g.V + 63) / 64;
+    const int more = g.parts - 1;         // a second step for every 64 k, with the low parts
+    const int steps = (DW ? g.rows / 64 : (g.V + 63) / 64) << more;
     const int ks0 = (int)((long long)steps * split / splits), ks1 = (int)((long long)steps * (split + 1) / splits);
     const unsigned ring_base = lds_address(ring);
     const int m0 = m_t * BM;
@@ -638,15 +653,16 @@ __device__ __forceinline__ void product_tile(const ProdArgs& g, kr_half8* ring, 
     const kr_half* a_base = DW ? g.G + m0 : g.G + (size_t)m0 * g.ldg;
     const kr_half* b_base = DW ? g.x : g.W;
     const long long ldb = DW ? g.C : g.ldw;
-    auto issue = [&](int n_t, int ks, int q) {
+    auto issue = [&](int n_t, int step, int q) {
         const unsigned so = ring_base + (unsigned)((q & 1) * STAGE * 16);
-        const int n0 = n_t * BN;
+        const int n0 = n_t * BN, ks = step >> more;
+        const kr_half* a = a_base + (step & more ? (size_t)g.rows * g.ldg : 0);
         if (wave >= WAVES / 2) {
             // B's k past the piece: the last row, against zeros of G
             copy_across<BN, COPIES>(b_base + n0 + (long long)ks * 64 * ldb, ldb, DW ? 63 : g.V - 1 - 64 * ks, g.C - n0,
                                     so + BM * 128, wave - WAVES / 2, lane);
         } else if (DW) {
-            copy_across<BM, COPIES>(a_base + (long long)ks * 64 * g.ldg, g.ldg, 63, (int)g.ldg - m0, so, wave, lane);
+            copy_across<BM, COPIES>(a + (long long)ks * 64 * g.ldg, g.ldg, 63, (int)g.ldg - m0, so, wave, lane);
         } else {
             #pragma unroll
             for (int i = 0; i < COPIES; i++) {
@@ -654,7 +670,7 @@ __device__ __forceinline__ void product_tile(const ProdArgs& g, kr_half8* ring, 
                 const int kc = (lane & 7) ^ ((row >> 1) & 7);
                 const unsigned off = (unsigned)min(row, M - 1 - m0) * (unsigned)(2 * g.ldg) +
                                      (unsigned)(16 * kc + 128 * ks);
-                copy16(a_base, off, so + 1024u * (unsigned)(wave * COPIES + i));
+                copy16(a, off, so + 1024u * (unsigned)(wave * COPIES + i));
             }
         }
     };
@@ -669,7 +685,8 @@ __device__ __forceinline__ void product_tile(const ProdArgs& g, kr_half8* ring, 
     int q = 0;
     // a short last piece has fewer steps than dx's splits: one without steps only adds zeros
     if (ks0 < ks1) issue(n_first, ks0, 0);
-    TargetRows rows{hits, min(64 * ks1, g.N), g.v0 + m0, min(BM, g.V - m0), 64 * ks0, 0};
+    // with low parts nothing is left of the targets' dz
+    TargetRows rows{hits, more ? 0 : min(64 * ks1, g.N), g.v0 + m0, min(BM, g.V - m0), 64 * ks0, 0};
     if (DW) rows.fill(g.targets, g.left, lane);
     for (int n_t = n_first; n_t < n_last; n_t++) {
         kr_float4 acc[4][TN];
@@ -850,10 +867,10 @@ struct GradPlan {
     size_t left, x, G, dx_part, dw_part, total;             // offsets in the workspace
 };
 
-GradPlan grad_plan(int N, int C, int V, bool dx, bool dw) {
+GradPlan grad_plan(int N, int C, int V, bool dx, bool dw, int parts) {
     GradPlan p{};
     p.rows = (N + 63) / 64 * 64;
-    const long long most = std::max<long long>(256, (88ll << 20) / p.rows / 256 * 256);
+    const long long most = std::max<long long>(256, (88ll << 20) / parts / p.rows / 256 * 256);
     p.pieces = (int)((V + most - 1) / most);
     p.piece = ((V + p.pieces - 1) / p.pieces + 255) / 256 * 256;
     p.pieces = (V + p.piece - 1) / p.piece;
@@ -863,13 +880,13 @@ GradPlan grad_plan(int N, int C, int V, bool dx, bool dw) {
     // a piece) 1410 / 1666, 4096 x 1024 x 4096 (64) 134 / 167
     p.big_products = p.big && C > 512 && (p.piece / 256) * ((C + 255) / 256) >= 100;
     const int tile = p.big_products ? 256 : 128, slots = p.big_products ? 256 : 512;
-    const int gx = (C + tile - 1) / tile, dx_steps = p.piece / 64, dw_steps = p.rows / 64;
+    const int gx = (C + tile - 1) / tile, dx_steps = p.piece / 64 * parts, dw_steps = p.rows / 64 * parts;
     const long long dx_tiles = (long long)(p.rows + tile - 1) / tile * gx, dw_tiles = (long long)p.piece / tile * gx;
     const long long total = (dx ? dx_tiles * dx_steps : 0) + (dw ? dw_tiles * dw_steps : 0);
     const long long each = std::max<long long>(8, total / (3 * slots));
     p.dx_splits = (int)std::max<long long>(1, std::min<long long>(64, dx_steps / each));
     p.dw_splits = dw_tiles >= slots / 4 ? 1 : (int)std::max<long long>(1, std::min<long long>(64, dw_steps / each));
-    p.dw_run = 64 * dw_steps <= kLooked && p.dw_splits == 1 ? gx : 1;
+    p.dw_run = p.rows <= kLooked && p.dw_splits == 1 ? gx : 1;
     p.dx_direct = p.dx_splits == 1 && p.pieces == 1;
     size_t at = 256;                                  // the scale
     p.left = at;
@@ -877,7 +894,7 @@ GradPlan grad_plan(int N, int C, int V, bool dx, bool dw) {
     p.x = at;
     at += up256((size_t)p.rows * C * 2);
     p.G = at;
-    at += up256((size_t)p.rows * p.piece * 2);
+    at += up256((size_t)p.rows * p.piece * 2 * parts);
     p.dx_part = at;
     if (dx && !p.dx_direct) at += up256((size_t)p.dx_splits * p.rows * C * 4);
     p.dw_part = at;
@@ -941,7 +958,7 @@ int kr_head_loss(const uint16_t* x, long long ldx, int N, int C, const uint16_t*
 
 size_t kr_head_loss_backward_workspace_bytes(int N, int C, int V, int dx, int dw) {
     if (!shape_ok(N, C, V) || N == 0) return 0;
-    return grad_plan(N, C, V, dx != 0, dw != 0).total;
+    return std::max(grad_plan(N, C, V, dx != 0, dw != 0, 1).total, grad_plan(N, C, V, dx != 0, dw != 0, 2).total);
 }
 
 int kr_head_loss_backward(const uint16_t* x, long long ldx, int N, int C, const uint16_t* W, long long ldw, int V,
@@ -956,9 +973,11 @@ int kr_head_loss_backward(const uint16_t* x, long long ldx, int N, int C, const 
     KR_REQUIRE(x && W && targets && lse && dloss && (dx || dW), "kr_head_loss_backward: null pointer");
     KR_REQUIRE((((uintptr_t)x | (uintptr_t)W | (uintptr_t)dx | (uintptr_t)dW) & 15) == 0,
                "kr_head_loss_backward: x, W, dx and dW must be 16-byte aligned");
-    const GradPlan p = grad_plan(N, C, V, dx != nullptr, dW != nullptr);
-    KR_REQUIRE(ws && ws_bytes >= p.total && ((uintptr_t)ws & 255) == 0,
-               "kr_head_loss_backward: workspace of %zu bytes, %zu needed (256-byte aligned)", ws_bytes, p.total);
+    const int parts = out_f32 ? 2 : 1;
+    const GradPlan p = grad_plan(N, C, V, dx != nullptr, dW != nullptr, parts);
+    const size_t need = kr_head_loss_backward_workspace_bytes(N, C, V, dx != nullptr, dW != nullptr);
+    KR_REQUIRE(ws && ws_bytes >= need && ((uintptr_t)ws & 255) == 0,
+               "kr_head_loss_backward: workspace of %zu bytes, %zu needed (256-byte aligned)", ws_bytes, need);
     char* base = static_cast<char*>(ws);
     float* scale = reinterpret_cast<float*>(base);
     kr_half* live = reinterpret_cast<kr_half*>(base + p.x);
@@ -977,6 +996,7 @@ int kr_head_loss_backward(const uint16_t* x, long long ldx, int N, int C, const 
     g.dloss = dloss;
     g.scale = scale;
     g.G = reinterpret_cast<kr_half*>(base + p.G);
+    g.G_low = parts == 2 ? g.G + (size_t)p.rows * p.piece : nullptr;
     g.left = reinterpret_cast<float*>(base + p.left);
     g.ldg = p.piece;
     g.N = N;
@@ -986,6 +1006,7 @@ int kr_head_loss_backward(const uint16_t* x, long long ldx, int N, int C, const 
     ProdArgs d{};
     d.G = g.G;
     d.ldg = g.ldg;
+    d.parts = parts;
     d.x = live;
     d.W_all = g.W = reinterpret_cast<const kr_half*>(W);
     d.targets = targets;

@@ -287,9 +287,9 @@ def head_loss_backward(x, W, targets, lse, dloss, out_dtype=None, dx: bool = Tru
     """Gradients of head_loss: x, W, targets as there, its lse, and dloss fp32 [N]
     (the gradient of each loss) -> (dx [N, C], dW [V, C]), fp16 or fp32 by
     out_dtype, None for one that is not wanted. Rows with target -1 or dloss 0 have
-    no gradient. The gradient of the logits is rounded to fp16 relative to the
-    largest |dloss|, but for the target's; sums are fp32. For fp16 outputs dloss may
-    carry a loss scale."""
+    no gradient. For fp16 outputs the gradient of the logits is rounded to fp16 relative
+    to the largest |dloss|, but for the target's, and dloss may carry a loss scale; for
+    fp32 outputs it keeps 22 bits (the products take twice as long). Sums are fp32."""
     N, C, V, ldx, ldw = _head_shapes(x, W, targets)
     dev = x.get_device()
     _head_vector(lse, torch.float32, "lse", N, dev)

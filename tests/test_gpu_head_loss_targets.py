@@ -1,7 +1,8 @@
-"""dW of the rows that are targets (kr_head_loss_backward): what fp16 leaves of a target's
-dz, of most of such a row, is added back, in float32 outputs to be seen apart from the
-outputs' own rounding. Against float64: one row of x for a row of W, many for one, lists
-longer than a workgroup holds, byte vocabularies, several column tiles, pieces."""
+"""dW of the rows that are targets (kr_head_loss_backward, fp16 outputs): what fp16 leaves of
+a target's dz, of most of such a row, is added back, so that the output's own rounding, at
+most half a step of it, is nearly all of the error. Against float64: one row of x for a
+row of W, many for one, lists longer than a workgroup holds, byte vocabularies, several
+column tiles, pieces."""
 import pytest
 import torch
 
@@ -37,12 +38,12 @@ def plain(x, W, t, w):
 
 def check(x, W, t, w):
     lse = ops.head_loss(x, W, t)[1]
-    _, dW = ops.head_loss_backward(x, W, t, lse, w, torch.float32)
+    _, dW = ops.head_loss_backward(x, W, t, lse, w)
     want, err = plain(x, W, t, w)
     off = (dW.double() - want).abs()
-    assert (off <= err).all(), (off / err).max()
-    half = ops.head_loss_backward(x, W, t, lse, w)[1]
-    assert torch.equal(half, dW.half())
+    # half a step of fp16 where the value before its rounding may be
+    half_step = torch.exp2(torch.floor(torch.log2(want.abs() + err)).clamp_min(-14) - 11)
+    assert (off <= half_step + err).all(), (off / (half_step + err)).max()
     return dW
 
 
@@ -82,4 +83,4 @@ def test_rows_that_hold_anything_reach_no_target():
     x[::3] = float("nan")
     lse = ops.head_loss(x, W, t)[1]
     w[::3] = 0
-    assert torch.equal(ops.head_loss_backward(x, W, t, lse, w, torch.float32)[1], want)
+    assert torch.equal(ops.head_loss_backward(x, W, t, lse, w)[1], want)
