@@ -211,10 +211,19 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN >= 8 ? 1 : 2) logits_ker
                     for (int r = 0; r < 4; r++) big = fmaxf(big, acc[i][t][r]);
                 big = fmaxf(big, kr_xor<16>(big));
                 big = fmaxf(big, kr_xor<32>(big));
-                // e^(z - big) as 2^(z log2 e - c); the rounding of c is taken back from the sum
+                // e^(z - big) as 2^(z log2 e - c); the rounding of c is taken back from the sum,
+                // or, where it may be more than 1, there is none: z - big, then the product
                 const float base = big == -INFINITY ? 0.0f : big;
-                const float c = base * kLog2e;
-                const float back = __builtin_amdgcn_exp2f(__builtin_fmaf(-base, kLog2e, c));
+                float c = base * kLog2e;
+                float back = __builtin_amdgcn_exp2f(__builtin_fmaf(-base, kLog2e, c));
+                if (fabsf(c) > 0x1p24f) {
+                    #pragma unroll
+                    for (int t = 0; t < TN; t++)
+                        #pragma unroll
+                        for (int r = 0; r < 4; r++) acc[i][t][r] -= base;
+                    c = 0.0f;
+                    back = 1.0f;
+                }
                 float sum = 0.0f;
                 #pragma unroll
                 for (int t = 0; t < TN; t++) {
