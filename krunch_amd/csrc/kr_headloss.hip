@@ -238,11 +238,19 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN >= 8 ? 1 : 2) logits_ker
                 if (m < g.N && lq == 0 && first < g.V)
                     g.part[(size_t)(n_t * WN + wn) * g.N + m] = float2{big, sum * back};
             } else {
-                // f e^(z - lse) as 2^(z log2 e - c) with f's sign set behind it
+                // f e^(z - lse) as 2^(z log2 e - c) with f's sign set behind it; beside a large
+                // lse c's rounding would show (3e-4 of f at 8000): z - lse first
                 float f = 0.0f, c = 0.0f;
                 if (target != -1 && m < g.N) {
                     f = (unsigned)target < (unsigned)g.v_all ? g.dloss[m] * g.scale[0] : NAN;
-                    c = g.lse[m] * kLog2e - __builtin_amdgcn_logf(fabsf(f));
+                    const float lse = g.lse[m];
+                    const bool first = fabsf(lse) > 32.0f;
+                    c = (first ? 0.0f : lse * kLog2e) - __builtin_amdgcn_logf(fabsf(f));
+                    if (first)
+                        #pragma unroll
+                        for (int t = 0; t < TN; t++)
+                            #pragma unroll
+                            for (int r = 0; r < 4; r++) acc[i][t][r] -= lse;
                 }
                 const float sign = f < 0.0f ? -1.0f : 1.0f;
                 kr_half* out = g.G + (size_t)m * g.ldg + c0;
