@@ -156,11 +156,11 @@ int kr_token_scores(const void* logits, int logits_f32, int N, int V, long long 
  * |dloss| is 2^14..2^15: by 2^-11 of each dz above 2^-28 of the largest |dloss|, by
  * 2^-39 of the largest |dloss| below; what that leaves of the target's dz is added
  * back, in dx and in dW. For fp32 outputs dz has a second such part: 2^-22 of each, and
- * products of twice the length.
- * Sums are fp32 in an order that depends on the sizes alone. ws:
- * kr_head_loss_backward_workspace_bytes (dx, dw: which of them is wanted), 256-byte
- * aligned, enough for both output types: at most 176 MB of dz at once (256 columns at
- * least), a copy of x and fp32 partial sums. Outputs must not overlap inputs. */
+ * products of twice the length. Sums are fp32 in an order that depends on the sizes and
+ * the output type alone. N C and V C are at most 2^33. ws:
+ * kr_head_loss_backward_workspace_bytes (dx, dw: which of them is wanted; enough for both
+ * output types), 256-byte aligned: at most 176 MB of dz at once (256 columns at least), a
+ * copy of x and fp32 partial sums. Outputs must not overlap inputs. */
 size_t kr_head_loss_workspace_bytes(int N, int C, int V);
 int kr_head_loss(const uint16_t* x, long long ldx, int N, int C, const uint16_t* W, long long ldw, int V,
                  const int32_t* targets, float* loss, float* lse, void* ws, size_t ws_bytes, void* stream);

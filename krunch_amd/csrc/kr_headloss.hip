@@ -872,6 +872,11 @@ bool shape_ok(int N, int C, int V) {
     return N >= 0 && N <= 1 << 24 && C >= 64 && C % 64 == 0 && C <= 1 << 14 && V >= 1 && V <= 1 << 24 &&
            (long long)N * V <= 1ll << 44;             // a launch's tiles stay below 2^31
 }
+// Backward, also what a thread for four values of dx or dW (and one for eight of x) can be
+// launched for, 2^32.
+bool grad_shape_ok(int N, int C, int V) {
+    return shape_ok(N, C, V) && (long long)N * C <= 1ll << 33 && (long long)V * C <= 1ll << 33;
+}
 constexpr int kLossRows = 1 << 16;                    // of a forward launch: bounds its parts
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
@@ -974,15 +979,15 @@ int kr_head_loss(const uint16_t* x, long long ldx, int N, int C, const uint16_t*
 }
 
 size_t kr_head_loss_backward_workspace_bytes(int N, int C, int V, int dx, int dw) {
-    if (!shape_ok(N, C, V) || N == 0) return 0;
+    if (!grad_shape_ok(N, C, V) || N == 0) return 0;
     return std::max(grad_plan(N, C, V, dx != 0, dw != 0, 1).total, grad_plan(N, C, V, dx != 0, dw != 0, 2).total);
 }
 
 int kr_head_loss_backward(const uint16_t* x, long long ldx, int N, int C, const uint16_t* W, long long ldw, int V,
                           const int32_t* targets, const float* lse, const float* dloss, int out_f32, void* dx,
                           void* dW, void* ws, size_t ws_bytes, void* stream) {
-    KR_REQUIRE(shape_ok(N, C, V),
-               "kr_head_loss_backward: bad shape N=%d C=%d V=%d (C a multiple of 64 up to 16384, N and V up to 2^24, N * V up to 2^44)",
+    KR_REQUIRE(grad_shape_ok(N, C, V),
+               "kr_head_loss_backward: bad shape N=%d C=%d V=%d (C a multiple of 64 up to 16384, N and V up to 2^24, N * V up to 2^44, N * C and V * C up to 2^33)",
                N, C, V);
     KR_REQUIRE(N >= 1, "kr_head_loss_backward: no rows");
     KR_REQUIRE(ldx >= C && ldw >= C && (ldx | ldw) % 8 == 0 && (ldx | ldw) < 1 << 21,
