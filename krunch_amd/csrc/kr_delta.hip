@@ -1207,12 +1207,10 @@ __device__ __forceinline__ void join_segments(const DeltaArgs& f, const float* s
         float* to = out + at + seg(i) * step + sum_at;
         #pragma unroll
         for (int r = 0; r < 4; r++) to[r * D] = x[r];
-        if (seg(i) * f.seg_chunks * kChunk >= live) {     // no token: x stays, and so does LDS,
-            fetch(i + 2, o);                              // which slower waves may still read
-            return;
-        }
+        // no token: x stays, and so does LDS, which slower waves may still read
+        const bool tokens = seg(i) * f.seg_chunks * kChunk < live;
         float* col = S[i & 1];
-        *reinterpret_cast<kr_float4*>(col + l16 * LD + rows + 4 * q4) = x;
+        if (tokens) *reinterpret_cast<kr_float4*>(col + l16 * LD + rows + 4 * q4) = x;
         // the map's parts, with a scale for each row
         Parts8 mp[KS];
         float big = 0.0f, up, m_down, x_down;
@@ -1223,6 +1221,7 @@ __device__ __forceinline__ void join_segments(const DeltaArgs& f, const float* s
         for (int s = 0; s < KS; s++) mp[s] = parts8(o.map[s], up);
         const kr_float4 add = {o.sum[0], o.sum[1], o.sum[2], o.sum[3]};
         fetch(i + 2, o);
+        if (!tokens) return;
         __syncthreads();
         float c[KS][8];
         big = 0.0f;

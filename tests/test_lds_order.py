@@ -6,15 +6,16 @@ CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
 
 
 def test_a_join_step_that_ends_early_leaves_lds_alone():
-    """A step of delta_join_kernel that returns before its barrier has not written the
-    column's buffer, which a slower wave may still read from the step two before."""
+    """A step of delta_join_kernel that returns before its barrier, as one without tokens
+    does, has not written the column's buffer, which a slower wave may still read from the
+    step two before."""
     text = open(os.path.join(CSRC, "kr_delta.hip")).read()
     step = text[text.index("auto take = [&]"):]
     step = step[:step.index("\n    };")]
-    early, barrier = step.index("return;"), step.index("__syncthreads()")
-    writes = [m.start() for m in re.finditer(r"\(col \+|S\[i & 1\]\s*\[", step)]
-    assert writes and early < barrier
-    assert all(w > early for w in writes)
+    early, barrier = step.index("if (!tokens) return;"), step.index("__syncthreads()")
+    writes = [x.strip() for x in step[:barrier].split("\n") if re.search(r"\(col \+|S\[i & 1\]\s*\[", x)]
+    assert early < barrier and writes
+    assert all(x.startswith("if (tokens) ") for x in writes)
 
 
 def test_a_split_without_steps_copies_nothing():
