@@ -465,11 +465,11 @@ int kr_wkv_heads(int B, int T, int H, int D, const uint16_t* r, long long ldr, c
  * (2^-22 of a value that enters the matrix units: a state element, a weight between two
  * tokens, what a token writes; and 2^-38 of the largest one of its column or row), in
  * an order that depends on B * H and T (the time axis is split over workgroups where
- * heads are few); a NaN or infinity of a token then also reaches y of up to 63 tokens before it. Calls of
- * at most 8 tokens are the same in both. Keys of length 1 and beta in 0..1 keep the
- * recurrence stable; others are computed, too. y must not overlap q, k or v. ws:
- * kr_gated_delta_workspace_bytes (chunked only, may be 0), 16-byte aligned, as q, k, v,
- * state and y. */
+ * heads are few); a NaN or infinity of a token then also reaches y of up to 63 tokens
+ * before it. Calls of at most 8 tokens are the same in both. Keys of length 1 and beta in
+ * 0..1 keep the recurrence stable; others are computed, too. y must not overlap q, k or
+ * v. ws: kr_gated_delta_workspace_bytes (chunked only: 12 D D bytes for each head and
+ * segment of a split, else 0), 16-byte aligned, as q, k, v, state and y. */
 size_t kr_gated_delta_workspace_bytes(int B, int T, int H, int D);
 int kr_gated_delta(int B, int T, int H, int D, const uint16_t* q, long long ldq, const uint16_t* k,
                    long long ldk, const uint16_t* v, long long ldv, const float* log_decay, long long ldg,
@@ -485,8 +485,9 @@ int kr_gated_delta(int B, int T, int H, int D, const uint16_t* q, long long ldq,
  * sums over a chunk's tokens, so its error is relative to those, not to a small
  * gradient behind a strong decay. T <= 4194240. ws:
  * kr_gated_delta_backward_workspace_bytes (for each head and 64 tokens two states and two
- * rows of D fp32 values a token: 8 D (D + 64) bytes), 256-byte aligned; it must not
- * overlap anything, nor outputs the inputs. Everything but log_decay, beta, lens and
+ * rows of D fp32 values a token, 8 D (D + 64) bytes; for each head one state more, and
+ * where the time axis is split five a segment, 20 D D bytes), 256-byte aligned; it must
+ * not overlap anything, nor outputs the inputs. Everything but log_decay, beta, lens and
  * their gradients is 16-byte aligned. */
 size_t kr_gated_delta_backward_workspace_bytes(int B, int T, int H, int D);
 int kr_gated_delta_backward(int B, int T, int H, int D, const uint16_t* q, long long ldq, const uint16_t* k,

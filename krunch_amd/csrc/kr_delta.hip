@@ -1151,9 +1151,9 @@ __global__ void __launch_bounds__(4 * D, 2) delta_both_kernel(DeltaArgs f, BackA
 // computed for all segments at once, the states at their starts follow one from
 // the other, and then all segments run. Backward, D -> map' D + sum.
 // z of the sums' launch: 0 sums, 1 maps, 2 D's sums; of the states': 0 forward, 1 back.
-// Three times the work, side by side: 1 x 1777 x 8 heads of 128 274 -> 78 us (14 segments:
-// sums 20, join 38, walk 24), gradients of 1 x 2000 x 12 of 64 394 -> 84 (29, 12, 29, and
-// 22 for the chunks' gradients).
+// Three times the work, side by side: 1 x 1777 x 8 heads of 128 274 -> 77 us (14 segments:
+// sums 19, join 36, walk 24), gradients of 1 x 2000 x 12 of 64 394 -> 83 (28, 12, 28, and
+// 21 for the chunks' gradients).
 // ---------------------------------------------------------------------------
 template <int D>
 __global__ void __launch_bounds__(4 * D, 2) delta_sums_kernel(DeltaArgs f, BackArgs g) {

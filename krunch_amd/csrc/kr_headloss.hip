@@ -93,11 +93,11 @@ __device__ __forceinline__ bool tile_of(int gy, int gx, int vb, int group_m, int
 // order that makes them 8 consecutive columns over two of its tiles.
 // Bound, at 256 x 256: the copies, one step ahead (a step takes 4,400 cycles, its matrix
 // instructions 2,050, LDS reads 770), and the epilogue that nothing overlaps (an
-// exponential each). Measured on MI355X, 8192 x 768 x 50277: losses 577 us
-// (1.10 PF/s; a library's product of the same sizes 703, 8192^3 at 1.16), dz 155 us for
+// exponential each). Measured on MI355X, 8192 x 768 x 50277: losses 580 us
+// (1.09 PF/s; a library's product of the same sizes 703, 8192^3 at 1.16), dz 156 us for
 // 10240 columns (0.83 PF/s, 168 MB stored). A bank conflict in every read of W cost 40 us of
 // the losses, a cursor over tiles that allows more stages 25. At 128 x 128, two workgroups
-// a CU: 30001 x 512 x 256 15 us, of which 6 are its 31 MB (64 x 256 tiles 16, 64 x 128
+// a CU: 30001 x 512 x 256 15.5 us, of which 6 are its 31 MB (64 x 256 tiles 16, 64 x 128
 // 23, 128 x 64 25).
 // ---------------------------------------------------------------------------
 template <int N>
@@ -298,7 +298,10 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN >= 8 ? 1 : 2) logits_ker
 // The forward pass of up to 16 rows: bound by W. Every wave walks 16-row blocks of W
 // through an LDS ring of its own (steps of 64 k, whole lines, no barriers, 80 KB a CU in
 // flight) beside x in LDS, and keeps a maximum and a sum per row. Measured on MI355X:
-// 1 x 768 x 50277 18.0 us with the join's 4 (77 MB: 15.1 at a copy's rate); the tile kernel 34.
+// 1 x 768 x 50277 17.7 us with the join's 4 (77 MB: 15.1 at a copy's rate). Limits: rows of
+// one matrix instruction, and x in LDS. us, this kernel / the tiles: 1 x 768 x 50277 18.4 /
+// 19.5, 8 rows 18.9 / 20.3, 16 19.4 / 21.0, of width 256 13.8 / 14.1, of 1536 33 / 31; over 4096
+// columns 1 row 13.8 / 14.9, 16 14.0 / 14.8.
 // ---------------------------------------------------------------------------
 constexpr int kFewRows = 16, kFewC = 1536, kFewWaves = 8, kFewStages = 6;
 
@@ -491,9 +494,12 @@ __global__ void __launch_bounds__(1024) grad_prepare_kernel(const kr_half* x, lo
 // read by the LDS's transposing reads: 16 lanes get 4 k of 16 columns.
 // Bound: copies (one step ahead) and the last round of workgroups: dW's tiles of a piece
 // take all N rows each, dx's splits fill up behind them. Measured on MI355X, a piece of
-// 10240 columns of 8192 x 768 x 50277: 282 us for both products (0.90 PF/s; a library's of
-// these sizes 0.77 dW, 1.04 dx); steps of 32 k, three ahead, 292. Pieces: dz of 176 MB at most stays in the memory-side
-// cache; 224, 288 and 420 MB 2045, 2062 and 1937 us for the call, 176 2037.
+// 10240 columns of 8192 x 768 x 50277: 283 us for both products (0.90 PF/s; a library's of
+// these sizes 0.77 dW, 1.04 dx); steps of 32 k, three ahead, 292. Pieces: a call's workspace
+// is what keeps dz at 176 MB, not its time, which goes by how the rounds of workgroups of a
+// piece come out. us, 176 / 352 / 420 / 880 MB: 8192 x 768 x 50277 2060 / 2226 / 2004 / 1993, 512
+// wide 1538 / 1647 / 1680 / 1659, 4096 x 768 1245 / 1092 / 1029 / 1038, 16384 x 768 4758 / 3885 /
+// 4007 / 3855, 30000 x 256 x 4096 360 / 331 / 332 / 331.
 // ---------------------------------------------------------------------------
 struct ProdArgs {
     const kr_half* G;                 // [rows][ldg]
@@ -588,7 +594,8 @@ __device__ __forceinline__ void store_out(void* out, size_t at, kr_float4 v, int
 // 6e-5 is left, the other dz's. All waves look through all rows and write the same list, so
 // that none waits for another. Measured on MI355X, gradients with / without: 8192 x 768 x 50277
 // 2069 / 2053 us, 20000 x 256 x 256 (half of all rows in every tile) 44.8 / 41.8, 97 x 1024 x
-// 50277 122.6 / 112.6 (three barriers and a step in a quarter of the tiles, which have two).
+// 50277 122.6 / 112.6 (three barriers and a step in a quarter of the tiles, which have two
+// steps without).
 constexpr int kHits = 1024, kLooked = 8 * 64;
 struct TargetRows {
     int2* list;                       // n; column | fp16 rest << 16
@@ -851,7 +858,9 @@ int launch_logits(const LossArgs& g, hipStream_t s) {
 
 // Which tiles. us, 128 x 128 / 256 x 256, width 768: losses over 50277 columns of 128
 // rows 23 / 32, 256 39 / 32, 1024 104 / 104, 4096 372 / 314; over 4096 columns of 2048 rows
-// (128 large tiles) 20 / 29, 8192 64 / 56.
+// (128 large tiles) 20 / 29, 8192 64 / 56. Gradients, of which dz is in them: over 50277
+// columns 128 rows 91 / 101, 256 141 / 131, 1024 336 / 334, 8192 2186 / 2056; over 4096
+// columns 2048 rows 80 / 88, 8192 219 / 211.
 bool big_tiles(int N, int V) {
     return N > 128 && (long long)((N + 255) / 256) * ((V + 255) / 256) >= 192;
 }
@@ -897,9 +906,9 @@ GradPlan grad_plan(int N, int C, int V, bool dx, bool dw, int parts) {
     p.piece = ((V + p.pieces - 1) / p.pieces + 255) / 256 * 256;
     p.pieces = (V + p.piece - 1) / p.piece;
     p.big = big_tiles(N, V);
-    // us for gradients, 128 x 128 / 256 x 256 tiles in the products: 8192 x 768 x 50277 2084 /
-    // 2014, 512 wide 1463 / 1596, 4096 x 256 wide 510 / 581, 16384 x 768 x 16384 (66 tiles of dW
-    // a piece) 1410 / 1666, 4096 x 1024 x 4096 (64) 134 / 167
+    // us for gradients, 128 x 128 / 256 x 256 tiles in the products: 8192 x 768 x 50277 2167 /
+    // 2061, 512 wide 1503 / 1711, 4096 x 256 wide 532 / 603, 16384 x 768 x 16384 (66 tiles of dW
+    // a piece) 1507 / 1838, 4096 x 1024 x 4096 (64) 135 / 187
     p.big_products = p.big && C > 512 && (p.piece / 256) * ((C + 255) / 256) >= 100;
     const int tile = p.big_products ? 256 : 128, slots = p.big_products ? 256 : 512;
     const int gx = (C + tile - 1) / tile, dx_steps = p.piece / 64 * parts, dw_steps = p.rows / 64 * parts;
